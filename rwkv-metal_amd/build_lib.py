@@ -38,7 +38,10 @@ FLAGS = [
 
 def _units():
     units = [("rq_quant.hip", [], "rq_quant.o"), ("rq_sb6.hip", [], "rq_sb6.o"),
-             ("rq_lora.hip", [], "rq_lora.o"),
+             ("rq_lora.hip", [], "rq_lora.o"), ("rq_clip.hip", [], "rq_clip.o"),
+             ("rq_embed.hip", [], "rq_embed.o"), ("rq_linear.hip", [], "rq_linear.o"),
+             ("rq_dpre.hip", [], "rq_dpre.o"),
+             ("rq_train_abi.cpp", ["-x", "hip"], "rq_train_abi.o"),
              ("rq_abi.cpp", ["-x", "hip"], "rq_abi.o")]
     for b in BITS:
         # MFMA results straight into VGPRs: the GEMV consumes every MFMA

@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "../../include/rwkvq.h"
+#include "rq_error.h"
 #include "rq_launch.h"
 #include "rq_mid.h"
 
@@ -94,11 +95,7 @@ static hipError_t launch_qmm(int transpose, const void* x, int x_dt, const uint3
     }
 }
 
-}  // namespace rq
-
-namespace {
-
-thread_local char g_err[512] = "";
+static thread_local char g_err[512] = "";
 
 int fail(int code, const char* fmt, ...) {
     va_list ap;
@@ -113,10 +110,23 @@ int ok() {
     return RQ_OK;
 }
 
+int launch_status(hipError_t e, const char* what) {
+    if (e != hipSuccess) return fail(RQ_ELAUNCH, "%s: HIP launch failed: %s", what, hipGetErrorString(e));
+    return ok();
+}
+
+}  // namespace rq
+
+using rq::aligned16;
+using rq::fail;
+using rq::launch_status;
+using rq::ok;
+using rq::valid_dt;
+
+namespace {
+
 bool valid_bits(int b) { return b == 2 || b == 3 || b == 4 || b == 5 || b == 6 || b == 8; }
 bool valid_gs(int g) { return g == 32 || g == 64 || g == 128; }
-bool valid_dt(int d) { return d == RQ_BF16 || d == RQ_F16 || d == RQ_F32; }
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 int check_common(int64_t rows, int64_t cols, int gs, int bits) {
     if (!valid_bits(bits)) return fail(RQ_EINVAL, "bits must be one of 2,3,4,5,6,8 (got %d)", bits);
@@ -129,18 +139,13 @@ int check_common(int64_t rows, int64_t cols, int gs, int bits) {
     return RQ_OK;
 }
 
-int launch_status(hipError_t e, const char* what) {
-    if (e != hipSuccess) return fail(RQ_ELAUNCH, "%s: HIP launch failed: %s", what, hipGetErrorString(e));
-    return ok();
-}
-
 }  // namespace
 
 extern "C" {
 
 int rq_abi_version(void) { return RWKVQ_ABI_VERSION; }
 
-const char* rq_last_error(void) { return g_err; }
+const char* rq_last_error(void) { return rq::g_err; }
 
 int rq_quantize(const void* w, rq_dtype w_dt, int64_t rows, int64_t cols, int group_size, int bits,
                 uint32_t* w_q, void* scales, void* biases, void* stream) {

@@ -7,7 +7,9 @@ quantize (mlx.nn.quantize).  LoRA engine: LoRALinear, add_lora,
 quantize_base_model, BIG_QUANT_TARGETS, save_lora / load_lora / merge_lora.
 Packed checkpoints: rwkvq.io.save_quantized / load_quantized.  The .rwkvq
 (rwkv-quant sb6) base: RwkvqLinear, RwkvqNativeLinear, RwkvqHybridLinear,
-add_lora_rwkvq, load_sidecar.
+add_lora_rwkvq, load_sidecar.  The rest of a training step: linear_act,
+embedding, grad_norm, clip_grad_norm, clip_grad_norm_ and the modules LinearAct
+and ScaledEmbedding (rwkvq.train).
 All compute runs in librwkvq_hip.so; tensors must be on the GPU.
 """
 from .ops import (VALID_BITS, VALID_GROUP_SIZES, BoundQmm, GroupedQmv, dequantize, grouped_qmv,
@@ -19,6 +21,8 @@ from . import io, sb6
 from .sb6 import RwkvqHybridLinear, RwkvqLinear, RwkvqNativeLinear, add_lora_rwkvq, load_sidecar
 from .lora import (BIG_QUANT_TARGETS, CMIX_TARGETS, TMIX_TARGETS, LoRALinear, add_lora,
                    load_lora, lora_state, merge_lora, quantize_base_model, save_lora)
+from .train import (ACTIVATIONS, LinearAct, ScaledEmbedding, clip_grad_norm, clip_grad_norm_,
+                    embedding, grad_norm, linear_act)
 
 __all__ = [
     "VALID_BITS", "VALID_GROUP_SIZES", "quantize", "dequantize", "quantized_matmul",
@@ -27,5 +31,6 @@ __all__ = [
     "is_quantizable", "quantize_model", "BIG_QUANT_TARGETS", "TMIX_TARGETS", "CMIX_TARGETS",
     "LoRALinear", "add_lora", "quantize_base_model", "lora_state", "save_lora", "load_lora",
     "merge_lora", "io", "sb6", "RwkvqLinear", "RwkvqNativeLinear", "RwkvqHybridLinear",
-    "add_lora_rwkvq", "load_sidecar",
+    "add_lora_rwkvq", "load_sidecar", "ACTIVATIONS", "linear_act", "LinearAct", "embedding",
+    "ScaledEmbedding", "grad_norm", "clip_grad_norm", "clip_grad_norm_",
 ]

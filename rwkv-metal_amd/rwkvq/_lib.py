@@ -38,6 +38,12 @@ class RqProblem(ctypes.Structure):
     ]
 
 
+class RqGrad(ctypes.Structure):
+    """Mirror of rq_grad (include/rwkvq_train.h)."""
+
+    _fields_ = [("g", _vp), ("out", _vp), ("n", _i64), ("dt", _i32), ("pad", _i32)]
+
+
 class RqGroupedPlan(ctypes.Structure):
     """Mirror of rq_grouped_plan."""
 
@@ -80,6 +86,22 @@ SIGNATURES = {
     "rq_grouped_plan_init": ([ctypes.POINTER(RqProblem), _i32, _i32, _i32, _i32, _i64, _i32, _i32,
                               _vp, _i64, ctypes.POINTER(RqGroupedPlan), _vp], _i32),
     "rq_grouped_plan_run": ([ctypes.POINTER(RqGroupedPlan), _vp], _i32),
+    # include/rwkvq_train.h; a list of rq_grad is passed by its address
+    "rq_linear_slope": ([_i32, _i32, _i32], _i32),
+    "rq_linear_workspace_bytes": ([_i32, _i64, _i64, _i64, _i32], _i64),
+    "rq_linear": ([_vp, _vp, _vp, _i32, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _i64,
+                   _vp], _i32),
+    "rq_linear_dpre": ([_vp, _i32, _vp, _i32, _i32, _i32, _i64, _i64, _vp, _vp, _vp, _i64, _vp],
+                       _i32),
+    "rq_linear_dx": ([_vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp], _i32),
+    "rq_linear_dw": ([_vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp], _i32),
+    "rq_embed": ([_vp, _i32, _i64, _vp, _i32, _i64, _i64, ctypes.c_float, _vp, _vp], _i32),
+    "rq_embed_grad_workspace_bytes": ([_i64, _i64, _i64], _i64),
+    "rq_embed_grad": ([_vp, _i32, _i64, _vp, _i32, _i64, _i64, ctypes.c_float, _i64, _vp, _vp,
+                       _i64, _vp], _i32),
+    "rq_grad_norm_workspace_bytes": ([_vp, _i64], _i64),
+    "rq_grad_norm": ([_vp, _i64, _vp, _vp, _i64, _vp], _i32),
+    "rq_clip_grads": ([_vp, _i64, ctypes.c_float, ctypes.c_float, _vp, _vp, _i64, _vp], _i32),
 }
 RQ_EUNSUPPORTED = -4
 

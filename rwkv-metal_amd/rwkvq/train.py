@@ -1,0 +1,587 @@
+"""The operators of a training step around the packed products.
+
+    linear_act(x, weight, bias, activation, residual)  act(x W^T + b) + r, one pass, with gradients
+    embedding(idx, weight, scale, padding_idx)          scale * W[idx] of a table that is trained
+    grad_norm(grads)                                    the 2-norm over a list of gradients
+    clip_grad_norm(grads, max_norm, out)                <- mlx.optimizers.clip_grad_norm
+    clip_grad_norm_(parameters, max_norm)               the same in place, on .grad
+    LinearAct, ScaledEmbedding                          the modules over the first two
+
+Reference call sites: the projections and low-rank tanh / sigmoid branches the
+stock quantizer leaves dense (rwkv_metal/lora/finetune.py:40-42,
+rwkv_metal/model/rwkv7_x070.py:108-111,142-182), the FFN's relu^2
+(rwkv7_x070.py:215-221), the table's lookup (rwkv7_x070.py:302) and the clip of
+the fine-tune loop (rwkv_metal/lora/finetune.py:108-205).
+
+Operands of one dtype stay in it; any other mix computes in float32, as in the
+packed products.  Tensors must live on the ROCm GPU; there is no CPU path.
+"""
+from __future__ import annotations
+
+import array
+import collections
+from typing import Iterable, List, Optional, Sequence, Tuple
+
+import torch
+from torch import Tensor, nn
+from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
+
+from ._lib import DTYPE_CODE, check, lib
+from .ops import _DeviceGuard, _eager, _float, _on_gpu, _ptr, _ready, _stream_on
+
+ACTIVATIONS = (None, "relu", "relu2", "silu", "gelu", "sigmoid", "tanh")
+_ACT_CODE = {a: i for i, a in enumerate(ACTIVATIONS)}
+_SLOPE_NONE, _SLOPE_Y, _SLOPE_F16, _SLOPE_F32 = range(4)
+_OP_FORWARD, _OP_DX, _OP_DW, _OP_DPRE = range(4)
+
+_workspaces: "collections.OrderedDict" = collections.OrderedDict()
+_WORKSPACES_MAX = 8
+
+
+def _workspace(device: torch.device, stream: int, nbytes: int) -> Optional[Tensor]:
+    """Scratch memory of the launches of one stream, which run in order: one
+    buffer per (device, stream), at most _WORKSPACES_MAX of them (least recently
+    used out).  Allocated while its stream is current, so torch's caching
+    allocator reuses a dropped one only on that stream, after the work queued
+    there.  Needs no initialisation."""
+    if nbytes <= 0:
+        return None
+    key = (device.index, stream)
+    ws = _workspaces.pop(key, None)
+    if ws is None or ws.numel() < nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _workspaces[key] = ws
+    while len(_workspaces) > _WORKSPACES_MAX:
+        _workspaces.popitem(last=False)
+    return ws
+
+
+def _addr(t: Optional[Tensor]) -> int:
+    return 0 if t is None or t.numel() == 0 else t.data_ptr()
+
+
+# -------------------------------------------------------------- linear_act
+
+_slope_kinds: dict = {}   # (activation code, dtype code, residual?) -> rq_linear_slope
+_linear_bytes: dict = {}  # (op, m, n, k, dtype code) -> rq_linear_workspace_bytes
+
+
+def _slope_kind(act: int, dt: int, residual: bool) -> int:
+    key = (act, dt, residual)
+    kind = _slope_kinds.get(key)
+    if kind is None:
+        kind = lib().rq_linear_slope(act, dt, int(residual))
+        check(min(kind, 0), "linear_act")
+        _slope_kinds[key] = kind
+    return kind
+
+
+def _linear_workspace(op: int, m: int, n: int, k: int, dt: int, device, stream):
+    key = (op, m, n, k, dt)
+    nbytes = _linear_bytes.get(key)
+    if nbytes is None:
+        nbytes = lib().rq_linear_workspace_bytes(op, m, n, k, dt)
+        check(min(nbytes, 0), "linear_act")
+        if len(_linear_bytes) > 4096:
+            _linear_bytes.clear()
+        _linear_bytes[key] = nbytes
+    ws = _workspace(device, stream, nbytes)
+    return (0, 0) if ws is None else (ws.data_ptr(), ws.numel())
+
+
+def _linear_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor],
+                 act: int, want_slope: bool) -> Tuple[Tensor, Tensor]:
+    """y, and the slopes where the backward pass reads them (else an empty tensor)."""
+    _on_gpu(x, weight, *[t for t in (bias, residual) if t is not None])
+    lead, k = x.shape[:-1], x.shape[-1]
+    n = weight.shape[0]
+    x, weight = _ready(x), _ready(weight)
+    bias = None if bias is None else _ready(bias)
+    residual = None if residual is None else _ready(residual)
+    m = 1
+    for s in lead:
+        m *= s
+    dt = DTYPE_CODE[x.dtype]
+    ydt = x.dtype if residual is None else residual.dtype
+    y = torch.empty(*lead, n, dtype=ydt, device=x.device)
+    kind = _slope_kind(act, dt, residual is not None) if want_slope else _SLOPE_NONE
+    slope = None
+    if kind >= _SLOPE_F16:
+        slope = torch.empty(*lead, n, device=x.device,
+                            dtype=torch.float16 if kind == _SLOPE_F16 else torch.float32)
+    if m and n:
+        with _DeviceGuard(x.device):
+            stream = _stream_on(x.device)
+            ws, nbytes = _linear_workspace(_OP_FORWARD, m, n, k, dt, x.device, stream)
+            rc = lib().rq_linear(_ptr(x), _ptr(weight), _addr(bias), dt, _addr(residual),
+                                 DTYPE_CODE[ydt], m, n, k, act, y.data_ptr(), _addr(slope), ws,
+                                 nbytes, stream)
+        if rc:
+            check(rc, "linear_act")
+    if slope is None and want_slope:
+        slope = x.new_empty(0)
+    return y, slope
+
+
+def _linear_backward_impl(dy: Tensor, x: Tensor, weight: Tensor, saved: Tensor, act: int, kind: int,
+                          want_x: bool, want_w: bool, want_b: bool):
+    """(dx, dw, db), each None unless wanted."""
+    _on_gpu(dy, x, weight)
+    k, n = x.shape[-1], weight.shape[0]
+    dy, x, weight = _ready(dy), _ready(x), _ready(weight)
+    m = dy.numel() // n if n else 0
+    dtype, device = x.dtype, x.device
+    dt = DTYPE_CODE[dtype]
+    dx = torch.empty_like(x) if want_x else None
+    dw = torch.empty_like(weight) if want_w else None
+    db = torch.empty(n, dtype=dtype, device=device) if want_b else None
+    if n == 0:
+        return (dx.zero_() if want_x else None), dw, db
+    L = lib()
+    with _DeviceGuard(device):
+        stream = _stream_on(device)
+        # where act'(v) is 1 and dy is in the operands' type, dy is g
+        is_g = kind == _SLOPE_NONE and dy.dtype == dtype
+        need_g = (want_x or want_w) and not is_g
+        g = torch.empty(dy.shape, dtype=dtype, device=device) if need_g else dy
+        if need_g or want_b:
+            ws, nbytes = _linear_workspace(_OP_DPRE, m, n, 0, dt, device, stream) if want_b else (0, 0)
+            rc = L.rq_linear_dpre(_ptr(dy), DTYPE_CODE[dy.dtype],
+                                  _ptr(saved) if kind != _SLOPE_NONE else 0, kind, act, dt, m, n,
+                                  _ptr(g) if need_g else 0, _addr(db), ws, nbytes, stream)
+            check(rc, "linear_act backward")
+        if want_x and dx.numel():
+            ws, nbytes = _linear_workspace(_OP_DX, m, n, k, dt, device, stream)
+            rc = L.rq_linear_dx(_ptr(g), _ptr(weight), dt, m, n, k, dx.data_ptr(), ws, nbytes, stream)
+            check(rc, "linear_act backward")
+        if want_w and dw.numel():
+            ws, nbytes = _linear_workspace(_OP_DW, m, n, k, dt, device, stream)
+            rc = L.rq_linear_dw(_ptr(g), _ptr(x), dt, m, n, k, dw.data_ptr(), ws, nbytes, stream)
+            check(rc, "linear_act backward")
+    return dx, dw, db
+
+
+def _linear_op_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor],
+                    act: int) -> Tuple[Tensor, Tensor]:
+    return _linear_impl(x, weight, bias, residual, act, True)
+
+
+_linear_op = torch.library.custom_op("rwkvq::linear_act", _linear_op_impl, mutates_args=())
+
+
+@_linear_op.register_fake
+def _(x, weight, bias, residual, act):
+    shape = (*x.shape[:-1], weight.shape[0])
+    kind = _slope_kind(act, DTYPE_CODE[x.dtype], residual is not None)
+    slope = (x.new_empty(0) if kind < _SLOPE_F16 else
+             x.new_empty(shape, dtype=torch.float16 if kind == _SLOPE_F16 else torch.float32))
+    return x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype), slope
+
+
+def _linear_backward_op_impl(dy: Tensor, x: Tensor, weight: Tensor, saved: Tensor, act: int,
+                             kind: int, wanted: List[bool]) -> Tuple[Tensor, Tensor, Tensor]:
+    got = _linear_backward_impl(dy, x, weight, saved, act, kind, *wanted)
+    return tuple(x.new_empty(0) if t is None else t for t in got)
+
+
+_linear_backward_op = torch.library.custom_op("rwkvq::linear_act_backward", _linear_backward_op_impl,
+                                              mutates_args=())
+
+
+@_linear_backward_op.register_fake
+def _(dy, x, weight, saved, act, kind, wanted):
+    return (torch.empty_like(x) if wanted[0] else x.new_empty(0),
+            torch.empty_like(weight) if wanted[1] else x.new_empty(0),
+            x.new_empty(weight.shape[0]) if wanted[2] else x.new_empty(0))
+
+
+def _linear_op_setup(ctx, inputs, output):
+    x, weight, bias, residual, act = inputs
+    ctx.act = act
+    ctx.kind = _slope_kind(act, DTYPE_CODE[x.dtype], residual is not None)
+    ctx.save_for_backward(x, weight, output[0] if ctx.kind == _SLOPE_Y else output[1])
+
+
+def _linear_op_backward(ctx, dy, _dslope):
+    x, weight, saved = ctx.saved_tensors
+    need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+    dx, dw, db = _linear_backward_op(dy.contiguous(), x, weight, saved, ctx.act, ctx.kind,
+                                     [need_x, need_w, need_b])
+    return (dx if need_x else None, dw if need_w else None, db if need_b else None,
+            dy if need_r else None, None)
+
+
+_linear_op.register_autograd(_linear_op_backward, setup_context=_linear_op_setup)
+
+
+class _LinearActFunction(torch.autograd.Function):
+    """The registered op's autograd formula without its dispatch, for plain eager
+    GPU tensors."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        need_pre = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        y, slope = _linear_impl(x, weight, bias, residual, act, need_pre)
+        ctx.act = act
+        ctx.kind = _slope_kind(act, DTYPE_CODE[x.dtype], residual is not None) if need_pre else 0
+        if need_pre:
+            ctx.save_for_backward(x, weight, y if ctx.kind == _SLOPE_Y else slope)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            x, weight, saved = ctx.saved_tensors
+            dx, dw, db = _linear_backward_impl(dy, x, weight, saved, ctx.act, ctx.kind, need_x,
+                                               need_w, need_b)
+        return dx, dw, db, dy if need_r else None, None
+
+
+def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
+               activation: Optional[str] = None, residual: Optional[Tensor] = None) -> Tensor:
+    """act(x @ weight^T + bias) + residual in one pass over the output.
+
+    x [..., k], weight [n, k], bias [n]; residual [..., n] is added after the
+    activation and may be float32 beside 16-bit operands: y then is too, a
+    float32 residual stream.  activation: None, "relu", "relu2" (relu(v)^2),
+    "silu", "gelu" (v Phi(v)), "sigmoid" or "tanh".  The sums, the activation and
+    the residual's addition are in float32, rounded once.
+
+    The backward pass keeps x, weight and the slope act'(v): read off y for relu
+    and relu2 without a residual, else a tensor of its own (float16 beside bf16
+    operands, float32 beside others and for relu2).  Its products take g = dy act'(v)
+    rounded to the operands' type."""
+    if activation not in _ACT_CODE:
+        raise ValueError(f"activation must be one of {ACTIVATIONS} (got {activation!r})")
+    _float(x, "x")
+    _float(weight, "weight")
+    if weight.dim() != 2:
+        raise ValueError("linear_act expects a 2-D weight")
+    if x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x has shape {tuple(x.shape)} but the weight expects an inner dimension of "
+                         f"{weight.shape[1]}")
+    if bias is not None:
+        _float(bias, "bias")
+        if bias.shape != (weight.shape[0],):
+            raise ValueError(f"bias must have shape {(weight.shape[0],)} (got {tuple(bias.shape)})")
+    if residual is not None:
+        _float(residual, "residual")
+        want = (*x.shape[:-1], weight.shape[0])
+        if residual.shape != want:
+            raise ValueError(f"residual must have shape {want} (got {tuple(residual.shape)})")
+    dt = x.dtype
+    if weight.dtype != dt or (bias is not None and bias.dtype != dt):
+        dt = torch.float32
+        x, weight = x.to(dt), weight.to(dt)
+        bias = None if bias is None else bias.to(dt)
+    if residual is not None and residual.dtype not in (dt, torch.float32):
+        residual = residual.to(torch.float32)
+    act = _ACT_CODE[activation]
+    ts = [t for t in (x, weight, bias, residual) if t is not None]
+    if _eager(*ts):
+        if not torch.is_grad_enabled() or not any(t.requires_grad for t in ts):
+            return _linear_impl(x, weight, bias, residual, act, False)[0]
+        if forward_ad._current_level < 0:
+            return _LinearActFunction.apply(x, weight, bias, residual, act)
+    return _linear_op(x, weight, bias, residual, act)[0]
+
+
+class LinearAct(nn.Linear):
+    """nn.Linear with an activation and an optional residual in its product's
+    output stage: forward(x, residual=None) = act(x W^T + b) + residual."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True,
+                 activation: Optional[str] = None, device=None, dtype=None):
+        super().__init__(in_features, out_features, bias, device=device, dtype=dtype)
+        if activation not in _ACT_CODE:
+            raise ValueError(f"activation must be one of {ACTIVATIONS} (got {activation!r})")
+        self.activation = activation
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, activation: Optional[str] = None) -> "LinearAct":
+        """The same parameters (shared, not copied) with an activation behind them."""
+        m = cls(linear.in_features, linear.out_features, linear.bias is not None, activation,
+                device="meta", dtype=linear.weight.dtype)
+        m.weight, m.bias = linear.weight, linear.bias
+        return m
+
+    def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Tensor:
+        return linear_act(x, self.weight, self.bias, self.activation, residual)
+
+    def extra_repr(self) -> str:
+        return f"{super().extra_repr()}, activation={self.activation}"
+
+
+# --------------------------------------------------------------- embedding
+
+_INDEX_TYPES = (torch.int64, torch.int32)
+
+
+def _embed_impl(idx: Tensor, weight: Tensor, scale: float) -> Tensor:
+    _on_gpu(weight, idx)
+    idx, weight = idx.contiguous(), weight.contiguous()
+    vocab, dim = weight.shape
+    out = torch.empty(*idx.shape, dim, dtype=weight.dtype, device=weight.device)
+    if out.numel():
+        with _DeviceGuard(weight.device):
+            rc = lib().rq_embed(_ptr(idx), idx.element_size(), idx.numel(), _ptr(weight),
+                                DTYPE_CODE[weight.dtype], vocab, dim, scale, out.data_ptr(),
+                                _stream_on(weight.device))
+        if rc:
+            check(rc, "embedding")
+    return out
+
+
+def _embed_grad_impl(dout: Tensor, idx: Tensor, vocab: int, scale: float, padding_idx: int) -> Tensor:
+    _on_gpu(dout, idx)
+    dout, idx = dout.contiguous(), idx.contiguous()
+    dim, n = dout.shape[-1], idx.numel()
+    dw = torch.empty(vocab, dim, dtype=dout.dtype, device=dout.device)
+    if dw.numel():
+        L = lib()
+        with _DeviceGuard(dout.device):
+            stream = _stream_on(dout.device)
+            nbytes = L.rq_embed_grad_workspace_bytes(n, vocab, dim)
+            check(min(nbytes, 0), "embedding backward")
+            ws = _workspace(dout.device, stream, nbytes)
+            rc = L.rq_embed_grad(_ptr(idx), idx.element_size(), n, _ptr(dout), DTYPE_CODE[dout.dtype],
+                                 vocab, dim, scale, padding_idx, dw.data_ptr(), ws.data_ptr(),
+                                 ws.numel(), stream)
+        check(rc, "embedding backward")
+    return dw
+
+
+def _embed_op_impl(idx: Tensor, weight: Tensor, scale: float, padding_idx: int) -> Tensor:
+    return _embed_impl(idx, weight, scale)
+
+
+_embed_op = torch.library.custom_op("rwkvq::embedding", _embed_op_impl, mutates_args=())
+_embed_grad_op = torch.library.custom_op("rwkvq::embedding_grad", _embed_grad_impl, mutates_args=())
+
+
+@_embed_op.register_fake
+def _(idx, weight, scale, padding_idx):
+    return weight.new_empty(*idx.shape, weight.shape[1])
+
+
+@_embed_grad_op.register_fake
+def _(dout, idx, vocab, scale, padding_idx):
+    return dout.new_empty(vocab, dout.shape[-1])
+
+
+def _embed_setup(ctx, inputs, output):
+    idx, weight, ctx.scale, ctx.padding_idx = inputs
+    ctx.vocab = weight.shape[0]
+    ctx.save_for_backward(idx)
+
+
+def _embed_backward(ctx, dout):
+    idx, = ctx.saved_tensors
+    dw = None
+    if ctx.needs_input_grad[1]:
+        dw = _embed_grad_op(dout, idx, ctx.vocab, ctx.scale, ctx.padding_idx)
+    return None, dw, None, None
+
+
+_embed_op.register_autograd(_embed_backward, setup_context=_embed_setup)
+
+
+class _EmbeddingFunction(torch.autograd.Function):
+    """The registered op's autograd formula without its dispatch."""
+
+    @staticmethod
+    def forward(ctx, idx, weight, scale, padding_idx):
+        ctx.save_for_backward(idx)
+        ctx.vocab, ctx.scale, ctx.padding_idx = weight.shape[0], scale, padding_idx
+        return _embed_impl(idx, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        idx, = ctx.saved_tensors
+        return None, _embed_grad_impl(dout, idx, ctx.vocab, ctx.scale, ctx.padding_idx), None, None
+
+
+def embedding(idx: Tensor, weight: Tensor, scale: float = 1.0,
+              padding_idx: Optional[int] = None) -> Tensor:
+    """scale * weight[idx], rounded once: idx integers of any shape, weight
+    [vocab, dim].  Indices outside the table give rows of NaN and no gradient.
+    The table's gradient is dense: scale times the float32 sum of each token's rows,
+    in an order that does not change from run to run; 0 for padding_idx."""
+    _float(weight, "weight")
+    if weight.dim() != 2:
+        raise ValueError("embedding expects a 2-D table")
+    if idx.dtype not in _INDEX_TYPES:
+        if idx.dtype not in (torch.int16, torch.uint8, torch.int8):
+            raise ValueError(f"indices must be an integer tensor (got {idx.dtype})")
+        idx = idx.to(torch.int32)
+    vocab = weight.shape[0]
+    pad = -1
+    if padding_idx is not None:
+        if not -vocab <= padding_idx < vocab:
+            raise ValueError(f"padding_idx {padding_idx} is outside the table of {vocab} rows")
+        pad = padding_idx % vocab
+    scale = float(scale)
+    if _eager(idx, weight):
+        if not (weight.requires_grad and torch.is_grad_enabled()):
+            return _embed_impl(idx, weight, scale)
+        if forward_ad._current_level < 0:
+            return _EmbeddingFunction.apply(idx, weight, scale, pad)
+    return _embed_op(idx, weight, scale, pad)
+
+
+class ScaledEmbedding(nn.Embedding):
+    """nn.Embedding whose rows are multiplied by `scale` in the lookup."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0,
+                 padding_idx: Optional[int] = None, device=None, dtype=None):
+        super().__init__(num_embeddings, embedding_dim, padding_idx, device=device, dtype=dtype)
+        self.scale = scale
+
+    def forward(self, idx: Tensor) -> Tensor:
+        return embedding(idx, self.weight, self.scale, self.padding_idx)
+
+    def extra_repr(self) -> str:
+        return f"{super().extra_repr()}, scale={self.scale}"
+
+
+# --------------------------------------------------- gradient norm and clip
+
+def _grad_list(grads: Sequence[Tensor], out: Optional[Sequence[Tensor]]) -> array.array:
+    """The tensors as an array of rq_grad: (g, out, n, dtype code), 8 bytes each
+    (the dtype's upper four are rq_grad's padding)."""
+    n = len(grads)
+    a = array.array("q", bytes(32 * n))
+    a[0::4] = array.array("q", map(Tensor.data_ptr, grads))
+    a[1::4] = a[0::4] if out is None else array.array("q", map(Tensor.data_ptr, out))
+    a[2::4] = array.array("q", map(Tensor.numel, grads))
+    a[3::4] = array.array("q", [DTYPE_CODE[t.dtype] for t in grads])
+    return a
+
+
+def _check_grads(grads: Sequence[Tensor]) -> torch.device:
+    for t in grads:
+        if not isinstance(t, Tensor):
+            raise ValueError(f"gradients must be tensors (got {type(t).__name__})")
+        if t.dtype not in DTYPE_CODE:
+            _float(t, "gradients")
+        if t.is_sparse:
+            raise ValueError("sparse gradients are not supported")
+    _on_gpu(*grads)
+    return grads[0].device
+
+
+def _dense(t: Tensor) -> bool:
+    """Whether the tensor's elements fill its memory without gaps, in any order
+    of the dimensions: the norm and the factor do not depend on the order."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _run_norm(grads, out, max_norm, eps, device) -> Tensor:
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    a = _grad_list(grads, out)
+    at, n = a.buffer_info()[0], len(grads)
+    L = lib()
+    with _DeviceGuard(device):
+        stream = _stream_on(device)
+        nbytes = L.rq_grad_norm_workspace_bytes(at, n)
+        check(min(nbytes, 0), "clip_grad_norm")
+        ws = _workspace(device, stream, max(nbytes, 16))
+        if max_norm is None:
+            rc = L.rq_grad_norm(at, n, norm.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+        else:
+            rc = L.rq_clip_grads(at, n, max_norm, eps, norm.data_ptr(), ws.data_ptr(), ws.numel(),
+                                 stream)
+    check(rc, "clip_grad_norm")
+    return norm
+
+
+def grad_norm(grads: Iterable[Tensor]) -> Tensor:
+    """sqrt(sum of squares of every element of every tensor), a float32 scalar on
+    the GPU (nothing waits for it).  The squares are added in float64.  An empty
+    list has norm 0 and gives a CPU tensor."""
+    grads = [t.detach() for t in grads]
+    if not grads:
+        return torch.zeros(())
+    device = _check_grads(grads)
+    return _run_norm([t if _dense(t) else t.contiguous() for t in grads], None, None, 0.0, device)
+
+
+def clip_grad_norm(grads: Iterable[Tensor], max_norm: float, out: Optional[Sequence[Tensor]] = None,
+                   eps: float = 1e-6) -> Tuple[List[Tensor], Tensor]:
+    """(clipped, norm): every gradient times min(max_norm / (norm + eps), 1), the
+    factor in float32 and one rounding, and the norm over all of them
+    (mlx.optimizers.clip_grad_norm).  out: contiguous tensors of the gradients'
+    shapes and dtypes to write to (they may be the gradients themselves); by
+    default views of one new buffer for each dtype.  A NaN norm makes every
+    gradient NaN."""
+    grads = [t.detach() for t in grads]
+    max_norm, eps = float(max_norm), float(eps)
+    if not max_norm >= 0 or not eps >= 0:
+        raise ValueError(f"max_norm and eps must not be negative (got {max_norm} and {eps})")
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"out has {len(out)} tensors for {len(grads)} gradients")
+    if not grads:
+        return [], torch.zeros(())
+    device = _check_grads(grads)
+    grads = [t if t.is_contiguous() else t.contiguous() for t in grads]
+    if out is None:
+        out = _new_like(grads)
+    else:
+        _on_gpu(grads[0], *out)
+        for t, o in zip(grads, out):
+            if o.shape != t.shape or o.dtype != t.dtype or not o.is_contiguous():
+                raise ValueError(f"out must be contiguous {t.dtype} of shape {tuple(t.shape)} (got "
+                                 f"{o.dtype} {tuple(o.shape)}, strides {o.stride()})")
+    return out, _run_norm(grads, out, max_norm, eps, device)
+
+
+def _new_like(grads: Sequence[Tensor]) -> List[Tensor]:
+    """A contiguous tensor for each, cut from one buffer per dtype."""
+    out: list = [None] * len(grads)
+    by: dict = {}
+    for i, t in enumerate(grads):
+        by.setdefault(t.dtype, []).append(i)
+    for dtype, places in by.items():
+        # whole 16-byte lines, so that every view stays on the wide path
+        per = 16 // dtype.itemsize
+        sizes = [-(-grads[i].numel() // per) * per for i in places]
+        flat = torch.empty(sum(sizes), dtype=dtype, device=grads[0].device)
+        for i, p in zip(places, flat.split(sizes)):
+            out[i] = p[:grads[i].numel()].view(grads[i].shape)
+    return out
+
+
+def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6) -> Tensor:
+    """Clips the .grad of the parameters (or one parameter) in place and returns
+    the norm over them, a float32 scalar on the GPU; parameters without a
+    gradient are left out.  Nothing is written where the norm is within
+    max_norm."""
+    if isinstance(parameters, Tensor):
+        parameters = [parameters]
+    grads = [p.grad.detach() for p in parameters if p.grad is not None]
+    max_norm, eps = float(max_norm), float(eps)
+    if not max_norm >= 0 or not eps >= 0:
+        raise ValueError(f"max_norm and eps must not be negative (got {max_norm} and {eps})")
+    if not grads:
+        return torch.zeros(())
+    device = _check_grads(grads)
+    dense = [t if _dense(t) else t.contiguous() for t in grads]
+    norm = _run_norm(dense, None, max_norm, eps, device)
+    for t, d in zip(grads, dense):
+        if t is not d:
+            t.copy_(d)
+    return norm
