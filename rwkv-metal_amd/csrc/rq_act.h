@@ -50,6 +50,41 @@ RQ_DEV float act_slope(int act, float v) {
     }
 }
 
+// The same of four values; one scalar branch for all of them.
+RQ_DEV f32x4_t act_value4(int act, f32x4_t v) {
+    switch (act) {
+#define RQ_ACT4(A)                                               \
+    case A:                                                      \
+        return f32x4_t{act_value(A, v[0]), act_value(A, v[1]),   \
+                       act_value(A, v[2]), act_value(A, v[3])};
+        RQ_ACT4(RQ_ACT_RELU)
+        RQ_ACT4(RQ_ACT_RELU2)
+        RQ_ACT4(RQ_ACT_SILU)
+        RQ_ACT4(RQ_ACT_GELU)
+        RQ_ACT4(RQ_ACT_SIGMOID)
+        RQ_ACT4(RQ_ACT_TANH)
+#undef RQ_ACT4
+        default: return v;
+    }
+}
+
+RQ_DEV f32x4_t act_slope4(int act, f32x4_t v) {
+    switch (act) {
+#define RQ_ACT4(A)                                               \
+    case A:                                                      \
+        return f32x4_t{act_slope(A, v[0]), act_slope(A, v[1]),   \
+                       act_slope(A, v[2]), act_slope(A, v[3])};
+        RQ_ACT4(RQ_ACT_RELU)
+        RQ_ACT4(RQ_ACT_RELU2)
+        RQ_ACT4(RQ_ACT_SILU)
+        RQ_ACT4(RQ_ACT_GELU)
+        RQ_ACT4(RQ_ACT_SIGMOID)
+        RQ_ACT4(RQ_ACT_TANH)
+#undef RQ_ACT4
+        default: return f32x4_t{1.f, 1.f, 1.f, 1.f};
+    }
+}
+
 // act'(v) from y = act(v): relu and relu2 only (relu2: v = sqrt(y)).
 RQ_DEV float act_slope_of_y(int act, float y) {
     if (act == RQ_ACT_RELU) return y > 0.f ? 1.f : 0.f;

@@ -31,7 +31,7 @@ struct DenseArgs {
 constexpr int kDenseMaxSide = 65535 * 64;  // of m, n and k: grids count 64 rows in y
 
 hipError_t launch_dense(const DenseArgs& a, void* workspace, hipStream_t stream);
-int64_t dense_workspace_bytes(int64_t m, int64_t n, int64_t k, int dt, bool a_t, bool b_t);
+int64_t dense_workspace_bytes(const DenseArgs& a);  // of a's sizes, type and orders
 
 
 // g = dy * act'(v) and db = its column sums (rq_linear_dpre).

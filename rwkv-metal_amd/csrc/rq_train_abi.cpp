@@ -33,8 +33,18 @@ int check_ptrs(const char* what, std::initializer_list<const void*> needed, std:
     return RQ_OK;
 }
 
+rq::DenseArgs forward_args(const void* x, const void* w, int64_t m, int64_t n, int64_t k, int dt) {
+    return {x, w, k, k, m, n, k, dt, false, false, nullptr, nullptr, RQ_ACT_NONE, nullptr, dt, nullptr, 0};
+}
+rq::DenseArgs dx_args(const void* g, const void* w, int64_t m, int64_t n, int64_t k, int dt, void* dx) {
+    return {g, w, n, k, m, k, n, dt, false, true, nullptr, nullptr, RQ_ACT_NONE, dx, dt, nullptr, 0};
+}
+rq::DenseArgs dw_args(const void* g, const void* x, int64_t m, int64_t n, int64_t k, int dt, void* dw) {
+    return {g, x, n, k, n, k, m, dt, true, true, nullptr, nullptr, RQ_ACT_NONE, dw, dt, nullptr, 0};
+}
+
 int run_dense(const char* what, const rq::DenseArgs& g, void* workspace, int64_t bytes, void* stream) {
-    const int64_t need = rq::dense_workspace_bytes(g.m, g.n, g.k, g.dt, g.a_t, g.b_t);
+    const int64_t need = rq::dense_workspace_bytes(g);
     if (need > 0 && (!workspace || bytes < need))
         return fail(RQ_EINVAL, "%s: needs a workspace of %lld bytes", what, (long long)need);
     return rq::launch_status(rq::launch_dense(g, workspace, (hipStream_t)stream), what);
@@ -60,9 +70,9 @@ int64_t rq_linear_workspace_bytes(int op, int64_t m, int64_t n, int64_t k, rq_dt
     if (int rc = check_sizes(what, m, n, k, dt)) return rc;
     ok();
     switch (op) {
-        case 0: return rq::dense_workspace_bytes(m, n, k, dt, false, false);
-        case 1: return rq::dense_workspace_bytes(m, k, n, dt, false, true);
-        case 2: return rq::dense_workspace_bytes(n, k, m, dt, true, true);
+        case 0: return rq::dense_workspace_bytes(forward_args(nullptr, nullptr, m, n, k, dt));
+        case 1: return rq::dense_workspace_bytes(dx_args(nullptr, nullptr, m, n, k, dt, nullptr));
+        case 2: return rq::dense_workspace_bytes(dw_args(nullptr, nullptr, m, n, k, dt, nullptr));
         case 3: return rq::dpre_workspace_bytes(m, n);
         default: return fail(RQ_EINVAL, "%s: unknown op %d", what, op);
     }
@@ -82,7 +92,14 @@ int rq_linear(const void* x, const void* w, const void* bias, rq_dtype dt, const
     if (k > 0 && (!x || !w)) return fail(RQ_EINVAL, "%s: NULL pointer", what);
     if (slope && kind != RQ_SLOPE_F16 && kind != RQ_SLOPE_F32)
         return fail(RQ_EINVAL, "%s: this activation keeps no slopes (rq_linear_slope)", what);
-    const rq::DenseArgs g{x, w, k, k, m, n, k, dt, false, false, bias, residual, act, y, y_dt, slope, kind};
+    rq::DenseArgs g = forward_args(x, w, m, n, k, dt);
+    g.bias = bias;
+    g.residual = residual;
+    g.act = act;
+    g.y = y;
+    g.y_dt = y_dt;
+    g.slope = slope;
+    g.slope_kind = kind;
     return run_dense(what, g, workspace, workspace_bytes, stream);
 }
 
@@ -113,8 +130,7 @@ int rq_linear_dx(const void* g, const void* w, rq_dtype dt, int64_t m, int64_t n
     if (m == 0 || k == 0) return ok();
     if (int rc = check_ptrs(what, {dx}, {g, w, dx, workspace})) return rc;
     if (n > 0 && (!g || !w)) return fail(RQ_EINVAL, "%s: NULL pointer", what);
-    const rq::DenseArgs a{g, w, n, k, m, k, n, dt, false, true, nullptr, nullptr, RQ_ACT_NONE, dx, dt, nullptr, 0};
-    return run_dense(what, a, workspace, workspace_bytes, stream);
+    return run_dense(what, dx_args(g, w, m, n, k, dt, dx), workspace, workspace_bytes, stream);
 }
 
 int rq_linear_dw(const void* g, const void* x, rq_dtype dt, int64_t m, int64_t n, int64_t k, void* dw,
@@ -124,8 +140,7 @@ int rq_linear_dw(const void* g, const void* x, rq_dtype dt, int64_t m, int64_t n
     if (n == 0 || k == 0) return ok();
     if (int rc = check_ptrs(what, {dw}, {g, x, dw, workspace})) return rc;
     if (m > 0 && (!g || !x)) return fail(RQ_EINVAL, "%s: NULL pointer", what);
-    const rq::DenseArgs a{g, x, n, k, n, k, m, dt, true, true, nullptr, nullptr, RQ_ACT_NONE, dw, dt, nullptr, 0};
-    return run_dense(what, a, workspace, workspace_bytes, stream);
+    return run_dense(what, dw_args(g, x, m, n, k, dt, dw), workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"
