@@ -44,19 +44,19 @@ typedef enum {
 
 /* What the backward pass takes act'(v) from: nothing (act'(v) = 1), the output
  * y, or a tensor of slopes act'(v) that the forward pass wrote. */
-enum { RQ_SLOPE_NONE = 0, RQ_SLOPE_Y = 1, RQ_SLOPE_F16 = 2, RQ_SLOPE_F32 = 3 };
+enum { RQ_SLOPE_NONE = 0, RQ_SLOPE_Y = 1, RQ_SLOPE_F16 = 2, RQ_SLOPE_F32 = 3, RQ_SLOPE_WIDE16 = 4 };
 
-/* The form of the slope for operands of type dt: RQ_SLOPE_Y where y alone gives
- * it (relu, and relu2 of bf16 or fp32, with no residual added), float16 for the
- * other activations of bf16 operands, whose slopes are bounded and keep three
- * bits more than in bf16, float32 otherwise.  RQ_EINVAL for an unknown act or dt. */
+/* The form of the slope for operands of type dt.  RQ_SLOPE_Y where y alone gives
+ * it: relu, and relu2 of fp32, with no residual added.  For bf16 operands 16 bits
+ * that keep three bits more than bf16: float16 where the slope is bounded, and for
+ * relu2, whose slope 2 v is not but has no sign, RQ_SLOPE_WIDE16: the float16 bits of
+ * a slope in [2^-14, 2^15), else 0x8000 + its bf16 bits.  float32 otherwise.
+ * RQ_EINVAL for an unknown act or dt. */
 int rq_linear_slope(rq_act act, rq_dtype dt, int has_residual);
 
-/* Bytes of workspace of rq_linear, rq_linear_dx and rq_linear_dw (0: none, the
- * pointer may be NULL) for x [m, k], w [n, k], operands of type dt; or a
- * negative return code.  op: 0 rq_linear, 1 rq_linear_dx, 2 rq_linear_dw,
- * 3 rq_linear_dpre. */
-int64_t rq_linear_workspace_bytes(int op, int64_t m, int64_t n, int64_t k, rq_dtype dt);
+/* Bytes of workspace of rq_linear for these sizes (0: none, the pointer may be
+ * NULL), or a negative return code. */
+int64_t rq_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, rq_dtype dt);
 
 /* y[m, n] = act(x[m, k] . w[n, k]^T + bias[n]) + residual[m, n].
  * x, w and bias (or NULL) in dt; residual (or NULL) and y in y_dt, which is dt
@@ -69,20 +69,20 @@ int rq_linear(const void* x, const void* w, const void* bias, rq_dtype dt, const
               rq_dtype y_dt, int64_t m, int64_t n, int64_t k, rq_act act, void* y, void* slope,
               void* workspace, int64_t workspace_bytes, void* stream);
 
-/* g = dy * act'(v) [m, n] in dt and db[n] = sum over m of g, in dt, from the
- * unrounded g.  Either output may be NULL.  dy in y_dt.  slope: y (in y_dt) for
- * RQ_SLOPE_Y, the forward's slopes for RQ_SLOPE_F16 / RQ_SLOPE_F32, NULL for
- * RQ_SLOPE_NONE. */
-int rq_linear_dpre(const void* dy, rq_dtype y_dt, const void* slope, int slope_kind, rq_act act,
-                   rq_dtype dt, int64_t m, int64_t n, void* g, void* db, void* workspace,
-                   int64_t workspace_bytes, void* stream);
-
-/* dx[m, k] = g[m, n] . w[n, k] and dw[n, k] = g[m, n]^T . x[m, k], everything
- * in dt, accumulated in fp32. */
-int rq_linear_dx(const void* g, const void* w, rq_dtype dt, int64_t m, int64_t n, int64_t k,
-                 void* dx, void* workspace, int64_t workspace_bytes, void* stream);
-int rq_linear_dw(const void* g, const void* x, rq_dtype dt, int64_t m, int64_t n, int64_t k,
-                 void* dw, void* workspace, int64_t workspace_bytes, void* stream);
+/* The gradients of rq_linear's x, w and bias: with g = dy * act'(v) [m, n]
+ *   dx[m, k] = g . w      dw[n, k] = g^T . x      db[n] = sum over m of g
+ * in dt, each written only where its pointer is not NULL (x and w may be NULL where
+ * no wanted gradient reads them).  dy is in y_dt (dt or RQ_F32).  slope: y (in y_dt) for
+ * RQ_SLOPE_Y, what rq_linear wrote for the kinds it writes, NULL for RQ_SLOPE_NONE.
+ * g is rounded to dt once for the two products (dy itself is g where the slope is 1 and
+ * the types are equal) and added up unrounded for db; all sums are fp32.
+ * rq_linear_backward_workspace_bytes: for the gradients wanted (has_*). */
+int64_t rq_linear_backward_workspace_bytes(int64_t m, int64_t n, int64_t k, rq_dtype dt, rq_dtype y_dt,
+                                           int slope_kind, int has_dx, int has_dw, int has_db);
+int rq_linear_backward(const void* dy, rq_dtype y_dt, const void* slope, int slope_kind, rq_act act,
+                       const void* x, const void* w, rq_dtype dt, int64_t m, int64_t n, int64_t k,
+                       void* dx, void* dw, void* db, void* workspace, int64_t workspace_bytes,
+                       void* stream);
 
 /* out[i, :] = scale * table[idx[i], :], i < n, table [vocab, dim] and out in
  * dt, rounded once.  idx: int32 (idx_bytes 4) or int64 (8).  An index outside

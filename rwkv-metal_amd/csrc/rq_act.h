@@ -85,6 +85,17 @@ RQ_DEV f32x4_t act_slope4(int act, f32x4_t v) {
     }
 }
 
+// RQ_SLOPE_WIDE16: a slope s >= 0 in 16 bits, float16 in [2^-14, 2^15), where that
+// keeps 11 bits, else bf16 with the unused sign bit as the mark.  Values >= 0
+// compare like their bits.
+RQ_DEV uint32_t wide16_bits(float s) {
+    constexpr uint32_t lo = 0x38800000u, hi = 0x47000000u;  // 2^-14 and 2^15
+    return __float_as_uint(s) - lo < hi - lo ? f32_to_f16_bits(s) : (f32_to_bf16_bits(s) | 0x8000u);
+}
+RQ_DEV float wide16_value(uint32_t b) {
+    return b & 0x8000u ? bf16_bits_to_f32(b & 0x7fffu) : f16_bits_to_f32(b);
+}
+
 // act'(v) from y = act(v): relu and relu2 only (relu2: v = sqrt(y)).
 RQ_DEV float act_slope_of_y(int act, float y) {
     if (act == RQ_ACT_RELU) return y > 0.f ? 1.f : 0.f;

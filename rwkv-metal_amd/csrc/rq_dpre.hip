@@ -30,8 +30,8 @@ RQ_DEV void store8(uint8_t* row, int64_t c, int64_t n, const float* f) {
     for (int h = 0; h < 8; h += kVec<DT>) store_cols<DT>(row, c + h, n, f + h);
 }
 
-// SDT: the slopes' type, -1 where act'(v) is 1; OFY: they are y, of type SDT.
-template <int DT, int YDT, int SDT, bool OFY>
+// KIND: RQ_SLOPE_*.  SDT: the type the slopes (or y) are held in, -1 where act'(v) is 1.
+template <int DT, int YDT, int KIND, int SDT>
 __global__ __launch_bounds__(kBlock) void dpre_kernel(const rq::DpreArgs a, float* __restrict__ part) {
     __shared__ float red[kWaves][kCols];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -47,6 +47,10 @@ __global__ __launch_bounds__(kBlock) void dpre_kernel(const rq::DpreArgs a, floa
             if (r0 + r >= a.m) break;
             load8<YDT>(dy + (r0 + r) * a.n * kSize<YDT>, c, a.n, f[r]);
             if constexpr (SDT >= 0) load8<SDT>(sl + (r0 + r) * a.n * kSize<SDT>, c, a.n, s[r]);
+            if constexpr (KIND == RQ_SLOPE_WIDE16) {  // read as bf16, which keeps the bits
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[r][j] = wide16_value(__float_as_uint(s[r][j]) >> 16);
+            }
         }
     }
     float sum[8];
@@ -58,7 +62,7 @@ __global__ __launch_bounds__(kBlock) void dpre_kernel(const rq::DpreArgs a, floa
             if (r0 + r >= a.m) break;
             if constexpr (SDT >= 0) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) f[r][j] *= OFY ? act_slope_of_y(a.act, s[r][j]) : s[r][j];
+                for (int j = 0; j < 8; ++j) f[r][j] *= KIND == RQ_SLOPE_Y ? act_slope_of_y(a.act, s[r][j]) : s[r][j];
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] += f[r][j];
@@ -111,10 +115,11 @@ __global__ __launch_bounds__(kBlock) void colsum_kernel(const float* __restrict_
 template <int DT, int YDT>
 void launch_as(const rq::DpreArgs& a, float* part, dim3 grid, hipStream_t s) {
     switch (a.slope_kind) {
-        case RQ_SLOPE_Y: dpre_kernel<DT, YDT, YDT, true><<<grid, kBlock, 0, s>>>(a, part); break;
-        case RQ_SLOPE_F16: dpre_kernel<DT, YDT, RQ_F16, false><<<grid, kBlock, 0, s>>>(a, part); break;
-        case RQ_SLOPE_F32: dpre_kernel<DT, YDT, RQ_F32, false><<<grid, kBlock, 0, s>>>(a, part); break;
-        default: dpre_kernel<DT, YDT, -1, false><<<grid, kBlock, 0, s>>>(a, part); break;
+        case RQ_SLOPE_Y: dpre_kernel<DT, YDT, RQ_SLOPE_Y, YDT><<<grid, kBlock, 0, s>>>(a, part); break;
+        case RQ_SLOPE_F16: dpre_kernel<DT, YDT, RQ_SLOPE_F16, RQ_F16><<<grid, kBlock, 0, s>>>(a, part); break;
+        case RQ_SLOPE_F32: dpre_kernel<DT, YDT, RQ_SLOPE_F32, RQ_F32><<<grid, kBlock, 0, s>>>(a, part); break;
+        case RQ_SLOPE_WIDE16: dpre_kernel<DT, YDT, RQ_SLOPE_WIDE16, RQ_BF16><<<grid, kBlock, 0, s>>>(a, part); break;
+        default: dpre_kernel<DT, YDT, RQ_SLOPE_NONE, -1><<<grid, kBlock, 0, s>>>(a, part); break;
     }
 }
 

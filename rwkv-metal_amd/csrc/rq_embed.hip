@@ -76,9 +76,9 @@ constexpr int kSortWaves = 16;
 constexpr int kSortBlock = 64 * kSortWaves;
 constexpr int kMinSortBlocks = 256;  // one for each CU; a power of two
 constexpr int kMaxIds = 512;         // ids of one block: 16 waves * 512 counters of LDS, 32 KB
-constexpr int kScan = 8;             // index loads of a lane in flight
+constexpr int kScan = 16;            // index loads of a lane in flight
 constexpr int kMaxShares = 1024;
-constexpr int kMaxDim = 65535 * 64;  // blockIdx.y counts columns by 64 in the last launch
+constexpr int kMaxDim = 65535 * 256;  // blockIdx.y counts columns by 256 and more
 
 struct SortPlan {
     int nb, ids;     // blocks, ids of a block
@@ -101,13 +101,16 @@ struct Work {
     int32_t* order;   // [n] position of the k-th token in sorted order
     int32_t* token;   // [n] its id
     int32_t* count;   // [1] tokens that take part
-    float* part;      // [shares][2][dim] sums that continue from the share before / into the next
+    float* part;      // [shares][2][part_ld(dim)] sums that continue from the share before / into the next
 };
+
+// Rows of whole 16-byte lines, also where the width is odd.
+__host__ RQ_DEV int64_t part_ld(int64_t dim) { return (dim + 3) & ~3ll; }
 
 size_t align16(size_t b) { return (b + 15) & ~(size_t)15; }
 
 size_t work_bytes(int64_t n, int64_t dim, const SortPlan& p) {
-    return 16 + 2 * align16((size_t)n * 4) + (size_t)p.shares * 2 * dim * 4;
+    return 16 + 2 * align16((size_t)n * 4) + (size_t)p.shares * 2 * part_ld(dim) * 4;
 }
 
 Work work_of(void* ws, int64_t n) {
@@ -130,30 +133,30 @@ __global__ __launch_bounds__(kSortBlock) void embed_sort_kernel(const void* __re
     __shared__ int32_t less[kSortWaves];          // tokens of lower blocks that the wave saw
     __shared__ int32_t wsum[kSortWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t me = blockIdx.x, mask = gridDim.x - 1;
+    const int32_t me = blockIdx.x, mask = gridDim.x - 1;
     for (int i = tid; i < kSortWaves * kMaxIds; i += kSortBlock) (&cnt[0][0])[i] = 0;
     __syncthreads();
 
     const int64_t part = ((n + kSortWaves - 1) / kSortWaves + 63) & ~63ll;
     const int64_t lo = wave * part, hi = lo + part < n ? lo + part : n;
     // the ids of kScan * 64 places from i on, -1 where nothing takes part
-    auto fetch = [&](int64_t i, int64_t* v) {
+    int32_t v[kScan];
+    auto fetch = [&](int64_t i) {
+        int64_t f[kScan];
 #pragma unroll
         for (int k = 0; k < kScan; ++k) {
             const int64_t at = i + k * 64 + lane;
-            v[k] = at < hi ? index_at(idx, wide, at) : -1;
+            f[k] = at < hi ? index_at(idx, wide, at) : -1;
         }
 #pragma unroll
-        for (int k = 0; k < kScan; ++k)
-            if (v[k] < 0 || v[k] >= vocab || v[k] == padding) v[k] = -1;
+        for (int k = 0; k < kScan; ++k) v[k] = f[k] < 0 || f[k] >= vocab || f[k] == padding ? -1 : (int32_t)f[k];
     };
     int32_t below = 0;
     for (int64_t i = lo; i < hi; i += kScan * 64) {
-        int64_t v[kScan];
-        fetch(i, v);
+        fetch(i);
 #pragma unroll
         for (int k = 0; k < kScan; ++k) {
-            const int64_t o = v[k] & mask;
+            const int32_t o = v[k] & mask;
             below += v[k] >= 0 && o < me;
             if (v[k] >= 0 && o == me) atomicAdd(&cnt[wave][v[k] >> nb_shift], 1);
         }
@@ -209,8 +212,7 @@ __global__ __launch_bounds__(kSortBlock) void embed_sort_kernel(const void* __re
     // the second scan: every wave places its own tokens in order
     volatile int32_t* next = cnt[wave];
     for (int64_t i = lo; i < hi; i += kScan * 64) {
-        int64_t v[kScan];
-        fetch(i, v);
+        if (part > kScan * 64) fetch(i);  // else they are still there
 #pragma unroll
         for (int k = 0; k < kScan; ++k) {
             const bool own = v[k] >= 0 && (v[k] & mask) == me;
@@ -224,7 +226,7 @@ __global__ __launch_bounds__(kSortBlock) void embed_sort_kernel(const void* __re
                 if (id == key) {
                     const int32_t place = base + __popcll(same & ((1ull << lane) - 1));
                     ws.order[place] = (int32_t)(i + k * 64 + lane);
-                    ws.token[place] = (int32_t)v[k];
+                    ws.token[place] = v[k];
                 }
                 __builtin_amdgcn_wave_barrier();
                 if (lane == lead) next[key] = base + __popcll(same);
@@ -235,24 +237,35 @@ __global__ __launch_bounds__(kSortBlock) void embed_sort_kernel(const void* __re
     }
 }
 
+template <int V>
+RQ_DEV void store_part(float* row, int64_t c, int64_t dim, const float* f) {
+#pragma unroll
+    for (int h = 0; h < V; h += 4)  // the row's padding takes what is past its end
+        if (c + h < dim) *(f32x4_t*)(row + c + h) = f32x4_t{f[h], f[h + 1], f[h + 2], f[h + 3]};
+}
+
 // A wave takes a share of the sorted tokens and 64 vectors of columns (blockIdx.y).
 template <int DT>
-__global__ __launch_bounds__(kBlock) void embed_sum_kernel(Work ws, int share, int64_t dim,
+__global__ __launch_bounds__(kBlock) void embed_sum_kernel(const int32_t* __restrict__ count,
+                                                           const int32_t* __restrict__ order,
+                                                           const int32_t* __restrict__ token,
+                                                           float* __restrict__ part, int share, int64_t dim,
                                                            const uint8_t* __restrict__ dout,
                                                            float scale, uint8_t* __restrict__ dtable) {
     constexpr int V = kVec<DT>;
-    const int64_t s = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
-    const int n = ws.count[0];
+    // the same for all lanes: tokens and rows are scalar loads, run ends scalar branches
+    const int64_t s = (int64_t)blockIdx.x * (kBlock / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = count[0];
     const int64_t b = s * share;
     if (b >= n) return;
     const int64_t e = b + share < n ? b + share : n;
     const int64_t c = ((int64_t)blockIdx.y * 64 + (threadIdx.x & 63)) * V;
     const bool in = c < dim;
-    bool open = b > 0 && ws.token[b - 1] == ws.token[b];  // the run began in an earlier share
+    bool open = b > 0 && token[b - 1] == token[b];  // the run began in an earlier share
     float acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.f;
-    int32_t id = ws.token[b];
+    int32_t id = token[b];
     for (int64_t i = b; i < e; i += 8) {
         float f[8][V];
         int32_t ids[8];
@@ -260,8 +273,8 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Work ws, int share, i
         for (int k = 0; k < 8; ++k) {
             ids[k] = -1;
             if (i + k < e) {
-                ids[k] = ws.token[i + k];
-                const uint8_t* row = dout + (int64_t)ws.order[i + k] * dim * kSize<DT>;
+                ids[k] = token[i + k];
+                const uint8_t* row = dout + (int64_t)order[i + k] * dim * kSize<DT>;
                 if (in) load_cols<DT>(row, c, dim, f[k]);
             }
         }
@@ -271,9 +284,7 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Work ws, int share, i
             if (ids[k] != id) {  // the run of `id` ends inside the share
                 if (in) {
                     if (open) {
-                        float* p = ws.part + (s * 2) * dim;
-                        for (int j = 0; j < V; ++j)
-                            if (c + j < dim) p[c + j] = acc[j];
+                        store_part<V>(part + (s * 2) * part_ld(dim), c, dim, acc);
                     } else {
 #pragma unroll
                         for (int j = 0; j < V; ++j) acc[j] *= scale;
@@ -290,11 +301,9 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(Work ws, int share, i
         }
     }
     if (!in) return;
-    const bool goes_on = e < n && ws.token[e] == id;
+    const bool goes_on = e < n && token[e] == id;
     if (open || goes_on) {
-        float* p = ws.part + (s * 2 + (open ? 0 : 1)) * dim;
-        for (int j = 0; j < V; ++j)
-            if (c + j < dim) p[c + j] = acc[j];
+        store_part<V>(part + (s * 2 + (open ? 0 : 1)) * part_ld(dim), c, dim, acc);
     } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] *= scale;
@@ -308,9 +317,9 @@ template <int DT>
 __global__ __launch_bounds__(kBlock) void embed_join_kernel(Work ws, int share, int64_t dim, float scale,
                                                             uint8_t* __restrict__ dtable) {
     constexpr int W = kBlock / 64;
-    __shared__ float red[W][64];
+    __shared__ f32x4_t red[W][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t s = blockIdx.x;
+    const int64_t s = blockIdx.x, ld = part_ld(dim);
     const int n = ws.count[0];
     const int64_t b = s * share, e = b + share;
     if (e >= n) return;
@@ -331,15 +340,16 @@ __global__ __launch_bounds__(kBlock) void embed_join_kernel(Work ws, int share, 
     const int64_t rows = last - s + 1;  // partial rows: this share's second, the others' first
     const int64_t q = (rows + W - 1) / W;
     const int64_t r0 = wave * q, r1 = r0 + q < rows ? r0 + q : rows;
-    const int64_t c = (int64_t)blockIdx.y * 64 + lane;
-    float acc = 0.f;
+    const int64_t c = ((int64_t)blockIdx.y * 64 + lane) * 4;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
     if (c < dim) {
         for (int64_t r = r0; r < r1; r += 8) {
-            float f[8];
+            f32x4_t f[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const int64_t x = r + k;
-                f[k] = x < r1 ? ws.part[((s + x) * 2 + (x == 0 ? 1 : 0)) * dim + c] : 0.f;
+                f[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                if (x < r1) f[k] = *(const f32x4_t*)(ws.part + ((s + x) * 2 + (x == 0 ? 1 : 0)) * ld + c);
             }
 #pragma unroll
             for (int k = 0; k < 8; ++k) acc += f[k];
@@ -347,11 +357,13 @@ __global__ __launch_bounds__(kBlock) void embed_join_kernel(Work ws, int share, 
     }
     red[wave][lane] = acc;
     __syncthreads();
-    if (wave == 0 && c < dim) {
-        float v = red[0][lane];
+    if (wave == 0) {
+        f32x4_t v = red[0][lane];
 #pragma unroll
         for (int w = 1; w < W; ++w) v += red[w][lane];
-        store_dt(dtable + (int64_t)id * dim * kSize<DT>, DT, c, v * scale);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < dim) store_dt(dtable + (int64_t)id * dim * kSize<DT>, DT, c + e, v[e] * scale);
     }
 }
 
@@ -422,14 +434,14 @@ int rq_embed_grad(const void* idx, int idx_bytes, int64_t n, const void* dout, r
     const bool wide = idx_bytes == 8;
     hipStream_t s = (hipStream_t)stream;
     const int per = 64 * (dt == RQ_F32 ? 4 : 8);
-    const int tiles = (int)((dim + per - 1) / per), jtiles = (int)((dim + 63) / 64);
+    const int tiles = (int)((dim + per - 1) / per), jtiles = (int)((dim + 255) / 256);
     const unsigned sums = (p.shares + kBlock / 64 - 1) / (kBlock / 64);
     RQ_DISPATCH_DT(dt, DT, {
         embed_sort_kernel<DT><<<p.nb, kSortBlock, 0, s>>>(idx, wide, n, vocab, dim, padding_idx,
                                                           __builtin_ctz(p.nb), p.ids, ws, (uint8_t*)dtable);
         if (n > 0)
-            embed_sum_kernel<DT><<<dim3(sums, tiles), kBlock, 0, s>>>(ws, p.share, dim, (const uint8_t*)dout,
-                                                                      scale, (uint8_t*)dtable);
+            embed_sum_kernel<DT><<<dim3(sums, tiles), kBlock, 0, s>>>(
+                ws.count, ws.order, ws.token, ws.part, p.share, dim, (const uint8_t*)dout, scale, (uint8_t*)dtable);
         if (p.shares > 1)
             embed_join_kernel<DT><<<dim3(p.shares - 1, jtiles), kBlock, 0, s>>>(ws, p.share, dim, scale,
                                                                                 (uint8_t*)dtable);

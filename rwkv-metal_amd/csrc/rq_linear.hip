@@ -23,6 +23,9 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4_p;
 
+// Row stride of the partial sums of a split contraction.
+__host__ RQ_DEV int64_t part_ld(int64_t n) { return (n + 3) & ~3ll; }
+
 template <int N_>
 struct Count {
     static constexpr int N = N_;
@@ -30,24 +33,40 @@ struct Count {
 
 // ------------------------------------------------------------ output stage
 
+// Four or eight neighbouring elements at any element-aligned address: rows of odd
+// width take the same wide accesses (global memory allows them unaligned).
+struct __attribute__((packed, aligned(2))) Bytes8 {
+    uint32_t w[2];
+};
+
 RQ_DEV f32x4_t load4(const void* p, int dt, int64_t at) {
-    if (dt == RQ_F32) return *(const f32x4_t*)((const float*)p + at);
-    const u32x2_t v = *(const u32x2_t*)((const uint16_t*)p + at);
+    if (dt == RQ_F32) {
+        float f[4];
+        load_vec<RQ_F32>((const uint8_t*)p + at * 4, f);
+        return f32x4_t{f[0], f[1], f[2], f[3]};
+    }
+    const Bytes8 v = *(const Bytes8*)((const uint16_t*)p + at);
     if (dt == RQ_BF16)
-        return f32x4_t{__uint_as_float(v[0] << 16), __uint_as_float(v[0] & 0xffff0000u),
-                       __uint_as_float(v[1] << 16), __uint_as_float(v[1] & 0xffff0000u)};
-    return f32x4_t{f16_bits_to_f32(v[0] & 0xffffu), f16_bits_to_f32(v[0] >> 16),
-                   f16_bits_to_f32(v[1] & 0xffffu), f16_bits_to_f32(v[1] >> 16)};
+        return f32x4_t{__uint_as_float(v.w[0] << 16), __uint_as_float(v.w[0] & 0xffff0000u),
+                       __uint_as_float(v.w[1] << 16), __uint_as_float(v.w[1] & 0xffff0000u)};
+    return f32x4_t{f16_bits_to_f32(v.w[0] & 0xffffu), f16_bits_to_f32(v.w[0] >> 16),
+                   f16_bits_to_f32(v.w[1] & 0xffffu), f16_bits_to_f32(v.w[1] >> 16)};
 }
 
 RQ_DEV void store4(void* p, int dt, int64_t at, const f32x4_t& v) {
     if (dt == RQ_F32) {
-        *(f32x4_t*)((float*)p + at) = v;
+        const float f[4] = {v[0], v[1], v[2], v[3]};
+        store_vec<RQ_F32>((uint8_t*)p + at * 4, f);
     } else {
-        *(u32x2_t*)((uint16_t*)p + at) =
-            dt == RQ_BF16 ? u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}
-                          : u32x2_t{f32_to_f16_bits(v[0]) | (f32_to_f16_bits(v[1]) << 16),
-                                    f32_to_f16_bits(v[2]) | (f32_to_f16_bits(v[3]) << 16)};
+        Bytes8 b;
+        if (dt == RQ_BF16) {
+            b.w[0] = pack_bf16x2(v[0], v[1]);
+            b.w[1] = pack_bf16x2(v[2], v[3]);
+        } else {
+            b.w[0] = f32_to_f16_bits(v[0]) | (f32_to_f16_bits(v[1]) << 16);
+            b.w[1] = f32_to_f16_bits(v[2]) | (f32_to_f16_bits(v[3]) << 16);
+        }
+        *(Bytes8*)((uint16_t*)p + at) = b;
     }
 }
 
@@ -55,8 +74,8 @@ RQ_DEV void store4(void* p, int dt, int64_t at, const f32x4_t& v) {
 RQ_DEV void store_out(const rq::DenseArgs& g, int64_t i, int64_t j, f32x4_t v) {
     const int64_t at = i * g.n + j;
     const int sdt = g.slope_kind == RQ_SLOPE_F16 ? RQ_F16 : RQ_F32;
-    const bool whole = (g.n & 3) == 0;  // four outputs are inside or outside together, and aligned
     if (j >= g.n) return;
+    const bool whole = j + 4 <= g.n;
     if (g.bias) {
         if (whole) {
             v += load4(g.bias, g.dt, j);
@@ -68,7 +87,11 @@ RQ_DEV void store_out(const rq::DenseArgs& g, int64_t i, int64_t j, f32x4_t v) {
     }
     if (g.slope) {
         const f32x4_t s = act_slope4(g.act, v);
-        if (whole) {
+        if (g.slope_kind == RQ_SLOPE_WIDE16) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e < g.n) ((uint16_t*)g.slope)[at + e] = (uint16_t)wide16_bits(s[e]);
+        } else if (whole) {
             store4(g.slope, sdt, at, s);
         } else {
 #pragma unroll
@@ -149,14 +172,16 @@ struct Side {
     uint32_t off[LD];   // of this thread's chunks, rows clamped to the last one inside
     int rows;           // outputs of the tile inside the matrix
     int64_t ld;
-    bool split;         // a transposed tile whose last chunk is cut: elements are checked
+    bool cut;           // a transposed tile whose last chunk is cut: every stage is checked
+    bool wide;          // rows hold 16 bytes at least
 
     RQ_DEV void init(const void* base, int64_t ld_, int64_t r0, int64_t all, int64_t k0) {
         ld = ld_;
         rows = (int)(all - r0 < R ? all - r0 : R);
         p = (const uint8_t*)base + (T ? k0 * ld + r0 : r0 * ld + k0) * ES;
         step = (T ? BK * ld : (int64_t)BK) * ES;
-        split = T && rows < R && rows % E != 0;
+        cut = T && rows < R && rows % E != 0;
+        wide = (T ? all : ld) >= E;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             int r, c;
@@ -178,7 +203,7 @@ struct Side {
     }
     // the chunks of the next stage, of which `left` contraction elements are inside
     RQ_DEV void load(u32x4_t* v, int64_t left) {
-        if (left >= BK && !split) {
+        if (left >= BK && !cut) {
 #pragma unroll
             for (int i = 0; i < LD; ++i) {
                 const Bytes16 b = *(const Bytes16*)(p + off[i]);
@@ -189,16 +214,19 @@ struct Side {
         }
         p += step;
     }
+    // A chunk cut by the end of its row: the row's last 16 bytes, shifted down.
     RQ_DEV void checked(u32x4_t* v, int64_t left) {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             int r, c;
             place(i, r, c);
             v[i] = u32x4_t{0u, 0u, 0u, 0u};
-            const int64_t in = T ? (c < left ? rows - r : 0) : (r < rows ? left - c : 0);
-            if (in >= E) {
-                const Bytes16 b = *(const Bytes16*)(p + off[i]);
-                v[i] = u32x4_t{b.w[0], b.w[1], b.w[2], b.w[3]};
+            const int64_t in64 = T ? (c < left ? rows - r : 0) : (r < rows ? left - c : 0);
+            const int in = in64 < E ? (int)in64 : E;
+            if (in <= 0) continue;
+            if (wide) {
+                const Bytes16 b = *(const Bytes16*)(p + off[i] - (E - in) * ES);
+                v[i] = down(u32x4_t{b.w[0], b.w[1], b.w[2], b.w[3]}, E - in);
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
@@ -208,6 +236,18 @@ struct Side {
                 }
             }
         }
+    }
+    // 128 bits shifted down by n < E elements, zeros from above
+    static RQ_DEV u32x4_t down(u32x4_t v, int n) {
+        if constexpr (ES == 2) {
+            if (n & 1)
+                v = u32x4_t{__builtin_amdgcn_alignbit(v[1], v[0], 16), __builtin_amdgcn_alignbit(v[2], v[1], 16),
+                            __builtin_amdgcn_alignbit(v[3], v[2], 16), v[3] >> 16};
+            n >>= 1;
+        }
+        if (n & 1) v = u32x4_t{v[1], v[2], v[3], 0u};
+        if (n & 2) v = u32x4_t{v[2], v[3], 0u, 0u};
+        return v;
     }
     static RQ_DEV void put(uint8_t* lds, const u32x4_t* v) {
 #pragma unroll
@@ -248,45 +288,36 @@ struct Side {
 template <int WM, int WN>
 constexpr int kOutRows = WM * WN > 4096 ? 8192 / WN : WM;
 
-// Eight neighbouring elements of type `dt` (DT or fp32), 16-byte aligned.
+// Eight neighbouring elements of type DT, or fp32.
 template <int DT>
 RQ_DEV void load8(const void* p, bool f32, int64_t at, f32x4_t& lo, f32x4_t& hi) {
+    float f[8];
     if (DT == RQ_F32 || f32) {
-        lo = ((const f32x4_t*)((const float*)p + at))[0];
-        hi = ((const f32x4_t*)((const float*)p + at))[1];
+        load_vec<RQ_F32>((const uint8_t*)p + at * 4, f);
+        load_vec<RQ_F32>((const uint8_t*)p + at * 4 + 16, f + 4);
     } else {
-        float f[8];
         load_vec<DT>((const uint8_t*)p + at * 2, f);
-        lo = f32x4_t{f[0], f[1], f[2], f[3]};
-        hi = f32x4_t{f[4], f[5], f[6], f[7]};
     }
+    lo = f32x4_t{f[0], f[1], f[2], f[3]};
+    hi = f32x4_t{f[4], f[5], f[6], f[7]};
 }
 
 template <int DT>
 RQ_DEV void store8(void* p, bool f32, int64_t at, const f32x4_t& lo, const f32x4_t& hi) {
+    const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     if (DT == RQ_F32 || f32) {
-        ((f32x4_t*)((float*)p + at))[0] = lo;
-        ((f32x4_t*)((float*)p + at))[1] = hi;
+        store_vec<RQ_F32>((uint8_t*)p + at * 4, f);
+        store_vec<RQ_F32>((uint8_t*)p + at * 4 + 16, f + 4);
     } else {
-        u32x4_t v;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            v[e] = DT == RQ_BF16 ? pack_bf16x2(lo[2 * e], lo[2 * e + 1])
-                                 : (f32_to_f16_bits(lo[2 * e]) | (f32_to_f16_bits(lo[2 * e + 1]) << 16));
-            v[e + 2] = DT == RQ_BF16 ? pack_bf16x2(hi[2 * e], hi[2 * e + 1])
-                                     : (f32_to_f16_bits(hi[2 * e]) | (f32_to_f16_bits(hi[2 * e + 1]) << 16));
-        }
-        *(u32x4_t*)((uint16_t*)p + at) = v;
+        store_vec<DT>((uint8_t*)p + at * 2, f);
     }
 }
 
 // `rows` rows of a wave's tile from LDS (row r at own + r * P) to row i0 + r, columns
-// j .. j + 7 of this lane (n % 8 == 0); every 64 / LPR-th row from r0 on is this lane's.
-// kBatch rows at a time, their loads together: one wave to a SIMD runs this in
+// j .. j + 7 of this lane (all inside); every 64 / LPR-th row from r0 on is this lane's.
+// BATCH rows at a time, their loads together: one wave to a SIMD runs this in
 // the large tiles, and every wait is felt.
-constexpr int kBatch = 4;
-
-template <int DT, int ACT, int ROWS, int P, int LPR>
+template <int DT, int ACT, int P, int LPR, int BATCH>
 RQ_DEV void out_rows(const rq::DenseArgs& g, const float* own, int64_t i0, int64_t j, int rows) {
     constexpr int STEP = 64 / LPR;
     const int r0 = (threadIdx.x & 63) / LPR;
@@ -296,17 +327,17 @@ RQ_DEV void out_rows(const rq::DenseArgs& g, const float* own, int64_t i0, int64
     const float* src = own + r0 * P + ((threadIdx.x & 63) % LPR) * 8;
     int64_t at = (i0 + r0) * g.n + j;
     const int64_t step = STEP * g.n;
-    for (int r = r0; r < rows; r += kBatch * STEP) {
-        f32x4_t lo[kBatch], hi[kBatch], rl[kBatch], rh[kBatch];
+    for (int r = r0; r < rows; r += BATCH * STEP) {
+        f32x4_t lo[BATCH], hi[BATCH], rl[BATCH], rh[BATCH];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
+        for (int u = 0; u < BATCH; ++u) {
             // rows of LDS are there for the whole tile, rows of memory are not
             lo[u] = ((const f32x4_t*)(src + u * STEP * P))[0];
             hi[u] = ((const f32x4_t*)(src + u * STEP * P))[1];
             if (res && r + u * STEP < rows) load8<DT>(g.residual, y32, at + u * step, rl[u], rh[u]);
         }
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
+        for (int u = 0; u < BATCH; ++u) {
             if (r + u * STEP >= rows) break;
             lo[u] += blo;
             hi[u] += bhi;
@@ -317,7 +348,17 @@ RQ_DEV void out_rows(const rq::DenseArgs& g, const float* own, int64_t i0, int64
                     sl[e] = act_slope(ACT, lo[u][e]);
                     sh[e] = act_slope(ACT, hi[u][e]);
                 }
-                store8<RQ_F16>(g.slope, g.slope_kind != RQ_SLOPE_F16, at + u * step, sl, sh);
+                if (ACT == RQ_ACT_RELU2 && g.slope_kind == RQ_SLOPE_WIDE16) {
+                    u32x4_t w;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        w[e] = wide16_bits(sl[2 * e]) | (wide16_bits(sl[2 * e + 1]) << 16);
+                        w[e + 2] = wide16_bits(sh[2 * e]) | (wide16_bits(sh[2 * e + 1]) << 16);
+                    }
+                    *(Bytes16*)((uint16_t*)g.slope + at + u * step) = Bytes16{{w[0], w[1], w[2], w[3]}};
+                } else {
+                    store8<RQ_F16>(g.slope, g.slope_kind == RQ_SLOPE_F32, at + u * step, sl, sh);
+                }
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -330,8 +371,8 @@ RQ_DEV void out_rows(const rq::DenseArgs& g, const float* own, int64_t i0, int64
             }
             store8<DT>(g.y, y32, at + u * step, lo[u], hi[u]);
         }
-        src += kBatch * STEP * P;
-        at += kBatch * step;
+        src += BATCH * STEP * P;
+        at += BATCH * step;
     }
 }
 
@@ -342,7 +383,9 @@ RQ_DEV void tile_out(const rq::DenseArgs& g, const f32x4_t (&acc)[MT][NT], float
                      float* part) {
     constexpr int WM = MT * 16, WN = NT * 16;
     constexpr int ROWS = kOutRows<WM, WN>, P = WN + 4, LPR = WN / 8;
-    static_assert(ROWS % (kBatch * 64 / LPR) == 0 || ROWS < kBatch * 64 / LPR, "");
+    // small tiles leave the registers to more blocks
+    constexpr int BATCH = MT * NT >= 16 ? 4 : 2;
+    static_assert(ROWS % (BATCH * (64 / LPR)) == 0, "rows of LDS are read in whole batches");
     static_assert(WM / ROWS <= 2, "");
     const int lane = threadIdx.x & 63;
     auto put = [&](auto half) {
@@ -360,25 +403,28 @@ RQ_DEV void tile_out(const rq::DenseArgs& g, const f32x4_t (&acc)[MT][NT], float
         __builtin_amdgcn_wave_barrier();
         const int64_t ib = i0 + h * ROWS;
         const int rows = (int)(g.m - ib < ROWS ? g.m - ib : ROWS);
-        if (part || (g.n & 7) != 0) {
-            float* o = part ? part + (int64_t)blockIdx.y * g.m * g.n : nullptr;
-            for (int r = lane / (WN / 4); r < rows; r += 256 / WN) {
-                const int64_t j = j0 + lane % (WN / 4) * 4, at = (ib + r) * g.n + j;
-                const f32x4_t v = *(const f32x4_t*)(own + r * P + lane % (WN / 4) * 4);
-                if (!part) {
-                    store_out(g, ib + r, j, v);
-                } else if ((g.n & 3) == 0) {
-                    if (j < g.n) *(f32x4_t*)(o + at) = v;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (j + e < g.n) o[at + e] = v[e];
+        const int64_t j = j0 + lane % LPR * 8;
+        if (part) {  // rows of whole 16-byte lines
+            const int64_t ld = part_ld(g.n);
+            float* o = part + ((int64_t)blockIdx.y * g.m + ib) * ld + j;
+            if (j < ld) {
+#pragma unroll 4
+                for (int r = lane / LPR; r < rows; r += 64 / LPR) {
+                    const float* v = own + r * P + lane % LPR * 8;
+                    *(f32x4_t*)(o + r * ld) = *(const f32x4_t*)v;
+                    if (j + 4 < ld) *(f32x4_t*)(o + r * ld + 4) = *(const f32x4_t*)(v + 4);
                 }
             }
-        } else if (const int64_t j = j0 + lane % LPR * 8; j < g.n) {
+        } else if (j + 8 > g.n) {  // the lane at the end of rows that are not whole eights
+            for (int r = lane / LPR; r < rows && j < g.n; r += 64 / LPR) {
+                const float* v = own + r * P + lane % LPR * 8;
+                store_out(g, ib + r, j, *(const f32x4_t*)v);
+                store_out(g, ib + r, j + 4, *(const f32x4_t*)(v + 4));
+            }
+        } else {
             switch (g.act) {
 #define RQ_OUT(A) \
-    case A: out_rows<DT, A, ROWS, P, LPR>(g, own, ib, j, rows); break;
+    case A: out_rows<DT, A, P, LPR, BATCH>(g, own, ib, j, rows); break;
                 RQ_OUT(RQ_ACT_NONE)
                 RQ_OUT(RQ_ACT_RELU)
                 RQ_OUT(RQ_ACT_RELU2)
@@ -406,8 +452,8 @@ RQ_DEV void tile_of(int64_t b, int64_t tiles, int64_t ti, int64_t tj, int64_t& i
     j = r / high;
 }
 
-template <int DT, bool AT, bool BT, int BM, int BN, int WM, int WN>
-constexpr int kTileLds = std::max(2 * (Side<DT, AT, BM>::BYTES + Side<DT, BT, BN>::BYTES),
+template <int DT, bool AT, bool BT, int BM, int BN, int WM, int WN, int NB = 2>
+constexpr int kTileLds = std::max(NB * (Side<DT, AT, BM>::BYTES + Side<DT, BT, BN>::BYTES),
                                   kBlock / 64 * kOutRows<WM, WN> * (WN + 4) * 4);
 
 template <int DT, bool AT, bool BT, int BM, int BN, int WM, int WN, int OCC>
@@ -533,7 +579,8 @@ RQ_DEV void mma_acc(const u32x4_t& a, const u32x4_t& b, f32x4_t& c) {
     else asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
-template <int DT, bool AT, bool BT, int BM, int BN, int WM, int WN, int OCC>
+// NB stages fit LDS: a stage is fetched NB - 1 stages ahead of its products.
+template <int DT, bool AT, bool BT, int BM, int BN, int WM, int WN, int OCC, int NB>
 __global__ __launch_bounds__(kBlock, OCC) void dense_direct(const rq::DenseArgs g, int64_t kper, float* part) {
     typedef Direct<DT, AT, BM> SA;
     typedef Direct<DT, BT, BN> SB;
@@ -603,13 +650,23 @@ __global__ __launch_bounds__(kBlock, OCC) void dense_direct(const rq::DenseArgs 
         }
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto sync = [&] {  // own loads have landed, own reads are done; then everybody's
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // own loads but the last STAGES' have landed, own reads are done; then everybody's
+    auto sync = [&](auto stages_left) {
+        constexpr int V = decltype(stages_left)::N * LD;
+        static_assert(V < 64, "vmcnt");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(V) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
 
     if (stages > 0) {
+        // Past the last stage the loads below and in the loop repeat it and the
+        // reads take what is there: nothing uses either, and every pass is the
+        // same code with the same counts.
+        int ahead = 0;  // stages fetched
+        auto move = [&] {
+            if (++ahead < stages) next();
+        };
         if (rest) {
             const uint8_t *pa = a.p, *pb = b.p;
             a.p += whole * a.step;
@@ -620,27 +677,31 @@ __global__ __launch_bounds__(kBlock, OCC) void dense_direct(const rq::DenseArgs 
             for (int i = 0; i < SB::LD; ++i) b.fetch_part(base + SA::BYTES + i * (kBlock * 16), i, rest);
             a.p = pa;
             b.p = pb;
+            ++ahead;
         } else {
 #pragma unroll
             for (int i = 0; i < LD; ++i) fetch(0, i);
-            if (stages > 1) next();
+            move();
         }
-        sync();
-        // Past the last stage the loop loads the last one again and reads what
-        // is there: nothing uses either, and every pass is the same code.
 #pragma unroll
-        for (int i = 0; i < LD; ++i) fetch(1, i);
-        if (stages > 2) next();
+        for (int v = 1; v < NB; ++v) {
+#pragma unroll
+            for (int i = 0; i < LD; ++i) fetch(v, i);
+            move();
+        }
+        sync(Count<NB - 1>{});
 #pragma unroll
         for (int i = 0; i < FR; ++i) read(0, 0, i);
+        int u = 0;
         for (int s = 0; s < stages; ++s) {
-            const int u = s & 1;
             products(Step<0, false>{}, u, 0);
-            sync();
-            products(Step<1, true>{}, u ^ 1, u);
-            if (s + 3 < stages) next();
+            sync(Count<NB - 2>{});
+            const int v = u;
+            u = u + 1 < NB ? u + 1 : 0;
+            products(Step<1, true>{}, u, v);
+            move();
         }
-        sync();
+        sync(Count<0>{});
         // the last products' results, of which the compiler knows no latency
         if constexpr (MT * NT == 64) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
     }
@@ -732,20 +793,13 @@ __global__ __launch_bounds__(kBlock) void dense_join(const rq::DenseArgs g, cons
     const int64_t i = blockIdx.y;
     if (j >= g.n) return;
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s) {
-        const float* p = part + ((int64_t)s * g.m + i) * g.n + j;
-        if ((g.n & 3) == 0) {
-            v += *(const f32x4_t*)p;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (j + e < g.n) v[e] += p[e];
-        }
-    }
+    const int64_t ld = part_ld(g.n);
+    const float* p = part + i * ld + j;
+    for (int s = 0; s < splits; ++s) v += *(const f32x4_t*)(p + s * g.m * ld);
     store_out(g, i, j, v);
 }
 
-enum Form { kDirect256, kDirect128, kTile128, kTile64, kFew };
+enum Form { kDirect256, kDirect128, kDeep128, kDirect128x64, kDirect64, kDeep64, kTile128, kTile64, kFew };
 
 struct Plan {
     Form form;
@@ -753,22 +807,79 @@ struct Plan {
     int64_t kper;  // contraction elements of a share
 };
 
+// What a product costs in each form, in us: a start, and for every tile on the
+// fullest of 256 CUs an amount of its own and an amount a stage, which is less where
+// several tiles of a CU run together, and more (`turned`) with two transposed
+// operands, half of that with one; a split adds its partial sums' traffic and a
+// launch.  The numbers are least squares over 90 sizes of m 1 - 4096, k and n 64 -
+// 8192 in all three orders and up to 16 shares on an MI355X (operands beyond the L2
+// caches): the fit is within 12 % (16-bit) and 7 % (fp32) of the times, and what it
+// chooses 2 % behind the best choice of each size.
+struct Cost {
+    int bm, bn, together;
+    float tile, turned, stage[4];  // stage: of 1 .. `together` tiles running together, all of them
+};
+constexpr float kStart = 3.f, kJoin = 2.9f, kJoinBytes = 6e6f;  // us, us, bytes a us
+constexpr Cost kCost[kFew] = {
+    {256, 256, 1, 7.2f, 1.21f, {1.02f}},
+    {128, 128, 2, 1.9f, 1.13f, {0.47f, 0.68f}},
+    {128, 128, 1, 2.6f, 1.33f, {0.36f}},
+    {128, 64, 2, 1.5f, 1.29f, {0.23f, 0.40f}},
+    {64, 64, 4, 0.7f, 1.06f, {0.34f, 0.41f, 0.46f, 0.48f}},
+    {64, 64, 2, 1.2f, 1.36f, {0.17f, 0.25f}},
+    {128, 128, 2, 2.1f, 2.44f, {0.79f, 0.83f}},  // the staged tiles on rows of odd width
+    {64, 64, 2, 0.34f, 1.87f, {0.45f, 0.46f}},
+};
+// fp32, 32 elements a stage: bound by the fp32 matrix instruction
+constexpr Cost kCost32[2] = {
+    {128, 128, 2, 2.6f, 1.11f, {2.1f, 3.9f}},
+    {64, 64, 2, 0.9f, 1.21f, {0.65f, 1.0f}},
+};
+
+float cost_of(const Cost& c, const rq::DenseArgs& a, int bk, int splits) {
+    const int64_t tiles = ((a.m + c.bm - 1) / c.bm) * ((a.n + c.bn - 1) / c.bn) * splits;
+    const float stages = (float)((a.k / splits + bk - 1) / bk);
+    const int64_t most = (tiles + 255) / 256;  // on one CU
+    const int rest = (int)(most % c.together);
+    const float all = (float)(most / c.together) * c.stage[c.together - 1] + (rest ? c.stage[rest - 1] : 0.f);
+    float t = kStart + most * c.tile + stages * all * (1.f + (c.turned - 1.f) * (a.a_t + a.b_t) / 2);
+    // two tensors written from the output stage: the large tile runs it one wave to a SIMD
+    if (a.slope && c.bm == 256) t += most * 12.f;
+    if (splits > 1) t += kJoin + (float)a.m * a.n * splits * 8.f / kJoinBytes;
+    return t;
+}
+
+// kFew: 1024 weights of 256 blocks' rows
+float cost_few(const rq::DenseArgs& a) {
+    const int mt = a.m <= 16 ? 1 : a.m <= 32 ? 2 : 4;
+    const float blocks = (float)((a.n + 15) / 16), k = (float)a.k * (a.dt == RQ_F32 ? 4 : 2) / 2048.f;
+    const float per = a.dt == RQ_F32 ? 1.34f * mt : a.k % 8 ? 2.25f + 0.53f * mt : 0.33f + 0.61f * mt;
+    return 3.9f + per * std::max(1.f, blocks / 256.f) * k;
+}
+
 Plan plan_of(const rq::DenseArgs& a) {
-    Plan p{kTile128, 1, a.k};
-    const char* e = getenv("RQ_TILE");
-    if (e) p.form = (Form)atoi(e);
-    const char* q = getenv("RQ_SPLIT");
-    const bool direct = a.dt != RQ_F32 && (a.lda | a.ldb) % 8 == 0 && a.k >= 64;
-    if (p.form <= kDirect128 && !direct) p.form = kTile128;
-    if (p.form == kFew && (a.a_t || a.b_t || a.m > 64)) p.form = kTile128;
-    if (q && p.form != kFew) {
-        const int bk = a.dt == RQ_F32 ? 32 : 64;
-        int s = atoi(q);
-        p.kper = ((a.k + s - 1) / s + bk - 1) / bk * bk;
-        if (p.kper < bk) p.kper = bk;
-        p.splits = (int)((a.k + p.kper - 1) / p.kper);
-        if (p.splits < 1) p.splits = 1;
-        if (p.splits > 1 && a.k - (p.splits - 1) * p.kper < bk) { p.splits = 1; p.kper = a.k; }
+    const bool f32 = a.dt == RQ_F32;
+    const int bk = f32 ? 32 : 64;
+    // rows of whole 16-byte lines, and a whole stage in the contraction
+    const bool direct = !f32 && (a.lda | a.ldb) % 8 == 0 && a.k >= 64;
+    Plan p{kTile64, 1, a.k};
+    float best = 1e30f;
+    if (!a.a_t && !a.b_t && a.m <= 64) {
+        p.form = kFew;
+        best = cost_few(a);
+    }
+    for (int f = direct ? kDirect256 : kTile128; f <= (direct ? kDeep64 : kTile64); ++f) {
+        const Cost& c = f32 ? kCost32[f - kTile128] : kCost[f];
+        for (int splits = 1; splits <= 32; splits *= 2) {
+            const int64_t per = ((a.k + splits - 1) / splits + bk - 1) / bk * bk;
+            // shares of two stages at least, and a whole one in the last
+            if (splits > 1 && (per < 2 * bk || a.k - (splits - 1) * per < bk)) break;
+            const float t = cost_of(c, a, bk, splits);
+            if (t < best) {
+                best = t;
+                p = {(Form)f, splits, splits > 1 ? per : a.k};
+            }
+        }
     }
     return p;
 }
@@ -788,11 +899,11 @@ hipError_t allow_lds(K* kernel, int lds) {
                             : hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
 }
 
-template <int DT, bool AT, bool BT, int BM, int BN, int WM, int WN, int OCC, bool DIRECT>
+template <int DT, bool AT, bool BT, int BM, int BN, int WM, int WN, int OCC, int NB>
 hipError_t launch_tile(const rq::DenseArgs& a, const Plan& p, float* part, hipStream_t s) {
-    constexpr int lds = kTileLds<DT, AT, BT, BM, BN, WM, WN>;
-    if constexpr (DIRECT) {
-        auto* kernel = dense_direct<DT, AT, BT, BM, BN, WM, WN, OCC>;
+    constexpr int lds = kTileLds<DT, AT, BT, BM, BN, WM, WN, NB ? NB : 2>;
+    if constexpr (NB > 0) {
+        auto* kernel = dense_direct<DT, AT, BT, BM, BN, WM, WN, OCC, NB>;
         if (hipError_t e = allow_lds(kernel, lds); e != hipSuccess) return e;
         return launch_lds(kernel, a, p, BM, BN, lds, part, s);
     } else {
@@ -814,14 +925,18 @@ hipError_t launch_few(const rq::DenseArgs& a, hipStream_t s) {
 template <int DT, bool AT, bool BT>
 hipError_t launch_as(const rq::DenseArgs& a, const Plan& p, float* part, hipStream_t s) {
     if constexpr (DT != RQ_F32) {
-        if (p.form == kDirect256) return launch_tile<DT, AT, BT, 256, 256, 128, 128, 1, true>(a, p, part, s);
-        if (p.form == kDirect128) return launch_tile<DT, AT, BT, 128, 128, 64, 64, 2, true>(a, p, part, s);
+        if (p.form == kDirect256) return launch_tile<DT, AT, BT, 256, 256, 128, 128, 1, 2>(a, p, part, s);
+        if (p.form == kDirect128) return launch_tile<DT, AT, BT, 128, 128, 64, 64, 2, 2>(a, p, part, s);
+        if (p.form == kDeep128) return launch_tile<DT, AT, BT, 128, 128, 64, 64, 2, 4>(a, p, part, s);
+        if (p.form == kDirect128x64) return launch_tile<DT, AT, BT, 128, 64, 64, 32, 2, 3>(a, p, part, s);
+        if (p.form == kDeep64) return launch_tile<DT, AT, BT, 64, 64, 32, 32, 2, 4>(a, p, part, s);
+        if (p.form == kDirect64) return launch_tile<DT, AT, BT, 64, 64, 32, 32, 4, 2>(a, p, part, s);
     }
     if constexpr (!AT && !BT) {
         if (p.form == kFew) return launch_few<DT>(a, s);
     }
-    if (p.form == kTile64) return launch_tile<DT, AT, BT, 64, 64, 32, 32, 2, false>(a, p, part, s);
-    return launch_tile<DT, AT, BT, 128, 128, 64, 64, 2, false>(a, p, part, s);
+    if (p.form == kTile64) return launch_tile<DT, AT, BT, 64, 64, 32, 32, 2, 0>(a, p, part, s);
+    return launch_tile<DT, AT, BT, 128, 128, 64, 64, 2, 0>(a, p, part, s);
 }
 
 }  // namespace
@@ -829,8 +944,14 @@ hipError_t launch_as(const rq::DenseArgs& a, const Plan& p, float* part, hipStre
 namespace rq {
 
 int64_t dense_workspace_bytes(const DenseArgs& a) {
-    const Plan p = plan_of(a);
-    return p.splits > 1 ? p.splits * a.m * a.n * 4 : 0;
+    int64_t most = 0;
+    DenseArgs b = a;
+    for (void* slope : {(void*)nullptr, (void*)&b}) {  // with and without slopes
+        b.slope = slope;
+        const Plan p = plan_of(b);
+        if (p.splits > 1) most = std::max(most, p.splits * a.m * part_ld(a.n) * 4);
+    }
+    return most;
 }
 
 hipError_t launch_dense(const DenseArgs& a, void* workspace, hipStream_t stream) {

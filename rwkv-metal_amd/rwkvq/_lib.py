@@ -88,13 +88,13 @@ SIGNATURES = {
     "rq_grouped_plan_run": ([ctypes.POINTER(RqGroupedPlan), _vp], _i32),
     # include/rwkvq_train.h; a list of rq_grad is passed by its address
     "rq_linear_slope": ([_i32, _i32, _i32], _i32),
-    "rq_linear_workspace_bytes": ([_i32, _i64, _i64, _i64, _i32], _i64),
+    "rq_linear_workspace_bytes": ([_i64, _i64, _i64, _i32], _i64),
     "rq_linear": ([_vp, _vp, _vp, _i32, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _i64,
                    _vp], _i32),
-    "rq_linear_dpre": ([_vp, _i32, _vp, _i32, _i32, _i32, _i64, _i64, _vp, _vp, _vp, _i64, _vp],
-                       _i32),
-    "rq_linear_dx": ([_vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp], _i32),
-    "rq_linear_dw": ([_vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp], _i32),
+    "rq_linear_backward_workspace_bytes": ([_i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32],
+                                           _i64),
+    "rq_linear_backward": ([_vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp,
+                            _vp, _vp, _i64, _vp], _i32),
     "rq_embed": ([_vp, _i32, _i64, _vp, _i32, _i64, _i64, ctypes.c_float, _vp, _vp], _i32),
     "rq_embed_grad_workspace_bytes": ([_i64, _i64, _i64], _i64),
     "rq_embed_grad": ([_vp, _i32, _i64, _vp, _i32, _i64, _i64, ctypes.c_float, _i64, _vp, _vp,

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import array
 import collections
+import operator
 from typing import Iterable, List, Optional, Sequence, Tuple
 
 import torch
@@ -32,8 +33,9 @@ from .ops import _DeviceGuard, _eager, _float, _on_gpu, _ptr, _ready, _stream_on
 
 ACTIVATIONS = (None, "relu", "relu2", "silu", "gelu", "sigmoid", "tanh")
 _ACT_CODE = {a: i for i, a in enumerate(ACTIVATIONS)}
-_SLOPE_NONE, _SLOPE_Y, _SLOPE_F16, _SLOPE_F32 = range(4)
-_OP_FORWARD, _OP_DX, _OP_DW, _OP_DPRE = range(4)
+_SLOPE_NONE, _SLOPE_Y, _SLOPE_F16, _SLOPE_F32, _SLOPE_WIDE16 = range(5)
+# the dtype a tensor of slopes is allocated in
+_SLOPE_DTYPE = {_SLOPE_F16: torch.float16, _SLOPE_F32: torch.float32, _SLOPE_WIDE16: torch.int16}
 
 _workspaces: "collections.OrderedDict" = collections.OrderedDict()
 _WORKSPACES_MAX = 8
@@ -64,7 +66,7 @@ def _addr(t: Optional[Tensor]) -> int:
 # -------------------------------------------------------------- linear_act
 
 _slope_kinds: dict = {}   # (activation code, dtype code, residual?) -> rq_linear_slope
-_linear_bytes: dict = {}  # (op, m, n, k, dtype code) -> rq_linear_workspace_bytes
+_linear_bytes: dict = {}  # the arguments of a workspace query -> its bytes
 
 
 def _slope_kind(act: int, dt: int, residual: bool) -> int:
@@ -77,11 +79,11 @@ def _slope_kind(act: int, dt: int, residual: bool) -> int:
     return kind
 
 
-def _linear_workspace(op: int, m: int, n: int, k: int, dt: int, device, stream):
-    key = (op, m, n, k, dt)
+def _linear_workspace(name: str, key: tuple, device, stream) -> Tuple[int, int]:
+    """Address and size of the workspace that the query `name` asks for with `key`."""
     nbytes = _linear_bytes.get(key)
     if nbytes is None:
-        nbytes = lib().rq_linear_workspace_bytes(op, m, n, k, dt)
+        nbytes = getattr(lib(), name)(*key)
         check(min(nbytes, 0), "linear_act")
         if len(_linear_bytes) > 4096:
             _linear_bytes.clear()
@@ -108,12 +110,12 @@ def _linear_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Op
     kind = _slope_kind(act, dt, residual is not None) if want_slope else _SLOPE_NONE
     slope = None
     if kind >= _SLOPE_F16:
-        slope = torch.empty(*lead, n, device=x.device,
-                            dtype=torch.float16 if kind == _SLOPE_F16 else torch.float32)
+        slope = torch.empty(*lead, n, device=x.device, dtype=_SLOPE_DTYPE[kind])
     if m and n:
         with _DeviceGuard(x.device):
             stream = _stream_on(x.device)
-            ws, nbytes = _linear_workspace(_OP_FORWARD, m, n, k, dt, x.device, stream)
+            ws, nbytes = _linear_workspace("rq_linear_workspace_bytes", (m, n, k, dt), x.device,
+                                           stream)
             rc = lib().rq_linear(_ptr(x), _ptr(weight), _addr(bias), dt, _addr(residual),
                                  DTYPE_CODE[ydt], m, n, k, act, y.data_ptr(), _addr(slope), ws,
                                  nbytes, stream)
@@ -131,34 +133,23 @@ def _linear_backward_impl(dy: Tensor, x: Tensor, weight: Tensor, saved: Tensor, 
     k, n = x.shape[-1], weight.shape[0]
     dy, x, weight = _ready(dy), _ready(x), _ready(weight)
     m = dy.numel() // n if n else 0
-    dtype, device = x.dtype, x.device
-    dt = DTYPE_CODE[dtype]
+    device = x.device
     dx = torch.empty_like(x) if want_x else None
     dw = torch.empty_like(weight) if want_w else None
-    db = torch.empty(n, dtype=dtype, device=device) if want_b else None
+    db = torch.empty(n, dtype=x.dtype, device=device) if want_b else None
     if n == 0:
         return (dx.zero_() if want_x else None), dw, db
-    L = lib()
+    dt, ydt = DTYPE_CODE[x.dtype], DTYPE_CODE[dy.dtype]
     with _DeviceGuard(device):
         stream = _stream_on(device)
-        # where act'(v) is 1 and dy is in the operands' type, dy is g
-        is_g = kind == _SLOPE_NONE and dy.dtype == dtype
-        need_g = (want_x or want_w) and not is_g
-        g = torch.empty(dy.shape, dtype=dtype, device=device) if need_g else dy
-        if need_g or want_b:
-            ws, nbytes = _linear_workspace(_OP_DPRE, m, n, 0, dt, device, stream) if want_b else (0, 0)
-            rc = L.rq_linear_dpre(_ptr(dy), DTYPE_CODE[dy.dtype],
-                                  _ptr(saved) if kind != _SLOPE_NONE else 0, kind, act, dt, m, n,
-                                  _ptr(g) if need_g else 0, _addr(db), ws, nbytes, stream)
-            check(rc, "linear_act backward")
-        if want_x and dx.numel():
-            ws, nbytes = _linear_workspace(_OP_DX, m, n, k, dt, device, stream)
-            rc = L.rq_linear_dx(_ptr(g), _ptr(weight), dt, m, n, k, dx.data_ptr(), ws, nbytes, stream)
-            check(rc, "linear_act backward")
-        if want_w and dw.numel():
-            ws, nbytes = _linear_workspace(_OP_DW, m, n, k, dt, device, stream)
-            rc = L.rq_linear_dw(_ptr(g), _ptr(x), dt, m, n, k, dw.data_ptr(), ws, nbytes, stream)
-            check(rc, "linear_act backward")
+        ws, nbytes = _linear_workspace("rq_linear_backward_workspace_bytes",
+                                       (m, n, k, dt, ydt, kind, want_x, want_w, want_b), device,
+                                       stream)
+        rc = lib().rq_linear_backward(
+            _ptr(dy), ydt, _ptr(saved) if kind != _SLOPE_NONE else 0, kind, act, _ptr(x),
+            _ptr(weight), dt, m, n, k, _addr(dx), _addr(dw), _addr(db), ws, nbytes, stream)
+    if rc:
+        check(rc, "linear_act backward")
     return dx, dw, db
 
 
@@ -174,8 +165,7 @@ _linear_op = torch.library.custom_op("rwkvq::linear_act", _linear_op_impl, mutat
 def _(x, weight, bias, residual, act):
     shape = (*x.shape[:-1], weight.shape[0])
     kind = _slope_kind(act, DTYPE_CODE[x.dtype], residual is not None)
-    slope = (x.new_empty(0) if kind < _SLOPE_F16 else
-             x.new_empty(shape, dtype=torch.float16 if kind == _SLOPE_F16 else torch.float32))
+    slope = x.new_empty(0) if kind < _SLOPE_F16 else x.new_empty(shape, dtype=_SLOPE_DTYPE[kind])
     return x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype), slope
 
 
@@ -252,9 +242,9 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
     the residual's addition are in float32, rounded once.
 
     The backward pass keeps x, weight and the slope act'(v): read off y for relu
-    and relu2 without a residual, else a tensor of its own (float16 beside bf16
-    operands, float32 beside others and for relu2).  Its products take g = dy act'(v)
-    rounded to the operands' type."""
+    (and float32 relu2) without a residual, else a tensor of its own, 16 bits with
+    three more of them significant than bf16's beside bf16 operands and float32
+    beside others.  Its products take g = dy act'(v) rounded to the operands' type."""
     if activation not in _ACT_CODE:
         raise ValueError(f"activation must be one of {ACTIVATIONS} (got {activation!r})")
     _float(x, "x")
@@ -451,28 +441,43 @@ class ScaledEmbedding(nn.Embedding):
 
 # --------------------------------------------------- gradient norm and clip
 
-def _grad_list(grads: Sequence[Tensor], out: Optional[Sequence[Tensor]]) -> array.array:
+_dtype_of = operator.attrgetter("dtype")
+
+
+def _grad_list(grads: Sequence[Tensor], out: Optional[Sequence[Tensor]], sizes: List[int],
+               codes: List[int]) -> array.array:
     """The tensors as an array of rq_grad: (g, out, n, dtype code), 8 bytes each
-    (the dtype's upper four are rq_grad's padding)."""
-    n = len(grads)
-    a = array.array("q", bytes(32 * n))
+    (the dtype's upper four are rq_grad's padding).  Column by column: a model has
+    hundreds of gradients, and a loop over them would take longer than the launches."""
+    a = array.array("q", bytes(32 * len(grads)))
     a[0::4] = array.array("q", map(Tensor.data_ptr, grads))
     a[1::4] = a[0::4] if out is None else array.array("q", map(Tensor.data_ptr, out))
-    a[2::4] = array.array("q", map(Tensor.numel, grads))
-    a[3::4] = array.array("q", [DTYPE_CODE[t.dtype] for t in grads])
+    a[2::4] = array.array("q", sizes)
+    a[3::4] = array.array("q", codes)
     return a
 
 
-def _check_grads(grads: Sequence[Tensor]) -> torch.device:
+def _check_grads(grads: Sequence[Tensor]) -> Tuple[torch.device, List[int]]:
+    """The one GPU that holds them all, and their dtype codes, or an error."""
+    try:
+        devices = set(map(Tensor.get_device, grads))
+        if len(devices) == 1 and -1 not in devices:
+            return grads[0].device, list(map(DTYPE_CODE.__getitem__, map(_dtype_of, grads)))
+    except (TypeError, KeyError):
+        pass
     for t in grads:
         if not isinstance(t, Tensor):
             raise ValueError(f"gradients must be tensors (got {type(t).__name__})")
-        if t.dtype not in DTYPE_CODE:
-            _float(t, "gradients")
-        if t.is_sparse:
-            raise ValueError("sparse gradients are not supported")
+        _float(t, "gradients")
     _on_gpu(*grads)
-    return grads[0].device
+    raise AssertionError("unreachable")
+
+
+def _contiguous(ts: Sequence[Tensor]) -> bool:
+    try:
+        return all(map(Tensor.is_contiguous, ts))
+    except RuntimeError:
+        raise ValueError("sparse gradients are not supported") from None
 
 
 def _dense(t: Tensor) -> bool:
@@ -488,9 +493,9 @@ def _dense(t: Tensor) -> bool:
     return True
 
 
-def _run_norm(grads, out, max_norm, eps, device) -> Tensor:
+def _run_norm(grads, out, sizes, codes, max_norm, eps, device) -> Tensor:
     norm = torch.empty((), dtype=torch.float32, device=device)
-    a = _grad_list(grads, out)
+    a = _grad_list(grads, out, sizes, codes)
     at, n = a.buffer_info()[0], len(grads)
     L = lib()
     with _DeviceGuard(device):
@@ -507,26 +512,30 @@ def _run_norm(grads, out, max_norm, eps, device) -> Tensor:
     return norm
 
 
+@torch.no_grad()
 def grad_norm(grads: Iterable[Tensor]) -> Tensor:
     """sqrt(sum of squares of every element of every tensor), a float32 scalar on
     the GPU (nothing waits for it).  The squares are added in float64.  An empty
     list has norm 0 and gives a CPU tensor."""
-    grads = [t.detach() for t in grads]
+    grads = list(grads)
     if not grads:
         return torch.zeros(())
-    device = _check_grads(grads)
-    return _run_norm([t if _dense(t) else t.contiguous() for t in grads], None, None, 0.0, device)
+    device, codes = _check_grads(grads)
+    if not _contiguous(grads):
+        grads = [t if _dense(t) else t.contiguous() for t in grads]
+    return _run_norm(grads, None, list(map(Tensor.numel, grads)), codes, None, 0.0, device)
 
 
+@torch.no_grad()
 def clip_grad_norm(grads: Iterable[Tensor], max_norm: float, out: Optional[Sequence[Tensor]] = None,
                    eps: float = 1e-6) -> Tuple[List[Tensor], Tensor]:
     """(clipped, norm): every gradient times min(max_norm / (norm + eps), 1), the
     factor in float32 and one rounding, and the norm over all of them
     (mlx.optimizers.clip_grad_norm).  out: contiguous tensors of the gradients'
-    shapes and dtypes to write to (they may be the gradients themselves); by
+    sizes and dtypes to write to (they may be the gradients themselves); by
     default views of one new buffer for each dtype.  A NaN norm makes every
     gradient NaN."""
-    grads = [t.detach() for t in grads]
+    grads = list(grads)
     max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0 or not eps >= 0:
         raise ValueError(f"max_norm and eps must not be negative (got {max_norm} and {eps})")
@@ -536,17 +545,18 @@ def clip_grad_norm(grads: Iterable[Tensor], max_norm: float, out: Optional[Seque
             raise ValueError(f"out has {len(out)} tensors for {len(grads)} gradients")
     if not grads:
         return [], torch.zeros(())
-    device = _check_grads(grads)
-    grads = [t if t.is_contiguous() else t.contiguous() for t in grads]
+    device, codes = _check_grads(grads)
+    sizes = list(map(Tensor.numel, grads))
     if out is None:
         out = _new_like(grads)
     else:
-        _on_gpu(grads[0], *out)
-        for t, o in zip(grads, out):
-            if o.shape != t.shape or o.dtype != t.dtype or not o.is_contiguous():
-                raise ValueError(f"out must be contiguous {t.dtype} of shape {tuple(t.shape)} (got "
-                                 f"{o.dtype} {tuple(o.shape)}, strides {o.stride()})")
-    return out, _run_norm(grads, out, max_norm, eps, device)
+        on, kinds = _check_grads(out)
+        if on != device:
+            raise ValueError(f"rwkvq ops take every operand on one device; got '{device}' and '{on}'")
+        if kinds != codes or list(map(Tensor.numel, out)) != sizes or not _contiguous(out):
+            raise ValueError("out must hold contiguous tensors of the gradients' sizes and dtypes")
+    src = grads if _contiguous(grads) else [t.contiguous() for t in grads]
+    return out, _run_norm(src, out, sizes, codes, max_norm, eps, device)
 
 
 def _new_like(grads: Sequence[Tensor]) -> List[Tensor]:
@@ -565,6 +575,7 @@ def _new_like(grads: Sequence[Tensor]) -> List[Tensor]:
     return out
 
 
+@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6) -> Tensor:
     """Clips the .grad of the parameters (or one parameter) in place and returns
     the norm over them, a float32 scalar on the GPU; parameters without a
@@ -572,15 +583,18 @@ def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6) -> Tensor:
     max_norm."""
     if isinstance(parameters, Tensor):
         parameters = [parameters]
-    grads = [p.grad.detach() for p in parameters if p.grad is not None]
+    grads = [g for g in (p.grad for p in parameters) if g is not None]
     max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0 or not eps >= 0:
         raise ValueError(f"max_norm and eps must not be negative (got {max_norm} and {eps})")
     if not grads:
         return torch.zeros(())
-    device = _check_grads(grads)
+    device, codes = _check_grads(grads)
+    sizes = list(map(Tensor.numel, grads))
+    if _contiguous(grads):
+        return _run_norm(grads, None, sizes, codes, max_norm, eps, device)
     dense = [t if _dense(t) else t.contiguous() for t in grads]
-    norm = _run_norm(dense, None, max_norm, eps, device)
+    norm = _run_norm(dense, None, sizes, codes, max_norm, eps, device)
     for t, d in zip(grads, dense):
         if t is not d:
             t.copy_(d)

@@ -251,3 +251,15 @@ def test_registered_op_and_its_gradients(rq, dev):
     want = torch.autograd.grad(rq.linear_act(x, w, b, "gelu", r), leaves, dy)
     for p, q in zip(torch.autograd.grad(y, leaves, dy), want):
         assert torch.equal(p, q)
+
+
+def test_slopes_of_relu2_over_the_whole_range_of_bf16(rq, dev):
+    """2 v from far below float16's range to far above it, through one weight."""
+    v = torch.logspace(-30, 15, 512, base=10.0, dtype=torch.float64)
+    x = v.to(torch.bfloat16)[:, None].to(dev).requires_grad_()
+    w = torch.ones(1, 1, dtype=torch.bfloat16, device=dev)
+    r = torch.zeros(512, 1, dtype=torch.float32, device=dev)
+    dx, = torch.autograd.grad(rq.linear_act(x, w, None, "relu2", r), x, torch.full_like(r, 2.0 ** -10))
+    want = 2 * x.detach().double() * 2.0 ** -10
+    # the slope's rounding (bf16 at worst), g's and dx's (both exact to bf16)
+    assert ((dx.double() - want).abs() <= 3 * 2.0 ** -8 * want).all()

@@ -28,8 +28,8 @@ def test_every_declared_entry_point_is_exported_and_bound(L):
     text = open(os.path.join(ROOT, "include", "rwkvq_train.h")).read()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     names = set(re.findall(r"^\s*\w+\s+(rq_\w+)\s*\(", text, flags=re.M))
-    assert names == {"rq_linear_slope", "rq_linear_workspace_bytes", "rq_linear", "rq_linear_dpre",
-                     "rq_linear_dx", "rq_linear_dw", "rq_embed", "rq_embed_grad_workspace_bytes",
+    assert names == {"rq_linear_slope", "rq_linear_workspace_bytes", "rq_linear",
+                     "rq_linear_backward_workspace_bytes", "rq_linear_backward", "rq_embed", "rq_embed_grad_workspace_bytes",
                      "rq_embed_grad", "rq_grad_norm_workspace_bytes", "rq_grad_norm", "rq_clip_grads"}
     for name in names:
         assert hasattr(L, name) and name in _lib.SIGNATURES
@@ -48,27 +48,31 @@ def test_linear_refusals(L):
     for name in ("x", "w", "b", "r", "y"):
         assert fwd(**{name: P + 2}) == -2 and "aligned" in err(L)
     assert fwd(m=0, x=0, w=0, y=0) == 0 and fwd(n=0, y=0) == 0
-    assert L.rq_linear_dpre(P, 0, P, 1, 3, 0, 4, 8, P, 0, 0, 0, None) == -1 and "slope" in err(L)
-    assert L.rq_linear_dpre(P, 0, 0, 2, 3, 0, 4, 8, P, 0, 0, 0, None) == -1 and "NULL" in err(L)
-    assert L.rq_linear_dpre(P, 0, 0, 0, 0, 0, 4, 8, 0, P, 0, 0, None) == -1 and "workspace" in err(L)
-    assert L.rq_linear_dpre(P, 1, 0, 0, 0, 0, 4, 8, P, 0, 0, 0, None) == -1 and "dy must" in err(L)
-    assert L.rq_linear_dpre(P, 0, 0, 0, 0, 0, 4, 8, 0, 0, 0, 0, None) == 0
-    for fn in (L.rq_linear_dx, L.rq_linear_dw):
-        assert fn(0, P, 0, 4, 8, 16, P, 0, 0, None) == -1 and "NULL" in err(L)
-        assert fn(P, P, 5, 4, 8, 16, P, 0, 0, None) == -1 and "dtype" in err(L)
-        assert fn(P, P + 8, 0, 4, 8, 16, P, 0, 0, None) == -2
-        assert fn(P, P, 0, 4, 8, 0, 0, 0, 0, None) == 0
-    assert L.rq_linear_workspace_bytes(4, 1, 1, 1, 0) == -1
-    assert L.rq_linear_workspace_bytes(0, -1, 1, 1, 0) == -1
+    def bwd(dy=P, ydt=0, s=0, kind=0, a=0, x=P, w=P, dt=0, m=4, n=8, k=16, dx=P, dw=P, db=0, ws=0, nb=0):
+        return L.rq_linear_backward(dy, ydt, s, kind, a, x, w, dt, m, n, k, dx, dw, db, ws, nb, None)
+
+    for kw, text in (({"dt": 3}, "dtype"), ({"ydt": 1}, "dy must have"), ({"m": -1}, "negative"),
+                     ({"a": -1}, "activation"), ({"kind": 5}, "slope kind"), ({"kind": 1, "s": P, "a": 3}, "slope of"),
+                     ({"kind": 2, "a": 3}, "NULL"), ({"dy": 0}, "NULL"), ({"x": 0}, "NULL"), ({"w": 0}, "NULL"),
+                     ({"db": P}, "workspace"), ({"kind": 2, "s": P, "a": 3}, "workspace"), ({"ydt": 2}, "workspace")):
+        assert bwd(**kw) == -1 and text in err(L), (kw, err(L))
+    for name in ("dy", "x", "w", "dx", "dw", "db"):
+        assert bwd(**{name: P + 8}) == -2
+    assert bwd(dx=0, dw=0) == 0 and bwd(n=0, dx=0) == 0 and bwd(k=0) == 0
+    need = L.rq_linear_backward_workspace_bytes(100, 33, 64, 0, 2, 0, 1, 1, 1)
+    assert need >= 100 * 33 * 2 + 4 * 33 * 4     # g and the four partial sums of db
+    assert L.rq_linear_backward_workspace_bytes(64, 64, 64, 0, 0, 0, 1, 0, 0) == 0
+    assert L.rq_linear_backward_workspace_bytes(64, 64, 64, 0, 1, 0, 1, 0, 0) == -1
+    assert L.rq_linear_workspace_bytes(-1, 1, 1, 0) == -1
 
 
 def test_where_the_backward_pass_takes_the_slope_from(L):
-    none, of_y, f16, f32 = range(4)
+    none, of_y, f16, f32, wide16 = range(5)
     for dt in range(3):
         assert L.rq_linear_slope(0, dt, 1) == none
         assert L.rq_linear_slope(1, dt, 0) == of_y
-        assert L.rq_linear_slope(2, dt, 0) == (f32 if dt == 1 else of_y)
-        assert L.rq_linear_slope(2, dt, 1) == f32
+        assert L.rq_linear_slope(2, dt, 0) == (wide16, f32, of_y)[dt]
+        assert L.rq_linear_slope(2, dt, 1) == (wide16, f32, f32)[dt]
         for a in (1, 3, 4, 5, 6):
             assert L.rq_linear_slope(a, dt, 1) == (f16 if dt == 0 else f32)
     assert L.rq_linear_slope(7, 0, 0) == -1 and L.rq_linear_slope(0, 9, 0) == -1

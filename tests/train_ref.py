@@ -40,10 +40,10 @@ def slope_error(name, dtype, residual):
     """The relative error of the slope as the backward pass reads it."""
     if name is None:
         return 0.0
-    if not residual and name == "relu2" and dtype != torch.float16:
-        return U[dtype]                       # from y: half its relative error, and the root's
-    if dtype == torch.bfloat16 and name != "relu2":
+    if dtype == torch.bfloat16:
         return U[torch.float16]
+    if not residual and name == "relu2":
+        return 2 * U32                        # from y: half its relative error, and the root's
     return U32
 
 
@@ -81,7 +81,9 @@ class Linear:
             es = torch.zeros_like(s)
         if name == "relu":                    # 0 or 1, unless v is too near 0 to tell
             es = (v.abs() <= ev).double()
-        elif T == torch.bfloat16 and name not in (None, "relu2"):
+        elif T == torch.bfloat16 and name == "relu2":   # below 2^-14 eight bits are kept
+            es = es + 2.0 ** -14 * U[torch.bfloat16]
+        elif T == torch.bfloat16 and name is not None:
             es = es + TINY[torch.float16]
         eg = D.abs() * es + 2 * U32 * g.abs()
         eg_r = eg + U[T] * (g.abs() + eg) + TINY[T]     # as the products take it
