@@ -6,48 +6,86 @@
 
 namespace {
 
-RQ_DEV float sigmoid_f(float v) { return 1.f / (1.f + expf(-v)); }
+// e^x for x <= 0 to about two units in the last place: 2^(x log2 e) by the
+// hardware's v_exp_f32 for the rounded product, times 1 + ln 2 times its rounding
+// error.  NaN stays; results below 2^-126 are 0.
+RQ_DEV float exp_neg(float x) {
+    x = x < -110.f ? -110.f : x;
+    const float h = x * 1.44269504f;
+    const float l = __builtin_fmaf(x, 1.92596303e-8f, __builtin_fmaf(x, 1.44269504f, -h));
+    return __builtin_amdgcn_exp2f(h) * __builtin_fmaf(l, 0.693147181f, 1.f);
+}
 
-// act(v).  `act` is the same in every lane, so the switch is a scalar branch.
-RQ_DEV float act_value(int act, float v) {
+// act(v) and act'(v).  One exponential of a value <= 0 and one reciprocal
+// (v_rcp_f32, one unit in the last place) serve both: the output stage of a large
+// tile runs one wave to a SIMD, where their instructions are felt (x [4096, 2048],
+// w [8192, 2048] with slopes: library expf, erff and divisions 179 us with silu and
+// 228 with gelu, these 156 and 158, no activation 114).  `act` is the same in every lane, so the switch is a scalar branch.
+//   sigmoid  e = exp(-|v|), r = 1 / (1 + e):  r or e r,  slope e r^2, which keep their
+//            relative precision where the function has saturated
+//   tanh     e = exp(-2 |v|):  +-(1 - e) r,  slope 4 e r^2;  below 1/4, where 1 - e
+//            cancels, its series to v^9
+//   gelu     v Phi(v), Phi from the approximation 7.1.26 of Abramowitz and Stegun's
+//            handbook (erf within 1.5e-7), whose exp(-v^2 / 2) is also the slope's density
+RQ_DEV void act_both(int act, float v, float& a, float& s) {
     switch (act) {
-        case RQ_ACT_RELU: return v < 0.f ? 0.f : v;  // NaN stays
+        case RQ_ACT_RELU:
+            a = v < 0.f ? 0.f : v;  // NaN stays
+            s = v > 0.f ? 1.f : 0.f;
+            return;
         case RQ_ACT_RELU2: {
             const float c = v < 0.f ? 0.f : v;
-            return c * c;
+            a = c * c;
+            s = v > 0.f ? 2.f * v : 0.f;
+            return;
         }
-        case RQ_ACT_SILU: return v * sigmoid_f(v);
-        case RQ_ACT_GELU: return v * (0.5f * (1.f + erff(v * 0.70710678118654752f)));
-        case RQ_ACT_SIGMOID: return sigmoid_f(v);
-        case RQ_ACT_TANH: return tanhf(v);
-        default: return v;
+        case RQ_ACT_SILU:
+        case RQ_ACT_SIGMOID: {
+            const float e = exp_neg(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.f + e);
+            const float sg = v < 0.f ? e * r : r, d = e * r * r;
+            a = act == RQ_ACT_SILU ? v * sg : sg;
+            s = act == RQ_ACT_SILU ? __builtin_fmaf(v, d, sg) : d;
+            return;
+        }
+        case RQ_ACT_GELU: {
+            const float x = fabsf(v), e = exp_neg(-0.5f * v * v);
+            const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(x, 0.3275911f * 0.707106781f, 1.f));
+            float q = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+            q = __builtin_fmaf(t, q, 1.421413741f);
+            q = __builtin_fmaf(t, q, -0.284496736f);
+            q = __builtin_fmaf(t, q, 0.254829592f);
+            const float tail = 0.5f * t * q * e;  // Phi(-|v|)
+            const float phi = v < 0.f ? tail : 1.f - tail;
+            a = v * phi;
+            s = __builtin_fmaf(v * 0.398942280f, e, phi);
+            return;
+        }
+        case RQ_ACT_TANH: {
+            const float x = fabsf(v), e = exp_neg(-2.f * x), r = __builtin_amdgcn_rcpf(1.f + e);
+            const float q = v * v;
+            float p = __builtin_fmaf(q, 0.0218694885f, -0.0539682540f);
+            p = __builtin_fmaf(q, p, 0.133333333f);
+            p = __builtin_fmaf(q, p, -0.333333333f);
+            a = x < 0.25f ? __builtin_fmaf(v * q, p, v) : copysignf((1.f - e) * r, v);
+            s = 4.f * e * r * r;
+            return;
+        }
+        default:
+            a = v;
+            s = 1.f;
     }
 }
 
-// act'(v).  The slopes of sigmoid and tanh are written in e = exp(-|v|), which
-// keeps their relative precision where the function has saturated: s (1 - s) =
-// e / (1 + e)^2, and 1 - tanh^2 v = 4 e' / (1 + e')^2 with e' = exp(-2 |v|).
+RQ_DEV float act_value(int act, float v) {
+    float a, s;
+    act_both(act, v, a, s);
+    return a;
+}
+
 RQ_DEV float act_slope(int act, float v) {
-    switch (act) {
-        case RQ_ACT_RELU: return v > 0.f ? 1.f : 0.f;
-        case RQ_ACT_RELU2: return v > 0.f ? 2.f * v : 0.f;
-        case RQ_ACT_SILU: {
-            const float s = sigmoid_f(v), e = expf(-fabsf(v));
-            return s + v * (e / ((1.f + e) * (1.f + e)));
-        }
-        case RQ_ACT_GELU:
-            return 0.5f * (1.f + erff(v * 0.70710678118654752f)) +
-                   v * (0.39894228040143268f * expf(-0.5f * v * v));
-        case RQ_ACT_SIGMOID: {
-            const float e = expf(-fabsf(v));
-            return e / ((1.f + e) * (1.f + e));
-        }
-        case RQ_ACT_TANH: {
-            const float e = expf(-2.f * fabsf(v));
-            return 4.f * e / ((1.f + e) * (1.f + e));
-        }
-        default: return 1.f;
-    }
+    float a, s;
+    act_both(act, v, a, s);
+    return s;
 }
 
 // The same of four values; one scalar branch for all of them.

@@ -21,6 +21,7 @@ from __future__ import annotations
 import array
 import collections
 import operator
+import threading
 from typing import Iterable, List, Optional, Sequence, Tuple
 
 import torch
@@ -42,14 +43,19 @@ _WORKSPACES_MAX = 8
 
 
 def _workspace(device: torch.device, stream: int, nbytes: int) -> Optional[Tensor]:
-    """Scratch memory of the launches of one stream, which run in order: one
-    buffer per (device, stream), at most _WORKSPACES_MAX of them (least recently
-    used out).  Allocated while its stream is current, so torch's caching
-    allocator reuses a dropped one only on that stream, after the work queued
-    there.  Needs no initialisation."""
+    """Scratch memory of a call's launches on one stream, which run in order: one
+    buffer per (device, stream, host thread), at most _WORKSPACES_MAX of them (least
+    recently used out).  The thread is part of the key because two threads' launches
+    on one stream can come in between each other.  Allocated while its stream is
+    current, so torch's caching allocator reuses a dropped one only on that stream,
+    after the work queued there.  A call that is captured into a graph gets a buffer
+    of the graph's own pool: its replays outlive what is kept here.  Needs no
+    initialisation."""
     if nbytes <= 0:
         return None
-    key = (device.index, stream)
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    key = (device.index, stream, threading.get_ident())
     ws = _workspaces.pop(key, None)
     if ws is None or ws.numel() < nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -59,14 +65,35 @@ def _workspace(device: torch.device, stream: int, nbytes: int) -> Optional[Tenso
     return ws
 
 
+_workspace_bytes: dict = {}  # (query, *its arguments) -> bytes
+
+
+def _queried_workspace(query: str, args: tuple, device: torch.device, stream: int,
+                       what: str) -> Optional[Tensor]:
+    """The workspace that the entry point `query` asks for with `args`.  The caller
+    holds it until its launches are queued."""
+    key = (query, *args)
+    nbytes = _workspace_bytes.get(key)
+    if nbytes is None:
+        nbytes = getattr(lib(), query)(*args)
+        check(min(nbytes, 0), what)
+        if len(_workspace_bytes) > 4096:
+            _workspace_bytes.clear()
+        _workspace_bytes[key] = nbytes
+    return _workspace(device, stream, nbytes)
+
+
 def _addr(t: Optional[Tensor]) -> int:
     return 0 if t is None or t.numel() == 0 else t.data_ptr()
+
+
+def _size(t: Optional[Tensor]) -> int:
+    return 0 if t is None else t.numel()
 
 
 # -------------------------------------------------------------- linear_act
 
 _slope_kinds: dict = {}   # (activation code, dtype code, residual?) -> rq_linear_slope
-_linear_bytes: dict = {}  # the arguments of a workspace query -> its bytes
 
 
 def _slope_kind(act: int, dt: int, residual: bool) -> int:
@@ -77,19 +104,6 @@ def _slope_kind(act: int, dt: int, residual: bool) -> int:
         check(min(kind, 0), "linear_act")
         _slope_kinds[key] = kind
     return kind
-
-
-def _linear_workspace(name: str, key: tuple, device, stream) -> Tuple[int, int]:
-    """Address and size of the workspace that the query `name` asks for with `key`."""
-    nbytes = _linear_bytes.get(key)
-    if nbytes is None:
-        nbytes = getattr(lib(), name)(*key)
-        check(min(nbytes, 0), "linear_act")
-        if len(_linear_bytes) > 4096:
-            _linear_bytes.clear()
-        _linear_bytes[key] = nbytes
-    ws = _workspace(device, stream, nbytes)
-    return (0, 0) if ws is None else (ws.data_ptr(), ws.numel())
 
 
 def _linear_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor],
@@ -114,11 +128,11 @@ def _linear_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Op
     if m and n:
         with _DeviceGuard(x.device):
             stream = _stream_on(x.device)
-            ws, nbytes = _linear_workspace("rq_linear_workspace_bytes", (m, n, k, dt), x.device,
-                                           stream)
+            ws = _queried_workspace("rq_linear_workspace_bytes", (m, n, k, dt), x.device, stream,
+                                    "linear_act")
             rc = lib().rq_linear(_ptr(x), _ptr(weight), _addr(bias), dt, _addr(residual),
-                                 DTYPE_CODE[ydt], m, n, k, act, y.data_ptr(), _addr(slope), ws,
-                                 nbytes, stream)
+                                 DTYPE_CODE[ydt], m, n, k, act, y.data_ptr(), _addr(slope),
+                                 _addr(ws), _size(ws), stream)
         if rc:
             check(rc, "linear_act")
     if slope is None and want_slope:
@@ -142,12 +156,13 @@ def _linear_backward_impl(dy: Tensor, x: Tensor, weight: Tensor, saved: Tensor, 
     dt, ydt = DTYPE_CODE[x.dtype], DTYPE_CODE[dy.dtype]
     with _DeviceGuard(device):
         stream = _stream_on(device)
-        ws, nbytes = _linear_workspace("rq_linear_backward_workspace_bytes",
-                                       (m, n, k, dt, ydt, kind, want_x, want_w, want_b), device,
-                                       stream)
+        ws = _queried_workspace("rq_linear_backward_workspace_bytes",
+                                (m, n, k, dt, ydt, kind, want_x, want_w, want_b), device, stream,
+                                "linear_act backward")
         rc = lib().rq_linear_backward(
             _ptr(dy), ydt, _ptr(saved) if kind != _SLOPE_NONE else 0, kind, act, _ptr(x),
-            _ptr(weight), dt, m, n, k, _addr(dx), _addr(dw), _addr(db), ws, nbytes, stream)
+            _ptr(weight), dt, m, n, k, _addr(dx), _addr(dw), _addr(db), _addr(ws), _size(ws),
+            stream)
     if rc:
         check(rc, "linear_act backward")
     return dx, dw, db
@@ -220,8 +235,13 @@ class _LinearActFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():  # a graph of this pass is wanted; it has none
+            return _LinearActFunction._once(ctx, dy)
+        return _LinearActFunction._gradients(ctx, dy)
+
+    @staticmethod
+    def _gradients(ctx, dy):
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         dx = dw = db = None
         if need_x or need_w or need_b:
@@ -229,6 +249,8 @@ class _LinearActFunction(torch.autograd.Function):
             dx, dw, db = _linear_backward_impl(dy, x, weight, saved, ctx.act, ctx.kind, need_x,
                                                need_w, need_b)
         return dx, dw, db, dy if need_r else None, None
+
+    _once = staticmethod(once_differentiable(_gradients.__func__))
 
 
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
@@ -335,13 +357,13 @@ def _embed_grad_impl(dout: Tensor, idx: Tensor, vocab: int, scale: float, paddin
         L = lib()
         with _DeviceGuard(dout.device):
             stream = _stream_on(dout.device)
-            nbytes = L.rq_embed_grad_workspace_bytes(n, vocab, dim)
-            check(min(nbytes, 0), "embedding backward")
-            ws = _workspace(dout.device, stream, nbytes)
+            ws = _queried_workspace("rq_embed_grad_workspace_bytes", (n, vocab, dim), dout.device,
+                                    stream, "embedding backward")
             rc = L.rq_embed_grad(_ptr(idx), idx.element_size(), n, _ptr(dout), DTYPE_CODE[dout.dtype],
-                                 vocab, dim, scale, padding_idx, dw.data_ptr(), ws.data_ptr(),
-                                 ws.numel(), stream)
-        check(rc, "embedding backward")
+                                 vocab, dim, scale, padding_idx, dw.data_ptr(), _addr(ws), _size(ws),
+                                 stream)
+        if rc:
+            check(rc, "embedding backward")
     return dw
 
 
@@ -390,10 +412,17 @@ class _EmbeddingFunction(torch.autograd.Function):
         return _embed_impl(idx, weight, scale)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
+        if torch.is_grad_enabled():  # a graph of this pass is wanted; it has none
+            return _EmbeddingFunction._once(ctx, dout)
+        return _EmbeddingFunction._gradients(ctx, dout)
+
+    @staticmethod
+    def _gradients(ctx, dout):
         idx, = ctx.saved_tensors
         return None, _embed_grad_impl(dout, idx, ctx.vocab, ctx.scale, ctx.padding_idx), None, None
+
+    _once = staticmethod(once_differentiable(_gradients.__func__))
 
 
 def embedding(idx: Tensor, weight: Tensor, scale: float = 1.0,

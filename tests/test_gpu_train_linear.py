@@ -76,6 +76,19 @@ def test_large_tiles(rq, dev):
     check(rq, dev, 1100, 640, 600, "fp32", "tanh", True, "")
 
 
+def test_largest_tiles(rq, dev):
+    """Enough outputs that the 256 x 256 tiles are the cheapest, whole and ragged,
+    with a contraction that is not whole stages; the gradients' long contractions."""
+    check(rq, dev, 4096, 4096, 136, "bf16", "relu2", False, "")
+    check(rq, dev, 3000, 5000, 72, "f16", "silu", True, "fp32")
+
+
+def test_many_rows_of_few_columns(rq, dev):
+    """More rows than a grid's second dimension has blocks, a gradient of one tile
+    over a contraction of as many."""
+    check(rq, dev, 70000, 8, 64, "bf16", "tanh", True, "")
+
+
 def test_empty(rq, dev):
     for m, n, k in ((0, 8, 8), (4, 0, 8), (4, 8, 0)):
         x, w, b, r, dy = make(dev, m, n, k, "bf16", True, "fp32", 1)
@@ -263,3 +276,16 @@ def test_slopes_of_relu2_over_the_whole_range_of_bf16(rq, dev):
     want = 2 * x.detach().double() * 2.0 ** -10
     # the slope's rounding (bf16 at worst), g's and dx's (both exact to bf16)
     assert ((dx.double() - want).abs() <= 3 * 2.0 ** -8 * want).all()
+
+
+def test_second_derivatives_are_refused(rq, dev):
+    x, w, _, _, dy = make(dev, 8, 16, 16, "fp32", False, "", 14)
+    x.requires_grad_()
+    dx, = torch.autograd.grad(rq.linear_act(x, w, None, "silu"), x, dy, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), x)
+    e = torch.randn(9, 4, device=dev, requires_grad=True)
+    g = torch.randn(3, 4, device=dev, requires_grad=True)
+    de, = torch.autograd.grad(rq.embedding(torch.tensor([1, 2, 1], device=dev), e), e, g, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(de.sum(), g)
