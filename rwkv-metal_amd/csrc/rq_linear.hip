@@ -129,9 +129,11 @@ RQ_DEV void store_out(const rq::DenseArgs& g, int64_t i, int64_t j, f32x4_t v) {
 // operand with a contiguous contraction has an output a row, and eight lanes
 // reading one chunk of eight rows hit all banks.  A transposed operand keeps its
 // memory order: blocks of 128 bytes of outputs, a contraction element a row.  Its
-// 16-bit fragments come from the transposing read (16 lanes take 32 bytes of four
-// rows, which the XOR with twice the row spreads over the banks), 32-bit ones
-// from single-word reads.
+// 16-bit fragments come from the transposing read: 32 lanes take 32 bytes each of
+// rows 0 - 3 and 8 - 11 at a time, eight different eighths of the 256 bytes of
+// banks by the key ((row % 4) ^ (row / 8 % 2)) * 2 (without its second term
+// SQ_LDS_BANK_CONFLICT counts half of all LDS cycles).  32-bit ones come from
+// single-word reads.
 //
 // The first MFMA operand is B, so that a lane holds four neighbouring outputs of a row.
 constexpr int kBlock = 256;
@@ -163,7 +165,7 @@ struct Side {
 
     static RQ_DEV int key(int row) {
         if constexpr (!T) return row & 7;
-        else if constexpr (ES == 2) return (row & 3) << 1;
+        else if constexpr (ES == 2) return ((row & 3) ^ (row >> 3 & 1)) << 1;
         else return row & 4;
     }
 
@@ -265,7 +267,7 @@ struct Side {
             const uint8_t* l = lds + r0 / BK * (BK * 128) + in / BK * (BK * 128);
             if constexpr (ES == 2) {
                 const int col = in % BK + 4 * (lr & 3);
-                const int at = (8 * lg + (lr >> 2)) * 128 + (((col >> 3) ^ key(lr >> 2)) << 4) + (lr & 1) * 8;
+                const int at = (8 * lg + (lr >> 2)) * 128 + (((col >> 3) ^ key(8 * lg + (lr >> 2))) << 4) + (lr & 1) * 8;
                 s16x4_t h[2];
 #pragma unroll
                 for (int v = 0; v < 2; ++v)
