@@ -814,10 +814,10 @@ struct Plan {
 // fullest of 256 CUs an amount of its own and an amount a stage, which is less where
 // several tiles of a CU run together, and more (`turned`) with two transposed
 // operands, half of that with one; a split adds its partial sums' traffic and a
-// launch.  The numbers are least squares over 90 sizes of m 1 - 4096, k and n 64 -
-// 8192 in all three orders and up to 16 shares on an MI355X (operands beyond the L2
-// caches): the fit is within 12 % (16-bit) and 7 % (fp32) of the times, and what it
-// chooses 2 % behind the best choice of each size.
+// launch.  The numbers are least squares over 2600 timings on an MI355X (operands
+// beyond the L2 caches): 100 sizes of m 1 - 4096, k and n 64 - 8192 in all three
+// orders, every form with up to 16 shares.  The fit is 12 % off (odd widths 21 %,
+// fp32 7 %), and what it chooses 2 % slower than the best of each size (4 %, 1 %).
 struct Cost {
     int bm, bn, together;
     float tile, turned, stage[4];  // stage: of 1 .. `together` tiles running together, all of them
