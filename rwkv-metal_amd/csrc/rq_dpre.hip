@@ -31,12 +31,15 @@ RQ_DEV void store8(uint8_t* row, int64_t c, int64_t n, const float* f) {
 }
 
 // KIND: RQ_SLOPE_*.  SDT: the type the slopes (or y) are held in, -1 where act'(v) is 1.
+// Neighbouring blocks take neighbouring columns of the same rows.
 template <int DT, int YDT, int KIND, int SDT>
-__global__ __launch_bounds__(kBlock) void dpre_kernel(const rq::DpreArgs a, float* __restrict__ part) {
+__global__ __launch_bounds__(kBlock) void dpre_kernel(const rq::DpreArgs a, uint32_t ctiles,
+                                                      float* __restrict__ part) {
     __shared__ float red[kWaves][kCols];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.y * kCols + lane * 8;
-    const int64_t r0 = (int64_t)blockIdx.x * kPart + wave * kRows;
+    const uint32_t rtile = blockIdx.x / ctiles, ctile = blockIdx.x % ctiles;
+    const int64_t c = (int64_t)ctile * kCols + lane * 8;
+    const int64_t r0 = (int64_t)rtile * kPart + wave * kRows;
     const bool in = c < a.n;
     const uint8_t* dy = (const uint8_t*)a.dy;
     const uint8_t* sl = (const uint8_t*)a.slope;
@@ -74,12 +77,12 @@ __global__ __launch_bounds__(kBlock) void dpre_kernel(const rq::DpreArgs a, floa
     for (int j = 0; j < 8; ++j) red[wave][lane * 8 + j] = sum[j];
     __syncthreads();
     for (int j = threadIdx.x; j < kCols; j += kBlock) {
-        const int64_t col = (int64_t)blockIdx.y * kCols + j;
+        const int64_t col = (int64_t)ctile * kCols + j;
         if (col >= a.n) break;
         float v = red[0][j];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) v += red[w][j];
-        part[(int64_t)blockIdx.x * a.n + col] = v;
+        part[(int64_t)rtile * a.n + col] = v;
     }
 }
 
@@ -113,13 +116,15 @@ __global__ __launch_bounds__(kBlock) void colsum_kernel(const float* __restrict_
 }
 
 template <int DT, int YDT>
-void launch_as(const rq::DpreArgs& a, float* part, dim3 grid, hipStream_t s) {
+void launch_as(const rq::DpreArgs& a, float* part, int64_t parts, hipStream_t s) {
+    const uint32_t ct = (uint32_t)((a.n + kCols - 1) / kCols);
+    const uint32_t grid = (uint32_t)parts * ct;
     switch (a.slope_kind) {
-        case RQ_SLOPE_Y: dpre_kernel<DT, YDT, RQ_SLOPE_Y, YDT><<<grid, kBlock, 0, s>>>(a, part); break;
-        case RQ_SLOPE_F16: dpre_kernel<DT, YDT, RQ_SLOPE_F16, RQ_F16><<<grid, kBlock, 0, s>>>(a, part); break;
-        case RQ_SLOPE_F32: dpre_kernel<DT, YDT, RQ_SLOPE_F32, RQ_F32><<<grid, kBlock, 0, s>>>(a, part); break;
-        case RQ_SLOPE_WIDE16: dpre_kernel<DT, YDT, RQ_SLOPE_WIDE16, RQ_BF16><<<grid, kBlock, 0, s>>>(a, part); break;
-        default: dpre_kernel<DT, YDT, RQ_SLOPE_NONE, -1><<<grid, kBlock, 0, s>>>(a, part); break;
+        case RQ_SLOPE_Y: dpre_kernel<DT, YDT, RQ_SLOPE_Y, YDT><<<grid, kBlock, 0, s>>>(a, ct, part); break;
+        case RQ_SLOPE_F16: dpre_kernel<DT, YDT, RQ_SLOPE_F16, RQ_F16><<<grid, kBlock, 0, s>>>(a, ct, part); break;
+        case RQ_SLOPE_F32: dpre_kernel<DT, YDT, RQ_SLOPE_F32, RQ_F32><<<grid, kBlock, 0, s>>>(a, ct, part); break;
+        case RQ_SLOPE_WIDE16: dpre_kernel<DT, YDT, RQ_SLOPE_WIDE16, RQ_BF16><<<grid, kBlock, 0, s>>>(a, ct, part); break;
+        default: dpre_kernel<DT, YDT, RQ_SLOPE_NONE, -1><<<grid, kBlock, 0, s>>>(a, ct, part); break;
     }
 }
 
@@ -133,10 +138,10 @@ hipError_t launch_dpre(const DpreArgs& a, void* workspace, hipStream_t stream) {
     const int64_t parts = (a.m + kPart - 1) / kPart;
     float* part = a.db ? (float*)workspace : nullptr;
     if (parts > 0) {
-        const dim3 grid((unsigned)parts, (unsigned)((a.n + kCols - 1) / kCols));
+        if (parts * ((a.n + kCols - 1) / kCols) * kBlock > UINT32_MAX) return hipErrorInvalidConfiguration;
         RQ_DISPATCH_DT(a.dt, DT, {
-            if (a.y_dt == DT) launch_as<DT, DT>(a, part, grid, stream);
-            else launch_as<DT, RQ_F32>(a, part, grid, stream);
+            if (a.y_dt == DT) launch_as<DT, DT>(a, part, parts, stream);
+            else launch_as<DT, RQ_F32>(a, part, parts, stream);
         });
     }
     if (a.db) colsum_kernel<<<(unsigned)((a.n + 63) / 64), kBlock, 0, stream>>>(part, parts, a.n, a.db, a.dt);

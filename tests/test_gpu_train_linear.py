@@ -289,3 +289,22 @@ def test_second_derivatives_are_refused(rq, dev):
     de, = torch.autograd.grad(rq.embedding(torch.tensor([1, 2, 1], device=dev), e), e, g, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(de.sum(), g)
+
+
+# (m, n, k): each at which one of the three products takes a form that the sizes
+# above do not reach -- large and small tiles, shallow and deep stages, odd widths
+# in large tiles, few rows by groups of 16, 32 and 64, shares of the contraction
+FORM_SIZES = [(5432, 2192, 64), (8720, 208, 64), (8376, 200, 456), (65, 8992, 72), (2831, 2196, 65),
+              (5619, 64, 2216), (195, 64, 8200), (202, 632, 8200), (8936, 64, 72), (8584, 66, 734),
+              (64, 1320, 8928), (64, 8720, 200), (68, 3818, 1654), (40, 200, 136), (40, 77, 131)]
+
+
+@pytest.mark.parametrize("i", range(len(FORM_SIZES)))
+def test_forms(rq, dev, i):
+    m, n, k = FORM_SIZES[i]
+    check(rq, dev, m, n, k, ("bf16", "f16")[i % 2], ACTS[1 + i % 6], i % 3 == 0, ("", "fp32")[i % 2])
+
+
+@pytest.mark.parametrize("size", [(6999, 392, 8), (461, 8, 6208), (1, 336, 8216), (50, 96, 1000)])
+def test_forms_of_float32(rq, dev, size):
+    check(rq, dev, *size, "fp32", "silu", True, "")
