@@ -267,3 +267,23 @@ def test_embedding_gradient_and_clip_in_a_hip_graph(rq, dev):
         torch.cuda.synchronize()
         for p, q in zip(got, want):
             assert torch.equal(p, q), f"replay {replay}"
+
+
+def test_offsets_past_32_bits(rq, dev):
+    """A table and a gradient of 70000 x 32768: byte offsets pass 2^32."""
+    vocab, dim = 70000, 32768
+    w = torch.zeros(vocab, dim, dtype=torch.bfloat16, device=dev)
+    w[-2:] = torch.arange(dim, device=dev) % 256
+    w.requires_grad_()
+    idx = torch.tensor([vocab - 1, 0, vocab - 2, vocab - 1, vocab], device=dev)
+    out = rq.embedding(idx, w, 2.0)
+    assert torch.equal(out[0].float(), 2.0 * (torch.arange(dim, device=dev) % 256)) and (out[1] == 0).all()
+    assert torch.equal(out[0], out[2]) and out[4].isnan().all()
+    dw, = torch.autograd.grad(out, w, torch.ones_like(out))
+    assert (dw[vocab - 1] == 4).all() and (dw[vocab - 2] == 2).all() and (dw[0] == 2).all()
+    assert int(torch.count_nonzero(dw[1:vocab - 2])) == 0
+    clipped, norm = rq.clip_grad_norm([dw, dw[:1]], 1.0, out=[dw, torch.empty_like(dw[:1])])
+    n = math.sqrt(dim * (16 + 4 + 4 + 4))
+    assert abs(norm.item() - n) <= 2 * U32 * n
+    want = torch.tensor(4 / (n + 1e-6), dtype=torch.float64)
+    assert (clipped[0][vocab - 1].double().cpu() - want).abs().max() <= 2.0 ** -7 * want

@@ -308,3 +308,19 @@ def test_forms(rq, dev, i):
 @pytest.mark.parametrize("size", [(6999, 392, 8), (461, 8, 6208), (1, 336, 8216), (50, 96, 1000)])
 def test_forms_of_float32(rq, dev, size):
     check(rq, dev, *size, "fp32", "silu", True, "")
+
+
+def test_offsets_past_32_bits(rq, dev):
+    """70000 x 32768 outputs: the last rows' byte offsets pass 2^32."""
+    g = torch.Generator().manual_seed(15)
+    m, n, k = 70000, 32768, 64
+    x = torch.randn(m, k, generator=g).to(torch.bfloat16).to(dev).requires_grad_()
+    w = (torch.randn(n, k, generator=g) * 0.2).to(torch.bfloat16).to(dev)
+    r = torch.zeros(m, n, dtype=torch.bfloat16, device=dev)
+    r[-3:] = 1
+    y = rq.linear_act(x, w, None, "sigmoid", r)
+    rows = torch.tensor([0, 1, 33000, 65535, m - 3, m - 2, m - 1], device=dev)
+    ref = Linear(x.detach()[rows], w, None, r[rows], "sigmoid", torch.ones(7, n, dtype=torch.bfloat16))
+    close(y.detach()[rows], ref.y, ref.ey, "y")
+    dx, = torch.autograd.grad(y, x, torch.ones((), dtype=torch.bfloat16, device=dev).expand(m, n))
+    close(dx[rows], ref.dx, ref.edx, "dx")
