@@ -3,7 +3,10 @@
 //
 // norm = sqrt(sum over all tensors and elements of g^2); out = T(g * c).
 // Memory bound: the norm reads S bytes, the scaling reads them again and writes
-// S (the factor is known only after the last element has been read).
+// S (the factor is known only after the last element has been read).  1.2 GB of
+// bf16: 225 us (5.4 TB/s) and 434 (5.6); twice the blocks or twice the chunk
+// change nothing.  288 adapters of 28 MB: three launches of 4 - 7 us and three of
+// 5 - 10.
 //
 // A launch takes its tensors' descriptors as kernel arguments (no table to
 // upload, nothing to keep alive, capturable), kClipTensors at most; longer

@@ -4,7 +4,9 @@
 //   g[i, j] = T(dy[i, j] * act'(v[i, j]))       db[j] = T(sum over i of dy act'(v))
 //
 // Memory bound: dy and the slopes in, g out, one pass; the column sums ride along
-// in registers, from the unrounded products.
+// in registers, from the unrounded products.  [4096, 8192] bf16 with 16-bit slopes,
+// 201 MB: 46 us, 4.4 TB/s (a copy reaches 5.1; blocks that walked down the rows of
+// one column tile instead of along the columns took 51).
 #include "rq_act.h"
 #include "rq_linear.h"
 #include "rq_vec.h"
