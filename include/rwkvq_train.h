@@ -117,7 +117,11 @@ typedef struct {
  * a host array of `count` entries, read before the call returns; the fields
  * `out` are not used.  rq_clip_grads also writes out = g * c, rounded once, c =
  * min(max_norm / (norm + eps), 1) in fp32; a NaN norm gives a NaN c.  Where c
- * is 1, tensors given in place are not touched. */
+ * is 1, tensors given in place are not touched.  An entry listed again (the same g,
+ * out, n and dt: tied weights) counts again in the norm and is scaled once.  An entry
+ * may read what another one writes, which then runs after it; RQ_EINVAL where that
+ * has no order (an entry that does both, or a g that overlaps its own out without being it) and
+ * where two outputs overlap otherwise. */
 int64_t rq_grad_norm_workspace_bytes(const rq_grad* grads, int64_t count);
 int rq_grad_norm(const rq_grad* grads, int64_t count, float* norm, void* workspace,
                  int64_t workspace_bytes, void* stream);

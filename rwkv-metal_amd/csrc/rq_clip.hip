@@ -18,6 +18,8 @@
 // added up by every block of the scaling launches, in the same order each time,
 // so that neither an atomic nor a launch of its own stands between the two.
 #include <algorithm>
+#include <utility>
+#include <vector>
 
 #include "rq_common.h"
 #include "rq_error.h"
@@ -293,6 +295,93 @@ int check_work(const char* what, const float* norm, const void* workspace, int64
     return RQ_OK;
 }
 
+// What a list's scaling launches may run side by side.  Blocks of one launch run in
+// any order, so an output must not be written twice, and not before another
+// tensor that shares its memory has been read.
+struct Scaling {
+    bool as_listed = true;       // every entry once, all together
+    std::vector<rq_grad> early;  // otherwise: entries without repeats whose outputs no other entry reads,
+    std::vector<rq_grad> late;   // and then those that others read
+};
+
+int64_t bytes_of(const rq_grad& t) { return t.n * (t.dt == RQ_F32 ? 4 : 2); }
+
+// The outputs by address, each with the entry that writes it.  The same tensor listed
+// again is one output; other outputs that share memory have no sound order.
+int order_scaling(const char* what, const rq_grad* grads, int64_t count, Scaling& plan) {
+    struct Span {
+        uintptr_t b, e;
+        int64_t i;
+    };
+    const auto out_of = [&](int64_t i) {
+        const uintptr_t b = (uintptr_t)grads[i].out;
+        return Span{b, b + (uintptr_t)bytes_of(grads[i]), i};
+    };
+    // Most lists need no order: outputs in ascending order, and gradients that are
+    // scaled in place or lie outside all outputs.
+    bool sorted = true;
+    uintptr_t end = 0, out_lo = UINTPTR_MAX, g_lo = UINTPTR_MAX, g_hi = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (grads[i].n == 0) continue;
+        const Span o = out_of(i);
+        sorted = sorted && o.b >= end;
+        end = std::max(end, o.e);
+        out_lo = std::min(out_lo, o.b);
+        if (grads[i].g == grads[i].out) continue;
+        g_lo = std::min(g_lo, (uintptr_t)grads[i].g);
+        g_hi = std::max(g_hi, (uintptr_t)grads[i].g + (uintptr_t)bytes_of(grads[i]));
+    }
+    const bool apart = g_lo >= end || g_hi <= out_lo;  // also where every entry is in place
+    if (sorted && apart) return RQ_OK;
+
+    std::vector<Span> outs;
+    outs.reserve((size_t)count);
+    for (int64_t i = 0; i < count; ++i)
+        if (grads[i].n > 0) outs.push_back(out_of(i));
+    std::sort(outs.begin(), outs.end(), [](const Span& a, const Span& b) { return a.b != b.b ? a.b < b.b : a.i < b.i; });
+    std::vector<uint8_t> again;  // entries that repeat another one
+    size_t kept = 0;
+    for (const Span& o : outs) {
+        if (kept > 0 && o.b < outs[kept - 1].e) {
+            const rq_grad &t = grads[o.i], &u = grads[outs[kept - 1].i];
+            if (t.out != u.out || t.g != u.g || t.n != u.n || t.dt != u.dt)
+                return rq::fail(RQ_EINVAL, "%s: the outputs of tensors %lld and %lld overlap", what,
+                                (long long)outs[kept - 1].i, (long long)o.i);
+            if (again.empty()) again.assign((size_t)count, 0);
+            again[o.i] = 1;
+        } else {
+            outs[kept++] = o;
+        }
+    }
+    outs.resize(kept);
+
+    std::vector<uint8_t> late;  // entries whose output another entry reads
+    if (!apart) {
+        std::vector<std::pair<int64_t, int64_t>> reads;  // (entry, the entry whose output it reads)
+        for (int64_t i = 0; i < count; ++i) {
+            if (grads[i].n == 0 || grads[i].g == grads[i].out) continue;  // in place: no other output is there
+            const uintptr_t b = (uintptr_t)grads[i].g, e = b + (uintptr_t)bytes_of(grads[i]);
+            auto o = std::upper_bound(outs.begin(), outs.end(), b, [](uintptr_t at, const Span& s) { return at < s.e; });
+            for (; o != outs.end() && o->b < e; ++o) {
+                if (late.empty()) late.assign((size_t)count, 0);
+                late[o->i] = 1;
+                reads.emplace_back(i, o->i);
+            }
+        }
+        for (const auto& [reader, writer] : reads)
+            if (late[reader])
+                return rq::fail(RQ_EINVAL, "%s: tensor %lld and the output of tensor %lld overlap", what,
+                                (long long)reader, (long long)writer);
+    }
+    if (again.empty() && late.empty()) return RQ_OK;
+    plan.as_listed = false;
+    for (int64_t i = 0; i < count; ++i) {
+        if (!again.empty() && again[i]) continue;
+        (!late.empty() && late[i] ? plan.late : plan.early).push_back(grads[i]);
+    }
+    return RQ_OK;
+}
+
 hipError_t launch_squares(const rq_grad* grads, int64_t count, double* part, hipStream_t s) {
     int64_t at = 0;
     for_lists(grads, count, [&](const ClipList& l, uint32_t chunks) {
@@ -332,6 +421,12 @@ int rq_clip_grads(const rq_grad* grads, int64_t count, float max_norm, float eps
     if (int rc = check_list("rq_clip_grads", grads, count, true)) return rc;
     if (!(max_norm >= 0.f) || !(eps >= 0.f))
         return rq::fail(RQ_EINVAL, "rq_clip_grads: max_norm and eps must not be negative");
+    Scaling plan;
+    try {  // host memory for lists whose entries share theirs
+        if (int rc = order_scaling("rq_clip_grads", grads, count, plan)) return rc;
+    } catch (...) {
+        return rq::fail(RQ_ELAUNCH, "rq_clip_grads: out of host memory");
+    }
     const int64_t parts = partials(grads, count);
     if (int rc = check_work("rq_clip_grads", norm, workspace, workspace_bytes, parts)) return rc;
     hipStream_t s = (hipStream_t)stream;
@@ -342,11 +437,17 @@ int rq_clip_grads(const rq_grad* grads, int64_t count, float max_norm, float eps
     if (e == hipSuccess && known) grad_norm_kernel<<<1, kBlock, 0, s>>>(part, (int)parts, norm);
     if (e == hipSuccess) {
         float* first = norm;  // one block of the first launch writes it
-        for_lists(grads, count, [&](const ClipList& l, uint32_t chunks) {
+        const auto scale = [&](const ClipList& l, uint32_t chunks) {
             const int blocks = (int)std::min<int64_t>(chunks, 2 * kNormBlocks);
             grad_scale_kernel<<<blocks, kBlock, 0, s>>>(l, chunks, part, (int)parts, max_norm, eps, first, known);
             if (!known) first = nullptr;
-        });
+        };
+        if (plan.as_listed) {
+            for_lists(grads, count, scale);
+        } else {
+            for_lists(plan.early.data(), (int64_t)plan.early.size(), scale);
+            for_lists(plan.late.data(), (int64_t)plan.late.size(), scale);
+        }
         e = hipGetLastError();
     }
     return rq::launch_status(e, "rq_clip_grads");

@@ -563,7 +563,9 @@ def clip_grad_norm(grads: Iterable[Tensor], max_norm: float, out: Optional[Seque
     (mlx.optimizers.clip_grad_norm).  out: contiguous tensors of the gradients'
     sizes and dtypes to write to (they may be the gradients themselves); by
     default views of one new buffer for each dtype.  A NaN norm makes every
-    gradient NaN."""
+    gradient NaN.  A gradient listed twice with one output counts twice in the norm
+    and is scaled once; outputs that overlap otherwise are refused, and so are
+    gradients and outputs that overlap in a way that leaves no order."""
     grads = list(grads)
     max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0 or not eps >= 0:
@@ -609,7 +611,8 @@ def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6) -> Tensor:
     """Clips the .grad of the parameters (or one parameter) in place and returns
     the norm over them, a float32 scalar on the GPU; parameters without a
     gradient are left out.  Nothing is written where the norm is within
-    max_norm."""
+    max_norm.  A gradient listed twice (tied weights) counts twice in the norm and is
+    scaled once; gradients that overlap otherwise are refused."""
     if isinstance(parameters, Tensor):
         parameters = [parameters]
     grads = [g for g in (p.grad for p in parameters) if g is not None]

@@ -1,0 +1,48 @@
+"""The training-step operators on the GPU at their edges: shared memory,
+saturated and non-finite values, parameters and modules, very long inputs.  The
+bounds are those of tests/train_ref.py unless a test derives its own."""
+import math
+
+import pytest
+import torch
+
+from train_ref import U32
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "fp32": torch.float32}
+
+
+# ---------------------------------------------------------- gradient clip
+
+@pytest.mark.parametrize("dt", DT)
+def test_clip_scales_a_gradient_listed_twice_once(rq, dev, dt):
+    """Tied weights: twice in the norm, one factor on the gradient."""
+    print(f"clip of a gradient listed twice {dt}", flush=True)
+    g = torch.Generator().manual_seed(1)
+    tied = torch.randn(700, 333, generator=g).to(DT[dt]).to(dev)
+    other = torch.randn(5000, generator=g).to(DT[dt]).to(dev)
+    kept = [tied.clone(), other.clone()]
+    want, same = rq.clip_grad_norm([*kept, kept[0].clone()], 2.0)   # three tensors of their own
+    n = math.sqrt(2 * (tied.double() ** 2).sum().item() + (other.double() ** 2).sum().item())
+    out, norm = rq.clip_grad_norm([tied, other, tied], 2.0, out=[tied, other, tied])
+    assert abs(norm.item() - n) <= 2 * U32 * n and torch.equal(norm, same)
+    for o, k in zip(out, want):
+        assert torch.equal(o, k)
+    p, q = torch.nn.Parameter(kept[0].clone()), torch.nn.Parameter(kept[0].clone())
+    p.grad = q.grad = kept[0].clone()
+    rq.clip_grad_norm_([p, q], 2.0)
+    assert torch.equal(p.grad, rq.clip_grad_norm([kept[0], kept[0].clone()], 2.0)[0][0])
+
+
+def test_clip_reads_a_gradient_before_it_is_scaled_in_place(rq, dev):
+    g = torch.Generator().manual_seed(2)
+    flat = torch.randn(300000, generator=g).to(dev)
+    ts = [flat, flat[1000:2000], flat[250000:]]
+    kept = [t.clone() for t in ts]
+    want, _ = rq.clip_grad_norm(kept, 1.0)
+    out, _ = rq.clip_grad_norm(ts, 1.0, out=[flat, torch.empty_like(kept[1]), torch.empty_like(kept[2])])
+    for o, k in zip(out, want):
+        assert torch.equal(o, k)
+    with pytest.raises(ValueError, match="overlap"):
+        rq.clip_grad_norm(ts, 1.0, out=ts)

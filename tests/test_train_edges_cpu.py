@@ -1,0 +1,58 @@
+"""Refusals and host logic of rwkvq.train at its edges, without a GPU: nothing
+here reaches a launch."""
+import ctypes
+
+import pytest
+import torch
+
+P = 0x1000  # never dereferenced: validation fails first
+
+
+@pytest.fixture(scope="module")
+def L():
+    from rwkvq import _lib
+    return _lib.lib()
+
+
+def err(L):
+    return L.rq_last_error().decode()
+
+
+def clip(L, *entries):
+    """rq_clip_grads of (g, out, elements[, dtype]) with a workspace that is too
+    small, which is the check behind the one of shared memory."""
+    from rwkvq._lib import RqGrad
+    a = (RqGrad * len(entries))(*[RqGrad(e[0], e[1], e[2], e[3] if len(e) > 3 else 2, 0) for e in entries])
+    assert L.rq_clip_grads(ctypes.addressof(a), len(entries), 1.0, 1e-6, P, P, 0, None) == -1
+    return err(L)
+
+
+def test_clip_refuses_outputs_that_share_memory(L):
+    a, b, c = 0x10000, 0x20000, 0x30000
+    for entries in (
+            [(a, a, 100), (a + 40, a + 40, 100)],               # in place, one inside the other
+            [(a + 40, a + 40, 100), (a, a, 11)],
+            [(a, c, 100), (b, c, 100)],                         # two gradients, one output
+            [(a, a, 100), (b, a, 100)],
+            [(a, a, 100), (a, a, 99)],                          # the same place, another size or type
+            [(a, a, 100), (a, a, 100, 0)],
+            [(a, a + 4, 100)],                                  # shifted onto itself
+            [(a, b, 100), (b, a, 100)],                         # exchanged
+            [(a, b, 100), (b, c, 100), (c, a, 100)],
+            [(b, c, 100), (a, b, 100), (c + 200, c + 4000, 100), (c + 4000, a, 9)]):
+        assert "overlap" in clip(L, *entries), entries
+
+
+def test_clip_takes_what_has_an_order(L):
+    a, b, c = 0x10000, 0x20000, 0x30000
+    for entries in (
+            [(a, a, 100), (a, a, 100)],                         # tied weights
+            [(b, b, 100), (a, a, 100), (b, b, 100), (a, a, 100)],
+            [(a, b, 100), (a, b, 100)],
+            [(a, b, 100), (a, c, 100)],                         # one gradient, two outputs
+            [(a, a, 100), (a + 40, b, 10)],                     # one reads what another scales in place
+            [(a + 40, b, 10), (a, a, 100), (a + 80, c, 10)],
+            [(c, c, 5), (b, b, 0), (a, a, 100), (b, b, 7)],     # in place in any order of addresses
+            [(a, a, 100), (a + 400, a + 400, 100)],             # side by side
+            [(a, c, 100), (b, c + 400, 100), (c + 1000, c + 800, 50)]):
+        assert "workspace" in clip(L, *entries), entries
