@@ -196,8 +196,9 @@ _linear_backward_op = torch.library.custom_op("rwkvq::linear_act_backward", _lin
 
 @_linear_backward_op.register_fake
 def _(dy, x, weight, saved, act, kind, wanted):
-    return (torch.empty_like(x) if wanted[0] else x.new_empty(0),
-            torch.empty_like(weight) if wanted[1] else x.new_empty(0),
+    # row-major whatever the operands' own strides, as the kernels write them
+    return (x.new_empty(x.shape) if wanted[0] else x.new_empty(0),
+            weight.new_empty(weight.shape) if wanted[1] else x.new_empty(0),
             x.new_empty(weight.shape[0]) if wanted[2] else x.new_empty(0))
 
 

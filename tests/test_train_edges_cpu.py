@@ -56,3 +56,24 @@ def test_clip_takes_what_has_an_order(L):
             [(a, a, 100), (a + 400, a + 400, 100)],             # side by side
             [(a, c, 100), (b, c + 400, 100), (c + 1000, c + 800, 50)]):
         assert "workspace" in clip(L, *entries), entries
+
+
+def meta(*shape, dt=torch.bfloat16):
+    return torch.empty(*shape, dtype=dt, device="meta")
+
+
+def test_fake_gradients_have_the_strides_that_the_kernels_write(rq):
+    """Row-major, also where an operand is a transposed view."""
+    x, w = meta(2, 16, 6).transpose(1, 2), meta(16, 5).t()
+    dx, dw, db = torch.ops.rwkvq.linear_act_backward(meta(2, 6, 5), x, w, meta(0), 0, 0, [True, True, True])
+    assert dx.shape == x.shape and dx.is_contiguous()
+    assert dw.shape == w.shape and dw.is_contiguous() and db.shape == (5,)
+    y, _ = torch.ops.rwkvq.linear_act(x, w, None, None, 0)
+    assert y.is_contiguous()
+    x.requires_grad_(), w.requires_grad_()
+    y = rq.linear_act(x, w, None, "gelu")
+    dx, dw = torch.autograd.grad(y, (x, w), meta(5, 2, 6).permute(1, 2, 0))
+    assert dx.is_contiguous() and dw.is_contiguous()
+    table = meta(4, 9).t().requires_grad_()
+    de, = torch.autograd.grad(rq.embedding(meta(3, dt=torch.int64), table), table, meta(4, 3).t())
+    assert de.shape == (9, 4) and de.is_contiguous()
