@@ -163,12 +163,15 @@ def _direct(*ts: Tensor) -> bool:
 
 def _eager(*ts: Tensor) -> bool:
     """_direct apart from autograd."""
+    # first: torch.compile knows this answer and cannot trace the queries behind it
+    if _is_compiling():
+        return False
     if _dispatch_modes() or _function_modes() or _functorch_active() or _tracing() is not None:
         return False
     for t in ts:
         if type(t) is not Tensor or not t.is_cuda:
             return False
-    return not _is_compiling()
+    return True
 
 
 # --------------------------------------------------------------- quantize

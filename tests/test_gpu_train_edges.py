@@ -13,6 +13,26 @@ pytestmark = pytest.mark.gpu
 DT = {"bf16": torch.bfloat16, "f16": torch.float16, "fp32": torch.float32}
 
 
+# --------------------------------------------------------- dense products
+
+def test_transposed_operands_under_compile(rq, dev):
+    """A traced training step over transposed views: the planned strides are those
+    that the kernels write."""
+    g = torch.Generator().manual_seed(3)
+    h = torch.randn(2, 64, 24, generator=g).to(torch.bfloat16).to(dev).requires_grad_()
+    wt = (torch.randn(64, 40, generator=g) * 0.1).to(torch.bfloat16).to(dev).requires_grad_()
+    dy = torch.randn(2, 24, 40, generator=g).to(torch.bfloat16).to(dev)
+
+    def step(h, wt):
+        y = rq.linear_act(h.transpose(1, 2), wt.t(), None, "silu")
+        return y * 2
+
+    want = torch.autograd.grad(step(h, wt), (h, wt), dy)
+    traced = torch.compile(step, backend="aot_eager", fullgraph=True)
+    for got, w in zip(torch.autograd.grad(traced(h, wt), (h, wt), dy), want):
+        assert torch.equal(got, w)
+
+
 # ---------------------------------------------------------- gradient clip
 
 @pytest.mark.parametrize("dt", DT)

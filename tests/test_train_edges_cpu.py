@@ -77,3 +77,18 @@ def test_fake_gradients_have_the_strides_that_the_kernels_write(rq):
     table = meta(4, 9).t().requires_grad_()
     de, = torch.autograd.grad(rq.embedding(meta(3, dt=torch.int64), table), table, meta(4, 3).t())
     assert de.shape == (9, 4) and de.is_contiguous()
+
+
+def test_compiled_calls_are_recorded_whole(rq):
+    """One graph, without a break, forward and backward."""
+    def step(idx, table, x, w):
+        h = rq.embedding(idx, table, 2.0)
+        return rq.linear_act(x.transpose(0, 1), w.t(), None, "silu", h)
+
+    args = [meta(7, dt=torch.int64), meta(9, 5), meta(6, 7), meta(6, 5)]
+    for t in args[1:]:
+        t.requires_grad_()
+    y = torch.compile(step, backend="aot_eager", fullgraph=True)(*args)
+    grads = torch.autograd.grad(y, args[1:], meta(7, 5))
+    # row-major gradients of the transposed views, seen from behind the transposition
+    assert [g.stride() for g in grads] == [(5, 1), (1, 6), (1, 6)]
