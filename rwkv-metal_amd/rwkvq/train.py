@@ -30,7 +30,8 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._lib import DTYPE_CODE, check, lib
-from .ops import _DeviceGuard, _eager, _float, _on_gpu, _ptr, _ready, _stream_on
+from .ops import (_DeviceGuard, _eager, _float, _functorch_active, _on_gpu, _ptr, _ready, _stream_on,
+                  _tracing)
 
 ACTIVATIONS = (None, "relu", "relu2", "silu", "gelu", "sigmoid", "tanh")
 _ACT_CODE = {a: i for i, a in enumerate(ACTIVATIONS)}
@@ -107,8 +108,8 @@ def _slope_kind(act: int, dt: int, residual: bool) -> int:
 
 
 def _linear_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor],
-                 act: int, want_slope: bool) -> Tuple[Tensor, Tensor]:
-    """y, and the slopes where the backward pass reads them (else an empty tensor)."""
+                 act: int, want_slope: bool) -> Tuple[Tensor, Optional[Tensor]]:
+    """y, and the slopes where they are wanted and the backward pass reads them."""
     _on_gpu(x, weight, *[t for t in (bias, residual) if t is not None])
     lead, k = x.shape[:-1], x.shape[-1]
     n = weight.shape[0]
@@ -135,8 +136,6 @@ def _linear_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Op
                                  _addr(ws), _size(ws), stream)
         if rc:
             check(rc, "linear_act")
-    if slope is None and want_slope:
-        slope = x.new_empty(0)
     return y, slope
 
 
@@ -169,17 +168,18 @@ def _linear_backward_impl(dy: Tensor, x: Tensor, weight: Tensor, saved: Tensor, 
 
 
 def _linear_op_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor],
-                    act: int) -> Tuple[Tensor, Tensor]:
-    return _linear_impl(x, weight, bias, residual, act, True)
+                    act: int, want_slope: bool = True) -> Tuple[Tensor, Tensor]:
+    y, slope = _linear_impl(x, weight, bias, residual, act, want_slope)
+    return y, x.new_empty(0) if slope is None else slope
 
 
 _linear_op = torch.library.custom_op("rwkvq::linear_act", _linear_op_impl, mutates_args=())
 
 
 @_linear_op.register_fake
-def _(x, weight, bias, residual, act):
+def _(x, weight, bias, residual, act, want_slope=True):
     shape = (*x.shape[:-1], weight.shape[0])
-    kind = _slope_kind(act, DTYPE_CODE[x.dtype], residual is not None)
+    kind = _slope_kind(act, DTYPE_CODE[x.dtype], residual is not None) if want_slope else _SLOPE_NONE
     slope = x.new_empty(0) if kind < _SLOPE_F16 else x.new_empty(shape, dtype=_SLOPE_DTYPE[kind])
     return x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype), slope
 
@@ -203,19 +203,28 @@ def _(dy, x, weight, saved, act, kind, wanted):
 
 
 def _linear_op_setup(ctx, inputs, output):
-    x, weight, bias, residual, act = inputs
-    ctx.act = act
+    x, weight, bias, residual, act, want_slope = inputs
+    ctx.set_materialize_grads(False)  # else the unused slopes get a gradient of zeros
+    ctx.act, ctx.want_slope = act, want_slope
     ctx.kind = _slope_kind(act, DTYPE_CODE[x.dtype], residual is not None)
-    ctx.save_for_backward(x, weight, output[0] if ctx.kind == _SLOPE_Y else output[1])
+    if want_slope:
+        ctx.save_for_backward(x, weight, output[0] if ctx.kind == _SLOPE_Y else output[1])
 
 
 def _linear_op_backward(ctx, dy, _dslope):
-    x, weight, saved = ctx.saved_tensors
-    need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
-    dx, dw, db = _linear_backward_op(dy.contiguous(), x, weight, saved, ctx.act, ctx.kind,
-                                     [need_x, need_w, need_b])
+    need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+    if dy is None:
+        return (None,) * 6
+    dx = dw = db = None
+    if need_x or need_w or need_b:
+        if not ctx.want_slope:
+            raise RuntimeError("rwkvq::linear_act was called with want_slope=False: only its residual has a "
+                               "gradient")
+        x, weight, saved = ctx.saved_tensors
+        dx, dw, db = _linear_backward_op(dy.contiguous(), x, weight, saved, ctx.act, ctx.kind,
+                                         [need_x, need_w, need_b])
     return (dx if need_x else None, dw if need_w else None, db if need_b else None,
-            dy if need_r else None, None)
+            dy if need_r else None, None, None)
 
 
 _linear_op.register_autograd(_linear_op_backward, setup_context=_linear_op_setup)
@@ -300,7 +309,17 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
             return _linear_impl(x, weight, bias, residual, act, False)[0]
         if forward_ad._current_level < 0:
             return _LinearActFunction.apply(x, weight, bias, residual, act)
-    return _linear_op(x, weight, bias, residual, act)[0]
+    return _linear_op(x, weight, bias, residual, act, _records(x, weight, bias))[0]
+
+
+def _records(*ts: Optional[Tensor]) -> bool:
+    """Whether a recorded call has to keep what gradients of these operands take.  A
+    functorch transform or torch.jit.trace may ask for them later."""
+    if not torch.is_grad_enabled():
+        return False
+    if any(t is not None and t.requires_grad for t in ts):
+        return True
+    return not torch.compiler.is_compiling() and (_functorch_active() or _tracing() is not None)
 
 
 class LinearAct(nn.Linear):

@@ -66,3 +66,30 @@ def test_clip_reads_a_gradient_before_it_is_scaled_in_place(rq, dev):
         assert torch.equal(o, k)
     with pytest.raises(ValueError, match="overlap"):
         rq.clip_grad_norm(ts, 1.0, out=ts)
+
+
+# --------------------------------------------------- parameters and modules
+
+def test_module_without_gradients_writes_only_its_output(rq, dev):
+    """No slopes: the forward under no_grad allocates y, and so does one where only
+    the residual has a gradient."""
+    m = rq.LinearAct(64, 4096, activation="silu", device=dev, dtype=torch.float16)
+    x = torch.randn(2048, 64, device=dev).to(torch.float16)
+    r = torch.randn(2048, 4096, device=dev).to(torch.float16).requires_grad_()
+
+    def peak(fn):
+        fn()
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        y = fn()
+        return torch.cuda.max_memory_allocated() - before, y
+
+    with torch.no_grad():
+        assert peak(lambda: m(x))[0] == 2 * 2048 * 4096
+        assert peak(lambda: torch.ops.rwkvq.linear_act(x, m.weight, m.bias, None, 3, False)[0])[0] < 2.1 * 2048 * 4096
+    m.requires_grad_(False)
+    used, y = peak(lambda: m(x, r))
+    assert used == 2 * 2048 * 4096
+    dy = torch.ones_like(y)
+    assert torch.equal(torch.autograd.grad(y, r, dy)[0], dy)

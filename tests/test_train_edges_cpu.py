@@ -92,3 +92,44 @@ def test_compiled_calls_are_recorded_whole(rq):
     grads = torch.autograd.grad(y, args[1:], meta(7, 5))
     # row-major gradients of the transposed views, seen from behind the transposition
     assert [g.stride() for g in grads] == [(5, 1), (1, 6), (1, 6)]
+
+
+def test_the_recorded_op_keeps_slopes_only_for_gradients_that_take_them(rq, monkeypatch):
+    seen = []
+    op = rq.train._linear_op
+    monkeypatch.setattr(rq.train, "_linear_op", lambda *a: seen.append(op(*a)) or seen[-1])
+    x, w, b, r = meta(6, 8), meta(5, 8), meta(5), meta(6, 5)
+
+    def slopes(grads=()):
+        for t in (x, w, b, r):
+            t.requires_grad_(any(t is g for g in grads))
+        y = rq.linear_act(x, w, b, "silu", r)
+        return y, seen[-1][1].numel()
+
+    assert slopes()[1] == 0 and slopes([r])[1] == 0
+    for t in (x, w, b):
+        assert slopes([t])[1] == 30
+    with torch.no_grad():
+        assert slopes([x, w])[1] == 0
+    y, _ = slopes([r])
+    assert torch.autograd.grad(y, r, meta(6, 5))[0].shape == (6, 5)
+    y, _ = op(x, w.requires_grad_(), b, r, 3, False)
+    with pytest.raises(RuntimeError, match="want_slope"):
+        torch.autograd.grad(y, w, meta(6, 5))
+
+
+def test_the_recorded_op_materialises_no_gradient_of_its_slopes(rq):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Calls(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    names = []
+    w = meta(5, 8).requires_grad_()
+    y, slope = torch.ops.rwkvq.linear_act(meta(6, 8), w, None, None, 3)
+    assert slope.numel() == 30
+    with Calls():
+        torch.autograd.grad(y, w, meta(6, 5))
+    assert any("linear_act_backward" in n for n in names) and not any("zeros" in n for n in names), names
