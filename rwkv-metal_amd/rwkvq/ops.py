@@ -146,7 +146,7 @@ _tracing = torch._C._get_tracing_state  # of torch.jit.trace, which records regi
 
 def _direct(*ts: Tensor) -> bool:
     """True when a call may run an op's body without the torch.library
-    dispatcher: plain GPU tensors, no autograd to record, no tracing, no
+    dispatcher: plain GPU tensors or parameters, no autograd to record, no tracing, no
     dispatch or function mode and no functorch transform.  Such a call does
     exactly what the registered op would do and skips about 13 us of host
     dispatch, which is longer than the small launches take on the GPU.
@@ -161,6 +161,9 @@ def _direct(*ts: Tensor) -> bool:
     return True
 
 
+_PLAIN = (Tensor, torch.nn.Parameter)  # a parameter of a subclass keeps the subclass as its type
+
+
 def _eager(*ts: Tensor) -> bool:
     """_direct apart from autograd."""
     # first: torch.compile knows this answer and cannot trace the queries behind it
@@ -169,7 +172,7 @@ def _eager(*ts: Tensor) -> bool:
     if _dispatch_modes() or _function_modes() or _functorch_active() or _tracing() is not None:
         return False
     for t in ts:
-        if type(t) is not Tensor or not t.is_cuda:
+        if type(t) not in _PLAIN or not t.is_cuda:
             return False
     return True
 

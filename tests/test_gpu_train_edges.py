@@ -93,3 +93,35 @@ def test_module_without_gradients_writes_only_its_output(rq, dev):
     assert used == 2 * 2048 * 4096
     dy = torch.ones_like(y)
     assert torch.equal(torch.autograd.grad(y, r, dy)[0], dy)
+
+
+def test_parameters_take_the_direct_path(rq, dev, monkeypatch):
+    """Modules and calls on their weights run the same code as plain tensors, not the
+    registered ops; other subclasses do not."""
+    class Other(torch.Tensor):
+        pass
+
+    g = torch.Generator().manual_seed(4)
+    lin = rq.LinearAct(64, 40, activation="tanh", device=dev, dtype=torch.bfloat16)
+    emb = rq.ScaledEmbedding(30, 64, scale=3.0, device=dev, dtype=torch.bfloat16)
+    idx = torch.randint(0, 30, (2, 7), generator=g).to(dev)
+    dy = torch.randn(2, 7, 40, generator=g).to(torch.bfloat16).to(dev)
+
+    def step(w, b, table):
+        y = rq.linear_act(rq.embedding(idx, table, 3.0), w, b, "tanh")
+        return [y, *torch.autograd.grad(y, (w, b, table), dy)]
+
+    want = step(*[t.detach().clone().requires_grad_() for t in (lin.weight, lin.bias, emb.weight)])
+
+    def refuse(*a):
+        raise AssertionError("the registered op was called")
+
+    for name in ("_linear_op", "_embed_op", "_embed_grad_op", "_linear_backward_op"):
+        monkeypatch.setattr(rq.train, name, refuse)
+    for got in (step(lin.weight, lin.bias, emb.weight), [lin(emb(idx))]):
+        for p, q in zip(got, want):
+            assert torch.equal(p, q)
+    with torch.no_grad():
+        assert torch.equal(lin(emb(idx)), want[0])
+    with pytest.raises(AssertionError, match="registered"):
+        rq.embedding(idx, emb.weight.detach().as_subclass(Other))
