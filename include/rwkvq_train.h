@@ -44,13 +44,16 @@ typedef enum {
 
 /* What the backward pass takes act'(v) from: nothing (act'(v) = 1), the output
  * y, or a tensor of slopes act'(v) that the forward pass wrote. */
-enum { RQ_SLOPE_NONE = 0, RQ_SLOPE_Y = 1, RQ_SLOPE_F16 = 2, RQ_SLOPE_F32 = 3, RQ_SLOPE_WIDE16 = 4 };
+enum { RQ_SLOPE_NONE = 0, RQ_SLOPE_Y = 1, RQ_SLOPE_BOUND16 = 2, RQ_SLOPE_F32 = 3, RQ_SLOPE_WIDE16 = 4 };
 
 /* The form of the slope for operands of type dt.  RQ_SLOPE_Y where y alone gives
  * it: relu, and relu2 of fp32, with no residual added.  For bf16 operands 16 bits
- * that keep three bits more than bf16: float16 where the slope is bounded, and for
- * relu2, whose slope 2 v is not but has no sign, RQ_SLOPE_WIDE16: the float16 bits of
- * a slope in [2^-14, 2^15), else 0x8000 + its bf16 bits.  float32 otherwise.
+ * that keep three bits more than bf16 where float16 is normal and bf16's elsewhere:
+ * RQ_SLOPE_BOUND16 of slopes s below 2: the sign and the float16 bits of |s| >= 2^-14,
+ * else the sign and 0x4000 + the bf16 bits of |s| (NaN: 0x7fff);
+ * RQ_SLOPE_WIDE16 of relu2, whose slope 2 v is not bounded but has no sign: the
+ * float16 bits of a slope in [2^-14, 2^15), else 0x8000 + its bf16 bits.  float32
+ * otherwise.
  * RQ_EINVAL for an unknown act or dt. */
 int rq_linear_slope(rq_act act, rq_dtype dt, int has_residual);
 
@@ -63,7 +66,7 @@ int64_t rq_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, rq_dtype dt);
  * or RQ_F32.  One pass: v is accumulated in fp32 (bf16 and f16 operands on the
  * 16-bit matrix instructions, fp32 ones on the fp32 instruction) and rounded
  * once, into y.  slope: NULL, or where the backward pass wants
- * it [m, n] float16 or float32 as rq_linear_slope says.  k == 0 gives act(bias) +
+ * it [m, n] in the 16 or 32 bits that rq_linear_slope says.  k == 0 gives act(bias) +
  * residual. */
 int rq_linear(const void* x, const void* w, const void* bias, rq_dtype dt, const void* residual,
               rq_dtype y_dt, int64_t m, int64_t n, int64_t k, rq_act act, void* y, void* slope,

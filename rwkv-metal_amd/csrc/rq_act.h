@@ -123,6 +123,23 @@ RQ_DEV f32x4_t act_slope4(int act, f32x4_t v) {
     }
 }
 
+// RQ_SLOPE_BOUND16: a slope |s| < 2 - 2^-11 in 16 bits, of which float16 needs the codes
+// below 0x4000 only.  A saturated sigmoid's or tanh's slope goes far below 2^-14,
+// where float16 loses bits (from |v| = 10 and 5 on) and then everything (17.5 and 9.4):
+// there the codes from 0x4000 on hold bf16's bits.
+RQ_DEV uint32_t bound16_bits(float s) {
+    const uint32_t m = __float_as_uint(s) & 0x7fffffffu, sign = __float_as_uint(s) >> 16 & 0x8000u;
+    const float a = __uint_as_float(m);
+    uint32_t c = m < 0x38800000u ? f32_to_bf16_bits(a) + 0x4000u : f32_to_f16_bits(a);
+    if (m >= 0x40000000u) c = 0x7fffu;  // NaN: finite sums have no such slope
+    return c | sign;
+}
+RQ_DEV float bound16_value(uint32_t b) {
+    const uint32_t c = b & 0x7fffu;
+    const float a = c < 0x4000u ? f16_bits_to_f32(c) : bf16_bits_to_f32(c == 0x7fffu ? c : c - 0x4000u);
+    return __uint_as_float(__float_as_uint(a) | (b & 0x8000u) << 16);
+}
+
 // RQ_SLOPE_WIDE16: a slope s >= 0 in 16 bits, float16 in [2^-14, 2^15), where that
 // keeps 11 bits, else bf16 with the unused sign bit as the mark.  Values >= 0
 // compare like their bits.
@@ -133,6 +150,9 @@ RQ_DEV uint32_t wide16_bits(float s) {
 RQ_DEV float wide16_value(uint32_t b) {
     return b & 0x8000u ? bf16_bits_to_f32(b & 0x7fffu) : f16_bits_to_f32(b);
 }
+
+// The bits of a slope of `act` in 16, and the slope.
+RQ_DEV uint32_t slope16_bits(int act, float s) { return act == RQ_ACT_RELU2 ? wide16_bits(s) : bound16_bits(s); }
 
 // act'(v) from y = act(v): relu and relu2 only (relu2: v = sqrt(y)).
 RQ_DEV float act_slope_of_y(int act, float y) {

@@ -52,9 +52,12 @@ __global__ __launch_bounds__(kBlock) void dpre_kernel(const rq::DpreArgs a, uint
             if (r0 + r >= a.m) break;
             load8<YDT>(dy + (r0 + r) * a.n * kSize<YDT>, c, a.n, f[r]);
             if constexpr (SDT >= 0) load8<SDT>(sl + (r0 + r) * a.n * kSize<SDT>, c, a.n, s[r]);
-            if constexpr (KIND == RQ_SLOPE_WIDE16) {  // read as bf16, which keeps the bits
+            if constexpr (KIND == RQ_SLOPE_BOUND16 || KIND == RQ_SLOPE_WIDE16) {  // read as bf16, which keeps the bits
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s[r][j] = wide16_value(__float_as_uint(s[r][j]) >> 16);
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t b = __float_as_uint(s[r][j]) >> 16;
+                    s[r][j] = KIND == RQ_SLOPE_WIDE16 ? wide16_value(b) : bound16_value(b);
+                }
             }
         }
     }
@@ -123,7 +126,7 @@ void launch_as(const rq::DpreArgs& a, float* part, int64_t parts, hipStream_t s)
     const uint32_t grid = (uint32_t)parts * ct;
     switch (a.slope_kind) {
         case RQ_SLOPE_Y: dpre_kernel<DT, YDT, RQ_SLOPE_Y, YDT><<<grid, kBlock, 0, s>>>(a, ct, part); break;
-        case RQ_SLOPE_F16: dpre_kernel<DT, YDT, RQ_SLOPE_F16, RQ_F16><<<grid, kBlock, 0, s>>>(a, ct, part); break;
+        case RQ_SLOPE_BOUND16: dpre_kernel<DT, YDT, RQ_SLOPE_BOUND16, RQ_BF16><<<grid, kBlock, 0, s>>>(a, ct, part); break;
         case RQ_SLOPE_F32: dpre_kernel<DT, YDT, RQ_SLOPE_F32, RQ_F32><<<grid, kBlock, 0, s>>>(a, ct, part); break;
         case RQ_SLOPE_WIDE16: dpre_kernel<DT, YDT, RQ_SLOPE_WIDE16, RQ_BF16><<<grid, kBlock, 0, s>>>(a, ct, part); break;
         default: dpre_kernel<DT, YDT, RQ_SLOPE_NONE, -1><<<grid, kBlock, 0, s>>>(a, ct, part); break;

@@ -25,7 +25,7 @@ struct DenseArgs {
     void* y;
     int y_dt;
     void* slope;           // [m, n]: act'(C + bias), or NULL
-    int slope_kind;        // RQ_SLOPE_F16, _F32 or _WIDE16 where slope is set
+    int slope_kind;        // RQ_SLOPE_BOUND16, _F32 or _WIDE16 where slope is set
 };
 
 constexpr int kDenseMaxSide = 65535 * 64;  // of m, n and k: grids count 64 rows in y

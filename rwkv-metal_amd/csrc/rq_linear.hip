@@ -73,7 +73,6 @@ RQ_DEV void store4(void* p, int dt, int64_t at, const f32x4_t& v) {
 // y and slope of the four outputs (i, j) .. (i, j + 3) whose sums are v.
 RQ_DEV void store_out(const rq::DenseArgs& g, int64_t i, int64_t j, f32x4_t v) {
     const int64_t at = i * g.n + j;
-    const int sdt = g.slope_kind == RQ_SLOPE_F16 ? RQ_F16 : RQ_F32;
     if (j >= g.n) return;
     const bool whole = j + 4 <= g.n;
     if (g.bias) {
@@ -87,16 +86,16 @@ RQ_DEV void store_out(const rq::DenseArgs& g, int64_t i, int64_t j, f32x4_t v) {
     }
     if (g.slope) {
         const f32x4_t s = act_slope4(g.act, v);
-        if (g.slope_kind == RQ_SLOPE_WIDE16) {
+        if (g.slope_kind != RQ_SLOPE_F32) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (j + e < g.n) ((uint16_t*)g.slope)[at + e] = (uint16_t)wide16_bits(s[e]);
+                if (j + e < g.n) ((uint16_t*)g.slope)[at + e] = (uint16_t)slope16_bits(g.act, s[e]);
         } else if (whole) {
-            store4(g.slope, sdt, at, s);
+            store4(g.slope, RQ_F32, at, s);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (j + e < g.n) store_dt(g.slope, sdt, at + e, s[e]);
+                if (j + e < g.n) ((float*)g.slope)[at + e] = s[e];
         }
     }
     v = act_value4(g.act, v);
@@ -350,16 +349,16 @@ RQ_DEV void out_rows(const rq::DenseArgs& g, const float* own, int64_t i0, int64
                     sl[e] = act_slope(ACT, lo[u][e]);
                     sh[e] = act_slope(ACT, hi[u][e]);
                 }
-                if (ACT == RQ_ACT_RELU2 && g.slope_kind == RQ_SLOPE_WIDE16) {
+                if (DT == RQ_BF16 && g.slope_kind != RQ_SLOPE_F32) {
                     u32x4_t w;
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        w[e] = wide16_bits(sl[2 * e]) | (wide16_bits(sl[2 * e + 1]) << 16);
-                        w[e + 2] = wide16_bits(sh[2 * e]) | (wide16_bits(sh[2 * e + 1]) << 16);
+                        w[e] = slope16_bits(ACT, sl[2 * e]) | (slope16_bits(ACT, sl[2 * e + 1]) << 16);
+                        w[e + 2] = slope16_bits(ACT, sh[2 * e]) | (slope16_bits(ACT, sh[2 * e + 1]) << 16);
                     }
                     *(Bytes16*)((uint16_t*)g.slope + at + u * step) = Bytes16{{w[0], w[1], w[2], w[3]}};
                 } else {
-                    store8<RQ_F16>(g.slope, g.slope_kind == RQ_SLOPE_F32, at + u * step, sl, sh);
+                    store8<RQ_F32>(g.slope, true, at + u * step, sl, sh);
                 }
             }
 #pragma unroll

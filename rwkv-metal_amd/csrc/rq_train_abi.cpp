@@ -84,7 +84,7 @@ int rq_linear_slope(rq_act act, rq_dtype dt, int has_residual) {
     // into every gradient, and y = v^2 underflows in f16 where v does not
     if (!has_residual && (act == RQ_ACT_RELU || (act == RQ_ACT_RELU2 && dt == RQ_F32))) return RQ_SLOPE_Y;
     if (dt != RQ_BF16) return RQ_SLOPE_F32;
-    return act == RQ_ACT_RELU2 ? RQ_SLOPE_WIDE16 : RQ_SLOPE_F16;
+    return act == RQ_ACT_RELU2 ? RQ_SLOPE_WIDE16 : RQ_SLOPE_BOUND16;
 }
 
 int64_t rq_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, rq_dtype dt) {
@@ -105,7 +105,7 @@ int rq_linear(const void* x, const void* w, const void* bias, rq_dtype dt, const
     if (m == 0 || n == 0) return ok();
     if (int rc = check_ptrs(what, {y}, {x, w, bias, residual, y, slope, workspace})) return rc;
     if (k > 0 && (!x || !w)) return fail(RQ_EINVAL, "%s: NULL pointer", what);
-    if (slope && kind < RQ_SLOPE_F16)
+    if (slope && kind < RQ_SLOPE_BOUND16)
         return fail(RQ_EINVAL, "%s: this activation keeps no slopes (rq_linear_slope)", what);
     rq::DenseArgs g = forward_args(x, w, m, n, k, dt);
     g.bias = bias;

@@ -35,9 +35,10 @@ from .ops import (_DeviceGuard, _eager, _float, _functorch_active, _on_gpu, _ptr
 
 ACTIVATIONS = (None, "relu", "relu2", "silu", "gelu", "sigmoid", "tanh")
 _ACT_CODE = {a: i for i, a in enumerate(ACTIVATIONS)}
-_SLOPE_NONE, _SLOPE_Y, _SLOPE_F16, _SLOPE_F32, _SLOPE_WIDE16 = range(5)
-# the dtype a tensor of slopes is allocated in
-_SLOPE_DTYPE = {_SLOPE_F16: torch.float16, _SLOPE_F32: torch.float32, _SLOPE_WIDE16: torch.int16}
+_SLOPE_NONE, _SLOPE_Y, _SLOPE_BOUND16, _SLOPE_F32, _SLOPE_WIDE16 = range(5)
+# the dtype a tensor of slopes is allocated in; BOUND16 holds float16 values but for
+# those below 2^-14, whose bits have a code of their own
+_SLOPE_DTYPE = {_SLOPE_BOUND16: torch.float16, _SLOPE_F32: torch.float32, _SLOPE_WIDE16: torch.int16}
 
 _workspaces: "collections.OrderedDict" = collections.OrderedDict()
 _WORKSPACES_MAX = 8
@@ -124,7 +125,7 @@ def _linear_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Op
     y = torch.empty(*lead, n, dtype=ydt, device=x.device)
     kind = _slope_kind(act, dt, residual is not None) if want_slope else _SLOPE_NONE
     slope = None
-    if kind >= _SLOPE_F16:
+    if kind >= _SLOPE_BOUND16:
         slope = torch.empty(*lead, n, device=x.device, dtype=_SLOPE_DTYPE[kind])
     if m and n:
         with _DeviceGuard(x.device):
@@ -180,7 +181,7 @@ _linear_op = torch.library.custom_op("rwkvq::linear_act", _linear_op_impl, mutat
 def _(x, weight, bias, residual, act, want_slope=True):
     shape = (*x.shape[:-1], weight.shape[0])
     kind = _slope_kind(act, DTYPE_CODE[x.dtype], residual is not None) if want_slope else _SLOPE_NONE
-    slope = x.new_empty(0) if kind < _SLOPE_F16 else x.new_empty(shape, dtype=_SLOPE_DTYPE[kind])
+    slope = x.new_empty(0) if kind < _SLOPE_BOUND16 else x.new_empty(shape, dtype=_SLOPE_DTYPE[kind])
     return x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype), slope
 
 
@@ -275,8 +276,8 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
 
     The backward pass keeps x, weight and the slope act'(v): read off y for relu
     (and float32 relu2) without a residual, else a tensor of its own, 16 bits with
-    three more of them significant than bf16's beside bf16 operands and float32
-    beside others.  Its products take g = dy act'(v) rounded to the operands' type."""
+    three more of them significant than bf16's (as many below 2^-14) beside bf16
+    operands and float32 beside others.  Its products take g = dy act'(v) rounded to the operands' type."""
     if activation not in _ACT_CODE:
         raise ValueError(f"activation must be one of {ACTIVATIONS} (got {activation!r})")
     _float(x, "x")

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from train_ref import U32
+from train_ref import U, U32, act, close
 
 pytestmark = pytest.mark.gpu
 
@@ -31,6 +31,25 @@ def test_transposed_operands_under_compile(rq, dev):
     traced = torch.compile(step, backend="aot_eager", fullgraph=True)
     for got, w in zip(torch.autograd.grad(traced(h, wt), (h, wt), dy), want):
         assert torch.equal(got, w)
+
+
+def slopes_of(rq, dev, name, v):
+    """act'(v) times 2^20 as one product with w = 1 gives it back: the slope's, g's and
+    dx's roundings, and 64 fp32 units for the functions where their parts do not cancel."""
+    x = v.to(torch.bfloat16)[:, None].to(dev).requires_grad_()
+    w = torch.ones(1, 1, dtype=torch.bfloat16, device=dev)
+    r = torch.zeros(len(v), 1, dtype=torch.float32, device=dev)
+    dx, = torch.autograd.grad(rq.linear_act(x, w, None, name, r), x, torch.full_like(r, 2.0 ** 20))
+    want = act(name, x.detach().double().cpu())[1] * 2.0 ** 20
+    return dx.double().cpu(), want, (3 * U[torch.bfloat16] + 64 * U32) * want.abs()
+
+
+@pytest.mark.parametrize("name,lo,hi", [("sigmoid", -80, 80), ("tanh", -40, 40), ("silu", -80, -3)])
+def test_slopes_of_saturated_values_beside_bf16(rq, dev, name, lo, hi):
+    """Far below float16's range they keep bf16's precision."""
+    got, want, bound = slopes_of(rq, dev, name, torch.linspace(lo, hi, 1000))
+    close(got, want, bound, "slope")
+    assert (want.abs() < 2.0 ** -20 * 2.0 ** -24).any()
 
 
 # ---------------------------------------------------------- gradient clip
