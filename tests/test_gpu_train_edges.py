@@ -33,6 +33,15 @@ def test_transposed_operands_under_compile(rq, dev):
         assert torch.equal(got, w)
 
 
+def act64(name, v):
+    """act(v) and act'(v); gelu's tail by erfc, which keeps its precision where the
+    distribution function of torch.special.ndtr has become 0 (v below -8.3)."""
+    if name != "gelu":
+        return act(name, v)
+    p = 0.5 * torch.special.erfc(-v / math.sqrt(2))
+    return v * p, p + v * torch.exp(-v * v / 2) / math.sqrt(2 * math.pi)
+
+
 def slopes_of(rq, dev, name, v):
     """act'(v) times 2^20 as one product with w = 1 gives it back: the slope's, g's and
     dx's roundings, and 64 fp32 units for the functions where their parts do not cancel."""
@@ -40,16 +49,30 @@ def slopes_of(rq, dev, name, v):
     w = torch.ones(1, 1, dtype=torch.bfloat16, device=dev)
     r = torch.zeros(len(v), 1, dtype=torch.float32, device=dev)
     dx, = torch.autograd.grad(rq.linear_act(x, w, None, name, r), x, torch.full_like(r, 2.0 ** 20))
-    want = act(name, x.detach().double().cpu())[1] * 2.0 ** 20
+    want = act64(name, x.detach().double().cpu())[1] * 2.0 ** 20
     return dx.double().cpu(), want, (3 * U[torch.bfloat16] + 64 * U32) * want.abs()
 
 
-@pytest.mark.parametrize("name,lo,hi", [("sigmoid", -80, 80), ("tanh", -40, 40), ("silu", -80, -3)])
+@pytest.mark.parametrize("name,lo,hi", [("sigmoid", -80, 80), ("tanh", -40, 40), ("silu", -80, -3), ("gelu", -13, -1.5)])
 def test_slopes_of_saturated_values_beside_bf16(rq, dev, name, lo, hi):
     """Far below float16's range they keep bf16's precision."""
     got, want, bound = slopes_of(rq, dev, name, torch.linspace(lo, hi, 1000))
     close(got, want, bound, "slope")
     assert (want.abs() < 2.0 ** -20 * 2.0 ** -24).any()
+
+
+def test_the_tail_of_gelu_in_float32(rq, dev):
+    """v Phi(v) and its slope for negative v to fp32's relative precision: the tail is a
+    product of factors that are each a few units off (24 in all); in the slope, for
+    v < -1.5, its parts cancel by at most a factor of two."""
+    for m in (3, 1000):    # both output stages
+        v = torch.linspace(-13, -1.5, m)
+        x = v[:, None].expand(m, 16).contiguous().to(dev).requires_grad_()
+        y = rq.linear_act(x, torch.eye(16, device=dev), None, "gelu")
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        a, s = act64("gelu", x.detach().double().cpu())
+        close(y, a, 24 * U32 * a.abs(), "y")
+        close(dx, s, 64 * U32 * s.abs(), "slope")
 
 
 # ---------------------------------------------------------- gradient clip
