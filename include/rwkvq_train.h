@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-/* relu2 is relu(v)^2; gelu is v * Phi(v) with the normal distribution's Phi;
+/* relu2 is relu(v)^2, whose slope 2 relu(v) of a NaN is NaN, relu's is 1; gelu is v * Phi(v) with the normal distribution's Phi;
  * silu is v * sigmoid(v). */
 typedef enum {
     RQ_ACT_NONE = 0,

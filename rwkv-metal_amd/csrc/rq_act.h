@@ -34,12 +34,12 @@ RQ_DEV void act_both(int act, float v, float& a, float& s) {
     switch (act) {
         case RQ_ACT_RELU:
             a = v < 0.f ? 0.f : v;  // NaN stays
-            s = v > 0.f ? 1.f : 0.f;
+            s = v <= 0.f ? 0.f : 1.f;  // of NaN: 1, the gradient goes on
             return;
         case RQ_ACT_RELU2: {
             const float c = v < 0.f ? 0.f : v;
             a = c * c;
-            s = v > 0.f ? 2.f * v : 0.f;
+            s = v <= 0.f ? 0.f : 2.f * v;
             return;
         }
         case RQ_ACT_SILU:
@@ -165,8 +165,8 @@ RQ_DEV uint32_t slope16_bits(int act, float s) { return act == RQ_ACT_RELU2 ? wi
 
 // act'(v) from y = act(v): relu and relu2 only (relu2: v = sqrt(y)).
 RQ_DEV float act_slope_of_y(int act, float y) {
-    if (act == RQ_ACT_RELU) return y > 0.f ? 1.f : 0.f;
-    return y > 0.f ? 2.f * sqrtf(y) : 0.f;
+    if (y <= 0.f) return 0.f;  // NaN is neither: as from v itself
+    return act == RQ_ACT_RELU ? 1.f : 2.f * sqrtf(y);
 }
 
 }  // namespace

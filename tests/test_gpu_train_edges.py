@@ -75,6 +75,30 @@ def test_the_tail_of_gelu_in_float32(rq, dev):
         close(dx, s, 64 * U32 * s.abs(), "slope")
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("residual", ("", "fp32"))
+@pytest.mark.parametrize("name", ("relu", "relu2"))
+def test_nan_in_front_of_relu(rq, dev, name, residual, dt):
+    """As through torch's relu: the gradient goes on through relu, and is NaN behind its
+    square; rows without a NaN do not see it."""
+    g = torch.Generator().manual_seed(5)
+    for m, n in ((6, 40), (300, 136)):
+        x, w = torch.randn(m, 64, generator=g), torch.randn(n, 64, generator=g)
+        b, dy = torch.randn(n, generator=g), torch.randn(m, n, generator=g)
+        x[2, 3] = float("nan")
+        leaves = [t.to(DT[dt]).to(dev).requires_grad_() for t in (x, w, b)]
+        r = torch.zeros(m, n, device=dev) if residual else None
+        y = rq.linear_act(*leaves, name, r)
+        got = torch.autograd.grad(y, leaves, dy.to(y.dtype).to(dev))
+        plain = [t.detach().float().cpu().requires_grad_() for t in leaves]
+        c = torch.relu(plain[0] @ plain[1].t() + plain[2])
+        want = torch.autograd.grad(c if name == "relu" else c * c, plain, dy.to(y.dtype).float())
+        for p, q in zip(got, want):
+            assert torch.equal(p.isnan().cpu(), q.isnan())
+        assert bool(got[0][2].isnan().all()) == (name == "relu2") and not got[0][3:].isnan().any()
+        assert name == "relu2" or (got[0][2] != 0).any()
+
+
 # ---------------------------------------------------------- gradient clip
 
 @pytest.mark.parametrize("dt", DT)
