@@ -140,32 +140,45 @@ def _linear_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Op
     return y, slope
 
 
-def _linear_backward_impl(dy: Tensor, x: Tensor, weight: Tensor, saved: Tensor, act: int, kind: int,
-                          want_x: bool, want_w: bool, want_b: bool):
-    """(dx, dw, db), each None unless wanted."""
-    _on_gpu(dy, x, weight)
-    k, n = x.shape[-1], weight.shape[0]
-    dy, x, weight = _ready(dy), _ready(x), _ready(weight)
+def _linear_backward_impl(dy: Tensor, x: Optional[Tensor], weight: Optional[Tensor],
+                          saved: Optional[Tensor], act: int, kind: int, want_b: bool,
+                          dtype: torch.dtype):
+    """(dx, dw, db) of operands of `dtype`: dw where x is given, dx where the weight is."""
+    _on_gpu(dy, *[t for t in (x, weight) if t is not None])
+    n, k = dy.shape[-1], 0 if x is weight is None else (weight if x is None else x).shape[-1]
+    dy = _ready(dy)
+    x = None if x is None else _ready(x)
+    weight = None if weight is None else _ready(weight)
     m = dy.numel() // n if n else 0
-    device = x.device
-    dx = torch.empty_like(x) if want_x else None
-    dw = torch.empty_like(weight) if want_w else None
-    db = torch.empty(n, dtype=x.dtype, device=device) if want_b else None
+    device = dy.device
+    dx = None if weight is None else torch.empty(*dy.shape[:-1], k, dtype=dtype, device=device)
+    dw = None if x is None else torch.empty(n, k, dtype=dtype, device=device)
+    db = torch.empty(n, dtype=dtype, device=device) if want_b else None
     if n == 0:
-        return (dx.zero_() if want_x else None), dw, db
-    dt, ydt = DTYPE_CODE[x.dtype], DTYPE_CODE[dy.dtype]
+        return None if dx is None else dx.zero_(), dw, db
+    dt, ydt = DTYPE_CODE[dtype], DTYPE_CODE[dy.dtype]
     with _DeviceGuard(device):
         stream = _stream_on(device)
         ws = _queried_workspace("rq_linear_backward_workspace_bytes",
-                                (m, n, k, dt, ydt, kind, want_x, want_w, want_b), device, stream,
-                                "linear_act backward")
+                                (m, n, k, dt, ydt, kind, dx is not None, dw is not None, want_b),
+                                device, stream, "linear_act backward")
         rc = lib().rq_linear_backward(
-            _ptr(dy), ydt, _ptr(saved) if kind != _SLOPE_NONE else 0, kind, act, _ptr(x),
-            _ptr(weight), dt, m, n, k, _addr(dx), _addr(dw), _addr(db), _addr(ws), _size(ws),
+            _ptr(dy), ydt, _addr(saved) if kind != _SLOPE_NONE else 0, kind, act, _addr(x),
+            _addr(weight), dt, m, n, k, _addr(dx), _addr(dw), _addr(db), _addr(ws), _size(ws),
             stream)
     if rc:
         check(rc, "linear_act backward")
     return dx, dw, db
+
+
+def _save(ctx, x, weight, residual, act, y, slope) -> None:
+    """Keeps for the backward pass what the gradients wanted read: x for dw, the weight for
+    dx, the slopes (or y) for all of them.  A frozen layer keeps no activations."""
+    need_x, need_w = ctx.needs_input_grad[:2]
+    ctx.act, ctx.dtype = act, x.dtype
+    ctx.kind = _slope_kind(act, DTYPE_CODE[x.dtype], residual is not None)
+    saved = y if ctx.kind == _SLOPE_Y else slope if ctx.kind >= _SLOPE_BOUND16 else None
+    ctx.save_for_backward(x if need_w else None, weight if need_x else None, saved)
 
 
 def _linear_op_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor],
@@ -185,10 +198,11 @@ def _(x, weight, bias, residual, act, want_slope=True):
     return x.new_empty(shape, dtype=x.dtype if residual is None else residual.dtype), slope
 
 
-def _linear_backward_op_impl(dy: Tensor, x: Tensor, weight: Tensor, saved: Tensor, act: int,
-                             kind: int, wanted: List[bool]) -> Tuple[Tensor, Tensor, Tensor]:
-    got = _linear_backward_impl(dy, x, weight, saved, act, kind, *wanted)
-    return tuple(x.new_empty(0) if t is None else t for t in got)
+def _linear_backward_op_impl(dy: Tensor, x: Optional[Tensor], weight: Optional[Tensor],
+                             saved: Optional[Tensor], act: int, kind: int, want_b: bool,
+                             dtype: torch.dtype) -> Tuple[Tensor, Tensor, Tensor]:
+    got = _linear_backward_impl(dy, x, weight, saved, act, kind, want_b, dtype)
+    return tuple(dy.new_empty(0, dtype=dtype) if t is None else t for t in got)
 
 
 _linear_backward_op = torch.library.custom_op("rwkvq::linear_act_backward", _linear_backward_op_impl,
@@ -196,20 +210,20 @@ _linear_backward_op = torch.library.custom_op("rwkvq::linear_act_backward", _lin
 
 
 @_linear_backward_op.register_fake
-def _(dy, x, weight, saved, act, kind, wanted):
+def _(dy, x, weight, saved, act, kind, want_b, dtype):
     # row-major whatever the operands' own strides, as the kernels write them
-    return (x.new_empty(x.shape) if wanted[0] else x.new_empty(0),
-            weight.new_empty(weight.shape) if wanted[1] else x.new_empty(0),
-            x.new_empty(weight.shape[0]) if wanted[2] else x.new_empty(0))
+    n = dy.shape[-1]
+    return (dy.new_empty(0 if weight is None else (*dy.shape[:-1], weight.shape[-1]), dtype=dtype),
+            dy.new_empty(0 if x is None else (n, x.shape[-1]), dtype=dtype),
+            dy.new_empty(n if want_b else 0, dtype=dtype))
 
 
 def _linear_op_setup(ctx, inputs, output):
     x, weight, bias, residual, act, want_slope = inputs
     ctx.set_materialize_grads(False)  # else the unused slopes get a gradient of zeros
-    ctx.act, ctx.want_slope = act, want_slope
-    ctx.kind = _slope_kind(act, DTYPE_CODE[x.dtype], residual is not None)
+    ctx.want_slope = want_slope
     if want_slope:
-        ctx.save_for_backward(x, weight, output[0] if ctx.kind == _SLOPE_Y else output[1])
+        _save(ctx, x, weight, residual, act, *output)
 
 
 def _linear_op_backward(ctx, dy, _dslope):
@@ -222,8 +236,9 @@ def _linear_op_backward(ctx, dy, _dslope):
             raise RuntimeError("rwkvq::linear_act was called with want_slope=False: only its residual has a "
                                "gradient")
         x, weight, saved = ctx.saved_tensors
-        dx, dw, db = _linear_backward_op(dy.contiguous(), x, weight, saved, ctx.act, ctx.kind,
-                                         [need_x, need_w, need_b])
+        dx, dw, db = _linear_backward_op(dy.contiguous(), x if need_w else None,
+                                         weight if need_x else None, saved, ctx.act, ctx.kind, need_b,
+                                         ctx.dtype)
     return (dx if need_x else None, dw if need_w else None, db if need_b else None,
             dy if need_r else None, None, None)
 
@@ -239,10 +254,8 @@ class _LinearActFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act):
         need_pre = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         y, slope = _linear_impl(x, weight, bias, residual, act, need_pre)
-        ctx.act = act
-        ctx.kind = _slope_kind(act, DTYPE_CODE[x.dtype], residual is not None) if need_pre else 0
         if need_pre:
-            ctx.save_for_backward(x, weight, y if ctx.kind == _SLOPE_Y else slope)
+            _save(ctx, x, weight, residual, act, y, slope)
         return y
 
     @staticmethod
@@ -257,8 +270,8 @@ class _LinearActFunction(torch.autograd.Function):
         dx = dw = db = None
         if need_x or need_w or need_b:
             x, weight, saved = ctx.saved_tensors
-            dx, dw, db = _linear_backward_impl(dy, x, weight, saved, ctx.act, ctx.kind, need_x,
-                                               need_w, need_b)
+            dx, dw, db = _linear_backward_impl(dy, x if need_w else None, weight if need_x else None,
+                                               saved, ctx.act, ctx.kind, need_b, ctx.dtype)
         return dx, dw, db, dy if need_r else None, None
 
     _once = staticmethod(once_differentiable(_gradients.__func__))
@@ -274,7 +287,8 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
     "silu", "gelu" (v Phi(v)), "sigmoid" or "tanh".  The sums, the activation and
     the residual's addition are in float32, rounded once.
 
-    The backward pass keeps x, weight and the slope act'(v): read off y for relu
+    The backward pass keeps x where the weight has a gradient, the weight where x has
+    one, and the slope act'(v): read off y for relu
     (and float32 relu2) without a residual, else a tensor of its own, 16 bits with
     three more of them significant than bf16's (as many below 2^-14) beside bf16
     operands and float32 beside others.  Its products take g = dy act'(v) rounded to the operands' type."""

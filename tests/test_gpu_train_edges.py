@@ -191,3 +191,21 @@ def test_parameters_take_the_direct_path(rq, dev, monkeypatch):
         assert torch.equal(lin(emb(idx)), want[0])
     with pytest.raises(AssertionError, match="registered"):
         rq.embedding(idx, emb.weight.detach().as_subclass(Other))
+
+
+@pytest.mark.parametrize("name", (None, "relu", "silu"))
+def test_a_frozen_layer_keeps_no_activations(rq, dev, name):
+    """Only what the gradients wanted read is kept, and the gradients are the same."""
+    g = torch.Generator().manual_seed(6)
+    x, w, b = [torch.randn(s, generator=g).to(torch.bfloat16).to(dev) for s in ((50, 64), (40, 64), (40,))]
+    dy = torch.randn(50, 40, generator=g).to(torch.bfloat16).to(dev)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(rq.linear_act(*leaves, name), leaves, dy)
+    for needs in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        ts, kept = [t.detach().clone().requires_grad_(i in needs) for i, t in enumerate(leaves)], []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.shape) or t, lambda t: t):
+            y = rq.linear_act(*ts, name)
+        shapes = [(50, 64)] * (1 in needs) + [(40, 64)] * (0 in needs) + [(50, 40)] * (name is not None)
+        assert sorted(kept) == sorted(shapes)
+        for i, got in zip(needs, torch.autograd.grad(y, [ts[i] for i in needs], dy)):
+            assert torch.equal(got, want[i])

@@ -65,7 +65,7 @@ def meta(*shape, dt=torch.bfloat16):
 def test_fake_gradients_have_the_strides_that_the_kernels_write(rq):
     """Row-major, also where an operand is a transposed view."""
     x, w = meta(2, 16, 6).transpose(1, 2), meta(16, 5).t()
-    dx, dw, db = torch.ops.rwkvq.linear_act_backward(meta(2, 6, 5), x, w, meta(0), 0, 0, [True, True, True])
+    dx, dw, db = torch.ops.rwkvq.linear_act_backward(meta(2, 6, 5), x, w, None, 0, 0, True, torch.bfloat16)
     assert dx.shape == x.shape and dx.is_contiguous()
     assert dw.shape == w.shape and dw.is_contiguous() and db.shape == (5,)
     y, _ = torch.ops.rwkvq.linear_act(x, w, None, None, 0)
@@ -133,3 +133,27 @@ def test_the_recorded_op_materialises_no_gradient_of_its_slopes(rq):
     with Calls():
         torch.autograd.grad(y, w, meta(6, 5))
     assert any("linear_act_backward" in n for n in names) and not any("zeros" in n for n in names), names
+
+
+def kept(fn):
+    """What a call saves for its backward pass."""
+    ts = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: ts.append(t) or t, lambda t: t):
+        y = fn()
+    return y, ts
+
+
+def test_only_what_the_gradients_read_is_kept_by_the_recorded_op(rq):
+    x, w, b = meta(6, 8), meta(5, 8), meta(5)
+    for needs, shapes in (((x,), {(5, 8), (6, 5)}), ((w,), {(6, 8), (6, 5)}), ((b,), {(6, 5)}),
+                          ((x, w, b), {(5, 8), (6, 8), (6, 5)})):
+        for t in (x, w, b):
+            t.requires_grad_(any(t is n for n in needs))
+        for name in ("silu", "relu"):       # slopes, and y
+            y, ts = kept(lambda: rq.linear_act(x, w, b, name))
+            assert {tuple(t.shape) for t in ts} == shapes and len(ts) == len(shapes)
+            grads = torch.autograd.grad(y, needs, meta(6, 5))
+            assert [g.shape for g in grads] == [t.shape for t in needs]
+        y, ts = kept(lambda: rq.linear_act(x, w, b))
+        assert {tuple(t.shape) for t in ts} == shapes - {(6, 5)}
+        torch.autograd.grad(y, needs[:1], meta(6, 5))
