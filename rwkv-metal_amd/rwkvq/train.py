@@ -19,9 +19,7 @@ packed products.  Tensors must live on the ROCm GPU; there is no CPU path.
 from __future__ import annotations
 
 import array
-import collections
 import operator
-import threading
 from typing import Iterable, List, Optional, Sequence, Tuple
 
 import torch
@@ -40,38 +38,19 @@ _SLOPE_NONE, _SLOPE_Y, _SLOPE_BOUND16, _SLOPE_F32, _SLOPE_WIDE16 = range(5)
 # those below 2^-14, whose bits have a code of their own
 _SLOPE_DTYPE = {_SLOPE_BOUND16: torch.float16, _SLOPE_F32: torch.float32, _SLOPE_WIDE16: torch.int16}
 
-_workspaces: "collections.OrderedDict" = collections.OrderedDict()
-_WORKSPACES_MAX = 8
 
-
-def _workspace(device: torch.device, stream: int, nbytes: int) -> Optional[Tensor]:
-    """Scratch memory of a call's launches on one stream, which run in order: one
-    buffer per (device, stream, host thread), at most _WORKSPACES_MAX of them (least
-    recently used out).  The thread is part of the key because two threads' launches
-    on one stream can come in between each other.  Allocated while its stream is
-    current, so torch's caching allocator reuses a dropped one only on that stream,
-    after the work queued there.  A call that is captured into a graph gets a buffer
-    of the graph's own pool: its replays outlive what is kept here.  Needs no
-    initialisation."""
-    if nbytes <= 0:
-        return None
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, stream, threading.get_ident())
-    ws = _workspaces.pop(key, None)
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _workspaces[key] = ws
-    while len(_workspaces) > _WORKSPACES_MAX:
-        _workspaces.popitem(last=False)
-    return ws
+def _workspace(device: torch.device, nbytes: int) -> Optional[Tensor]:
+    """Scratch memory of one call's launches, from torch's caching allocator and
+    back to it when the call returns: the allocator hands it on only to later work of
+    the stream that was current here, which is the one launched on.  Nothing is kept
+    from call to call (a backward pass takes as much as its output's gradient)."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
 
 
 _workspace_bytes: dict = {}  # (query, *its arguments) -> bytes
 
 
-def _queried_workspace(query: str, args: tuple, device: torch.device, stream: int,
-                       what: str) -> Optional[Tensor]:
+def _queried_workspace(query: str, args: tuple, device: torch.device, what: str) -> Optional[Tensor]:
     """The workspace that the entry point `query` asks for with `args`.  The caller
     holds it until its launches are queued."""
     key = (query, *args)
@@ -82,7 +61,7 @@ def _queried_workspace(query: str, args: tuple, device: torch.device, stream: in
         if len(_workspace_bytes) > 4096:
             _workspace_bytes.clear()
         _workspace_bytes[key] = nbytes
-    return _workspace(device, stream, nbytes)
+    return _workspace(device, nbytes)
 
 
 def _addr(t: Optional[Tensor]) -> int:
@@ -130,7 +109,7 @@ def _linear_impl(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Op
     if m and n:
         with _DeviceGuard(x.device):
             stream = _stream_on(x.device)
-            ws = _queried_workspace("rq_linear_workspace_bytes", (m, n, k, dt), x.device, stream,
+            ws = _queried_workspace("rq_linear_workspace_bytes", (m, n, k, dt), x.device,
                                     "linear_act")
             rc = lib().rq_linear(_ptr(x), _ptr(weight), _addr(bias), dt, _addr(residual),
                                  DTYPE_CODE[ydt], m, n, k, act, y.data_ptr(), _addr(slope),
@@ -161,7 +140,7 @@ def _linear_backward_impl(dy: Tensor, x: Optional[Tensor], weight: Optional[Tens
         stream = _stream_on(device)
         ws = _queried_workspace("rq_linear_backward_workspace_bytes",
                                 (m, n, k, dt, ydt, kind, dx is not None, dw is not None, want_b),
-                                device, stream, "linear_act backward")
+                                device, "linear_act backward")
         rc = lib().rq_linear_backward(
             _ptr(dy), ydt, _addr(saved) if kind != _SLOPE_NONE else 0, kind, act, _addr(x),
             _addr(weight), dt, m, n, k, _addr(dx), _addr(dw), _addr(db), _addr(ws), _size(ws),
@@ -393,7 +372,7 @@ def _embed_grad_impl(dout: Tensor, idx: Tensor, vocab: int, scale: float, paddin
         with _DeviceGuard(dout.device):
             stream = _stream_on(dout.device)
             ws = _queried_workspace("rq_embed_grad_workspace_bytes", (n, vocab, dim), dout.device,
-                                    stream, "embedding backward")
+                                    "embedding backward")
             rc = L.rq_embed_grad(_ptr(idx), idx.element_size(), n, _ptr(dout), DTYPE_CODE[dout.dtype],
                                  vocab, dim, scale, padding_idx, dw.data_ptr(), _addr(ws), _size(ws),
                                  stream)
@@ -566,7 +545,7 @@ def _run_norm(grads, out, sizes, codes, max_norm, eps, device) -> Tensor:
         stream = _stream_on(device)
         nbytes = L.rq_grad_norm_workspace_bytes(at, n)
         check(min(nbytes, 0), "clip_grad_norm")
-        ws = _workspace(device, stream, max(nbytes, 16))
+        ws = _workspace(device, max(nbytes, 16))
         if max_norm is None:
             rc = L.rq_grad_norm(at, n, norm.data_ptr(), ws.data_ptr(), ws.numel(), stream)
         else:

@@ -209,3 +209,23 @@ def test_a_frozen_layer_keeps_no_activations(rq, dev, name):
         assert sorted(kept) == sorted(shapes)
         for i, got in zip(needs, torch.autograd.grad(y, [ts[i] for i in needs], dy)):
             assert torch.equal(got, want[i])
+
+
+def test_no_workspace_outlives_its_call(rq, dev):
+    """The backward pass's g (64 MB here), the table gradient's and the clip's scratch
+    memory go back to the allocator."""
+    x = torch.zeros(8192, 64, dtype=torch.bfloat16, device=dev)
+    w = torch.zeros(4096, 64, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    table = torch.zeros(500, 64, device=dev, requires_grad=True)
+    idx = torch.arange(9000, device=dev) % 500
+
+    def step():
+        rq.linear_act(x, w, None, "silu").sum().backward()
+        rq.embedding(idx, table).sum().backward()
+        rq.clip_grad_norm_([w, table], 1.0)
+        w.grad = table.grad = None
+
+    torch.ones(8, device=dev).sum()
+    before = torch.cuda.memory_allocated()
+    step()
+    assert torch.cuda.memory_allocated() == before
