@@ -14,7 +14,7 @@ rwkv_metal/model/rwkv7_x070.py:108-111,142-182), the FFN's relu^2
 the fine-tune loop (rwkv_metal/lora/finetune.py:108-205).
 
 Operands of one dtype stay in it; any other mix computes in float32, as in the
-packed products.  Tensors must live on the ROCm GPU; there is no CPU path.
+packed products, and under torch.autocast linear_act computes in its dtype.  Tensors must live on the ROCm GPU; there is no CPU path.
 """
 from __future__ import annotations
 
@@ -262,7 +262,8 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
 
     x [..., k], weight [n, k], bias [n]; residual [..., n] is added after the
     activation and may be float32 beside 16-bit operands: y then is too, a
-    float32 residual stream.  activation: None, "relu", "relu2" (relu(v)^2),
+    float32 residual stream.  Under torch.autocast x, weight and bias are cast to its
+    dtype, as nn.Linear casts them.  activation: None, "relu", "relu2" (relu(v)^2),
     "silu", "gelu" (v Phi(v)), "sigmoid" or "tanh".  The sums, the activation and
     the residual's addition are in float32, rounded once.
 
@@ -290,8 +291,14 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
         if residual.shape != want:
             raise ValueError(f"residual must have shape {want} (got {tuple(residual.shape)})")
     dt = x.dtype
-    if weight.dtype != dt or (bias is not None and bias.dtype != dt):
-        dt = torch.float32
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        cast = torch.get_autocast_dtype("cuda")
+    elif weight.dtype != dt or (bias is not None and bias.dtype != dt):
+        cast = torch.float32
+    else:
+        cast = None
+    if cast is not None:
+        dt = cast
         x, weight = x.to(dt), weight.to(dt)
         bias = None if bias is None else bias.to(dt)
     if residual is not None and residual.dtype not in (dt, torch.float32):

@@ -229,3 +229,28 @@ def test_no_workspace_outlives_its_call(rq, dev):
     before = torch.cuda.memory_allocated()
     step()
     assert torch.cuda.memory_allocated() == before
+
+
+@pytest.mark.parametrize("to", ("bf16", "f16"))
+def test_linear_act_under_autocast(rq, dev, to):
+    """float32 parameters compute in autocast's dtype, as nn.Linear's do, and get float32
+    gradients; a float32 residual stream stays one."""
+    T = DT[to]
+    g = torch.Generator().manual_seed(7)
+    lin = torch.nn.Linear(64, 40, device=dev)
+    m = rq.LinearAct.from_linear(lin, "silu")
+    x = torch.randn(3, 9, 64, generator=g).to(dev).requires_grad_()
+    r = torch.randn(3, 9, 40, generator=g).to(dev)
+    for res in (None, r):
+        with torch.autocast("cuda", dtype=T):
+            y, plain = m(x, res), lin(x)
+        assert plain.dtype == T and y.dtype == (T if res is None else torch.float32)
+        cast = [t.detach().to(T).requires_grad_() for t in (x, lin.weight, lin.bias)]
+        want = rq.linear_act(*cast, "silu", res)
+        assert torch.equal(y, want)
+        dy = torch.randn(3, 9, 40, generator=g).to(dev).to(y.dtype)
+        for p, q in zip(torch.autograd.grad(y, (x, lin.weight, lin.bias), dy),
+                        torch.autograd.grad(want, cast, dy)):
+            assert p.dtype == torch.float32 and torch.equal(p, q.float())
+    with torch.autocast("cuda", dtype=T, enabled=False):
+        assert m(x).dtype == torch.float32
