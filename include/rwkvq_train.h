@@ -98,7 +98,7 @@ int rq_embed(const void* idx, int idx_bytes, int64_t n, const void* table, rq_dt
  * with idx[i] == v, every row written (0 where no index points, and for
  * padding_idx; -1: none).  Indices outside [0, vocab) are left out.  dout [n,
  * dim] and dtable in dt.  The rows of one token are added in fp32, in an order
- * that depends on the sizes only.  n and vocab below 2^31. */
+ * that depends on the sizes only.  n below 2^31, vocab at most 2^30. */
 int64_t rq_embed_grad_workspace_bytes(int64_t n, int64_t vocab, int64_t dim);
 int rq_embed_grad(const void* idx, int idx_bytes, int64_t n, const void* dout, rq_dtype dt,
                   int64_t vocab, int64_t dim, float scale, int64_t padding_idx, void* dtable,

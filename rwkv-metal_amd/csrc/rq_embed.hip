@@ -42,6 +42,7 @@ RQ_DEV int64_t index_at(const void* idx, bool wide, int64_t i) {
 
 constexpr int kBlock = 256;
 constexpr int kRowLoads = 4;  // 16-byte loads a lane has in flight
+constexpr int64_t kLookupRows = 1 << 25;  // of one launch: a grid holds fewer than 2^32 threads, 64 of them a row
 
 // A wave takes kRowLoads * 64 vectors of one row.
 template <int DT>
@@ -81,6 +82,7 @@ constexpr int kSortBlock = 64 * kSortWaves;
 constexpr int kMinSortBlocks = 256;  // one for each CU; a power of two
 constexpr int kMaxIds = 512;         // ids of one block: 16 waves * 512 counters of LDS, 32 KB
 constexpr int kScan = 16;            // index loads of a lane in flight
+constexpr int64_t kMaxVocab = 1 << 30;  // 2^21 sort blocks of 1024 threads: a grid holds fewer than 2^32
 constexpr int kMaxShares = 1024;
 constexpr int kMaxDim = 65535 * 256;  // blockIdx.y counts columns by 256 and more
 
@@ -405,19 +407,23 @@ int rq_embed(const void* idx, int idx_bytes, int64_t n, const void* table, rq_dt
     if (!some) return rq::ok();
     const int64_t per = (int64_t)kRowLoads * 64 * (dt == RQ_F32 ? 4 : 8);
     const int64_t segs = (dim + per - 1) / per;
-    const int64_t blocks = (n + kBlock / 64 - 1) / (kBlock / 64);
-    if (blocks > INT32_MAX) return rq::fail(RQ_EINVAL, "rq_embed: too many indices");
     const bool wide = idx_bytes == 8;
-    RQ_DISPATCH_DT(dt, DT, embed_kernel<DT><<<dim3((unsigned)blocks, (unsigned)segs), kBlock, 0, (hipStream_t)stream>>>(
-                               idx, wide, n, (const uint8_t*)table, vocab, dim, scale, (uint8_t*)out));
-    return rq::launch_status(hipGetLastError(), "rq_embed");
+    hipError_t e = hipSuccess;
+    for (int64_t i = 0; i < n && e == hipSuccess; i += kLookupRows) {
+        const int64_t count = std::min(n - i, kLookupRows), blocks = (count + kBlock / 64 - 1) / (kBlock / 64);
+        RQ_DISPATCH_DT(dt, DT, embed_kernel<DT><<<dim3((unsigned)blocks, (unsigned)segs), kBlock, 0, (hipStream_t)stream>>>(
+                                   (const uint8_t*)idx + i * idx_bytes, wide, count, (const uint8_t*)table, vocab, dim,
+                                   scale, (uint8_t*)out + i * dim * kSize<DT>));
+        e = hipGetLastError();
+    }
+    return rq::launch_status(e, "rq_embed");
 }
 
 int64_t rq_embed_grad_workspace_bytes(int64_t n, int64_t vocab, int64_t dim) {
     if (n < 0 || vocab < 0 || dim < 0)
         return rq::fail(RQ_EINVAL, "rq_embed_grad_workspace_bytes: negative size");
-    if (n > INT32_MAX || vocab > INT32_MAX || dim > kMaxDim)
-        return rq::fail(RQ_EINVAL, "rq_embed_grad_workspace_bytes: n and vocab must be below 2^31, dim at most %d",
+    if (n > INT32_MAX || vocab > kMaxVocab || dim > kMaxDim)
+        return rq::fail(RQ_EINVAL, "rq_embed_grad_workspace_bytes: n must be below 2^31, vocab at most 2^30, dim at most %d",
                         kMaxDim);
     rq::ok();
     return vocab == 0 || dim == 0 ? 0 : (int64_t)work_bytes(n, dim, sort_plan(n, vocab));
@@ -428,7 +434,8 @@ int rq_embed_grad(const void* idx, int idx_bytes, int64_t n, const void* dout, r
                   int64_t workspace_bytes, void* stream) {
     if (int rc = check_embed("rq_embed_grad", idx, idx_bytes, n, dout, dt, vocab, dim, dtable, vocab > 0 && dim > 0))
         return rc;
-    if (n > INT32_MAX || vocab > INT32_MAX) return rq::fail(RQ_EINVAL, "rq_embed_grad: n and vocab must be below 2^31");
+    if (n > INT32_MAX || vocab > kMaxVocab)
+        return rq::fail(RQ_EINVAL, "rq_embed_grad: n must be below 2^31, vocab at most 2^30");
     if (vocab == 0 || dim == 0) return rq::ok();
     const SortPlan p = sort_plan(n, vocab);
     if (!workspace || workspace_bytes < (int64_t)work_bytes(n, dim, p))

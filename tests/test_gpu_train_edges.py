@@ -254,3 +254,15 @@ def test_linear_act_under_autocast(rq, dev, to):
             assert p.dtype == torch.float32 and torch.equal(p, q.float())
     with torch.autocast("cuda", dtype=T, enabled=False):
         assert m(x).dtype == torch.float32
+
+
+# --------------------------------------------------------------- embedding
+
+def test_lookup_of_more_rows_than_a_grid_holds(rq, dev):
+    """2^26 + 5 tokens: 64 threads each are past the 2^32 of one launch."""
+    n = 2 ** 26 + 5
+    idx = torch.arange(n, dtype=torch.int32, device=dev) % 251
+    w = torch.arange(251 * 8, device=dev).view(251, 8).to(torch.bfloat16)
+    out = rq.embedding(idx, w)
+    for a in range(0, n, 2 ** 23):
+        assert torch.equal(out[a:a + 2 ** 23], w[idx[a:a + 2 ** 23].long()])

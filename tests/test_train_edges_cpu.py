@@ -157,3 +157,9 @@ def test_only_what_the_gradients_read_is_kept_by_the_recorded_op(rq):
         y, ts = kept(lambda: rq.linear_act(x, w, b))
         assert {tuple(t.shape) for t in ts} == shapes - {(6, 5)}
         torch.autograd.grad(y, needs[:1], meta(6, 5))
+
+
+def test_the_largest_vocabulary_of_a_table_gradient(L):
+    assert L.rq_embed_grad_workspace_bytes(1, 2 ** 30, 8) > 0
+    assert L.rq_embed_grad_workspace_bytes(1, 2 ** 30 + 1, 8) == -1 and "2^30" in err(L)
+    assert L.rq_embed_grad(P, 8, 1, P, 0, 2 ** 30 + 1, 8, 1.0, -1, P, P, 1 << 40, None) == -1 and "2^30" in err(L)
