@@ -559,7 +559,7 @@ struct Direct : Side<DT, T, R> {
     // chunk i of a wave to LDS at `lds` (the wave's first byte of it)
     RQ_DEV void fetch(uint32_t lds, int i) const {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                     :: "s"(lds), "v"(this->off[i]), "s"(this->p) : "memory");
+                     :: "s"(lds), "v"(this->off[i]), "s"(this->p) : "memory", "m0");
     }
     // the same of a stage `left` contraction elements long: what is past them comes from a line of zeros
     RQ_DEV void fetch_part(uint32_t lds, int i, int left) const {
@@ -567,7 +567,7 @@ struct Direct : Side<DT, T, R> {
         S::place(i, r, c);
         const uint8_t* q = c < left ? this->p + this->off[i] : (const uint8_t*)&kZero16;
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                     :: "s"(lds), "v"(q) : "memory");
+                     :: "s"(lds), "v"(q) : "memory", "m0");
     }
 };
 
@@ -708,8 +708,15 @@ __global__ __launch_bounds__(kBlock, OCC) void dense_direct(const rq::DenseArgs 
             move();
         }
         sync(Count<0>{});
-        // the last products' results, of which the compiler knows no latency
-        if constexpr (MT * NT == 64) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+        if constexpr (MT * NT == 64) {
+            // the compiler knows no latency of the last products: a wait, and every sum
+            // passes through an asm behind it, so that none is read before
+            asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+            for (int p = 0; p < MT; ++p)
+#pragma unroll
+                for (int q = 0; q < NT; ++q) asm volatile("" : "+a"(acc[p][q]));
+        }
     }
     tile_out<DT, MT, NT>(g, acc, (float*)lds + wave * kOutRows<WM, WN> * (WN + 4), i0 + wm, j0 + wn, part);
 }
