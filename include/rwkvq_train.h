@@ -49,8 +49,8 @@ enum { RQ_SLOPE_NONE = 0, RQ_SLOPE_Y = 1, RQ_SLOPE_BOUND16 = 2, RQ_SLOPE_F32 = 3
 /* The form of the slope for operands of type dt.  RQ_SLOPE_Y where y alone gives
  * it: relu, and relu2 of fp32, with no residual added.  For bf16 operands 16 bits
  * that keep three bits more than bf16 where float16 is normal and bf16's elsewhere:
- * RQ_SLOPE_BOUND16 of slopes s below 2: the sign and the float16 bits of |s| >= 2^-14,
- * else the sign and 0x4000 + the bf16 bits of |s| (NaN: 0x7fff);
+ * RQ_SLOPE_BOUND16 of slopes s below 2: the float16 bits of s, or where |s| < 2^-14 its
+ * sign and 0x4000 + the bf16 bits of |s| (a 0 may have either);
  * RQ_SLOPE_WIDE16 of relu2, whose slope 2 v is not bounded but has no sign: the
  * float16 bits of a slope in [2^-14, 2^15), else 0x8000 + its bf16 bits.  float32
  * otherwise.

@@ -20,7 +20,8 @@ RQ_DEV float exp_neg(float x) {
 // (v_rcp_f32, one unit in the last place) serve both: the output stage of a large
 // tile runs one wave to a SIMD, where their instructions are felt (x [4096, 2048],
 // w [8192, 2048] with slopes: library expf, erff and divisions 179 us with silu and
-// 228 with gelu, these 156 and 158, no activation 114).  `act` is the same in every lane, so the switch is a scalar branch.
+// 228 with gelu, these 158 and 155; tanh 171, relu2 134, no activation 114).  `act` is
+// the same in every lane, so the switch is a scalar branch.
 //   sigmoid  e = exp(-|v|), r = 1 / (1 + e):  r or e r,  slope e r^2, which keep their
 //            relative precision where the function has saturated
 //   tanh     e = exp(-2 |v|):  +-(1 - e) r,  slope 4 e r^2;  below 1/4, where 1 - e
@@ -51,9 +52,11 @@ RQ_DEV void act_both(int act, float v, float& a, float& s) {
             return;
         }
         case RQ_ACT_GELU: {
-            const float x = fabsf(v) < 16.f ? fabsf(v) : 16.f;  // past it the tail is 0; an infinite v^2 has no rounding error
-            const float h = x * x, l = __builtin_fmaf(x, x, -h);
-            const float e = exp_neg(-0.5f * h) * __builtin_fmaf(l, -0.5f, 1.f);
+            const float x = __builtin_amdgcn_fmed3f(fabsf(v), 0.f, 16.f);  // past 16 the tail is 0
+            // exp(-x^2 / 2) = 2^-(x c x), the rounding errors of both products in l
+            const float p = x * 0.721347520f, h = p * x;
+            const float l = __builtin_fmaf(x, __builtin_fmaf(x, 0.721347520f, -p) + x * 9.62981495e-9f, __builtin_fmaf(p, x, -h));
+            const float e = __builtin_amdgcn_exp2f(-h) * __builtin_fmaf(l, -0.693147181f, 1.f);
             const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(x, 0.35f, 1.f));
             float q = __builtin_fmaf(t, -0.029163115f, 0.14405745f);
             q = __builtin_fmaf(t, q, -0.25589612f);
@@ -132,21 +135,25 @@ RQ_DEV f32x4_t act_slope4(int act, f32x4_t v) {
     }
 }
 
-// RQ_SLOPE_BOUND16: a slope |s| < 2 - 2^-11 in 16 bits, of which float16 needs the codes
-// below 0x4000 only.  A saturated sigmoid's or tanh's slope goes far below 2^-14,
-// where float16 loses bits (from |v| = 10 and 5 on) and then everything (17.5 and 9.4):
-// there the codes from 0x4000 on hold bf16's bits.
+// RQ_SLOPE_BOUND16: a slope |s| < 2 - 2^-11 in 16 bits: its float16 bits, of which no such
+// slope needs the codes 0x4000 - 0x7bff.  A saturated sigmoid's or tanh's slope goes far
+// below 2^-14, where float16 loses bits (from |v| = 10 and 5 on) and then everything
+// (17.5 and 9.4): those codes hold its bf16 bits.
 RQ_DEV uint32_t bound16_bits(float s) {
-    const uint32_t m = __float_as_uint(s) & 0x7fffffffu, sign = __float_as_uint(s) >> 16 & 0x8000u;
-    const float a = __uint_as_float(m);
-    uint32_t c = m < 0x38800000u ? f32_to_bf16_bits(a) + 0x4000u : f32_to_f16_bits(a);
-    if (m >= 0x40000000u) c = 0x7fffu;  // NaN: finite sums have no such slope
-    return c | sign;
+    return fabsf(s) < 6.103515625e-05f ? (f32_to_bf16_bits(s) + 0x4000u) & 0xffffu : f32_to_f16_bits(s);
+}
+// Two of them, without a branch: the output stage feels every instruction.
+RQ_DEV uint32_t bound16_pair(float s0, float s1) {
+    typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+    const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2_t, pack_bf16x2(s0, s1)) + (uint16_t)0x4000);
+    const uint32_t lo = fabsf(s0) < 6.103515625e-05f ? b : f32_to_f16_bits(s0);
+    const uint32_t hi = fabsf(s1) < 6.103515625e-05f ? b : f32_to_f16_bits(s1) << 16;
+    return (lo & 0xffffu) | (hi & 0xffff0000u);
 }
 RQ_DEV float bound16_value(uint32_t b) {
     const uint32_t c = b & 0x7fffu;
-    const float a = c < 0x4000u ? f16_bits_to_f32(c) : bf16_bits_to_f32(c == 0x7fffu ? c : c - 0x4000u);
-    return __uint_as_float(__float_as_uint(a) | (b & 0x8000u) << 16);
+    if (c < 0x4000u || c >= 0x7c00u) return f16_bits_to_f32(b);
+    return __uint_as_float((b & 0x8000u) << 16 | (c - 0x4000u) << 16);
 }
 
 // RQ_SLOPE_WIDE16: a slope s >= 0 in 16 bits, float16 in [2^-14, 2^15), where that
@@ -160,8 +167,11 @@ RQ_DEV float wide16_value(uint32_t b) {
     return b & 0x8000u ? bf16_bits_to_f32(b & 0x7fffu) : f16_bits_to_f32(b);
 }
 
-// The bits of a slope of `act` in 16, and the slope.
+// The 16 bits of a slope of `act`, and of two.
 RQ_DEV uint32_t slope16_bits(int act, float s) { return act == RQ_ACT_RELU2 ? wide16_bits(s) : bound16_bits(s); }
+RQ_DEV uint32_t slope16_pair(int act, float s0, float s1) {
+    return act == RQ_ACT_RELU2 ? wide16_bits(s0) | wide16_bits(s1) << 16 : bound16_pair(s0, s1);
+}
 
 // act'(v) from y = act(v): relu and relu2 only (relu2: v = sqrt(y)).
 RQ_DEV float act_slope_of_y(int act, float y) {

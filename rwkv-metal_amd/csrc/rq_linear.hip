@@ -353,8 +353,8 @@ RQ_DEV void out_rows(const rq::DenseArgs& g, const float* own, int64_t i0, int64
                     u32x4_t w;
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        w[e] = slope16_bits(ACT, sl[2 * e]) | (slope16_bits(ACT, sl[2 * e + 1]) << 16);
-                        w[e + 2] = slope16_bits(ACT, sh[2 * e]) | (slope16_bits(ACT, sh[2 * e + 1]) << 16);
+                        w[e] = slope16_pair(ACT, sl[2 * e], sl[2 * e + 1]);
+                        w[e + 2] = slope16_pair(ACT, sh[2 * e], sh[2 * e + 1]);
                     }
                     *(Bytes16*)((uint16_t*)g.slope + at + u * step) = Bytes16{{w[0], w[1], w[2], w[3]}};
                 } else {
@@ -384,8 +384,8 @@ RQ_DEV void tile_out(const rq::DenseArgs& g, const f32x4_t (&acc)[MT][NT], float
                      float* part) {
     constexpr int WM = MT * 16, WN = NT * 16;
     constexpr int ROWS = kOutRows<WM, WN>, P = WN + 4, LPR = WN / 8;
-    // small tiles leave the registers to more blocks
-    constexpr int BATCH = MT * NT >= 16 ? 4 : 2;
+    // four rows together: the same with a residual, tanh 181 us instead of 171 (4096 x 2048 x 8192 with slopes)
+    constexpr int BATCH = 2;
     static_assert(ROWS % (BATCH * (64 / LPR)) == 0, "rows of LDS are read in whole batches");
     static_assert(WM / ROWS <= 2, "");
     const int lane = threadIdx.x & 63;
