@@ -23,6 +23,7 @@
 
 #include "rq_common.h"
 #include "rq_error.h"
+#include "rq_vec.h"
 #include "../../include/rwkvq_train.h"
 
 namespace {
@@ -67,63 +68,33 @@ RQ_DEV Piece piece_of(const ClipList& l, uint32_t chunk) {
     return p;
 }
 
-// Values of 16 bytes of type DT as fp32.
-template <int DT>
-RQ_DEV void unpack16(const uint4& v, float* f) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    if constexpr (DT == RQ_F32) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[2 * i] = dt_traits<DT>::to_f32((uint16_t)(w[i] & 0xffffu));
-            f[2 * i + 1] = dt_traits<DT>::to_f32((uint16_t)(w[i] >> 16));
-        }
-    }
-}
-
-template <int DT>
-RQ_DEV uint4 pack16(const float* f) {
-    if constexpr (DT == RQ_F32)
-        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                          __float_as_uint(f[3]));
-    uint32_t w[4];
-    if constexpr (DT != RQ_F32) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = DT == RQ_BF16 ? pack_bf16x2(f[2 * i], f[2 * i + 1])
-                                 : (f32_to_f16_bits(f[2 * i]) | (f32_to_f16_bits(f[2 * i + 1]) << 16));
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 constexpr int kLoads = kChunkBytes / 16 / kBlock;
+
+// The thread's vectors of a chunk, all their loads in flight; 16 bytes at any
+// element alignment, so that a view behind an odd-sized one runs the same path.
+RQ_DEV void load_chunk(const Piece& p, int nv, Bytes16 (&v)[kLoads]) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int k = threadIdx.x + i * kBlock;
+        v[i] = k < nv ? ((const Bytes16*)p.g)[k] : Bytes16{{0u, 0u, 0u, 0u}};
+    }
+}
 
 template <int DT>
 RQ_DEV double chunk_squares(const Piece& p) {
-    constexpr int E = DT == RQ_F32 ? 4 : 8;  // elements of 16 bytes
+    constexpr int E = kVec<DT>;
     double s = 0.0;
-    const int tid = threadIdx.x;
-    int64_t done = 0;
-    if (((uintptr_t)p.g & 15) == 0) {
-        const int nv = (int)(p.n / E);
-        uint4 v[kLoads];
+    const int nv = (int)(p.n / E);
+    Bytes16 v[kLoads];
+    load_chunk(p, nv, v);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int c = tid + i * kBlock;
-            v[i] = c < nv ? ((const uint4*)p.g)[c] : make_uint4(0, 0, 0, 0);
-        }
+    for (int i = 0; i < kLoads; ++i) {
+        float f[E];
+        unpack_vec<DT>(v[i], f);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            float f[E];
-            unpack16<DT>(v[i], f);
-#pragma unroll
-            for (int j = 0; j < E; ++j) s = __builtin_fma((double)f[j], (double)f[j], s);
-        }
-        done = (int64_t)nv * E;
+        for (int j = 0; j < E; ++j) s = __builtin_fma((double)f[j], (double)f[j], s);
     }
-    for (int64_t i = done + tid; i < p.n; i += kBlock) {
+    for (int64_t i = (int64_t)nv * E + threadIdx.x; i < p.n; i += kBlock) {
         const double f = load_dt(p.g, DT, i);
         s = __builtin_fma(f, f, s);
     }
@@ -132,30 +103,21 @@ RQ_DEV double chunk_squares(const Piece& p) {
 
 template <int DT>
 RQ_DEV void chunk_scale(const Piece& p, float c) {
-    constexpr int E = DT == RQ_F32 ? 4 : 8;
-    const int tid = threadIdx.x;
-    int64_t done = 0;
-    if ((((uintptr_t)p.g | (uintptr_t)p.out) & 15) == 0) {
-        const int nv = (int)(p.n / E);
-        uint4 v[kLoads];
+    constexpr int E = kVec<DT>;
+    const int nv = (int)(p.n / E);
+    Bytes16 v[kLoads];
+    load_chunk(p, nv, v);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int k = tid + i * kBlock;
-            if (k < nv) v[i] = ((const uint4*)p.g)[k];
-        }
+    for (int i = 0; i < kLoads; ++i) {
+        const int k = threadIdx.x + i * kBlock;
+        if (k >= nv) break;
+        float f[E];
+        unpack_vec<DT>(v[i], f);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int k = tid + i * kBlock;
-            if (k >= nv) break;
-            float f[E];
-            unpack16<DT>(v[i], f);
-#pragma unroll
-            for (int j = 0; j < E; ++j) f[j] *= c;
-            ((uint4*)p.out)[k] = pack16<DT>(f);
-        }
-        done = (int64_t)nv * E;
+        for (int j = 0; j < E; ++j) f[j] *= c;
+        store_vec<DT>(p.out + (int64_t)k * 16, f);
     }
-    for (int64_t i = done + tid; i < p.n; i += kBlock)
+    for (int64_t i = (int64_t)nv * E + threadIdx.x; i < p.n; i += kBlock)
         store_dt(p.out, DT, i, load_dt(p.g, DT, i) * c);
 }
 

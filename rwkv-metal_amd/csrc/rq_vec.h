@@ -17,9 +17,9 @@ constexpr int kVec = DT == RQ_F32 ? 4 : 8;  // elements of 16 bytes
 template <int DT>
 constexpr int kSize = DT == RQ_F32 ? 4 : 2;
 
+// Its values as fp32.
 template <int DT>
-RQ_DEV void load_vec(const uint8_t* p, float* f) {
-    const Bytes16 v = *(const Bytes16*)p;
+RQ_DEV void unpack_vec(const Bytes16& v, float* f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (DT == RQ_F32) {
@@ -29,6 +29,11 @@ RQ_DEV void load_vec(const uint8_t* p, float* f) {
             f[2 * i + 1] = dt_traits<DT>::to_f32((uint16_t)(v.w[i] >> 16));
         }
     }
+}
+
+template <int DT>
+RQ_DEV void load_vec(const uint8_t* p, float* f) {
+    unpack_vec<DT>(*(const Bytes16*)p, f);
 }
 
 template <int DT>
