@@ -300,7 +300,10 @@ int order_scaling(const char* what, const rq_grad* grads, int64_t count, Scaling
     outs.reserve((size_t)count);
     for (int64_t i = 0; i < count; ++i)
         if (grads[i].n > 0) outs.push_back(out_of(i));
-    std::sort(outs.begin(), outs.end(), [](const Span& a, const Span& b) { return a.b != b.b ? a.b < b.b : a.i < b.i; });
+    const auto before = [](const Span& a, const Span& b) { return a.b != b.b ? a.b < b.b : a.i < b.i; };
+    // gradients are often allocated from the last parameter to the first; 288 tensors in no order sort in 7 us
+    if (!sorted && outs.front().b > outs.back().b) std::reverse(outs.begin(), outs.end());
+    if (!std::is_sorted(outs.begin(), outs.end(), before)) std::sort(outs.begin(), outs.end(), before);
     std::vector<uint8_t> again;  // entries that repeat another one
     size_t kept = 0;
     for (const Span& o : outs) {
@@ -320,14 +323,19 @@ int order_scaling(const char* what, const rq_grad* grads, int64_t count, Scaling
     std::vector<uint8_t> late;  // entries whose output another entry reads
     if (!apart) {
         std::vector<std::pair<int64_t, int64_t>> reads;  // (entry, the entry whose output it reads)
+        auto o = outs.begin();  // the first output that ends past the gradient: mostly the last one's or the next
         for (int64_t i = 0; i < count; ++i) {
             if (grads[i].n == 0 || grads[i].g == grads[i].out) continue;  // in place: no other output is there
             const uintptr_t b = (uintptr_t)grads[i].g, e = b + (uintptr_t)bytes_of(grads[i]);
-            auto o = std::upper_bound(outs.begin(), outs.end(), b, [](uintptr_t at, const Span& s) { return at < s.e; });
-            for (; o != outs.end() && o->b < e; ++o) {
+            const bool here = (o == outs.begin() || o[-1].e <= b) && (o == outs.end() || b < o->e);
+            const bool next = !here && o != outs.end() && o->e <= b && (o + 1 == outs.end() || b < o[1].e);
+            if (next) ++o;
+            else if (!here)
+                o = std::upper_bound(outs.begin(), outs.end(), b, [](uintptr_t at, const Span& s) { return at < s.e; });
+            for (auto w = o; w != outs.end() && w->b < e; ++w) {
                 if (late.empty()) late.assign((size_t)count, 0);
-                late[o->i] = 1;
-                reads.emplace_back(i, o->i);
+                late[w->i] = 1;
+                reads.emplace_back(i, w->i);
             }
         }
         for (const auto& [reader, writer] : reads)
