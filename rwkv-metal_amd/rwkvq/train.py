@@ -482,6 +482,16 @@ class ScaledEmbedding(nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx, device=device, dtype=dtype)
         self.scale = scale
 
+    @classmethod
+    def from_pretrained(cls, embeddings: Tensor, freeze: bool = True, padding_idx: Optional[int] = None,
+                        scale: float = 1.0) -> "ScaledEmbedding":
+        """The module over a table that is there (shared, not copied)."""
+        if embeddings.dim() != 2:
+            raise ValueError("embedding expects a 2-D table")
+        m = cls(*embeddings.shape, scale=scale, padding_idx=padding_idx, device="meta", dtype=embeddings.dtype)
+        m.weight = nn.Parameter(embeddings, requires_grad=not freeze)
+        return m
+
     def forward(self, idx: Tensor) -> Tensor:
         return embedding(idx, self.weight, self.scale, self.padding_idx)
 
@@ -633,7 +643,8 @@ def clip_grad_norm_(parameters, max_norm: float, eps: float = 1e-6) -> Tensor:
     the norm over them, a float32 scalar on the GPU; parameters without a
     gradient are left out.  Nothing is written where the norm is within
     max_norm.  A gradient listed twice (tied weights) counts twice in the norm and is
-    scaled once; gradients that overlap otherwise are refused."""
+    scaled once; gradients that overlap otherwise are refused.  The gradients are
+    written through their memory: autograd's version counters do not see it."""
     if isinstance(parameters, Tensor):
         parameters = [parameters]
     grads = [g for g in (p.grad for p in parameters) if g is not None]

@@ -163,3 +163,14 @@ def test_the_largest_vocabulary_of_a_table_gradient(L):
     assert L.rq_embed_grad_workspace_bytes(1, 2 ** 30, 8) > 0
     assert L.rq_embed_grad_workspace_bytes(1, 2 ** 30 + 1, 8) == -1 and "2^30" in err(L)
     assert L.rq_embed_grad(P, 8, 1, P, 0, 2 ** 30 + 1, 8, 1.0, -1, P, P, 1 << 40, None) == -1 and "2^30" in err(L)
+
+
+def test_embedding_over_a_table_that_is_there(rq):
+    """The constructor of nn.Embedding that the module inherits."""
+    t = torch.randn(10, 4, dtype=torch.bfloat16)
+    e = rq.ScaledEmbedding.from_pretrained(t, padding_idx=-1, scale=3.0)
+    assert type(e) is rq.ScaledEmbedding and e.scale == 3.0 and e.padding_idx == 9
+    assert e.weight.data_ptr() == t.data_ptr() and not e.weight.requires_grad
+    assert rq.ScaledEmbedding.from_pretrained(t, freeze=False).weight.requires_grad
+    with pytest.raises(ValueError, match="2-D"):
+        rq.ScaledEmbedding.from_pretrained(t[0])
