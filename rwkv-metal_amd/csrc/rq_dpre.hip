@@ -3,6 +3,11 @@
 //
 //   g[i, j] = T(dy[i, j] * act'(v[i, j]))       db[j] = T(sum over i of dy act'(v))
 //
+// g is rounded to the operands' type T because the 16-bit matrix instructions of
+// the two products take it so: their results are off by 1.41 roundings of T instead of
+// one (bf16 0.0024 against 0.0017 of their norm).  g in two parts of T would
+// double both products, which take 227 of the 420 us of a 4096 x 2048 x 8192 step;
+// float32 operands keep all of g.  db adds the unrounded products.
 // Memory bound: dy and the slopes in, g out, one pass; the column sums ride along
 // in registers, from the unrounded products.  [4096, 8192] bf16 with 16-bit slopes,
 // 201 MB: 46 us, 4.4 TB/s (a copy reaches 5.1; blocks that walked down the rows of

@@ -191,7 +191,7 @@ __global__ __launch_bounds__(kSortBlock) void embed_sort_kernel(const void* __re
         total += less[w] + wsum[w];
     }
     if (me == mask && tid == 0) ws.count[0] = total;
-    // absent ids: their flag goes where the counts of wave 0 were read
+    // the counts become each wave's first places; which ids do not occur is kept beside them
     __shared__ uint8_t absent[kMaxIds];
     if (tid < ids) {
         absent[tid] = mine == 0;

@@ -28,13 +28,14 @@ struct DenseArgs {
     int slope_kind;        // RQ_SLOPE_BOUND16, _F32 or _WIDE16 where slope is set
 };
 
-constexpr int kDenseMaxSide = 65535 * 64;  // of m, n and k: grids count 64 rows in y
+// Of m, n and k.  Offsets from a tile's first element stay in 32 bits: 256 rows of 2
+// bytes or 128 of 4 an element, this long, are 2^31 bytes.
+constexpr int kDenseMaxSide = 1 << 22;
 
 hipError_t launch_dense(const DenseArgs& a, void* workspace, hipStream_t stream);
 int64_t dense_workspace_bytes(const DenseArgs& a);  // of a's sizes, type and orders
 
-
-// g = dy * act'(v) and db = its column sums (rq_linear_dpre).
+// g = dy * act'(v) and db = its column sums, the start of rq_linear_backward.
 struct DpreArgs {
     const void* dy;
     int y_dt;

@@ -553,6 +553,10 @@ struct Step {
     static constexpr bool FETCH = FETCH_;
 };
 
+// m0 is written for the loads and named as clobbered; that it is a register the
+// compiler reserves, which it warns of, is why it has to be named.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int DT, bool T, int R>
 struct Direct : Side<DT, T, R> {
     typedef Side<DT, T, R> S;
@@ -570,6 +574,7 @@ struct Direct : Side<DT, T, R> {
                      :: "s"(lds), "v"(q) : "memory", "m0");
     }
 };
+#pragma clang diagnostic pop
 
 // mma with its sums in the accumulation registers, where the 256 x 256 tile's fill
 // all 256: left to itself the compiler moves them between the two files, up to
@@ -904,7 +909,8 @@ hipError_t launch_lds(K* kernel, const rq::DenseArgs& a, const Plan& p, int bm, 
     return hipGetLastError();
 }
 
-// More than 64 KB of LDS has to be asked for, once a kernel and device.
+// More than 64 KB of LDS has to be asked for.  Asked on every launch: a record of
+// which device has been asked would have to be kept for each kernel.
 template <class K>
 hipError_t allow_lds(K* kernel, int lds) {
     return lds <= 64 * 1024 ? hipSuccess

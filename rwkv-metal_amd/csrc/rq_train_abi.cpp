@@ -20,7 +20,6 @@ int check_sizes(const char* what, int64_t m, int64_t n, int64_t k, int dt) {
     if (!valid_dt(dt)) return fail(RQ_EINVAL, "%s: unsupported dtype", what);
     if (m < 0 || n < 0 || k < 0)
         return fail(RQ_EINVAL, "%s: negative size (m=%lld n=%lld k=%lld)", what, (long long)m, (long long)n, (long long)k);
-    // grids count tiles of 64 rows in y, and offsets inside a tile stay in 32 bits
     if (m > rq::kDenseMaxSide || n > rq::kDenseMaxSide || k > rq::kDenseMaxSide)
         return fail(RQ_EINVAL, "%s: a size is more than %d", what, rq::kDenseMaxSide);
     return RQ_OK;

@@ -271,7 +271,8 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
     one, and the slope act'(v): read off y for relu
     (and float32 relu2) without a residual, else a tensor of its own, 16 bits with
     three more of them significant than bf16's (as many below 2^-14) beside bf16
-    operands and float32 beside others.  Its products take g = dy act'(v) rounded to the operands' type."""
+    operands and float32 beside others.  Its products take g = dy act'(v) rounded to the operands' type
+    (past 65504 an infinity beside float16)."""
     if activation not in _ACT_CODE:
         raise ValueError(f"activation must be one of {ACTIVATIONS} (got {activation!r})")
     _float(x, "x")
