@@ -1,0 +1,857 @@
+// rq_wkv7.hip -- the recurrence of RWKV-7's time mixing: over a sequence, its
+// gradients, and one token.
+//
+//   d_t = exp(-exp(w_t)),  S_t = S_{t-1} diag(d_t) + (S_{t-1} a_t) b_t^T + v_t k_t^T,  y_t = S_t r_t
+//
+// The tokens are taken in chunks of 16.  With the running sums L of log d within a
+// chunk (Lx without the token's own) and
+//   A~ = a e^Lx   R~ = r e^L   B~ = b e^-L   K~ = k e^-L   B^ = b e^(Lend - L)   K^ = k e^(Lend - L)
+//   Mab = strict(A~ B~^T)  Mak = strict(A~ K~^T)  Mrb = incl(R~ B~^T)  Mrk = incl(R~ K~^T)
+// (strict: below the diagonal, incl: with it) a chunk is
+//   SA = (1 - Mab)^-1 (A~ S^T + Mak V)      the rows S_{t-1} a_t
+//   Y  = R~ S^T + Mrb SA + Mrk V
+//   S' = S diag(e^Lend) + SA^T B^ + V^T K^
+// and its adjoint, from dY and dS' backwards in time, has the same form:
+//   dZ = (1 - Mab)^-T (B^ dS'^T + Mrb^T dY)
+//   dV = K^ dS'^T + Mak^T dZ + Mrk^T dY
+//   dS = dS' diag(e^Lend) + dZ^T A~ + dY^T R~
+// so that one kernel runs both, the second with its tokens in reverse order.
+// The other gradients take one chunk each and nothing of the others but the states:
+//   dr = e^L (dY S + dMrb B~ + dMrk K~)             dMrb = incl(dY SA^T), dMrk = incl(dY V^T)
+//   da = e^Lx (dZ S + dMab B~ + dMak K~)            dMab = strict(dZ SA^T), dMak = strict(dZ V^T)
+//   db = e^-L (e^Lend SA dS' + dMrb^T R~ + dMab^T A~), dk alike with V, dMrk, dMak
+//   dlog d_t: what of the loss passes token t's decay (grads_kernel).
+//
+// All products are fp32 MFMAs (v_mfma_f32_16x16x4_f32): the state lives in fp32 and
+// feeds itself for thousands of tokens.
+//
+// e^-L overflows where the decays of a chunk are strong.  Below 2^-32 over one
+// chunk (RWKV-7's own decays reach 2^-14) a chunk's pair matrices are formed by VALU from
+// e^(L_t - L_s), whose exponents are sums of the terms between s and t and never
+// positive; that also serves decays of 0.
+#include <algorithm>
+
+#include "rq_common.h"
+#include "rq_error.h"
+#include "rq_wkv7.h"
+
+namespace {
+
+using namespace rq;
+
+constexpr int kHead = RQ_WKV7_HEAD;
+constexpr int kChunk = RQ_WKV7_CHUNK;
+constexpr int kRow = kHead + 4;  // LDS row of a [16, 64] array: lanes 16 rows apart meet in no bank
+constexpr float kStrong = -32.f;  // log2 of the weakest product of decays that e^-L stands for
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2Log2e = 0.5287663729448977f;  // log2(log2 e)
+
+RQ_DEV f32x4_t mfma4(float a, float b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// Four steps of a contraction: lane (m = lane & 15, g = lane >> 4) holds A[m][4g + i] in
+// a[i] and B[4g + i][m] in b[i]; c[i] is C[4g + i][m].  A result is the next product's B as it lies.
+RQ_DEV f32x4_t mma16(const f32x4_t& a, const f32x4_t& b, f32x4_t c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = mfma4(a[i], b[i], c);
+    return c;
+}
+
+RQ_DEV float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// log2 of the decay: -exp(w) log2 e.
+RQ_DEV float log2_decay(float w) { return -exp2_hw(fmaf(w, kLog2e, kLog2Log2e)); }
+
+template <int CTRL>
+RQ_DEV float dpp(float x) {  // 0 where the row of 16 lanes ends
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kRowShl = 0x100, kRowShr = 0x110, kRowBcast = 0x150;
+
+// Over the 16 lanes of a row, in time: forwards lane m is token m, backwards 15 - m.
+template <bool REV>
+RQ_DEV float upto(float x) {  // the sum of the tokens up to and with the lane's own
+    constexpr int C = REV ? kRowShl : kRowShr;
+    x += dpp<C + 1>(x);
+    x += dpp<C + 2>(x);
+    x += dpp<C + 4>(x);
+    x += dpp<C + 8>(x);
+    return x;
+}
+template <bool REV>
+RQ_DEV float before(float x) {  // the previous token's value, 0 for the first
+    return dpp<(REV ? kRowShl : kRowShr) + 1>(x);
+}
+template <bool REV>
+RQ_DEV float of_last(float x) {  // the last token's value
+    return dpp<kRowBcast + (REV ? 0 : 15)>(x);
+}
+
+struct Span {
+    int64_t start, len, chunk0;  // first token (row of the flattened batch), tokens, first chunk
+    RQ_DEV int64_t chunks() const { return (len + kChunk - 1) / kChunk; }
+};
+
+RQ_DEV int64_t clamp_token(int32_t v, int64_t time) { return v < 0 ? 0 : (v > time ? time : v); }
+
+RQ_DEV Span span_of(const WkvShape& s, int64_t n) {
+    if (!s.cu) return {n * s.time, s.time, n * ((s.time + kChunk - 1) / kChunk)};
+    const int64_t from = clamp_token(s.cu[n], s.time), to = clamp_token(s.cu[n + 1], s.time);
+    return {from, to > from ? to - from : 0, from / kChunk + n};
+}
+
+// ------------------------------------------------------- operands of a chunk
+
+// The 16 channels from `ch` of a token's head, as they are stored.
+template <int DT>
+struct Raw {
+    uint4 v[DT == RQ_F32 ? 4 : 2];
+};
+template <int DT>
+RQ_DEV Raw<DT> load_raw(const void* p, int64_t at, bool there) {
+    Raw<DT> r;
+    const uint4* q = (const uint4*)((const uint8_t*)p + at * (DT == RQ_F32 ? 4 : 2));
+#pragma unroll
+    for (int i = 0; i < (DT == RQ_F32 ? 4 : 2); ++i) r.v[i] = there ? q[i] : make_uint4(0, 0, 0, 0);
+    return r;
+}
+template <int DT>
+RQ_DEV void unpack_raw(const Raw<DT>& r, float* f) {
+#pragma unroll
+    for (int i = 0; i < (DT == RQ_F32 ? 4 : 2); ++i) {
+        const uint32_t u[4] = {r.v[i].x, r.v[i].y, r.v[i].z, r.v[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == RQ_F32) {
+                f[4 * i + j] = __uint_as_float(u[j]);
+            } else {
+                f[8 * i + 2 * j] = dt_traits<DT>::to_f32((uint16_t)(u[j] & 0xffffu));
+                f[8 * i + 2 * j + 1] = dt_traits<DT>::to_f32((uint16_t)(u[j] >> 16));
+            }
+        }
+    }
+}
+
+// What the scan reads of a chunk.  Backwards the tensors change places: to_sa is B^, to_y K^,
+// from_sa A~, from_x R~, and the matrices are transposed.
+struct Chunk {
+    float to_sa[kChunk][kRow];    // A~
+    float to_y[kChunk][kRow];     // R~
+    float from_sa[kChunk][kRow];  // B^
+    float from_x[kChunk][kRow];   // K^
+    f32x4_t inv[64];              // (1 - Mab)^-1, [lane] as an A operand
+    f32x4_t sa_x[64];             // Mak
+    f32x4_t y_sa[64];             // Mrb
+    f32x4_t y_x[64];              // Mrk
+    float decay[kHead];           // e^Lend
+};
+
+// X^T of X = (1 - M)^-1 from m[i] = M^T[4g + i][lane & 15], nonzero above the diagonal:
+// rows from the last, X^T[s] = e_s + sum over u > s of M^T[s, u] X^T[u], four at a time.
+RQ_DEV f32x4_t unit_inverse(const f32x4_t& m, int lane) {
+    const int g = lane >> 4, col = lane & 15;
+    f32x4_t x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = 4 * g + i == col ? 1.f : 0.f;
+#define RQ_STEP(U, I, V) x[I] = fmaf(dpp<kRowBcast + U>(mm[I]), V, x[I])
+#define RQ_BLOCK(G)                                                                        \
+    {                                                                                      \
+        f32x4_t mm;                                                                        \
+        _Pragma("unroll") for (int i = 0; i < 4; ++i) mm[i] = g == G ? m[i] : 0.f;         \
+        RQ_STEP(4 * G + 3, 0, x[3]);                                                       \
+        RQ_STEP(4 * G + 3, 1, x[3]);                                                       \
+        RQ_STEP(4 * G + 3, 2, x[3]);                                                       \
+        RQ_STEP(4 * G + 2, 0, x[2]);                                                       \
+        RQ_STEP(4 * G + 2, 1, x[2]);                                                       \
+        RQ_STEP(4 * G + 1, 0, x[1]);                                                       \
+        if constexpr (G > 0) {                                                             \
+            f32x4_t rows;                                                                  \
+            _Pragma("unroll") for (int i = 0; i < 4; ++i) {                                \
+                rows[i] = __shfl(x[i], 16 * G + col);                                      \
+                mm[i] = g < G ? m[i] : 0.f;                                                \
+            }                                                                              \
+            _Pragma("unroll") for (int i = 0; i < 4; ++i) {                                \
+                RQ_STEP(4 * G + 3, i, rows[3]);                                            \
+                RQ_STEP(4 * G + 2, i, rows[2]);                                            \
+                RQ_STEP(4 * G + 1, i, rows[1]);                                            \
+                RQ_STEP(4 * G + 0, i, rows[0]);                                            \
+            }                                                                              \
+        }                                                                                  \
+    }
+    RQ_BLOCK(3)
+    RQ_BLOCK(2)
+    RQ_BLOCK(1)
+    RQ_BLOCK(0)
+#undef RQ_BLOCK
+#undef RQ_STEP
+    return x;
+}
+
+// One pair matrix of a chunk whose decays are too strong for e^-L: entry (t, s) is the sum over
+// the channels of late_t early_s e^(log d between them), the later token's own decay among them
+// unless `strict`.  Rows are the source's tokens, columns the target's, as mma16 leaves them.
+template <bool REV>
+__device__ __attribute__((noinline)) f32x4_t strong_pairs(const float* late, const float* early, const float* g2,
+                                                          bool strict, int lane) {
+    const int g = lane >> 4, m = lane & 15;
+    f32x4_t out = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < kChunk; ++s) {
+        float sum = 0.f;
+        const bool after = REV ? m < s : m > s;
+        for (int c = 0; c < 16; ++c) {
+            const float e = __shfl(early[c], 16 * g + s);
+            float between = upto<REV>(after ? g2[c] : 0.f);
+            if (strict) between = before<REV>(between);
+            sum += late[c] * e * exp2_hw(between);
+        }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if constexpr (REV) {  // the rows are the later tokens
+            for (int i = 0; i < 4; ++i) {
+                const float x = __shfl(sum, 4 * g + i);
+                if (m == s) out[i] = x;
+            }
+        } else {
+            for (int i = 0; i < 4; ++i)
+                if (4 * g + i == s) out[i] = sum;
+        }
+    }
+    return out;
+}
+
+// ------------------------------------------------------------------ the scan
+
+// Wave `pair` of four forms one of the matrices Mab, Mak / Mrb, Mrb / Mak, Mrk of a chunk, from
+// its two tensors, and one of the four arrays.  Lane (m, g): token m, channels 16g .. 16g + 15.
+template <int DT, bool REV>
+struct Producer {
+    int lane, pair;
+    const void *late_p, *early_p, *w_p;
+    Raw<DT> late, early, w;
+    bool there;
+
+    RQ_DEV Producer(const WkvScan& p, int lane_, int pair_) : lane(lane_), pair(pair_) {
+        const bool is_a = pair == 0 || pair == (REV ? 2 : 1), is_b = pair == 0 || pair == (REV ? 1 : 2);
+        late_p = is_a ? p.in.a : p.in.r;
+        early_p = is_b ? p.in.b : p.in.k;
+        w_p = p.in.w;
+    }
+    // `row`: the flattened row of the lane's token and head, where it exists
+    RQ_DEV void load(int64_t row, bool exists) {
+        there = exists;
+        const int64_t at = row * kHead + 16 * (lane >> 4);
+        late = load_raw<DT>(late_p, at, exists);
+        early = load_raw<DT>(early_p, at, exists);
+        w = load_raw<DT>(w_p, at, exists);
+    }
+    RQ_DEV static void store(float (*to)[kRow], const float* f, int lane) {
+        f32x4_t* at = (f32x4_t*)&to[lane & 15][16 * (lane >> 4)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at[i] = f32x4_t{f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]};
+    }
+    RQ_DEV void produce(Chunk& c) {
+        const bool strict = pair == 0 || pair == (REV ? 2 : 1);
+        float x[16], y[16], g2[16], l[16];
+        unpack_raw<DT>(late, x);
+        unpack_raw<DT>(early, y);
+        unpack_raw<DT>(w, g2);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            g2[i] = there ? log2_decay(g2[i]) : 0.f;
+            l[i] = upto<REV>(g2[i]);
+        }
+        bool strong = false;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) strong |= !(of_last<REV>(l[i]) >= kStrong);
+        strong = __any(strong);
+        f32x4_t m = {0.f, 0.f, 0.f, 0.f};
+        float hat[16];  // the earlier tensor times e^(Lend - L)
+        if (!strong) {
+            float late_s[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float end = of_last<REV>(l[i]);
+                late_s[i] = x[i] * exp2_hw(strict ? before<REV>(l[i]) : l[i]);
+                hat[i] = y[i] * exp2_hw(end - l[i]);
+                y[i] *= exp2_hw(-l[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = REV ? mfma4(late_s[i], y[i], m) : mfma4(y[i], late_s[i], m);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = late_s[i];
+        } else {
+            float late_m[16], early_m[16], g2_m[16];  // copies: those of the usual way stay in registers
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                late_m[i] = x[i];
+                early_m[i] = y[i];
+                g2_m[i] = g2[i];
+            }
+            m = strong_pairs<REV>(late_m, early_m, g2_m, strict, lane);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                hat[i] = y[i] * exp2_hw(before<!REV>(upto<!REV>(g2[i])));
+                x[i] *= exp2_hw(strict ? before<REV>(l[i]) : l[i]);
+            }
+        }
+        const int row = 4 * (lane >> 4), col = lane & 15;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = (strict ? row + i < col : row + i <= col) ? m[i] : 0.f;
+        // every array has one writer
+        if (pair == 0) store(REV ? c.from_sa : c.to_sa, x, lane);
+        if (pair == 3) store(REV ? c.from_x : c.to_y, x, lane);
+        if (pair == 1) store(REV ? c.to_sa : c.from_x, hat, lane);
+        if (pair == 2) store(REV ? c.to_y : c.from_sa, hat, lane);
+        if (pair == 0) c.inv[lane] = unit_inverse(m, lane);
+        if (pair == 1) c.sa_x[lane] = m;
+        if (pair == 2) c.y_sa[lane] = m;
+        if (pair == 3) {
+            c.y_x[lane] = m;
+            if (col == (REV ? 0 : 15)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) c.decay[4 * row + i] = exp2_hw(l[i]);
+            }
+        }
+    }
+};
+
+// Four producer waves prepare chunk c + 1 while TILES waves, each with 16 of the 64 values, take
+// chunk c.  A scan wave holds its state transposed, acc[q][i] = S[value lane & 15][key 16q + 4g + i]:
+// the layout in which a product's result comes and in which the next takes it.
+template <int DT, int XDT, int YDT, bool REV, int TILES>
+__global__ __launch_bounds__(64 * (4 + TILES)) void wkv7_scan_kernel(WkvScan p) {
+    __shared__ Chunk buf[2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = lane >> 4, m = lane & 15;
+    const int64_t pairs = p.shape.seqs * p.shape.heads;  // of a sequence and a head
+    const int64_t which = blockIdx.x % pairs;
+    const int64_t seq = which / p.shape.heads, head = which % p.shape.heads, H = p.shape.heads;
+    const Span span = span_of(p.shape, seq);
+    const int64_t n = span.chunks();
+    // the chunk's token of index i, i in processing order
+    const auto token = [&](int64_t c, int i) { return REV ? kChunk * (n - 1 - c) + (kChunk - 1 - i) : kChunk * c + i; };
+
+    if (wave < 4) {
+        // the wave that inverts shares its SIMD with no scan wave of TILES == 1
+        Producer<DT, REV> prod(p, lane, (wave + 1) & 3);
+        const auto load = [&](int64_t c) {
+            const int64_t t = token(c, m);
+            const bool exists = c < n && t < span.len;
+            prod.load((span.start + (exists ? t : 0)) * H + head, exists);
+        };
+        if (n > 0) {
+            load(0);
+            prod.produce(buf[0]);
+            load(1);
+        }
+        __syncthreads();
+        for (int64_t c = 0; c < n; ++c) {
+            if (c + 1 < n) {
+                prod.produce(buf[(c + 1) & 1]);
+                load(c + 2);
+            }
+            __syncthreads();
+        }
+        return;
+    }
+    const int value = 16 * ((int)(blockIdx.x / pairs) * TILES + wave - 4) + m;
+    const int64_t state_at = (which * kHead + value) * kHead + 4 * g;
+    f32x4_t acc[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        acc[q] = p.state ? *(const f32x4_t*)(p.state + state_at + 16 * q) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float x[4];
+    const auto load_x = [&](int64_t c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t t = token(c, 4 * g + i);
+            x[i] = c < n && t < span.len ? load_dt(p.x, XDT, ((span.start + t) * H + head) * kHead + value) : 0.f;
+        }
+    };
+    load_x(0);
+    __syncthreads();
+    for (int64_t c = 0; c < n; ++c) {
+        const Chunk& b = buf[c & 1];
+        const int64_t slot = (span.chunk0 + (REV ? n - 1 - c : c)) * H + head;
+        const f32x4_t v = {x[0], x[1], x[2], x[3]};
+        load_x(c + 1);
+        if (p.states) {
+            float* to = p.states + (slot * kHead + value) * kHead + 4 * g;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *(f32x4_t*)(to + 16 * q) = acc[q];
+        }
+        f32x4_t z = {0.f, 0.f, 0.f, 0.f}, sa = z, y = z;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z = mma16(*(const f32x4_t*)&b.to_sa[m][16 * q + 4 * g], acc[q], z);
+        z = mma16(b.sa_x[lane], v, z);
+        sa = mma16(b.inv[lane], z, sa);
+        if (p.y) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) y = mma16(*(const f32x4_t*)&b.to_y[m][16 * q + 4 * g], acc[q], y);
+            y = mma16(b.y_sa[lane], sa, y);
+            y = mma16(b.y_x[lane], v, y);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4_t d = *(const f32x4_t*)&b.decay[16 * q + 4 * g];
+            f32x4_t fs, fx;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[q][i] *= d[i];
+                fs[i] = b.from_sa[4 * g + i][16 * q + m];
+                fx[i] = b.from_x[4 * g + i][16 * q + m];
+            }
+            acc[q] = mma16(fx, v, acc[q]);
+            acc[q] = mma16(fs, sa, acc[q]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t t = token(c, 4 * g + i);
+            if (t < span.len && p.y) store_dt(p.y, YDT, ((span.start + t) * H + head) * kHead + value, y[i]);
+            // rows in the order of time, the missing ones 0
+            if (p.sa) p.sa[(slot * kChunk + (REV ? kChunk - 1 - (4 * g + i) : 4 * g + i)) * kHead + value] = sa[i];
+        }
+        __syncthreads();
+    }
+    if (p.state_out) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *(f32x4_t*)(p.state_out + state_at + 16 * q) = acc[q];
+    }
+}
+
+// ----------------------------------------------------------- the gradients
+
+// Over a lane's four tokens and the four lanes of its key: lane (m, g) holds tokens 4g + i.
+RQ_DEV float groups_before(float x, int g) {  // the sum over the groups before the lane's own
+    float a = __shfl_up(x, 16), b = __shfl_up(x, 32), c = __shfl_up(x, 48);
+    return (g > 0 ? a : 0.f) + (g > 1 ? b : 0.f) + (g > 2 ? c : 0.f);
+}
+RQ_DEV float groups_after(float x, int g) {
+    float a = __shfl_down(x, 16), b = __shfl_down(x, 32), c = __shfl_down(x, 48);
+    return (g < 3 ? a : 0.f) + (g < 2 ? b : 0.f) + (g < 1 ? c : 0.f);
+}
+RQ_DEV float over_groups(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+constexpr int kPairRow = 20;  // LDS row of a [16, 16] matrix
+
+struct GradLds {
+    float m[4][kChunk][kPairRow];       // dMab, dMak, dMrb, dMrk, [s][t], s < t
+    float own[2][kChunk];               // the diagonals of dMrb, dMrk
+    float strong[4][5][kChunk][16];     // r, a, b, k and log2 d of a wave's 16 keys
+};
+
+// The parts of the gradients that come from the pairs within a chunk of strong decays, for the
+// lane's key and tokens 4g + i: gr, ga, gb, gk, and in `cross` what of the loss passes each
+// token's decay.
+__device__ __attribute__((noinline)) void strong_grads(const GradLds& lds, int wave, int lane, float* gr, float* ga,
+                                                       float* gb, float* gk, float* cross) {
+    const int g = lane >> 4, key = lane & 15;
+    const auto& in = lds.strong[wave];
+    for (int i = 0; i < 4; ++i) {
+        const int own = 4 * g + i;
+        gr[i] = ga[i] = gb[i] = gk[i] = cross[i] = 0.f;
+        float e = in[4][own][key];  // log2 of the decay from s to own
+        for (int s = own - 1; s >= 0; --s) {
+            gr[i] += (lds.m[2][s][own] * in[2][s][key] + lds.m[3][s][own] * in[3][s][key]) * exp2_hw(e);
+            e += in[4][s][key];
+        }
+        e = 0.f;
+        for (int s = own - 1; s >= 0; --s) {
+            ga[i] += (lds.m[0][s][own] * in[2][s][key] + lds.m[1][s][own] * in[3][s][key]) * exp2_hw(e);
+            e += in[4][s][key];
+        }
+        e = 0.f;
+        for (int t = own + 1; t < kChunk; ++t) {
+            const float f = in[1][t][key] * exp2_hw(e);
+            e += in[4][t][key];
+            const float h = in[0][t][key] * exp2_hw(e);
+            gb[i] += lds.m[0][own][t] * f + lds.m[2][own][t] * h;
+            gk[i] += lds.m[1][own][t] * f + lds.m[3][own][t] * h;
+        }
+        for (int s = 0; s < own; ++s) {
+            e = 0.f;
+            for (int t = s + 1; t < kChunk; ++t) {
+                if (t > own)  // a's decays end before t
+                    cross[i] += in[1][t][key] * exp2_hw(e) *
+                                (lds.m[0][s][t] * in[2][s][key] + lds.m[1][s][t] * in[3][s][key]);
+                e += in[4][t][key];
+                if (t >= own)
+                    cross[i] += in[0][t][key] * exp2_hw(e) *
+                                (lds.m[2][s][t] * in[2][s][key] + lds.m[3][s][t] * in[3][s][key]);
+            }
+        }
+    }
+}
+
+// Four contiguous values of a row as fp32.
+template <int DT>
+RQ_DEV f32x4_t load4(const void* p, int64_t at, bool there) {
+    if (!there) return f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if constexpr (DT == RQ_F32) {
+        return *(const f32x4_t*)((const float*)p + at);
+    } else {
+        const uint2 u = *(const uint2*)((const uint16_t*)p + at);
+        return f32x4_t{dt_traits<DT>::to_f32((uint16_t)(u.x & 0xffffu)), dt_traits<DT>::to_f32((uint16_t)(u.x >> 16)),
+                       dt_traits<DT>::to_f32((uint16_t)(u.y & 0xffffu)), dt_traits<DT>::to_f32((uint16_t)(u.y >> 16))};
+    }
+}
+
+// A block is one chunk of one head; each of its four waves has 16 keys, and one of the four pair
+// matrices for all.  In products over the values a lane holds rows of tokens (A) and columns of
+// keys (B); the results, tokens 4g + i of key lane & 15, are where the gradients are formed.
+template <int DT, int YDT>
+__global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
+    __shared__ GradLds lds;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = lane >> 4, m = lane & 15;
+    const int64_t H = p.shape.heads, slot = blockIdx.x, head = slot % H, chunk = slot / H;
+    Span span;
+    if (p.shape.cu) {  // the last sequence that begins at this chunk or before
+        int64_t lo = 0, hi = p.shape.seqs;
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) / 2;
+            if (clamp_token(p.shape.cu[mid], p.shape.time) / kChunk + mid <= chunk) lo = mid;
+            else hi = mid;
+        }
+        span = span_of(p.shape, lo);
+    } else {
+        span = span_of(p.shape, chunk / ((p.shape.time + kChunk - 1) / kChunk));
+    }
+    const int64_t c = chunk - span.chunk0;
+    if (c < 0 || c >= span.chunks()) return;
+    const int64_t t0 = kChunk * c;
+
+    // rows of tokens: dy, dz, sa, v of token m, values 16q + 4g + i
+    const bool there = t0 + m < span.len;
+    const int64_t row = (span.start + t0 + m) * H + head;
+    f32x4_t dy[4], dz[4], sa[4], v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        dy[q] = load4<YDT>(p.dy, row * kHead + 16 * q + 4 * g, there);
+        v[q] = load4<DT>(p.in.v, row * kHead + 16 * q + 4 * g, there);
+        dz[q] = load4<RQ_F32>(p.dz, (slot * kChunk + m) * kHead + 16 * q + 4 * g, true);
+        sa[q] = load4<RQ_F32>(p.sa, (slot * kChunk + m) * kHead + 16 * q + 4 * g, true);
+    }
+    const int key = 16 * wave + m;
+    // this wave's tensors: tokens 4g + i of its key
+    float r[4], a[4], b[4], k[4], g2[4], l[4], w[4];
+    bool has[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t t = t0 + 4 * g + i, at = ((span.start + t) * H + head) * kHead + key;
+        has[i] = t < span.len;
+        r[i] = has[i] ? load_dt(p.in.r, DT, at) : 0.f;
+        a[i] = has[i] ? load_dt(p.in.a, DT, at) : 0.f;
+        b[i] = has[i] ? load_dt(p.in.b, DT, at) : 0.f;
+        k[i] = has[i] ? load_dt(p.in.k, DT, at) : 0.f;
+        w[i] = has[i] ? load_dt(p.in.w, DT, at) : 0.f;
+    }
+    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+    f32x4_t gr = zero, ga = zero, gb = zero, gk = zero;
+    float through = 0.f;  // sum over the values of S dS' of this key
+    const float* s_at = p.states + slot * kHead * kHead + key;
+    const float* d_at = p.dstates + slot * kHead * kHead + key;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        f32x4_t s, d;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[i] = s_at[(16 * q + 4 * g + i) * kHead];
+            d[i] = d_at[(16 * q + 4 * g + i) * kHead];
+            through = fmaf(s[i], d[i], through);
+        }
+        gr = mma16(dy[q], s, gr);
+        ga = mma16(dz[q], s, ga);
+        gb = mma16(sa[q], d, gb);
+        gk = mma16(v[q], d, gk);
+    }
+    through = over_groups(through);
+    {
+        f32x4_t pm = zero;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) pm = mma16((wave & 1) ? v[q] : sa[q], wave < 2 ? dz[q] : dy[q], pm);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = 4 * g + i;
+            lds.m[wave][s][m] = s < m ? pm[i] : 0.f;
+            if (wave >= 2 && s == m) lds.own[wave - 2][m] = pm[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        g2[i] = has[i] ? log2_decay(w[i]) : 0.f;
+        l[i] = i ? l[i - 1] + g2[i] : g2[i];
+    }
+    const float off = groups_before(l[3], g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l[i] += off;
+    const float end = __shfl(l[3], 48 + m);
+    const bool strong = __any(!(end >= kStrong));
+    if (strong) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            auto& in = lds.strong[wave];
+            in[0][4 * g + i][m] = r[i];
+            in[1][4 * g + i][m] = a[i];
+            in[2][4 * g + i][m] = b[i];
+            in[3][4 * g + i][m] = k[i];
+            in[4][4 * g + i][m] = g2[i];
+        }
+    }
+    __syncthreads();
+    float to_end[4], el[4], ex[4];  // e^(Lend - L), e^L, e^Lx
+    {
+        float after = groups_after((g2[0] + g2[1]) + (g2[2] + g2[3]), g);
+        float prev = off;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            el[i] = exp2_hw(l[i]);
+            ex[i] = exp2_hw(prev);
+            prev = l[i];
+        }
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {
+            to_end[i] = exp2_hw(after);
+            after += g2[i];
+        }
+    }
+    float enters[4], leaves_r[4], leaves_a[4];  // what each token adds to, and takes from, the state
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        gb[i] *= to_end[i];
+        gk[i] *= to_end[i];
+        gr[i] *= el[i];
+        ga[i] *= ex[i];
+        enters[i] = b[i] * gb[i] + k[i] * gk[i];
+        leaves_r[i] = r[i] * gr[i];
+        leaves_a[i] = a[i] * ga[i];
+    }
+    float cross[4];
+    if (strong) {
+        float pr[4], pa[4], pb[4], pk[4], pc[4];
+        strong_grads(lds, wave, lane, pr, pa, pb, pk, pc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            gr[i] += pr[i];
+            ga[i] += pa[i];
+            gb[i] += pb[i];
+            gk[i] += pk[i];
+            cross[i] = pc[i];
+        }
+    } else {
+        f32x4_t rs, as, bs, ks, pr = zero, pa = zero, pb = zero, pk = zero;
+        float il[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            il[i] = exp2_hw(-l[i]);
+            rs[i] = r[i] * el[i];
+            as[i] = a[i] * ex[i];
+            bs[i] = b[i] * il[i];
+            ks[i] = k[i] * il[i];
+        }
+        f32x4_t by_t[4], by_s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            by_s[j] = *(const f32x4_t*)&lds.m[j][m][4 * g];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) by_t[j][i] = lds.m[j][4 * g + i][m];
+        }
+        pa = mma16(by_t[0], bs, pa);
+        pa = mma16(by_t[1], ks, pa);
+        pr = mma16(by_t[2], bs, pr);
+        pr = mma16(by_t[3], ks, pr);
+        pb = mma16(by_s[0], as, pb);
+        pb = mma16(by_s[2], rs, pb);
+        pk = mma16(by_s[1], as, pk);
+        pk = mma16(by_s[3], rs, pk);
+        // a pair (s, t) passes the decays behind s up to t (before t, for a): sums of what ends
+        // minus what begins at each token and behind it
+        float q[4], qa[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            pr[i] *= el[i];
+            pa[i] *= ex[i];
+            pb[i] *= il[i];
+            pk[i] *= il[i];
+            q[i] = r[i] * pr[i] - b[i] * pb[i] - k[i] * pk[i];
+            qa[i] = a[i] * pa[i];
+            gr[i] += pr[i];
+            ga[i] += pa[i];
+            gb[i] += pb[i];
+            gk[i] += pk[i];
+        }
+        float sum = groups_after((q[0] + qa[0]) + (q[1] + qa[1]) + (q[2] + qa[2]) + (q[3] + qa[3]), g);
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {
+            cross[i] = sum + q[i];
+            sum += q[i] + qa[i];
+        }
+    }
+    // a token's own pair passes no decay: kept out of the sums above, where it would cancel
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float ob = lds.own[0][4 * g + i], ok = lds.own[1][4 * g + i];
+        gr[i] += ob * b[i] + ok * k[i];
+        gb[i] += ob * r[i];
+        gk[i] += ok * r[i];
+    }
+    // the state's own way through the chunk, what entered before and what leaves at or behind
+    const float whole = exp2_hw(end) * through;
+    float into = groups_before((enters[0] + enters[1]) + (enters[2] + enters[3]), g);
+    float out_of = groups_after((leaves_r[0] + leaves_a[0]) + (leaves_r[1] + leaves_a[1]) +
+                                    (leaves_r[2] + leaves_a[2]) + (leaves_r[3] + leaves_a[3]), g);
+    float gw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        gw[i] = cross[i] + whole + into;
+        into += enters[i];
+    }
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+        gw[i] += out_of + leaves_r[i];
+        out_of += leaves_r[i] + leaves_a[i];
+        // d log d / dw = -exp(w), inf where the decay, and with it what passes it, is 0
+        gw[i] = gw[i] == 0.f ? 0.f : gw[i] * (g2[i] * kLn2);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (!has[i]) continue;
+        const int64_t at = ((span.start + t0 + 4 * g + i) * H + head) * kHead + key;
+        if (p.dr) store_dt(p.dr, DT, at, gr[i]);
+        if (p.dw) store_dt(p.dw, DT, at, gw[i]);
+        if (p.dk) store_dt(p.dk, DT, at, gk[i]);
+        if (p.da) store_dt(p.da, DT, at, ga[i]);
+        if (p.db) store_dt(p.db, DT, at, gb[i]);
+    }
+}
+
+// ----------------------------------------------------------------- one token
+
+// A block is one head of one sequence: four lanes a row of the state, 16 keys each.
+template <int DT, int YDT>
+__global__ __launch_bounds__(256) void wkv7_step_kernel(WkvStep p) {
+    __shared__ float in[6][kHead];
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, value = tid >> 2, part = tid & 3;
+    f32x4_t s[4];
+    const int64_t at = (row * kHead + value) * kHead + 4 * part;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        s[j] = p.state ? *(const f32x4_t*)(p.state + at + 16 * j) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const void* const of[6] = {p.in.r, p.in.w, p.in.k, p.in.v, p.in.a, p.in.b};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int i = tid + 256 * j, which = i >> 6;
+        if (which < 6) {
+            const void* from = which == 0 ? of[0] : which == 1 ? of[1] : which == 2 ? of[2] : which == 3 ? of[3] : which == 4 ? of[4] : of[5];
+            const float x = load_dt(from, DT, row * kHead + (i & 63));
+            in[which][i & 63] = which == 1 ? exp2_hw(log2_decay(x)) : x;
+        }
+    }
+    __syncthreads();
+    float sa = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f32x4_t a = *(const f32x4_t*)&in[4][16 * j + 4 * part];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sa = fmaf(s[j][i], a[i], sa);
+    }
+    sa += __shfl_xor(sa, 1);
+    sa += __shfl_xor(sa, 2);
+    const float v = in[3][value];
+    float y = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int c = 16 * j + 4 * part;
+        const f32x4_t r = *(const f32x4_t*)&in[0][c], d = *(const f32x4_t*)&in[1][c], k = *(const f32x4_t*)&in[2][c],
+                      b = *(const f32x4_t*)&in[5][c];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[j][i] = fmaf(s[j][i], d[i], fmaf(sa, b[i], v * k[i]));
+            y = fmaf(s[j][i], r[i], y);
+        }
+        if (p.state_out) *(f32x4_t*)(p.state_out + at + 16 * j) = s[j];
+    }
+    y += __shfl_xor(y, 1);
+    y += __shfl_xor(y, 2);
+    if (part == 0) store_dt(p.y, YDT, row * kHead + value, y);
+}
+
+// ------------------------------------------------- rows of no sequence
+
+struct RestTensors {
+    void* p[6];
+};
+
+// One block a token outside [cu[0], cu[seqs]), in grid-sized strides.
+template <int SIZE>
+__global__ __launch_bounds__(256) void wkv7_rest_kernel(WkvShape s, RestTensors to) {
+    const int64_t first = clamp_token(s.cu[0], s.time), last = clamp_token(s.cu[s.seqs], s.time);
+    const int64_t behind = last > first ? last : first;
+    const int64_t rows = first + (s.time - behind), vecs = s.heads * kHead * SIZE / 16;
+    for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
+        const int64_t t = i < first ? i : behind + (i - first);
+#pragma unroll
+        for (int j = 0; j < 6; ++j) {
+            if (!to.p[j]) continue;
+            uint4* at = (uint4*)to.p[j] + t * vecs;
+            for (int64_t x = threadIdx.x; x < vecs; x += 256) at[x] = make_uint4(0, 0, 0, 0);
+        }
+    }
+}
+
+template <int DT, int XDT, int YDT, bool REV>
+hipError_t scan_tiles(const WkvScan& a, hipStream_t s) {
+    const int64_t pairs = a.shape.seqs * a.shape.heads;
+    if (pairs >= 192) wkv7_scan_kernel<DT, XDT, YDT, REV, 4><<<dim3((unsigned)pairs), 512, 0, s>>>(a);
+    else wkv7_scan_kernel<DT, XDT, YDT, REV, 1><<<dim3((unsigned)(4 * pairs)), 320, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+template <int DT, int ODT>
+hipError_t scan_dt(const WkvScan& a, hipStream_t s) {
+    return a.reverse ? scan_tiles<DT, ODT, DT, true>(a, s) : scan_tiles<DT, DT, ODT, false>(a, s);
+}
+
+template <int DT, int ODT>
+hipError_t grads_dt(const WkvGrads& a, hipStream_t s) {
+    wkv7_grads_kernel<DT, ODT><<<dim3((unsigned)(wkv_chunks(a.shape) * a.shape.heads)), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+template <int DT, int ODT>
+hipError_t step_dt(const WkvStep& a, hipStream_t s) {
+    wkv7_step_kernel<DT, ODT><<<dim3((unsigned)a.rows), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+namespace rq {
+
+#define RQ_BY_TYPES(F, DT_, ODT_, ...)                                        \
+    if (DT_ == RQ_F32) return F<RQ_F32, RQ_F32>(__VA_ARGS__);                 \
+    if (DT_ == RQ_BF16)                                                       \
+        return ODT_ == RQ_F32 ? F<RQ_BF16, RQ_F32>(__VA_ARGS__) : F<RQ_BF16, RQ_BF16>(__VA_ARGS__); \
+    return ODT_ == RQ_F32 ? F<RQ_F16, RQ_F32>(__VA_ARGS__) : F<RQ_F16, RQ_F16>(__VA_ARGS__);
+
+hipError_t launch_wkv_scan(const WkvScan& a, hipStream_t s) {
+    RQ_BY_TYPES(scan_dt, a.in.dt, (a.reverse ? a.x_dt : a.y_dt), a, s)
+}
+
+hipError_t launch_wkv_grads(const WkvGrads& a, hipStream_t s) { RQ_BY_TYPES(grads_dt, a.in.dt, a.dy_dt, a, s) }
+
+hipError_t launch_wkv_step(const WkvStep& a, hipStream_t s) { RQ_BY_TYPES(step_dt, a.in.dt, a.y_dt, a, s) }
+
+hipError_t launch_wkv_rest(const WkvShape& s, int dt, void* const* tensors, int n, hipStream_t stream) {
+    RestTensors to{};
+    for (int i = 0; i < n; ++i) to.p[i] = tensors[i];
+    const unsigned blocks = (unsigned)std::min<int64_t>(s.time, 1024);
+    if (dt == RQ_F32) wkv7_rest_kernel<4><<<dim3(blocks), 256, 0, stream>>>(s, to);
+    else wkv7_rest_kernel<2><<<dim3(blocks), 256, 0, stream>>>(s, to);
+    return hipGetLastError();
+}
+
+}  // namespace rq

@@ -1,0 +1,306 @@
+"""What an RWKV-7 block runs between its products.
+
+    wkv7(r, w, k, v, a, b, state, cu_seqlens)   the time mixing's recurrence, with gradients
+    wkv7_step(r, w, k, v, a, b, state, out)     its form for one token of every sequence
+
+Reference call sites: wkv7 / wkv7_train / wkv7_infer (rwkv_metal/kernel/wkv7.py:67-214,
+330-381, called at rwkv_metal/model/rwkv7_x070.py:184-187), wkv7_step
+(rwkv7_x070.py:174-182) and the carried state (rwkv_metal/model/state.py:33-127).
+
+Inputs of one dtype stay in it; any other mix computes in float32, as in the packed
+products.  States are float32.  Tensors must live on the ROCm GPU; there is no CPU path.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch import Tensor
+from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
+
+from ._lib import DTYPE_CODE, check, lib
+from .ops import _DeviceGuard, _eager, _float, _on_gpu, _ptr, _ready, _stream_on
+from .train import _addr, _queried_workspace, _records, _size
+
+HEAD_SIZE = 64   # channels of a head
+CHUNK = 16       # tokens between two states that are kept for the backward pass
+
+
+# -------------------------------------------------------------- recurrence
+
+def _sizes(r: Tensor, cu: Optional[Tensor]) -> Tuple[int, int, int, int]:
+    batch, time, heads = r.shape[:3]
+    return batch, time, heads, batch if cu is None else cu.numel() - 1
+
+
+def _chunks(batch: int, time: int, seqs: int, packed: bool) -> int:
+    return time // CHUNK + seqs if packed else batch * -(-time // CHUNK)
+
+
+def _wkv7_impl(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state: Optional[Tensor],
+               cu: Optional[Tensor], out_dtype: torch.dtype, keep: bool):
+    """(y, last state, and where they are kept the states and S a that the backward pass reads)."""
+    _on_gpu(r, w, k, v, a, b, *[t for t in (state, cu) if t is not None])
+    r, w, k, v, a, b = map(_ready, (r, w, k, v, a, b))
+    state = None if state is None else _ready(state)
+    batch, time, heads, seqs = _sizes(r, cu)
+    f32 = {"dtype": torch.float32, "device": r.device}
+    y = torch.empty(r.shape, dtype=out_dtype, device=r.device)
+    last = torch.empty(seqs, heads, HEAD_SIZE, HEAD_SIZE, **f32)
+    states = sa = None
+    if keep:
+        n = _chunks(batch, time, seqs, cu is not None)
+        states = torch.empty(n, heads, HEAD_SIZE, HEAD_SIZE, **f32)
+        sa = torch.empty(n, heads, CHUNK, HEAD_SIZE, **f32)
+    L, dt, odt = lib(), DTYPE_CODE[r.dtype], DTYPE_CODE[out_dtype]
+    with _DeviceGuard(r.device):
+        stream = _stream_on(r.device)
+        if time == 1 and cu is None and not keep:
+            rc = L.rq_wkv7_step(_ptr(r), _ptr(w), _ptr(k), _ptr(v), _ptr(a), _ptr(b), dt, batch, heads,
+                                _addr(state), _ptr(y), odt, _ptr(last), stream)
+        else:
+            rc = L.rq_wkv7(_ptr(r), _ptr(w), _ptr(k), _ptr(v), _ptr(a), _ptr(b), dt, batch, time, heads,
+                           0 if cu is None else cu.data_ptr(), seqs, _addr(state), _ptr(y), odt, _ptr(last),
+                           _addr(states), _addr(sa), stream)
+    if rc:
+        check(rc, "wkv7")
+    return y, last, states, sa
+
+
+def _wkv7_backward_impl(r, w, k, v, a, b, cu, states, sa, dy, dlast, want_state: bool):
+    """The gradients of the six and, where it is wanted, of the first state."""
+    _on_gpu(r, w, k, v, a, b, states, sa, dy, *[t for t in (dlast, cu) if t is not None])
+    r, w, k, v, a, b, dy = map(_ready, (r, w, k, v, a, b, dy))
+    dlast = None if dlast is None else _ready(dlast)
+    batch, time, heads, seqs = _sizes(r, cu)
+    grads = [torch.empty_like(r) for _ in range(6)]
+    dstate = None
+    if want_state:
+        dstate = torch.empty(seqs, heads, HEAD_SIZE, HEAD_SIZE, dtype=torch.float32, device=r.device)
+    with _DeviceGuard(r.device):
+        stream = _stream_on(r.device)
+        ws = _queried_workspace("rq_wkv7_backward_workspace_bytes", (batch, time, heads, seqs, cu is not None),
+                                r.device, "wkv7 backward")
+        rc = lib().rq_wkv7_backward(_ptr(r), _ptr(w), _ptr(k), _ptr(v), _ptr(a), _ptr(b), DTYPE_CODE[r.dtype],
+                                    batch, time, heads, 0 if cu is None else cu.data_ptr(), seqs, _ptr(states),
+                                    _ptr(sa), _ptr(dy), DTYPE_CODE[dy.dtype], _addr(dlast),
+                                    *[_ptr(g) for g in grads], _addr(dstate), _addr(ws), _size(ws), stream)
+    if rc:
+        check(rc, "wkv7 backward")
+    return (*grads, dstate)
+
+
+def _wkv7_op_impl(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state: Optional[Tensor],
+                  cu: Optional[Tensor], out_dtype: torch.dtype,
+                  keep: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    y, last, states, sa = _wkv7_impl(r, w, k, v, a, b, state, cu, out_dtype, keep)
+    none = last.new_empty(0)
+    return y, last, none if states is None else states, last.new_empty(0) if sa is None else sa
+
+
+_wkv7_op = torch.library.custom_op("rwkvq::wkv7", _wkv7_op_impl, mutates_args=())
+
+
+@_wkv7_op.register_fake
+def _(r, w, k, v, a, b, state, cu, out_dtype, keep):
+    batch, time, heads, seqs = _sizes(r, cu)
+    n = _chunks(batch, time, seqs, cu is not None)
+    f32 = {"dtype": torch.float32}
+    return (r.new_empty(r.shape, dtype=out_dtype), r.new_empty(seqs, heads, HEAD_SIZE, HEAD_SIZE, **f32),
+            r.new_empty((n, heads, HEAD_SIZE, HEAD_SIZE) if keep else 0, **f32),
+            r.new_empty((n, heads, CHUNK, HEAD_SIZE) if keep else 0, **f32))
+
+
+def _wkv7_backward_op_impl(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor,
+                           cu: Optional[Tensor], states: Tensor, sa: Tensor, dy: Tensor,
+                           dlast: Optional[Tensor], want_state: bool
+                           ) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    *grads, dstate = _wkv7_backward_impl(r, w, k, v, a, b, cu, states, sa, dy, dlast, want_state)
+    return (*grads, states.new_empty(0) if dstate is None else dstate)
+
+
+_wkv7_backward_op = torch.library.custom_op("rwkvq::wkv7_backward", _wkv7_backward_op_impl, mutates_args=())
+
+
+@_wkv7_backward_op.register_fake
+def _(r, w, k, v, a, b, cu, states, sa, dy, dlast, want_state):
+    _, _, heads, seqs = _sizes(r, cu)
+    return (*[r.new_empty(r.shape) for _ in range(6)],
+            states.new_empty((seqs, heads, HEAD_SIZE, HEAD_SIZE) if want_state else 0))
+
+
+def _gradients(ctx, dy, dlast, backward):
+    """The gradients of wkv7's seven tensors from those of its two results (None: 0)."""
+    r, w, k, v, a, b, cu, states, sa = ctx.saved_tensors
+    if dy is None and dlast is None:
+        return (None,) * 7
+    if dy is None:
+        dy = torch.zeros(r.shape, dtype=ctx.out_dtype, device=r.device)
+    got = backward(r, w, k, v, a, b, cu, states, sa, dy.contiguous(), dlast, ctx.needs_input_grad[6])
+    return tuple(g if need else None for g, need in zip(got, ctx.needs_input_grad))
+
+
+def _wkv7_op_setup(ctx, inputs, output):
+    r, w, k, v, a, b, state, cu, ctx.out_dtype, ctx.keep = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(r, w, k, v, a, b, cu, *output[2:])
+
+
+def _wkv7_op_backward(ctx, dy, dlast, _dstates, _dsa):
+    if not ctx.keep:
+        raise RuntimeError("rwkvq::wkv7 was called with keep=False: it has no gradients")
+    return (*_gradients(ctx, dy, dlast, _wkv7_backward_op), None, None, None)
+
+
+_wkv7_op.register_autograd(_wkv7_op_backward, setup_context=_wkv7_op_setup)
+
+
+class _Wkv7Function(torch.autograd.Function):
+    """The registered op's autograd formula without its dispatch, for plain eager
+    GPU tensors."""
+
+    @staticmethod
+    def forward(ctx, r, w, k, v, a, b, state, cu, out_dtype):
+        y, last, states, sa = _wkv7_impl(r, w, k, v, a, b, state, cu, out_dtype, True)
+        ctx.set_materialize_grads(False)
+        ctx.out_dtype = out_dtype
+        ctx.save_for_backward(r, w, k, v, a, b, cu, states, sa)
+        return y, last
+
+    @staticmethod
+    def backward(ctx, dy, dlast):
+        if torch.is_grad_enabled():  # a graph of this pass is wanted; it has none
+            return _Wkv7Function._once(ctx, dy, dlast)
+        return _Wkv7Function._run(ctx, dy, dlast)
+
+    @staticmethod
+    def _run(ctx, dy, dlast):
+        return (*_gradients(ctx, dy, dlast, _wkv7_backward_impl), None, None)
+
+    _once = staticmethod(once_differentiable(_run.__func__))
+
+
+def _same_dtype(six):
+    """The six in one dtype, float32 where they come in several."""
+    dt = six[0].dtype
+    if all(t.dtype == dt for t in six):
+        return six, dt
+    return [t.to(torch.float32) for t in six], torch.float32
+
+
+def _check_inputs(six, dims: int) -> None:
+    for name, t in zip("rwkvab", six):
+        _float(t, name)
+        if t.shape != six[0].shape:
+            raise ValueError(f"r, w, k, v, a and b must have one shape (got {tuple(six[0].shape)} and "
+                             f"{tuple(t.shape)} of {name})")
+    if six[0].dim() != dims or six[0].shape[-1] != HEAD_SIZE:
+        lead = "[batch, time, heads, 64]" if dims == 4 else "[batch, heads, 64]"
+        raise ValueError(f"r, w, k, v, a and b must be {lead} (got {tuple(six[0].shape)})")
+
+
+def _check_state(state: Tensor, seqs: int, heads: int, name: str = "state") -> None:
+    want = (seqs, heads, HEAD_SIZE, HEAD_SIZE)
+    if state.dtype != torch.float32 or state.shape != want:
+        raise ValueError(f"{name} must be float32 of shape {want} (got {state.dtype} {tuple(state.shape)})")
+
+
+def _out_dtype(out_dtype: Optional[torch.dtype], dt: torch.dtype) -> torch.dtype:
+    if out_dtype is None:
+        return dt
+    if out_dtype not in (dt, torch.float32):
+        raise ValueError(f"out_dtype must be the inputs' {dt} or float32 (got {out_dtype})")
+    return out_dtype
+
+
+def wkv7(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state: Optional[Tensor] = None,
+         cu_seqlens: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
+    """(y, last state) of the recurrence, for every head with its state S [64, 64]:
+
+        S_t = S_{t-1} diag(exp(-exp(w_t))) + (S_{t-1} a_t) b_t^T + v_t k_t^T,   y_t = S_t r_t
+
+    r, w, k, v, a, b: [batch, time, heads, 64] of any length.  state: float32 [batch, heads,
+    64 values, 64 keys] before the first token, 0 by default.  y has the inputs' dtype or
+    out_dtype (float32 is the other choice); the state, its products and all sums are float32.
+
+    cu_seqlens: packed sequences in a batch of one; n + 1 int32 values on the GPU, from 0,
+    not decreasing.  Sequence i is the tokens cu_seqlens[i] to cu_seqlens[i + 1] with state i of
+    [n, heads, 64, 64] (an empty one keeps its state); y and the gradients are 0 behind the
+    last.  Nothing waits for their values: boundaries outside the batch are moved into it, and
+    where they decrease the results are undefined.
+
+    In a padded batch a token with w = -inf, k = 0 and b = 0 leaves the state as it was.
+
+    Differentiable in all six and the first state, from both results (once).  The backward pass
+    keeps every 16th state, a sixteenth of 16 KB for each token and head."""
+    six = [r, w, k, v, a, b]
+    _check_inputs(six, 4)
+    six, dt = _same_dtype(six)
+    odt = _out_dtype(out_dtype, dt)
+    batch, time, heads = six[0].shape[:3]
+    seqs = batch
+    if cu_seqlens is not None:
+        if cu_seqlens.dtype not in (torch.int32, torch.int64) or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+            raise ValueError("cu_seqlens must hold the n + 1 boundaries of n sequences as int32 or int64")
+        if batch != 1:
+            raise ValueError(f"packed sequences take a batch of 1 (got {batch})")
+        seqs = cu_seqlens.numel() - 1
+        if seqs == 0 and time:
+            raise ValueError("cu_seqlens holds no sequence")
+        cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+    if state is not None:
+        _check_state(state, seqs, heads)
+    ts = six if state is None else [*six, state]
+    if _eager(*ts):
+        if not torch.is_grad_enabled() or not any(t.requires_grad for t in ts):
+            return _wkv7_impl(*six, state, cu_seqlens, odt, False)[:2]
+        if forward_ad._current_level < 0:
+            return _Wkv7Function.apply(*six, state, cu_seqlens, odt)
+    return _wkv7_op(*six, state, cu_seqlens, odt, _records(*ts))[:2]
+
+
+# --------------------------------------------------------------- one token
+
+def _step_impl(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state: Tensor, out: Tensor,
+               out_dtype: torch.dtype) -> Tensor:
+    _on_gpu(r, w, k, v, a, b, state, out)
+    r, w, k, v, a, b = map(_ready, (r, w, k, v, a, b))
+    y = torch.empty(r.shape, dtype=out_dtype, device=r.device)
+    with _DeviceGuard(r.device):
+        rc = lib().rq_wkv7_step(_ptr(r), _ptr(w), _ptr(k), _ptr(v), _ptr(a), _ptr(b), DTYPE_CODE[r.dtype],
+                                r.shape[0], r.shape[1], _ptr(state), _ptr(y), DTYPE_CODE[out_dtype], _ptr(out),
+                                _stream_on(r.device))
+    if rc:
+        check(rc, "wkv7_step")
+    return y
+
+
+@torch.no_grad()
+def wkv7_step(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state: Tensor,
+              out: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
+    """(y, new state) of one token of every sequence: r .. b [batch, heads, 64], state
+    [batch, heads, 64, 64].  out: a contiguous float32 tensor for the new state, `state` itself for an
+    update in place.  Without gradients (wkv7 over a time of 1 has them)."""
+    six = [r, w, k, v, a, b]
+    _check_inputs(six, 3)
+    six, dt = _same_dtype(six)
+    odt = _out_dtype(out_dtype, dt)
+    _check_state(state, *six[0].shape[:2])
+    if out is None:
+        out = torch.empty(state.shape, dtype=torch.float32, device=state.device)
+    else:
+        _check_state(out, *six[0].shape[:2], "out")
+        if not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError("out must be contiguous and 16-byte aligned")
+        if out.numel() and out.data_ptr() != state.data_ptr() and _overlap(out, state):
+            raise ValueError("out may be the state itself, but must not overlap it otherwise")
+    return _step_impl(*six, _ready(state), out, odt), out
+
+
+def _overlap(x: Tensor, y: Tensor) -> bool:
+    """Whether the memory that the two span has bytes in common."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + 4 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    (x0, x1), (y0, y1) = span(x), span(y)
+    return x0 < y1 and y0 < x1
