@@ -70,6 +70,26 @@ int rq_wkv7_step(const void* r, const void* w, const void* k, const void* v, con
                  rq_dtype dt, int64_t batch, int64_t heads, const float* state, void* y, rq_dtype y_dt,
                  float* state_out, void* stream);
 
+/* token[i] from the logits [rows, vocab] of dt (vocab at most 2^20, no alignment of the rows) and
+ * u[i] in [0, 1), in this order, with e_j = exp((l_j - max l) / temperature):
+ *   1. the top_k largest stay (0: all);
+ *   2. of these, from the largest, those before whom less than top_p of their sum lies (1: all);
+ *   3. of these, those with e_j >= min_p;
+ *   4. the first by index at which the running sum of what stays exceeds u times the whole.
+ * Equal logits rank by index.  A temperature of 0 takes the largest logit.  logprob[i] (or NULL) is the log of the
+ * token's share of what stays.  -inf logits never come; +inf ones share everything.  A row with a NaN, or of
+ * -inf alone, gives token -1 and a NaN.  The sums are taken in float64 from terms rounded to 2^-36
+ * (2^-33 past 2^17 logits), exactly.
+ *
+ * temperature, top_k, top_p, min_p: one for each row, or NULL for the value behind it.  Values on the
+ * device are not checked: a temperature that is not above 0 is 0, top_k below 1 is 0, a top_p of 0 or less keeps the
+ * largest alone and one that is not below 1 all, min_p is moved into [0, 1] (NaN: 0), u into [0, 1) (NaN: 0).
+ * u, temperature, top_p and min_p are 4-byte aligned, top_k and token 8-byte. */
+int rq_sample(const void* logits, rq_dtype dt, int64_t rows, int64_t vocab, const float* u,
+              const float* temperature, float temperature_all, const int64_t* top_k, int64_t top_k_all,
+              const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* token,
+              float* logprob, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

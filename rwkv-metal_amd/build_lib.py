@@ -42,6 +42,7 @@ def _units():
              ("rq_embed.hip", [], "rq_embed.o"), ("rq_linear.hip", [], "rq_linear.o"),
              ("rq_dpre.hip", [], "rq_dpre.o"),
              ("rq_wkv7.hip", [], "rq_wkv7.o"),
+             ("rq_sample.hip", [], "rq_sample.o"),
              ("rq_rwkv7_abi.cpp", ["-x", "hip"], "rq_rwkv7_abi.o"),
              ("rq_train_abi.cpp", ["-x", "hip"], "rq_train_abi.o"),
              ("rq_abi.cpp", ["-x", "hip"], "rq_abi.o")]

@@ -1,4 +1,4 @@
-// rq_rwkv7_abi.cpp -- the extern "C" boundary of the recurrence
+// rq_rwkv7_abi.cpp -- the extern "C" boundary of the recurrence and the sampler
 // (include/rwkvq_rwkv7.h): argument checks, then the launchers.
 #include <hip/hip_runtime.h>
 
@@ -6,6 +6,7 @@
 
 #include "../../include/rwkvq_rwkv7.h"
 #include "rq_error.h"
+#include "rq_sample.h"
 #include "rq_wkv7.h"
 
 using rq::aligned16;
@@ -159,6 +160,31 @@ int rq_wkv7_step(const void* r, const void* w, const void* k, const void* v, con
     if (int rc = check_ptrs(what, {r, w, k, v, a, b, y}, {state, state_out})) return rc;
     return rq::launch_status(
         rq::launch_wkv_step({{r, w, k, v, a, b, dt}, batch * heads, state, y, y_dt, state_out}, (hipStream_t)stream), what);
+}
+
+int rq_sample(const void* logits, rq_dtype dt, int64_t rows, int64_t vocab, const float* u, const float* temperature,
+              float temperature_all, const int64_t* top_k, int64_t top_k_all, const float* top_p, float top_p_all,
+              const float* min_p, float min_p_all, int64_t* token, float* logprob, void* stream) {
+    const char* what = "rq_sample";
+    if (!valid_dt(dt)) return fail(RQ_EINVAL, "%s: unsupported dtype", what);
+    if (rows < 0 || vocab < 0) return fail(RQ_EINVAL, "%s: negative size (rows=%lld vocab=%lld)", what, (long long)rows, (long long)vocab);
+    if (vocab > rq::kSampleMaxVocab) return fail(RQ_EINVAL, "%s: a vocabulary of more than %lld", what, (long long)rq::kSampleMaxVocab);
+    if (rows > (1 << 21)) return fail(RQ_EINVAL, "%s: more than %d rows", what, 1 << 21);
+    if (rows > 0 && vocab == 0) return fail(RQ_EINVAL, "%s: rows without a logit", what);
+    if (!temperature && !(temperature_all >= 0.f)) return fail(RQ_EINVAL, "%s: a temperature is 0 or more", what);
+    if (!top_k && top_k_all < 0) return fail(RQ_EINVAL, "%s: top_k is 0 or more", what);
+    if (!top_p && !(top_p_all > 0.f && top_p_all <= 1.f)) return fail(RQ_EINVAL, "%s: top_p lies in (0, 1]", what);
+    if (!min_p && !(min_p_all >= 0.f && min_p_all <= 1.f)) return fail(RQ_EINVAL, "%s: min_p lies in [0, 1]", what);
+    if (rows == 0) return ok();
+    if (!logits || !u || !token) return fail(RQ_EINVAL, "%s: NULL pointer", what);
+    const uintptr_t fours = (uintptr_t)u | (uintptr_t)temperature | (uintptr_t)top_p | (uintptr_t)min_p | (uintptr_t)logprob;
+    if (((uintptr_t)logits & (dt == RQ_F32 ? 3u : 1u)) || (fours & 3u) || (((uintptr_t)top_k | (uintptr_t)token) & 7u))
+        return fail(RQ_EALIGN, "%s: pointers must be aligned to their elements", what);
+    return rq::launch_status(
+        rq::launch_sample({logits, dt, rows, vocab, u, temperature, top_k, top_p, min_p, temperature_all, top_k_all,
+                           top_p_all, min_p_all, token, logprob},
+                          (hipStream_t)stream),
+        what);
 }
 
 }  // extern "C"

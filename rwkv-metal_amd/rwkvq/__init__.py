@@ -9,8 +9,8 @@ Packed checkpoints: rwkvq.io.save_quantized / load_quantized.  The .rwkvq
 (rwkv-quant sb6) base: RwkvqLinear, RwkvqNativeLinear, RwkvqHybridLinear,
 add_lora_rwkvq, load_sidecar.  The rest of a training step: linear_act,
 embedding, grad_norm, clip_grad_norm, clip_grad_norm_ and the modules LinearAct
-and ScaledEmbedding (rwkvq.train).  Between the products of an RWKV-7 block: wkv7,
-wkv7_step (rwkvq.rwkv7).
+and ScaledEmbedding (rwkvq.train).  Between the products of an RWKV-7 block and
+behind its head: wkv7, wkv7_step and sample (rwkvq.rwkv7).
 All compute runs in librwkvq_hip.so; tensors must be on the GPU.
 """
 from .ops import (VALID_BITS, VALID_GROUP_SIZES, BoundQmm, GroupedQmv, dequantize, grouped_qmv,
@@ -24,7 +24,7 @@ from .lora import (BIG_QUANT_TARGETS, CMIX_TARGETS, TMIX_TARGETS, LoRALinear, ad
                    load_lora, lora_state, merge_lora, quantize_base_model, save_lora)
 from .train import (ACTIVATIONS, LinearAct, ScaledEmbedding, clip_grad_norm, clip_grad_norm_,
                     embedding, grad_norm, linear_act)
-from .rwkv7 import wkv7, wkv7_step
+from .rwkv7 import sample, wkv7, wkv7_step
 
 __all__ = [
     "VALID_BITS", "VALID_GROUP_SIZES", "quantize", "dequantize", "quantized_matmul",
@@ -35,5 +35,5 @@ __all__ = [
     "merge_lora", "io", "sb6", "RwkvqLinear", "RwkvqNativeLinear", "RwkvqHybridLinear",
     "add_lora_rwkvq", "load_sidecar", "ACTIVATIONS", "linear_act", "LinearAct", "embedding",
     "ScaledEmbedding", "grad_norm", "clip_grad_norm", "clip_grad_norm_",
-    "wkv7", "wkv7_step",
+    "wkv7", "wkv7_step", "sample",
 ]

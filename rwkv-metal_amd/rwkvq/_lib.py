@@ -108,6 +108,8 @@ SIGNATURES = {
     "rq_wkv7_backward_workspace_bytes": ([_i64, _i64, _i64, _i64, _i32], _i64),
     "rq_wkv7_backward": ([_vp] * 6 + [_i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _vp] +
                          [_vp] * 7 + [_vp, _i64, _vp], _i32),
+    "rq_sample": ([_vp, _i32, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _i64, _vp, ctypes.c_float, _vp,
+                   ctypes.c_float, _vp, _vp, _vp], _i32),
     "rq_wkv7_step": ([_vp] * 6 + [_i32, _i64, _i64, _vp, _vp, _i32, _vp, _vp], _i32),
 }
 RQ_EUNSUPPORTED = -4

@@ -1,7 +1,8 @@
-"""What an RWKV-7 block runs between its products.
+"""What an RWKV-7 block runs between its products, and the token choice behind its head.
 
     wkv7(r, w, k, v, a, b, state, cu_seqlens)   the time mixing's recurrence, with gradients
     wkv7_step(r, w, k, v, a, b, state, out)     its form for one token of every sequence
+    sample(logits, u, temperature, top_k, top_p, min_p)   tokens from given uniform numbers
 
 Reference call sites: wkv7 / wkv7_train / wkv7_infer (rwkv_metal/kernel/wkv7.py:67-214,
 330-381, called at rwkv_metal/model/rwkv7_x070.py:184-187), wkv7_step
@@ -12,7 +13,7 @@ products.  States are float32.  Tensors must live on the ROCm GPU; there is no C
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -304,3 +305,72 @@ def _overlap(x: Tensor, y: Tensor) -> bool:
         return t.data_ptr(), t.data_ptr() + 4 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
     (x0, x1), (y0, y1) = span(x), span(y)
     return x0 < y1 and y0 < x1
+
+
+# ------------------------------------------------------------------ sampler
+
+def _sample_impl(logits: Tensor, u: Tensor, temperature: Optional[Tensor], top_k: Optional[Tensor],
+                 top_p: Optional[Tensor], min_p: Optional[Tensor], temperature_all: float, top_k_all: int,
+                 top_p_all: float, min_p_all: float) -> Tuple[Tensor, Tensor]:
+    rows = [None if t is None else t.contiguous() for t in (temperature, top_k, top_p, min_p)]
+    _on_gpu(logits, u, *[t for t in rows if t is not None])
+    logits, u = logits.contiguous(), u.contiguous()
+    token = torch.empty(u.shape, dtype=torch.int64, device=u.device)
+    logprob = torch.empty(u.shape, dtype=torch.float32, device=u.device)
+    with _DeviceGuard(logits.device):
+        rc = lib().rq_sample(_ptr(logits), DTYPE_CODE[logits.dtype], u.numel(), logits.shape[-1], _ptr(u),
+                             _addr(rows[0]), temperature_all, _addr(rows[1]), top_k_all, _addr(rows[2]), top_p_all,
+                             _addr(rows[3]), min_p_all, _ptr(token), _ptr(logprob), _stream_on(logits.device))
+    if rc:
+        check(rc, "sample")
+    return token, logprob
+
+
+_sample_op = torch.library.custom_op("rwkvq::sample", _sample_impl, mutates_args=())
+
+
+@_sample_op.register_fake
+def _(logits, u, temperature, top_k, top_p, min_p, temperature_all, top_k_all, top_p_all, min_p_all):
+    return u.new_empty(u.shape, dtype=torch.int64), u.new_empty(u.shape, dtype=torch.float32)
+
+
+def _parameter(x, name: str, lead, whole: bool):
+    """(a value for each row, a value for all) of a parameter that is one or the other."""
+    if not isinstance(x, Tensor):
+        return None, (int(x) if whole else float(x))
+    if x.is_floating_point() if whole else not x.is_floating_point():
+        raise ValueError(f"{name} must hold {'integers' if whole else 'floating numbers'} (got {x.dtype})")
+    if x.shape != lead:
+        if x.dim() > len(lead):
+            raise ValueError(f"{name} must be a number or have shape {tuple(lead)} (got {tuple(x.shape)})")
+        x = x.expand(lead)
+    return x.to(torch.int64 if whole else torch.float32), (0 if whole else 1.0)
+
+
+@torch.no_grad()
+def sample(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] = 1.0, top_k: Union[int, Tensor] = 0,
+           top_p: Union[float, Tensor] = 1.0, min_p: Union[float, Tensor] = 0.0) -> Tuple[Tensor, Tensor]:
+    """(tokens int64, their log-probabilities float32) for logits [..., vocab] and numbers u [...] in
+    [0, 1), float32.  With e_i = exp((l_i - max l) / temperature), in this order:
+
+    1. the top_k largest stay (0: all);
+    2. of these, from the largest, those before whom less than top_p of their sum lies (1: all);
+    3. of these, those with e_i >= min_p;
+    4. the token is the first by index at which the running sum of what stays exceeds u times
+       the whole.
+
+    Equal logits rank by index.  Each parameter is a number, or a tensor [...] with one for each row
+    (numbers of 32 bits).  A temperature of 0, or a top_k of 1, takes the largest.  -inf logits never
+    come; a row of nothing else, or with a NaN in it, gives -1 and a NaN.  The sums are exact
+    (terms of float64 rounded to 2^-36 of the largest), so the same inputs give the same tokens.  Without gradients."""
+    _float(logits, "logits")
+    if logits.dim() < 1 or u.dtype != torch.float32 or u.shape != logits.shape[:-1]:
+        raise ValueError(f"u must be float32 of shape {tuple(logits.shape[:-1])} (got {u.dtype} {tuple(u.shape)})")
+    lead = u.shape
+    t, t_all = _parameter(temperature, "temperature", lead, False)
+    k, k_all = _parameter(top_k, "top_k", lead, True)
+    p, p_all = _parameter(top_p, "top_p", lead, False)
+    m, m_all = _parameter(min_p, "min_p", lead, False)
+    given = [x for x in (t, k, p, m) if x is not None]
+    op = _sample_impl if _eager(logits, u, *given) else _sample_op
+    return op(logits, u, t, k, p, m, t_all, min(k_all, 1 << 62), p_all, m_all)

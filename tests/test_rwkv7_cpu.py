@@ -1,4 +1,4 @@
-"""Argument checks of the recurrence's C entry points, without a GPU: nothing here reaches a
+"""Argument checks of the C entry points of the recurrence and the sampler, without a GPU: nothing here reaches a
 launch."""
 import os
 import re
@@ -25,7 +25,8 @@ def test_every_declared_entry_point_is_exported_and_bound(L):
     text = open(os.path.join(ROOT, "include", "rwkvq_rwkv7.h")).read()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     names = set(re.findall(r"^\s*\w+\s+(rq_\w+)\s*\(", text, flags=re.M))
-    assert {"rq_wkv7", "rq_wkv7_backward", "rq_wkv7_step", "rq_wkv7_chunks"} <= names
+    assert names == {"rq_wkv7", "rq_wkv7_backward", "rq_wkv7_step", "rq_wkv7_chunks",
+                     "rq_wkv7_backward_workspace_bytes", "rq_sample"}
     for name in names:
         assert hasattr(L, name) and name in _lib.SIGNATURES
 
@@ -97,6 +98,23 @@ def test_step_refusals(L):
     assert step(batch=0) == 0
 
 
+def test_sampler_refusals(L):
+    def call(x=P, dt=0, rows=2, vocab=10, u=P, t=0, ta=1.0, k=0, ka=0, p=0, pa=1.0, m=0, ma=0.0, token=P, lp=0):
+        return L.rq_sample(x, dt, rows, vocab, u, t, ta, k, ka, p, pa, m, ma, token, lp, None)
+
+    nan = float("nan")
+    for kw, text in (({"dt": 3}, "dtype"), ({"rows": -1}, "negative"), ({"vocab": -1}, "negative"), ({"vocab": 0}, "without a logit"),
+                     ({"vocab": 2 ** 20 + 1}, "vocabulary"), ({"rows": 2 ** 21 + 1}, "rows"), ({"ta": -0.5}, "temperature"),
+                     ({"ta": nan}, "temperature"), ({"ka": -1}, "top_k"), ({"pa": 0.0}, "top_p"), ({"pa": 1.25}, "top_p"),
+                     ({"pa": nan}, "top_p"), ({"ma": -1.0}, "min_p"), ({"ma": 1.5}, "min_p"), ({"x": 0}, "NULL"),
+                     ({"u": 0}, "NULL"), ({"token": 0}, "NULL")):
+        assert call(**kw) == -1 and text in err(L), (kw, err(L))
+    for kw in ({"x": P + 1}, {"x": P + 2, "dt": 2}, {"u": P + 2}, {"t": P + 1}, {"k": P + 4}, {"p": P + 2}, {"m": P + 2},
+               {"token": P + 4}, {"lp": P + 2}):
+        assert call(**kw) == -2 and "aligned" in err(L), kw
+    assert call(rows=0, x=0, u=0, token=0) == 0
+
+
 def test_no_cpu_path():
     import rwkvq
     six = [torch.zeros(1, 2, 1, 64) for _ in range(6)]
@@ -104,3 +122,5 @@ def test_no_cpu_path():
         rwkvq.wkv7(*six)
     with pytest.raises(RuntimeError, match="no CPU"):
         rwkvq.wkv7_step(*[x[:, 0] for x in six], torch.zeros(1, 1, 64, 64))
+    with pytest.raises(RuntimeError, match="no CPU"):
+        rwkvq.sample(torch.zeros(2, 5), torch.zeros(2))
