@@ -16,7 +16,7 @@ using rq::valid_dt;
 
 namespace {
 
-// A grid holds fewer than 2^32 threads: 512 for each head of a sequence in the scan, 256 for each
+// A grid holds fewer than 2^32 threads: 768 for each head of a sequence in the scan, 256 for each
 // head of a chunk and of a decode step.
 constexpr int64_t kMaxHeadsOfSeqs = 1 << 22, kMaxHeadsOfChunks = 1 << 23, kMaxTokens = 1ll << 31;
 

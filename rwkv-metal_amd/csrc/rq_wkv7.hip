@@ -82,6 +82,11 @@ RQ_DEV float before(float x) {  // the previous token's value, 0 for the first
     return dpp<(REV ? kRowShl : kRowShr) + 1>(x);
 }
 template <bool REV>
+RQ_DEV float before_or_one(float x) {  // 1 for the first
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(1.f), __float_as_int(x),
+                                                      (REV ? kRowShl : kRowShr) + 1, 0xf, 0xf, false));
+}
+template <bool REV>
 RQ_DEV float of_last(float x) {  // the last token's value
     return dpp<kRowBcast + (REV ? 0 : 15)>(x);
 }
@@ -131,18 +136,29 @@ RQ_DEV void unpack_raw(const Raw<DT>& r, float* f) {
     }
 }
 
-// What the scan reads of a chunk.  Backwards the tensors change places: to_sa is B^, to_y K^,
-// from_sa A~, from_x R~, and the matrices are transposed.
-struct Chunk {
-    float to_sa[kChunk][kRow];    // A~
-    float to_y[kChunk][kRow];     // R~
-    float from_sa[kChunk][kRow];  // B^
-    float from_x[kChunk][kRow];   // K^
-    f32x4_t inv[64];              // (1 - Mab)^-1, [lane] as an A operand
-    f32x4_t sa_x[64];             // Mak
-    f32x4_t y_sa[64];             // Mrb
-    f32x4_t y_x[64];              // Mrk
-    float decay[kHead];           // e^Lend
+// What the block's waves hand on: the arrays of three chunks and the matrices of two.  Backwards
+// the tensors change places: to_sa is B^, to_y K^, from_sa A~, from_x R~, and the matrices are transposed.
+typedef float Rows[kChunk][kRow];
+struct Arrays {
+    Rows to_sa;    // A~
+    Rows to_y;     // R~
+    Rows from_sa;  // B^
+    Rows from_x;   // K^
+    Rows x;        // V
+    float decay[kHead];  // e^Lend
+};
+struct Matrices {  // [lane] as A operands
+    f32x4_t inv[64];   // (1 - Mab)^-1
+    f32x4_t sa_x[64];  // Mak
+    f32x4_t y_sa[64];  // Mrb
+    f32x4_t y_x[64];   // Mrk
+};
+struct ScanLds {
+    Arrays arrays[3];
+    Rows inverse[2][2];  // B~ and K~
+    Matrices matrices[2];
+    Rows y[2];
+    int strong[3][4];    // whether a wave's channels hold strong decays
 };
 
 // X^T of X = (1 - M)^-1 from m[i] = M^T[4g + i][lane & 15], nonzero above the diagonal:
@@ -220,195 +236,275 @@ __device__ __attribute__((noinline)) f32x4_t strong_pairs(const float* late, con
 
 // ------------------------------------------------------------------ the scan
 
-// Wave `pair` of four forms one of the matrices Mab, Mak / Mrb, Mrb / Mak, Mrk of a chunk, from
-// its two tensors, and one of the four arrays.  Lane (m, g): token m, channels 16g .. 16g + 15.
-template <int DT, bool REV>
-struct Producer {
-    int lane, pair;
-    const void *late_p, *early_p, *w_p;
-    Raw<DT> late, early, w;
-    bool there;
-
-    RQ_DEV Producer(const WkvScan& p, int lane_, int pair_) : lane(lane_), pair(pair_) {
-        const bool is_a = pair == 0 || pair == (REV ? 2 : 1), is_b = pair == 0 || pair == (REV ? 1 : 2);
-        late_p = is_a ? p.in.a : p.in.r;
-        early_p = is_b ? p.in.b : p.in.k;
-        w_p = p.in.w;
-    }
-    // `row`: the flattened row of the lane's token and head, where it exists
-    RQ_DEV void load(int64_t row, bool exists) {
-        there = exists;
-        const int64_t at = row * kHead + 16 * (lane >> 4);
-        late = load_raw<DT>(late_p, at, exists);
-        early = load_raw<DT>(early_p, at, exists);
-        w = load_raw<DT>(w_p, at, exists);
-    }
-    RQ_DEV static void store(float (*to)[kRow], const float* f, int lane) {
-        f32x4_t* at = (f32x4_t*)&to[lane & 15][16 * (lane >> 4)];
+// Four contiguous values as they are stored.
+template <int DT>
+struct __attribute__((aligned(DT == RQ_F32 ? 16 : 8))) Raw4 {
+    uint32_t v[DT == RQ_F32 ? 4 : 2];
+};
+template <int DT>
+RQ_DEV Raw4<DT> load_raw4(const void* p, int64_t at) {
+    return *(const Raw4<DT>*)((const uint8_t*)p + at * (DT == RQ_F32 ? 4 : 2));
+}
+template <int DT>
+RQ_DEV f32x4_t unpack_raw4(const Raw4<DT>& r) {
+    f32x4_t f;
+    if constexpr (DT == RQ_F32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) at[i] = f32x4_t{f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]};
-    }
-    RQ_DEV void produce(Chunk& c) {
-        const bool strict = pair == 0 || pair == (REV ? 2 : 1);
-        float x[16], y[16], g2[16], l[16];
-        unpack_raw<DT>(late, x);
-        unpack_raw<DT>(early, y);
-        unpack_raw<DT>(w, g2);
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(r.v[i]);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            g2[i] = there ? log2_decay(g2[i]) : 0.f;
-            l[i] = upto<REV>(g2[i]);
+        for (int i = 0; i < 2; ++i) {
+            f[2 * i] = dt_traits<DT>::to_f32((uint16_t)(r.v[i] & 0xffffu));
+            f[2 * i + 1] = dt_traits<DT>::to_f32((uint16_t)(r.v[i] >> 16));
         }
+    }
+    return f;
+}
+
+template <int DT>
+RQ_DEV void store4(void* p, int64_t at, f32x4_t f) {
+    Raw4<DT> r;
+    if constexpr (DT == RQ_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.v[i] = __float_as_uint(f[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            r.v[i] = dt_traits<DT>::from_f32(f[2 * i]) | ((uint32_t)dt_traits<DT>::from_f32(f[2 * i + 1]) << 16);
+    }
+    *(Raw4<DT>*)((uint8_t*)p + at * (DT == RQ_F32 ? 4 : 2)) = r;
+}
+
+// A producer wave's share of the arrays: 16 channels of the chunk's 16 tokens.  Lane (m, g): token m,
+// four channels.
+template <int DT, int XDT, bool REV>
+struct Elementwise {
+    int lane, wave;
+    bool there;
+    Raw4<DT> r, w, k, a, b;
+    Raw4<XDT> x;
+
+    // `row`: the flattened row of the lane's token and head, or any that exists.  A load under a
+    // condition would be waited for where the condition ends.
+    RQ_DEV void load(const WkvInputs& in, const void* of_x, int64_t row, bool exists) {
+        there = exists;
+        const int64_t at = row * kHead + 16 * wave + 4 * (lane >> 4);
+        r = load_raw4<DT>(in.r, at);
+        w = load_raw4<DT>(in.w, at);
+        k = load_raw4<DT>(in.k, at);
+        a = load_raw4<DT>(in.a, at);
+        b = load_raw4<DT>(in.b, at);
+        x = load_raw4<XDT>(of_x, at);
+    }
+    RQ_DEV void run(Arrays& to, Rows* inverse, int& strong_flag) const {
+        const int m = lane & 15, c = 16 * wave + 4 * (lane >> 4);
+        const f32x4_t zero = {0.f, 0.f, 0.f, 0.f}, fw = unpack_raw4<DT>(w);
+        const f32x4_t fr = there ? unpack_raw4<DT>(r) : zero, fk = there ? unpack_raw4<DT>(k) : zero,
+                      fa = there ? unpack_raw4<DT>(a) : zero, fb = there ? unpack_raw4<DT>(b) : zero;
+        f32x4_t l, g2, el, ex, il, hat;
         bool strong = false;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) strong |= !(of_last<REV>(l[i]) >= kStrong);
+        for (int i = 0; i < 4; ++i) {
+            g2[i] = there ? log2_decay(fw[i]) : 0.f;
+            l[i] = upto<REV>(g2[i]);
+            strong |= !(of_last<REV>(l[i]) >= kStrong);
+        }
         strong = __any(strong);
-        f32x4_t m = {0.f, 0.f, 0.f, 0.f};
-        float hat[16];  // the earlier tensor times e^(Lend - L)
-        if (!strong) {
-            float late_s[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float end = of_last<REV>(l[i]);
-                late_s[i] = x[i] * exp2_hw(strict ? before<REV>(l[i]) : l[i]);
-                hat[i] = y[i] * exp2_hw(end - l[i]);
-                y[i] *= exp2_hw(-l[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) m = REV ? mfma4(late_s[i], y[i], m) : mfma4(y[i], late_s[i], m);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = late_s[i];
-        } else {
-            float late_m[16], early_m[16], g2_m[16];  // copies: those of the usual way stay in registers
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                late_m[i] = x[i];
-                early_m[i] = y[i];
-                g2_m[i] = g2[i];
-            }
-            m = strong_pairs<REV>(late_m, early_m, g2_m, strict, lane);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                hat[i] = y[i] * exp2_hw(before<!REV>(upto<!REV>(g2[i])));
-                x[i] *= exp2_hw(strict ? before<REV>(l[i]) : l[i]);
-            }
+        for (int i = 0; i < 4; ++i) {
+            el[i] = exp2_hw(l[i]);
+            ex[i] = before_or_one<REV>(el[i]);
+            il[i] = exp2_hw(-l[i]);
+            hat[i] = of_last<REV>(el[i]) * il[i];
         }
-        const int row = 4 * (lane >> 4), col = lane & 15;
+        if (strong) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m[i] = (strict ? row + i < col : row + i <= col) ? m[i] : 0.f;
-        // every array has one writer
-        if (pair == 0) store(REV ? c.from_sa : c.to_sa, x, lane);
-        if (pair == 3) store(REV ? c.from_x : c.to_y, x, lane);
-        if (pair == 1) store(REV ? c.to_sa : c.from_x, hat, lane);
-        if (pair == 2) store(REV ? c.to_y : c.from_sa, hat, lane);
-        if (pair == 0) c.inv[lane] = unit_inverse(m, lane);
-        if (pair == 1) c.sa_x[lane] = m;
-        if (pair == 2) c.y_sa[lane] = m;
-        if (pair == 3) {
-            c.y_x[lane] = m;
-            if (col == (REV ? 0 : 15)) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) c.decay[4 * row + i] = exp2_hw(l[i]);
-            }
+            for (int i = 0; i < 4; ++i) hat[i] = exp2_hw(before<!REV>(upto<!REV>(g2[i])));
         }
+        *(f32x4_t*)&(REV ? to.from_sa : to.to_sa)[m][c] = fa * ex;
+        *(f32x4_t*)&(REV ? to.from_x : to.to_y)[m][c] = fr * el;
+        *(f32x4_t*)&(REV ? to.to_sa : to.from_sa)[m][c] = fb * hat;
+        *(f32x4_t*)&(REV ? to.to_y : to.from_x)[m][c] = fk * hat;
+        *(f32x4_t*)&to.x[m][c] = there ? unpack_raw4<XDT>(x) : zero;
+        *(f32x4_t*)&inverse[0][m][c] = fb * il;
+        *(f32x4_t*)&inverse[1][m][c] = fk * il;
+        if (m == (REV ? 0 : 15)) *(f32x4_t*)&to.decay[c] = el;
+        if (lane == 0) strong_flag = strong;
     }
 };
 
-// Four producer waves prepare chunk c + 1 while TILES waves, each with 16 of the 64 values, take
-// chunk c.  A scan wave holds its state transposed, acc[q][i] = S[value lane & 15][key 16q + 4g + i]:
-// the layout in which a product's result comes and in which the next takes it.
-template <int DT, int XDT, int YDT, bool REV, int TILES>
-__global__ __launch_bounds__(64 * (4 + TILES)) void wkv7_scan_kernel(WkvScan p) {
-    __shared__ Chunk buf[2];
+// Wave `pair` of four forms one of Mab, Mak / Mrb, Mrb / Mak, Mrk from the arrays: an entry is a product
+// of a row of the later tensor and one of the earlier one.  Lane (m, g): token m, a quarter of the channels.
+template <int DT, bool REV>
+RQ_DEV void form_matrix(const WkvInputs& in, const Arrays& from, const Rows* inverse, bool strong, Matrices& to, int lane,
+                        int pair, int64_t row, bool exists) {
+    const int m = lane & 15, g = lane >> 4;
+    const bool is_a = pair == 0 || pair == (REV ? 2 : 1), is_b = pair == 0 || pair == (REV ? 1 : 2);
+    f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+    if (!strong) {
+        const Rows& late = is_a ? (REV ? from.from_sa : from.to_sa) : (REV ? from.from_x : from.to_y);
+        const Rows& early = inverse[is_b ? 0 : 1];
+        f32x4_t l[4], e[4], other = x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            l[j] = *(const f32x4_t*)&late[m][16 * g + 4 * j];
+            e[j] = *(const f32x4_t*)&early[m][16 * g + 4 * j];
+        }
+        // two sums: a product of this shape waits for the one before only where they share the sum
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+            x = REV ? mma16(l[j], e[j], x) : mma16(e[j], l[j], x);
+            other = REV ? mma16(l[j + 1], e[j + 1], other) : mma16(e[j + 1], l[j + 1], other);
+        }
+        x += other;
+    } else {
+        float late[16], early[16], g2[16];
+        const int64_t at = row * kHead + 16 * g;
+        unpack_raw<DT>(load_raw<DT>(is_a ? in.a : in.r, at, exists), late);
+        unpack_raw<DT>(load_raw<DT>(is_b ? in.b : in.k, at, exists), early);
+        unpack_raw<DT>(load_raw<DT>(in.w, at, exists), g2);
+        for (int i = 0; i < 16; ++i) g2[i] = exists ? log2_decay(g2[i]) : 0.f;
+        x = strong_pairs<REV>(late, early, g2, is_a, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (is_a ? 4 * g + i < m : 4 * g + i <= m) ? x[i] : 0.f;
+    if (pair == 0) to.inv[lane] = unit_inverse(x, lane);
+    if (pair == 1) to.sa_x[lane] = x;
+    if (pair == 2) to.y_sa[lane] = x;
+    if (pair == 3) to.y_x[lane] = x;
+}
+
+constexpr int kScanThreads = 12 * 64;
+
+// Four scan waves, each with 16 of the 64 values, take chunk c while four waves form the matrices of chunk
+// c + 1 and four others the arrays of chunk c + 2, load chunk c + 3 and store the y of chunk c - 1.  A scan wave
+// holds its state transposed, acc[q][i] = S[value lane & 15][key 16q + 4g + i]: the layout in which a product's
+// result comes and in which the next takes it.  It reads nothing from memory: on this machine loads and
+// stores are waited for in their order, and a load behind a store waits for the store too.
+template <int DT, int XDT, int YDT, bool REV>
+__global__ __launch_bounds__(kScanThreads) void wkv7_scan_kernel(WkvScan p) {
+    __shared__ ScanLds lds;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int g = lane >> 4, m = lane & 15;
-    const int64_t pairs = p.shape.seqs * p.shape.heads;  // of a sequence and a head
-    const int64_t which = blockIdx.x % pairs;
-    const int64_t seq = which / p.shape.heads, head = which % p.shape.heads, H = p.shape.heads;
+    const int64_t H = p.shape.heads, seq = blockIdx.x / H, head = blockIdx.x % H;
     const Span span = span_of(p.shape, seq);
     const int64_t n = span.chunks();
     // the chunk's token of index i, i in processing order
     const auto token = [&](int64_t c, int i) { return REV ? kChunk * (n - 1 - c) + (kChunk - 1 - i) : kChunk * c + i; };
 
+    const auto exists = [&](int64_t c) { return token(c, m) < span.len; };
+    const auto row = [&](int64_t c) { return (span.start + (exists(c) ? token(c, m) : 0)) * H + head; };  // where n > 0
     if (wave < 4) {
-        // the wave that inverts shares its SIMD with no scan wave of TILES == 1
-        Producer<DT, REV> prod(p, lane, (wave + 1) & 3);
+        Elementwise<DT, XDT, REV> el{lane, wave};
         const auto load = [&](int64_t c) {
-            const int64_t t = token(c, m);
-            const bool exists = c < n && t < span.len;
-            prod.load((span.start + (exists ? t : 0)) * H + head, exists);
+            if (c < n) el.load(p.in, p.x, row(c), exists(c));
         };
-        if (n > 0) {
-            load(0);
-            prod.produce(buf[0]);
-            load(1);
-        }
+        const auto arrays = [&](int64_t c, int ring) {
+            if (c < n) el.run(lds.arrays[ring], lds.inverse[c & 1], lds.strong[ring][wave]);
+        };
+        const auto store_y = [&](int64_t c) {
+            if (c < 0 || !p.y || !exists(c)) return;
+            const int at = 16 * wave + 4 * g;
+            store4<YDT>(p.y, row(c) * kHead + at, *(const f32x4_t*)&lds.y[c & 1][m][at]);
+        };
+        load(0);
+        arrays(0, 0);
+        load(1);
         __syncthreads();
+        arrays(1, 1);
+        load(2);
+        __syncthreads();
+        int ring = 2;  // of chunk c + 2
         for (int64_t c = 0; c < n; ++c) {
-            if (c + 1 < n) {
-                prod.produce(buf[(c + 1) & 1]);
-                load(c + 2);
-            }
+            arrays(c + 2, ring);
+            store_y(c - 1);
+            load(c + 3);
+            ring = ring == 2 ? 0 : ring + 1;
+            __syncthreads();
+        }
+        store_y(n - 1);
+        return;
+    }
+    if (wave < 8) {
+        const auto matrix = [&](int64_t c, int ring) {
+            if (c >= n) return;
+            const int* f = lds.strong[ring];
+            form_matrix<DT, REV>(p.in, lds.arrays[ring], lds.inverse[c & 1], f[0] | f[1] | f[2] | f[3], lds.matrices[c & 1],
+                                 lane, wave - 4, row(c), exists(c));
+        };
+        __syncthreads();
+        matrix(0, 0);
+        __syncthreads();
+        int ring = 1;  // of chunk c + 1
+        for (int64_t c = 0; c < n; ++c) {
+            matrix(c + 1, ring);
+            ring = ring == 2 ? 0 : ring + 1;
             __syncthreads();
         }
         return;
     }
-    const int value = 16 * ((int)(blockIdx.x / pairs) * TILES + wave - 4) + m;
-    const int64_t state_at = (which * kHead + value) * kHead + 4 * g;
+    const int value = 16 * (wave - 8) + m;
+    const int64_t state_at = ((int64_t)blockIdx.x * kHead + value) * kHead + 4 * g;
     f32x4_t acc[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
         acc[q] = p.state ? *(const f32x4_t*)(p.state + state_at + 16 * q) : f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float x[4];
-    const auto load_x = [&](int64_t c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t t = token(c, 4 * g + i);
-            x[i] = c < n && t < span.len ? load_dt(p.x, XDT, ((span.start + t) * H + head) * kHead + value) : 0.f;
-        }
-    };
-    load_x(0);
     __syncthreads();
+    __syncthreads();
+    int ring = 0;
     for (int64_t c = 0; c < n; ++c) {
-        const Chunk& b = buf[c & 1];
+        const Arrays& b = lds.arrays[ring];
+        const Matrices& mat = lds.matrices[c & 1];
+        ring = ring == 2 ? 0 : ring + 1;
         const int64_t slot = (span.chunk0 + (REV ? n - 1 - c : c)) * H + head;
-        const f32x4_t v = {x[0], x[1], x[2], x[3]};
-        load_x(c + 1);
         if (p.states) {
             float* to = p.states + (slot * kHead + value) * kHead + 4 * g;
 #pragma unroll
             for (int q = 0; q < 4; ++q) *(f32x4_t*)(to + 16 * q) = acc[q];
         }
-        f32x4_t z = {0.f, 0.f, 0.f, 0.f}, sa = z, y = z;
+        const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+        f32x4_t to_sa[4], to_y[4], fs[4], fx[4], v;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) z = mma16(*(const f32x4_t*)&b.to_sa[m][16 * q + 4 * g], acc[q], z);
-        z = mma16(b.sa_x[lane], v, z);
-        sa = mma16(b.inv[lane], z, sa);
-        if (p.y) {
+        for (int i = 0; i < 4; ++i) v[i] = b.x[4 * g + i][value];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) y = mma16(*(const f32x4_t*)&b.to_y[m][16 * q + 4 * g], acc[q], y);
-            y = mma16(b.y_sa[lane], sa, y);
-            y = mma16(b.y_x[lane], v, y);
-        }
+        for (int q = 0; q < 4; ++q) to_sa[q] = *(const f32x4_t*)&b.to_sa[m][16 * q + 4 * g];
+        const f32x4_t sa_x = mat.sa_x[lane], inv = mat.inv[lane];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) to_y[q] = *(const f32x4_t*)&b.to_y[m][16 * q + 4 * g];
+        const f32x4_t y_sa = mat.y_sa[lane], y_x = mat.y_x[lane];
+        f32x4_t z[2] = {zero, zero}, y[2] = {zero, zero};
+        z[0] = mma16(sa_x, v, z[0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z[q & 1] = mma16(to_sa[q], acc[q], z[q & 1]);
+        z[0] += z[1];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) y[q & 1] = mma16(to_y[q], acc[q], y[q & 1]);
+        y[1] = mma16(y_x, v, y[1]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const f32x4_t d = *(const f32x4_t*)&b.decay[16 * q + 4 * g];
-            f32x4_t fs, fx;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                acc[q][i] *= d[i];
-                fs[i] = b.from_sa[4 * g + i][16 * q + m];
-                fx[i] = b.from_x[4 * g + i][16 * q + m];
+                fs[q][i] = b.from_sa[4 * g + i][16 * q + m];
+                fx[q][i] = b.from_x[4 * g + i][16 * q + m];
             }
-            acc[q] = mma16(fx, v, acc[q]);
-            acc[q] = mma16(fs, sa, acc[q]);
         }
+        const f32x4_t sa = mma16(inv, z[0], zero);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t t = token(c, 4 * g + i);
-            if (t < span.len && p.y) store_dt(p.y, YDT, ((span.start + t) * H + head) * kHead + value, y[i]);
-            // rows in the order of time, the missing ones 0
-            if (p.sa) p.sa[(slot * kChunk + (REV ? kChunk - 1 - (4 * g + i) : 4 * g + i)) * kHead + value] = sa[i];
+        for (int q = 0; q < 4; ++q) {
+            acc[q] *= *(const f32x4_t*)&b.decay[16 * q + 4 * g];
+            acc[q] = mma16(fx[q], v, acc[q]);
+        }
+        y[0] = mma16(y_sa, sa, y[0]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // one step of each sum in turn
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[q] = mfma4(fs[q][i], sa[i], acc[q]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds.y[c & 1][4 * g + i][value] = y[0][i] + y[1][i];
+        if (p.sa) {  // rows in the order of time, the missing ones 0
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                p.sa[(slot * kChunk + (REV ? kChunk - 1 - (4 * g + i) : 4 * g + i)) * kHead + value] = sa[i];
         }
         __syncthreads();
     }
@@ -488,14 +584,8 @@ __device__ __attribute__((noinline)) void strong_grads(const GradLds& lds, int w
 // Four contiguous values of a row as fp32.
 template <int DT>
 RQ_DEV f32x4_t load4(const void* p, int64_t at, bool there) {
-    if (!there) return f32x4_t{0.f, 0.f, 0.f, 0.f};
-    if constexpr (DT == RQ_F32) {
-        return *(const f32x4_t*)((const float*)p + at);
-    } else {
-        const uint2 u = *(const uint2*)((const uint16_t*)p + at);
-        return f32x4_t{dt_traits<DT>::to_f32((uint16_t)(u.x & 0xffffu)), dt_traits<DT>::to_f32((uint16_t)(u.x >> 16)),
-                       dt_traits<DT>::to_f32((uint16_t)(u.y & 0xffffu)), dt_traits<DT>::to_f32((uint16_t)(u.y >> 16))};
-    }
+    const f32x4_t x = unpack_raw4<DT>(load_raw4<DT>(p, at));
+    return there ? x : f32x4_t{0.f, 0.f, 0.f, 0.f};
 }
 
 // A block is one chunk of one head; each of its four waves has 16 keys, and one of the four pair
@@ -525,7 +615,7 @@ __global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
 
     // rows of tokens: dy, dz, sa, v of token m, values 16q + 4g + i
     const bool there = t0 + m < span.len;
-    const int64_t row = (span.start + t0 + m) * H + head;
+    const int64_t row = (span.start + t0 + (there ? m : 0)) * H + head;
     f32x4_t dy[4], dz[4], sa[4], v[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -540,14 +630,18 @@ __global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
     bool has[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t t = t0 + 4 * g + i, at = ((span.start + t) * H + head) * kHead + key;
+        const int64_t t = t0 + 4 * g + i;
         has[i] = t < span.len;
-        r[i] = has[i] ? load_dt(p.in.r, DT, at) : 0.f;
-        a[i] = has[i] ? load_dt(p.in.a, DT, at) : 0.f;
-        b[i] = has[i] ? load_dt(p.in.b, DT, at) : 0.f;
-        k[i] = has[i] ? load_dt(p.in.k, DT, at) : 0.f;
-        w[i] = has[i] ? load_dt(p.in.w, DT, at) : 0.f;
+        const int64_t at = ((span.start + (has[i] ? t : t0)) * H + head) * kHead + key;
+        r[i] = load_dt(p.in.r, DT, at);
+        a[i] = load_dt(p.in.a, DT, at);
+        b[i] = load_dt(p.in.b, DT, at);
+        k[i] = load_dt(p.in.k, DT, at);
+        w[i] = load_dt(p.in.w, DT, at);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (!has[i]) r[i] = a[i] = b[i] = k[i] = 0.f;
     const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
     f32x4_t gr = zero, ga = zero, gb = zero, gk = zero;
     float through = 0.f;  // sum over the values of S dS' of this key
@@ -802,17 +896,12 @@ __global__ __launch_bounds__(256) void wkv7_rest_kernel(WkvShape s, RestTensors 
     }
 }
 
-template <int DT, int XDT, int YDT, bool REV>
-hipError_t scan_tiles(const WkvScan& a, hipStream_t s) {
-    const int64_t pairs = a.shape.seqs * a.shape.heads;
-    if (pairs >= 192) wkv7_scan_kernel<DT, XDT, YDT, REV, 4><<<dim3((unsigned)pairs), 512, 0, s>>>(a);
-    else wkv7_scan_kernel<DT, XDT, YDT, REV, 1><<<dim3((unsigned)(4 * pairs)), 320, 0, s>>>(a);
-    return hipGetLastError();
-}
-
 template <int DT, int ODT>
 hipError_t scan_dt(const WkvScan& a, hipStream_t s) {
-    return a.reverse ? scan_tiles<DT, ODT, DT, true>(a, s) : scan_tiles<DT, DT, ODT, false>(a, s);
+    const dim3 grid((unsigned)(a.shape.seqs * a.shape.heads));
+    if (a.reverse) wkv7_scan_kernel<DT, ODT, DT, true><<<grid, kScanThreads, 0, s>>>(a);
+    else wkv7_scan_kernel<DT, DT, ODT, false><<<grid, kScanThreads, 0, s>>>(a);
+    return hipGetLastError();
 }
 
 template <int DT, int ODT>
