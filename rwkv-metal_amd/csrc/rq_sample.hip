@@ -6,8 +6,16 @@
 //   the token: the first by index at which the running sum of what stays exceeds u times the whole
 //
 // Nothing is sorted: what stays is everything above a threshold and the first few, by
-// index, of those that equal it.  The threshold of top_k is found by counts of the logits'
-// bits, eight at a time from the top, that of top_p by sums in the same way.
+// index, of those that equal it.  A block takes a row, in few passes over it:
+//   1. the largest logit;
+//   2. a bound that everything that stays reaches and little else does.  top_k up to 1024: the
+//      k-th largest of the 1024 lanes' maxima.  top_p alone: the sums of e_i in 2048 bins of
+//      equal width below the largest logit, then the bin in which the border lies;
+//   3. the logits that reach it, by index, into LDS: few enough for everything else.
+// Where they are too many for that (a flat row) or nothing bounds them, the row is read
+// again instead: for the border by bins and then among the logits of one bin, or, where
+// too many share a bin (many equal ones, a range of 10^38), by the logits' bits, eight at a time
+// from the top; and for the sums of what stays.
 //
 // The sums decide which token comes, so they are exact: every e_i is a float64 rounded to
 // a multiple of 2^-36 (coarser for a vocabulary past 2^17), and a row's sum of such
@@ -67,15 +75,25 @@ struct Weights {
     RQ_DEV double quanta(double e) const { return (e + grid) - grid; }
 };
 
+constexpr int kBins = 2048;  // for sums below the largest logit
+constexpr int kBin = 1024;   // logits of one bin that are told apart in LDS
+constexpr int kPart = 384;   // logits of a wave's part of the row that are kept in LDS
+
 struct Lds {
-    double sums[256];
-    uint32_t counts[256];
+    double sums[kBins];  // of the bins; of 256 of them by bits
+    double bin_sums[kBin];
+    uint32_t bin_keys[kBin];
+    uint32_t in_bin;
+    double part_e[kWaves][kPart];  // what each adds
+    uint32_t part_key[kWaves][kPart], part_at[kWaves][kPart];
+    uint32_t part_n[kWaves];
+    uint32_t digits[2][kWaves][16];
     double wave_sum[kWaves];
     uint32_t wave_count[kWaves];
-    float wave_max[kWaves];
-    int64_t wave_at[kWaves];
-    double found_sum;
-    uint32_t found_bin, found_count;
+    float wave_max[kWaves], wave_min[kWaves];
+    unsigned long long first;
+    double found_sum, total;
+    uint32_t found, found_key;
     int nan;
 };
 
@@ -85,93 +103,334 @@ RQ_DEV double wave_sum64(double x) {
     return x;
 }
 
+RQ_DEV uint32_t wave_sum32(uint32_t x) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+    return x;
+}
+
+// Eight neighbouring logits as they are stored.
+template <int DT>
+struct Raw8 {
+    Bytes16 v[kLane / kVec<DT>];
+};
+
+// A wave's logits, a run of whole steps of 512; every pass reads them again, from the caches but
+// for the first.
 template <int DT>
 struct Row {
     const uint8_t* p;
-    int64_t n, from, steps;  // the wave's first logit and its steps
+    int64_t n, from;  // the wave's first logit
+    int whole, steps; // steps of 512 logits, and with the last one, of fewer
     int lane;
-    // f(index of the first, eight logits), in the order of the index within a wave; -inf past the end
+
+    RQ_DEV Row(const void* logits, int64_t row, int64_t vocab, int wave, int lane_)
+        : p((const uint8_t*)logits + row * vocab * kSize<DT>), n(vocab), lane(lane_) {
+        const int64_t per = (vocab + kWaves * kStep - 1) / (kWaves * kStep);
+        from = wave * per * kStep;
+        const int64_t left = vocab > from ? vocab - from : 0;
+        whole = (int)std::min<int64_t>(per, left / kStep);
+        steps = (int)std::min<int64_t>(per, (left + kStep - 1) / kStep);
+    }
+    RQ_DEV int64_t at(int s) const { return from + (int64_t)s * kStep + lane * kLane; }
+    RQ_DEV void fetch(int s, Raw8<DT>& to) const {
+        const int64_t i = at(s);
+        if (s < whole) {
+#pragma unroll
+            for (int j = 0; j < kLane / kVec<DT>; ++j) to.v[j] = *(const Bytes16*)(p + (i + j * kVec<DT>)*kSize<DT>);
+            return;
+        }
+        uint32_t w[kLane / kVec<DT> * 4];  // -inf past the end
+        if constexpr (DT == RQ_F32) {
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) w[j] = i + j < n ? ((const uint32_t*)p)[i + j] : 0xff800000u;
+        } else {
+            constexpr uint32_t kNone = DT == RQ_BF16 ? 0xff80u : 0xfc00u;
+#pragma unroll
+            for (int j = 0; j < kLane; j += 2) {
+                const uint32_t lo = i + j < n ? ((const uint16_t*)p)[i + j] : kNone;
+                const uint32_t hi = i + j + 1 < n ? ((const uint16_t*)p)[i + j + 1] : kNone;
+                w[j / 2] = lo | (hi << 16);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kLane / kVec<DT>; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) to.v[j].w[x] = w[4 * j + x];
+    }
+    // f(step, eight logits) in the order of the index, while it gives true; two steps in flight
     template <class F>
     RQ_DEV void each(F f) const {
-        for (int64_t s = 0; s < steps; ++s) {
+        if (steps == 0) return;
+        Raw8<DT> now, next;
+        fetch(0, now);
+        for (int s = 0; s < steps; ++s) {
+            if (s + 1 < steps) fetch(s + 1, next);
             float l[kLane];
-            const int64_t at = load(s, l);
-            f(at, l);
-        }
-    }
-    RQ_DEV int64_t load(int64_t s, float* l) const {
-        const int64_t at = from + s * kStep + lane * kLane;
-        if (at + kLane <= n) {
 #pragma unroll
-            for (int i = 0; i < kLane; i += kVec<DT>) load_vec<DT>(p + (at + i) * kSize<DT>, l + i);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kLane; ++i) l[i] = at + i < n ? load_dt(p, DT, at + i) : -INFINITY;
+            for (int j = 0; j < kLane / kVec<DT>; ++j) unpack_vec<DT>(now.v[j], l + j * kVec<DT>);
+            if (!f(s, l)) return;
+            now = next;
         }
-        return at;
     }
 };
 
-// The class of equal keys in which the running total from the largest key reaches `want` (counts, or
-// sums where SUMS): its key, and in `before` the total of the larger ones.  `weight(l, key)` is
-// what a logit adds, 0 for one that is out; `extra` is added for `extra_key`.
-template <bool SUMS, int DT, class W>
-RQ_DEV uint32_t select_key(const Row<DT>& row, Lds& lds, double want, double& before, W weight, uint32_t extra_key,
-                           double extra) {
-    uint32_t prefix = 0, mask = 0;
-    before = 0.0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        __syncthreads();
-        if (threadIdx.x < 256) {
-            lds.sums[threadIdx.x] = 0.0;
-            lds.counts[threadIdx.x] = 0;
+// Bins of equal width that grow as the logits fall.
+struct Bins {
+    float top, scale;
+    RQ_DEV Bins(float top_, float range) : top(top_), scale((float)(kBins - 1) / range) {}
+    RQ_DEV int of(float l) const {
+        const float x = l == top ? 0.f : (top - l) * scale;
+        return x < (float)(kBins - 1) ? (int)x : kBins - 1;
+    }
+};
+
+template <int BINS>
+RQ_DEV void clear_bins(Lds& lds) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < BINS; i += kThreads) lds.sums[i] = 0.0;
+    if (threadIdx.x == 0) lds.in_bin = 0;
+    __syncthreads();
+}
+
+// The bin, from the first, in which the running total reaches `want` (less than 0: `share` of the
+// whole, at least `quantum`); lds.found, the total before it lds.found_sum, what was looked for lds.total.
+template <int BINS>
+RQ_DEV void find_bin(Lds& lds, double before, double want, double share, double quantum) {
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        constexpr int PER = BINS / 64;
+        const int lane = threadIdx.x;
+        double sum = 0.0;
+#pragma unroll 8
+        for (int i = 0; i < PER; ++i) sum += lds.sums[lane * PER + i];
+        double upto = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const double x = __shfl_up(upto, d);
+            if (lane >= d) upto += x;
         }
-        __syncthreads();
-        row.each([&](int64_t, const float* l) {
+        if (want < 0.0) want = fmax(share * __shfl(upto, 63), quantum);
+        double at = before + (upto - sum);
+        if (at < want && before + upto >= want) {
+            int i = 0;
+            while (i < PER - 1 && at + lds.sums[lane * PER + i] < want) at += lds.sums[lane * PER + i++];
+            lds.found = lane * PER + i;
+            lds.found_sum = at;
+            lds.total = want;
+        }
+    }
+    __syncthreads();
+}
+
+// Among the logits of one bin, whose keys and terms lie in LDS: the class of equal keys in which the running total
+// from the largest key reaches `want`, and in `before` the total of the larger ones.  `extra` is added
+// for extra_key, which is below all others.
+RQ_DEV uint32_t key_in_bin(Lds& lds, double base, double want, double& before, uint32_t extra_key, bool with_extra) {
+    const uint32_t n = lds.in_bin;
+    if (threadIdx.x == 0 && with_extra) {  // reached where none of the others is
+        lds.found_key = extra_key;
+        lds.found_sum = -1.0;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+        const uint32_t key = lds.bin_keys[i];
+        double above = base, same = 0.0;
+        for (uint32_t j = 0; j < n; ++j) {
+            const uint32_t other = lds.bin_keys[j];
+            const double x = lds.bin_sums[j];
+            above += other > key ? x : 0.0;
+            same += other == key ? x : 0.0;
+        }
+        if (above < want && above + same >= want) {
+            lds.found_key = key;
+            lds.found_sum = above;
+        }
+    }
+    __syncthreads();
+    before = lds.found_sum;
+    const uint32_t key = lds.found_key;
+    if (before < 0.0) {
+        before = base;
+        for (uint32_t j = 0; j < n; ++j) before += lds.bin_sums[j];
+    }
+    __syncthreads();
+    return key;
+}
+
+RQ_DEV void add_to_bin(Lds& lds, uint32_t key, double x) {
+    const uint32_t at = atomicAdd(&lds.in_bin, 1u);
+    if (at < kBin) {
+        lds.bin_keys[at] = key;
+        lds.bin_sums[at] = x;
+    }
+}
+
+// The same over the whole row, once its bins are found (lds.found ...).  weight(l, key) is what a logit adds, and
+// may_weigh(l, key) whether that is more than 0 without working it out.
+template <int DT, class M, class W>
+RQ_DEV uint32_t key_in_row(const Row<DT>& row, Lds& lds, const Bins& bins, double& before, M may_weigh, W weight,
+                           uint32_t extra_key, double extra) {
+    const int bin = lds.found;
+    const double base = lds.found_sum, want = lds.total;
+    row.each([&](int, const float* l) {
+#pragma unroll
+        for (int i = 0; i < kLane; ++i) {
+            const uint32_t key = key_of(l[i]);
+            if (!may_weigh(l[i], key) || bins.of(l[i]) != bin) continue;
+            const double x = weight(l[i], key);
+            if (x > 0.0) add_to_bin(lds, key, x);
+        }
+        return true;
+    });
+    __syncthreads();
+    const bool with_extra = extra > 0.0 && bins.of(of_key(extra_key)) == bin;
+    if (lds.in_bin <= kBin) return key_in_bin(lds, base, want, before, extra_key, with_extra);
+    // by bits: digit d of a key goes to bin 255 - d
+    uint32_t prefix = 0, mask = 0;
+    before = base;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        clear_bins<256>(lds);
+        row.each([&](int, const float* l) {
 #pragma unroll
             for (int i = 0; i < kLane; ++i) {
                 const uint32_t key = key_of(l[i]);
-                if (l[i] == -INFINITY || (key & mask) != prefix) continue;
+                if ((key & mask) != prefix || !may_weigh(l[i], key) || bins.of(l[i]) != bin) continue;
                 const double x = weight(l[i], key);
-                if constexpr (SUMS) {
-                    if (x > 0.0) unsafeAtomicAdd(&lds.sums[(key >> shift) & 255], x);
-                } else {
-                    atomicAdd(&lds.counts[(key >> shift) & 255], (uint32_t)x);
-                }
+                if (x > 0.0) unsafeAtomicAdd(&lds.sums[255 - ((key >> shift) & 255)], x);
             }
+            return true;
         });
-        __syncthreads();
-        if (threadIdx.x < 64) {  // four bins a lane, from the largest
-            const int lane = threadIdx.x;
-            double bin[4], sum = 0.0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int b = 255 - 4 * lane - i;
-                bin[i] = SUMS ? lds.sums[b] : (double)lds.counts[b];
-                if (extra > 0.0 && (extra_key & mask) == prefix && (int)((extra_key >> shift) & 255) == b) bin[i] += extra;
-                sum += bin[i];
-            }
-            double upto = sum;
-            for (int d = 1; d < 64; d <<= 1) {
-                const double x = __shfl_up(upto, d);
-                if (lane >= d) upto += x;
-            }
-            double at = before + (upto - sum);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (at < want && at + bin[i] >= want) {
-                    lds.found_bin = 255 - 4 * lane - i;
-                    lds.found_sum = at;
-                }
-                at += bin[i];
-            }
-        }
-        __syncthreads();
+        if (threadIdx.x == 0 && with_extra && (extra_key & mask) == prefix)
+            unsafeAtomicAdd(&lds.sums[255 - ((extra_key >> shift) & 255)], extra);
+        find_bin<256>(lds, before, want, 0.0, 0.0);
         before = lds.found_sum;
-        prefix |= (lds.found_bin & 255u) << shift;
+        prefix |= (255u - lds.found) << shift;
         mask |= 0xffu << shift;
     }
     return prefix;
+}
+
+// The k-th largest of the keys that the waves hold, four bits at a time: `n` a lane, key(j) its j-th (0:
+// none).  `above` is the number of larger ones.  1 <= k <= their number.
+template <class K>
+RQ_DEV uint32_t kth_key(Lds& lds, int n, K key, uint32_t k, uint32_t& above) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t prefix = 0;
+    above = 0;
+#pragma unroll 1
+    for (int shift = 28, turn = 0; shift >= 0; shift -= 4, turn ^= 1) {
+        uint32_t mine = 0;  // lane d: the keys of this wave that are at least prefix with digit d
+        for (int j = 0; j < n; ++j) {
+            const uint32_t x = key(j);
+#pragma unroll
+            for (uint32_t d = 1; d < 16; ++d) {
+                const uint32_t c = __popcll(__ballot(x >= (prefix | (d << shift))));
+                mine += lane == (int)d ? c : 0;
+            }
+        }
+        if (lane < 16) lds.digits[turn][wave][lane] = mine;
+        __syncthreads();
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) c += lds.digits[turn][i][lane & 15];
+        // the largest digit that k keys reach
+        const uint64_t reach = __ballot(lane > 0 && lane < 16 && c >= k);
+        const int d = reach ? 63 - __builtin_clzll(reach) : 0;
+        const uint32_t over = __shfl(c, d + 1);  // keys with a larger digit
+        if (d < 15) above = over;
+        prefix |= (uint32_t)d << shift;
+    }
+    return prefix;
+}
+
+// The row's logits for which reaches(l, key) holds into LDS, each wave's by index.  Whether they fit.
+template <int DT, class P>
+RQ_DEV bool gather(const Row<DT>& row, Lds& lds, P reaches) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t have = 0;
+    row.each([&](int s, const float* l) {
+        uint32_t at = have;
+        uint32_t in = 0;
+#pragma unroll
+        for (int i = 0; i < kLane; ++i) {
+            const bool is = l[i] > -INFINITY && reaches(l[i], key_of(l[i]));
+            const uint64_t who = __ballot(is);
+            in |= (uint32_t)is << i;
+            at += __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+            have += __popcll(who);
+        }
+        if (have > kPart) return false;
+#pragma unroll
+        for (int i = 0; i < kLane; ++i) {
+            if (in >> i & 1) {
+                lds.part_key[wave][at] = key_of(l[i]);
+                lds.part_at[wave][at] = (uint32_t)(row.at(s) + i);
+                ++at;
+            }
+        }
+        return true;
+    });
+    if (lane == 0) lds.part_n[wave] = have;
+    return __syncthreads_and(have <= kPart);
+}
+
+// How many of `here` equal logits behind `so_far` others stay.
+RQ_DEV uint32_t staying(int64_t ties, uint32_t so_far, uint32_t here) {
+    const int64_t left = ties - (int64_t)so_far;
+    return left <= 0 ? 0u : (uint32_t)std::min<int64_t>(left, here);
+}
+
+// Of the waves' sums and equal logits (lds.wave_sum, wave_count): the whole, the number that the
+// running sum has to exceed, and the wave in which it does, with what lies before it.
+struct Place {
+    double whole, target, at;
+    uint32_t so_far;
+    int wave;
+};
+RQ_DEV Place find_wave(const Lds& lds, int64_t ties, double tie, float u, double quantum) {
+    Place f{0.0, 0.0, 0.0, 0, 0};
+    uint32_t so_far = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        f.whole += lds.wave_sum[i] + staying(ties, so_far, lds.wave_count[i]) * tie;
+        so_far += lds.wave_count[i];
+    }
+    // at most one quantum below the whole: the last that stays, where u is 1 or more
+    f.target = u > 0.f ? fmin((double)u * f.whole, f.whole - quantum) : 0.0;
+    for (int i = 0; i < kWaves; ++i) {
+        const double here = lds.wave_sum[i] + staying(ties, f.so_far, lds.wave_count[i]) * tie;
+        f.wave = i;
+        if (f.at + here > f.target) break;
+        f.at += here;
+        f.so_far += lds.wave_count[i];
+    }
+    return f;
+}
+
+RQ_DEV void choose(const SampleArgs& p, int64_t r, int64_t at, float l, const Weights& w, float temperature, double whole) {
+    p.token[r] = at;
+    if (p.logprob) {
+        const double z = w.inf ? 0.0 : ((double)l - w.top) / (double)temperature;
+        p.logprob[r] = (float)(z - log(whole));
+    }
+}
+
+RQ_DEV uint32_t scan32(uint32_t x, int lane) {  // up to and with the lane's own
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+RQ_DEV double scan64(double x, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
 }
 
 template <int DT>
@@ -179,56 +438,53 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
     __shared__ Lds lds;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t r = blockIdx.x, n = p.vocab;
-    const int64_t steps = (n + kWaves * kStep - 1) / (kWaves * kStep);
-    const Row<DT> row{(const uint8_t*)p.logits + r * n * kSize<DT>, n, wave * steps * kStep, steps, lane};
+    const Row<DT> row(p.logits, r, n, wave, lane);
     const float temperature = p.temperature ? p.temperature[r] : p.temperature_all;
-    const int64_t top_k = p.top_k ? p.top_k[r] : p.top_k_all;
+    int64_t top_k = p.top_k ? p.top_k[r] : p.top_k_all;
     const float top_p = p.top_p ? p.top_p[r] : p.top_p_all;
     float min_p = p.min_p ? p.min_p[r] : p.min_p_all;
+    const float u = p.u[r];
     min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
 
-    // the largest logit, and the first place that has it
-    float top = -INFINITY;
-    int64_t top_at = n;
+    float top = -INFINITY, low = INFINITY;
     uint32_t there = 0;
     bool nan = false;
-    row.each([&](int64_t at, const float* l) {
+    row.each([&](int, const float* l) {
 #pragma unroll
         for (int i = 0; i < kLane; ++i) {
             nan |= l[i] != l[i];
-            there += l[i] > -INFINITY;
-            if (l[i] > top) {
-                top = l[i];
-                top_at = at + i;
-            }
+            const bool is = l[i] > -INFINITY;
+            there += is;
+            top = fmaxf(top, l[i]);
+            low = is ? fminf(low, l[i]) : low;
         }
+        return true;
     });
+    const float lane_top = top;
 #pragma unroll
     for (int d = 32; d; d >>= 1) {
-        const float x = __shfl_xor(top, d);
-        const int64_t at = __shfl_xor((long long)top_at, d);
-        there += __shfl_xor(there, d);
-        if (x > top || (x == top && at < top_at)) {
-            top = x;
-            top_at = at;
-        }
+        top = fmaxf(top, __shfl_xor(top, d));
+        low = fminf(low, __shfl_xor(low, d));
     }
-    if (threadIdx.x == 0) lds.nan = 0;
+    there = wave_sum32(there);
+    if (threadIdx.x == 0) {
+        lds.nan = 0;
+        lds.first = ~0ull;
+    }
     __syncthreads();
     if (__any(nan) && lane == 0) lds.nan = 1;
     if (lane == 0) {
         lds.wave_max[wave] = top;
-        lds.wave_at[wave] = top_at;
+        lds.wave_min[wave] = low;
         lds.wave_count[wave] = there;
     }
     __syncthreads();
     there = 0;
+#pragma unroll
     for (int i = 0; i < kWaves; ++i) {
         there += lds.wave_count[i];
-        if (lds.wave_max[i] > top || (lds.wave_max[i] == top && lds.wave_at[i] < top_at)) {
-            top = lds.wave_max[i];
-            top_at = lds.wave_at[i];
-        }
+        top = fmaxf(top, lds.wave_max[i]);
+        low = fminf(low, lds.wave_min[i]);
     }
     if (lds.nan || there == 0) {  // nothing to choose from
         if (threadIdx.x == 0) {
@@ -237,9 +493,18 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
         }
         return;
     }
-    if (!(temperature > 0.f) || top_k == 1) {
+    if (!(temperature > 0.f) || top_k == 1) {  // the first that has the largest
+        unsigned long long first = ~0ull;
+        row.each([&](int s, const float* l) {
+#pragma unroll
+            for (int i = kLane - 1; i >= 0; --i)
+                if (l[i] == top) first = std::min<unsigned long long>(first, row.at(s) + i);
+            return true;
+        });
+        if (first != ~0ull) atomicMin(&lds.first, first);
+        __syncthreads();
         if (threadIdx.x == 0) {
-            p.token[r] = top_at;
+            p.token[r] = (int64_t)lds.first;
             if (p.logprob) p.logprob[r] = 0.f;
         }
         return;
@@ -248,33 +513,132 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
     const Weights w{(double)top, 1.4426950408889634 / (double)temperature,
                     6755399441055744.0 / (double)(1ll << bits), top == INFINITY};
     const double quantum = 1.0 / (double)(1ll << bits);
+    if (top_k < 0 || top_k >= (int64_t)there) top_k = 0;
+    const bool by_sum = top_p < 1.f;
+    // past 26 temperatures below the largest, e_i is rounded to 0
+    const Bins sum_bins(top, fminf(top - low, 26.f * temperature));
 
     // what stays: keys above `least`, and the first `ties` that equal it
     uint32_t least = 0;
     int64_t ties = 0;
-    if (top_k > 0 && top_k < (int64_t)there) {
-        double before;
-        least = select_key<false, DT>(row, lds, (double)top_k, before, [](float, uint32_t) { return 1.0; }, 0, 0.0);
-        ties = top_k - (int64_t)before;
-    }
-    if (top_p < 1.f) {
-        const double tied = ties ? (double)ties * w.quanta(w.exact(of_key(least))) : 0.0;
-        const auto weight = [&](float l, uint32_t key) { return key > least ? w.quanta(w.exact(l)) : 0.0; };
-        double sum = 0.0;
-        row.each([&](int64_t, const float* l) {
+    bool listed = false;
+    if (top_k > 0) {
+        const uint32_t mine = lane_top > -INFINITY ? key_of(lane_top) : 0;
+        uint32_t above;
+        if (top_k <= kThreads && __syncthreads_count(mine != 0) >= (int)top_k) {
+            const uint32_t bound = kth_key(lds, 1, [&](int) { return mine; }, (uint32_t)top_k, above);
+            listed = gather(row, lds, [&](float, uint32_t key) { return key >= bound; });
+        }
+        if (listed) {
+            uint32_t longest = 0;
 #pragma unroll
-            for (int i = 0; i < kLane; ++i)
-                if (l[i] > -INFINITY) sum += weight(l[i], key_of(l[i]));
-        });
-        sum = wave_sum64(sum);
-        __syncthreads();
-        if (lane == 0) lds.wave_sum[wave] = sum;
-        __syncthreads();
-        sum = tied;
-        for (int i = 0; i < kWaves; ++i) sum += lds.wave_sum[i];
-        const double want = fmax(top_p > 0.f ? (double)top_p * sum : 0.0, quantum);
-        double before;
-        const uint32_t key = select_key<true, DT>(row, lds, want, before, weight, least, tied);
+            for (int i = 0; i < kWaves; ++i) longest = std::max(longest, lds.part_n[i]);
+            least = kth_key(lds, (longest + 63) / 64,
+                            [&](int j) {
+                                const uint32_t i = lane + 64 * j;
+                                return i < lds.part_n[wave] ? lds.part_key[wave][i] : 0u;
+                            },
+                            (uint32_t)top_k, above);
+            ties = top_k - above;
+        } else {
+            // logits further below count as one bin: their range may be that of the type
+            const Bins bins(top, fminf(top - low, 64.f));
+            const auto any = [](float l, uint32_t) { return l > -INFINITY; };
+            double before;
+            clear_bins<kBins>(lds);
+            row.each([&](int, const float* l) {
+#pragma unroll
+                for (int i = 0; i < kLane; ++i)
+                    if (l[i] > -INFINITY) unsafeAtomicAdd(&lds.sums[bins.of(l[i])], 1.0);
+                return true;
+            });
+            find_bin<kBins>(lds, 0.0, (double)top_k, 0.0, 0.0);
+            least = key_in_row(row, lds, bins, before, any, [](float, uint32_t) { return 1.0; }, 0, 0.0);
+            ties = top_k - (int64_t)before;
+            listed = gather(row, lds, [&](float, uint32_t key) { return key >= least; });
+        }
+    }
+    if (by_sum) {
+        const double tied = ties ? (double)ties * w.quanta(w.exact(of_key(least))) : 0.0;
+        double before, want;
+        uint32_t key;
+        clear_bins<kBins>(lds);
+        if (threadIdx.x == 0 && ties) unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(least))], tied);
+        if (listed) {
+            for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
+                const uint32_t k = lds.part_key[wave][i];
+                if (k <= least) continue;
+                const double x = w.quanta(w.exact(of_key(k)));
+                lds.part_e[wave][i] = x;
+                unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(k))], x);
+            }
+            find_bin<kBins>(lds, 0.0, -1.0, fmax((double)top_p, 0.0), quantum);
+            const int bin = lds.found;
+            const double base = lds.found_sum;
+            want = lds.total;
+            for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
+                const uint32_t k = lds.part_key[wave][i];
+                if (k > least && sum_bins.of(of_key(k)) == bin && lds.part_e[wave][i] > 0.0) add_to_bin(lds, k, lds.part_e[wave][i]);
+            }
+            __syncthreads();
+            if (lds.in_bin <= kBin) {
+                key = key_in_bin(lds, base, want, before, least, ties && sum_bins.of(of_key(least)) == bin);
+            } else {
+                listed = false;  // found again from the row
+            }
+            __syncthreads();
+        }
+        const auto may_weigh = [&](float l, uint32_t k) { return k > least && l > -INFINITY; };
+        const auto weight = [&](float l, uint32_t) { return w.quanta(w.exact(l)); };
+        const bool from_row = !listed;
+        if (from_row) {
+            if (top_k == 0) {
+                row.each([&](int, const float* l) {
+                    double x[kLane];
+#pragma unroll
+                    for (int i = 0; i < kLane; ++i) x[i] = w.quanta(w.exact(l[i]));
+#pragma unroll
+                    for (int i = 0; i < kLane; ++i)
+                        if (x[i] > 0.0) unsafeAtomicAdd(&lds.sums[sum_bins.of(l[i])], x[i]);
+                    return true;
+                });
+            } else {
+                clear_bins<kBins>(lds);
+                if (threadIdx.x == 0 && ties) unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(least))], tied);
+                row.each([&](int, const float* l) {
+#pragma unroll
+                    for (int i = 0; i < kLane; ++i) {
+                        const uint32_t k = key_of(l[i]);
+                        if (!may_weigh(l[i], k)) continue;
+                        const double x = weight(l[i], k);
+                        if (x > 0.0) unsafeAtomicAdd(&lds.sums[sum_bins.of(l[i])], x);
+                    }
+                    return true;
+                });
+            }
+            find_bin<kBins>(lds, 0.0, -1.0, fmax((double)top_p, 0.0), quantum);
+            want = lds.total;
+            const int bin = lds.found;
+            const double base = lds.found_sum;
+            if (top_k == 0) listed = gather(row, lds, [&](float l, uint32_t) { return sum_bins.of(l) <= bin; });
+            if (listed) {
+                for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
+                    const uint32_t k = lds.part_key[wave][i];
+                    const double x = w.quanta(w.exact(of_key(k)));
+                    lds.part_e[wave][i] = x;
+                    if (x > 0.0 && sum_bins.of(of_key(k)) == bin) add_to_bin(lds, k, x);
+                }
+                __syncthreads();
+            }
+            if (listed && lds.in_bin <= kBin) {
+                key = key_in_bin(lds, base, want, before, 0, false);
+            } else {
+                __syncthreads();
+                if (threadIdx.x == 0) lds.in_bin = 0;
+                __syncthreads();
+                key = key_in_row(row, lds, sum_bins, before, may_weigh, weight, least, tied);
+            }
+        }
         // as many of that class as are needed to reach it
         const double each = w.quanta(w.exact(of_key(key)));
         double more = __builtin_ceil((want - before) / each);
@@ -283,113 +647,145 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
         ties = ties && key == least ? std::min<int64_t>(ties, (int64_t)more) : (int64_t)more;
         least = key;
     }
+    if (!listed && top_k == 0 && !by_sum && min_p > 0.f) {
+        // a little below the border (NaN where any logit may stay): the terms themselves decide
+        const float border = (float)(log((double)min_p) * (double)temperature) * 1.0001f - 1e-6f * fabsf(top);
+        if (!w.inf) listed = gather(row, lds, [&](float l, uint32_t) { return !(l - top < border); });
+    }
 
-    // each wave's part of what stays, by index
     const double tie_e = ties ? w.exact(of_key(least)) : 0.0;
     const double tie = ties && tie_e >= (double)min_p ? w.quanta(tie_e) : 0.0;
     const auto above = [&](float l, uint32_t key) {
-        if (!(l > -INFINITY) || key <= least) return 0.0;
         const double e = w.exact(l);
-        return e >= (double)min_p ? w.quanta(e) : 0.0;
+        return l > -INFINITY && key > least && e >= (double)min_p ? w.quanta(e) : 0.0;
     };
+
+    if (listed) {
+        double sum = 0.0;
+        uint32_t equal = 0;
+        const uint32_t mine = lds.part_n[wave];
+        for (uint32_t i = lane; i < mine; i += 64) {
+            const uint32_t key = lds.part_key[wave][i];
+            const double x = above(of_key(key), key);
+            lds.part_e[wave][i] = x;
+            sum += x;
+            equal += ties && key == least;
+        }
+        sum = wave_sum64(sum);
+        equal = wave_sum32(equal);
+        __syncthreads();
+        if (lane == 0) {
+            lds.wave_sum[wave] = sum;
+            lds.wave_count[wave] = equal;
+        }
+        __syncthreads();
+        Place f = find_wave(lds, ties, tie, u, quantum);
+        if (wave != f.wave) return;
+        for (uint32_t i0 = 0; i0 < mine; i0 += 64) {
+            const uint32_t i = i0 + lane;
+            const uint32_t key = i < mine ? lds.part_key[wave][i] : 0u;
+            double x = i < mine ? lds.part_e[wave][i] : 0.0;
+            const uint32_t is = i < mine && ties && key == least;
+            const uint32_t equals = scan32(is, lane);
+            if (is) x = staying(ties, f.so_far + equals - 1, 1) ? tie : 0.0;
+            const double upto = scan64(x, lane);
+            const uint64_t over = __ballot(f.at + upto > f.target);
+            if (over) {
+                if (lane == __builtin_ctzll(over)) choose(p, r, lds.part_at[wave][i], of_key(key), w, temperature, f.whole);
+                return;
+            }
+            f.at += __shfl(upto, 63);
+            f.so_far += __shfl(equals, 63);
+        }
+        return;
+    }
+
+    // from the row: each wave's part, then the one in which the token lies, by all waves
     double sum = 0.0;
     uint32_t equal = 0;
-    row.each([&](int64_t, const float* l) {
+    row.each([&](int, const float* l) {
+        bool some = false;
 #pragma unroll
         for (int i = 0; i < kLane; ++i) {
             const uint32_t key = key_of(l[i]);
-            sum += above(l[i], key);
-            equal += key == least;
+            some |= key > least && l[i] > -INFINITY;
+            equal += ties && key == least;
         }
+        if (__any(some)) {
+#pragma unroll
+            for (int i = 0; i < kLane; ++i) sum += above(l[i], key_of(l[i]));
+        }
+        return true;
     });
     sum = wave_sum64(sum);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) equal += __shfl_xor(equal, d);
+    equal = wave_sum32(equal);
     __syncthreads();
     if (lane == 0) {
         lds.wave_sum[wave] = sum;
         lds.wave_count[wave] = equal;
     }
     __syncthreads();
-    const auto kept = [&](int64_t so_far, uint32_t here) {  // of `here` ties behind `so_far`
-        const int64_t left = ties - so_far;
-        return left <= 0 ? 0.0 : (double)std::min<int64_t>(left, here);
-    };
-    double whole = 0.0;
-    int64_t so_far = 0;
-    for (int i = 0; i < kWaves; ++i) {
-        whole += lds.wave_sum[i] + kept(so_far, lds.wave_count[i]) * tie;
-        so_far += lds.wave_count[i];
-    }
-    const float u = p.u[r];
-    // at most one quantum below the whole: the last that stays, where u is 1 or more
-    const double target = u > 0.f ? fmin((double)u * whole, whole - quantum) : 0.0;
-    double at = 0.0;
-    int mine = -1;
-    so_far = 0;
-    for (int i = 0; i < kWaves && mine < 0; ++i) {
-        const double here = lds.wave_sum[i] + kept(so_far, lds.wave_count[i]) * tie;
-        if (at + here > target) {
-            mine = i;
-        } else {
-            at += here;
-            so_far += lds.wave_count[i];
-        }
-    }
-    if (wave != mine) return;
-    for (int64_t s = 0; s < steps; ++s) {
-        float l[kLane];
-        const int64_t first = row.load(s, l);
-        double x[kLane], lane_sum = 0.0;
-        uint32_t lane_ties = 0;
+    Place f = find_wave(lds, ties, tie, u, quantum);
+    const Row<DT> part(p.logits, r, n, f.wave, lane);
+    const int64_t end = std::min<int64_t>(n, part.from + (int64_t)part.steps * kStep);
+    constexpr int kOwn = 4;  // neighbouring logits of a thread
+    for (int64_t i0 = part.from; i0 < end; i0 += kOwn * kThreads) {
+        const int64_t first = i0 + (int64_t)threadIdx.x * kOwn;
+        float l[kOwn];
+        double x[kOwn], lane_sum = 0.0;
+        uint32_t lane_equal = 0;
 #pragma unroll
-        for (int i = 0; i < kLane; ++i) lane_ties += key_of(l[i]) == least;
-        uint32_t ties_upto = lane_ties;
+        for (int i = 0; i < kOwn; ++i) l[i] = load_dt(part.p, DT, std::min(first + i, n - 1));
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t y = __shfl_up(ties_upto, d);
-            if (lane >= d) ties_upto += y;
-        }
-        int64_t before_me = so_far + (ties_upto - lane_ties);
-#pragma unroll
-        for (int i = 0; i < kLane; ++i) {
+        for (int i = 0; i < kOwn; ++i) {
+            if (first + i >= end) l[i] = -INFINITY;
             const uint32_t key = key_of(l[i]);
-            if (key == least) {
-                x[i] = before_me < ties ? tie : 0.0;
-                ++before_me;
-            } else {
-                x[i] = above(l[i], key);
-            }
+            lane_equal += ties && key == least;
+            x[i] = above(l[i], key);
+        }
+        uint32_t equals = scan32(lane_equal, lane);
+        __syncthreads();
+        if (lane == 63) lds.wave_count[wave] = equals;
+        __syncthreads();
+        uint32_t so_far = f.so_far + equals - lane_equal, here_equal = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            so_far += i < wave ? lds.wave_count[i] : 0;
+            here_equal += lds.wave_count[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            if (ties && key_of(l[i]) == least) x[i] = staying(ties, so_far++, 1) ? tie : 0.0;
             lane_sum += x[i];
         }
-        double upto = lane_sum;
+        const double upto = scan64(lane_sum, lane);
+        if (lane == 63) lds.wave_sum[wave] = upto;
+        __syncthreads();
+        double at = f.at, here = 0.0;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const double y = __shfl_up(upto, d);
-            if (lane >= d) upto += y;
+        for (int i = 0; i < kWaves; ++i) {
+            at += i < wave ? lds.wave_sum[i] : 0.0;
+            here += lds.wave_sum[i];
         }
-        const uint64_t over = __ballot(at + upto > target);
-        if (over) {
-            if (lane == __builtin_ctzll(over)) {
-                double here = at + (upto - lane_sum);
-                bool done = false;
+        if (f.at + here > f.target) {
+            const uint64_t over = __ballot(at + upto > f.target);
+            if (at <= f.target && over && lane == __builtin_ctzll(over)) {
+                at += upto - lane_sum;
+                int i = 0;
 #pragma unroll
-                for (int i = 0; i < kLane; ++i) {
-                    here += x[i];
-                    if (!done && here > target) {
-                        done = true;
-                        p.token[r] = first + i;
-                        if (p.logprob) {
-                            const double z = w.inf ? 0.0 : ((double)l[i] - w.top) / (double)temperature;
-                            p.logprob[r] = (float)(z - log(whole));
-                        }
-                    }
+                for (int j = 0; j < kOwn; ++j) {
+                    at += x[j];
+                    i += at <= f.target;
                 }
+                float chosen = l[0];
+#pragma unroll
+                for (int j = 1; j < kOwn; ++j) chosen = i == j ? l[j] : chosen;
+                choose(p, r, first + i, chosen, w, temperature, f.whole);
             }
             return;
         }
-        at += __shfl(upto, 63);
-        so_far += __shfl(ties_upto, 63);
+        f.at += here;
+        f.so_far += here_equal;
     }
 }
 
