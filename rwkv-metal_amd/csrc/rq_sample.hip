@@ -44,34 +44,33 @@ RQ_DEV uint32_t key_of(float l) {
 }
 RQ_DEV float of_key(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 
-// 2^x for x <= 0: 2^n times the Taylor series of exp(f ln 2), |f| <= 1/2; twelve terms leave
-// 0.35^12 / 12! = 6e-15.
-RQ_DEV double exp2_64(double x) {
-    if (!(x > -80.0)) return 0.0;
-    const double n = __builtin_rint(x), t = (x - n) * 0.6931471805599453;
-    double s = 1.0 / 39916800;
-    s = fma(s, t, 1.0 / 3628800);
-    s = fma(s, t, 1.0 / 362880);
-    s = fma(s, t, 1.0 / 40320);
-    s = fma(s, t, 1.0 / 5040);
-    s = fma(s, t, 1.0 / 720);
-    s = fma(s, t, 1.0 / 120);
-    s = fma(s, t, 1.0 / 24);
-    s = fma(s, t, 1.0 / 6);
-    s = fma(s, t, 0.5);
-    s = fma(s, t, 1.0);
-    s = fma(s, t, 1.0);
-    return __builtin_ldexp(s, (int)n);
-}
+constexpr int kTable = 32;  // powers 2^(j / 32): each in banks of its own
 
+// e^((l - top) / temperature) in float64: x = 32 log2 of it is split into a whole number and f, |f| <= 1/2; with
+// t = f ln 2 / 32, |t| <= 0.0109, four terms of the series of e^t leave t^5 / 120 = 1.3e-12, less than a quantum's share.
 struct Weights {
-    double top, scale;  // the largest logit, log2(e) / temperature
-    double grid;        // 1.5 * 2^52 quanta: a sum with it is rounded to whole quanta
-    bool inf;           // the largest logit is +inf
+    double top, scale;    // the largest logit, 32 log2(e) / temperature
+    double grid;          // 1.5 * 2^52 quanta: a sum with it is rounded to whole quanta
+    const double* table;
+    bool inf;             // the largest logit is +inf
     RQ_DEV double exact(float l) const {
-        if (inf) return l == INFINITY ? 1.0 : 0.0;
-        return exp2_64(((double)l - top) * scale);
+        constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52
+        constexpr double k = 0.6931471805599453 / kTable;
+        // past 2^-40 everything is rounded to 0
+        const double x = fmax(((double)l - top) * scale, -40.0 * kTable);
+        const double r = x + kWhole;
+        const int n = (int)(uint32_t)__double_as_longlong(r);
+        const double f = x - (r - kWhole);
+        double s = k * k * k * k / 24;
+        s = fma(s, f, k * k * k / 6);
+        s = fma(s, f, k * k / 2);
+        s = fma(s, f, k);
+        s = fma(s, f, 1.0);
+        long long power = __double_as_longlong(table[n & (kTable - 1)]);
+        power += (long long)(n >> 5) << 52;
+        return s * __longlong_as_double(power);
     }
+    RQ_DEV double at(float l) const { return inf ? (l == INFINITY ? 1.0 : 0.0) : exact(l); }
     RQ_DEV double quanta(double e) const { return (e + grid) - grid; }
 };
 
@@ -80,6 +79,7 @@ constexpr int kBin = 1024;   // logits of one bin that are told apart in LDS
 constexpr int kPart = 384;   // logits of a wave's part of the row that are kept in LDS
 
 struct Lds {
+    double table[kTable];
     double sums[kBins];  // of the bins; of 256 of them by bits
     double bin_sums[kBin];
     uint32_t bin_keys[kBin];
@@ -90,23 +90,58 @@ struct Lds {
     uint32_t digits[2][kWaves][16];
     double wave_sum[kWaves];
     uint32_t wave_count[kWaves];
-    float wave_max[kWaves], wave_min[kWaves];
+    uint32_t wave_max[kWaves], wave_min[kWaves];  // keys, and their complements
     unsigned long long first;
     double found_sum, total;
     uint32_t found, found_key;
     int nan;
 };
 
-RQ_DEV double wave_sum64(double x) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+// Over a wave by data-parallel moves: rows of 16 lanes, then the rows.
+template <int CTRL, int ROWS = 0xf>
+RQ_DEV uint32_t moved(uint32_t x, uint32_t none) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS = 0xf>
+RQ_DEV double moved64(double x) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x);
+    const uint64_t lo = moved<CTRL, ROWS>((uint32_t)u, 0), hi = moved<CTRL, ROWS>((uint32_t)(u >> 32), 0);
+    return __longlong_as_double((long long)(lo | (hi << 32)));
+}
+// each lane's and all before it
+template <class T, class F, class M>
+RQ_DEV T scan_by(T x, F join, M) {
+    x = join(x, M::template of<0x111>(x));
+    x = join(x, M::template of<0x112>(x));
+    x = join(x, M::template of<0x114>(x));
+    x = join(x, M::template of<0x118>(x));
+    x = join(x, M::template of<0x142, 0xa>(x));
+    x = join(x, M::template of<0x143, 0xc>(x));
     return x;
 }
-
-RQ_DEV uint32_t wave_sum32(uint32_t x) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-    return x;
+struct Moved32 {
+    template <int CTRL, int ROWS = 0xf>
+    static RQ_DEV uint32_t of(uint32_t x) { return moved<CTRL, ROWS>(x, 0); }
+};
+struct Moved64 {
+    template <int CTRL, int ROWS = 0xf>
+    static RQ_DEV double of(double x) { return moved64<CTRL, ROWS>(x); }
+};
+RQ_DEV uint32_t scan32(uint32_t x) {
+    return scan_by(x, [](uint32_t a, uint32_t b) { return a + b; }, Moved32());
+}
+RQ_DEV double scan64(double x) {
+    return scan_by(x, [](double a, double b) { return a + b; }, Moved64());
+}
+RQ_DEV uint32_t last32(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
+RQ_DEV double last64(double x) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x);
+    return __longlong_as_double((long long)((uint64_t)last32((uint32_t)u) | ((uint64_t)last32((uint32_t)(u >> 32)) << 32)));
+}
+RQ_DEV double wave_sum64(double x) { return last64(scan64(x)); }
+RQ_DEV uint32_t wave_sum32(uint32_t x) { return last32(scan32(x)); }
+RQ_DEV uint32_t wave_max32(uint32_t x) {  // of keys: 0 is below all
+    return last32(scan_by(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; }, Moved32()));
 }
 
 // Eight neighbouring logits as they are stored.
@@ -158,19 +193,21 @@ struct Row {
 #pragma unroll
             for (int x = 0; x < 4; ++x) to.v[j].w[x] = w[4 * j + x];
     }
-    // f(step, eight logits) in the order of the index, while it gives true; two steps in flight
+    // f(step, eight logits) in the order of the index, while it gives true; three steps in flight
     template <class F>
     RQ_DEV void each(F f) const {
         if (steps == 0) return;
-        Raw8<DT> now, next;
+        Raw8<DT> now, next, third;
         fetch(0, now);
+        if (steps > 1) fetch(1, next);
         for (int s = 0; s < steps; ++s) {
-            if (s + 1 < steps) fetch(s + 1, next);
+            if (s + 2 < steps) fetch(s + 2, third);
             float l[kLane];
 #pragma unroll
             for (int j = 0; j < kLane / kVec<DT>; ++j) unpack_vec<DT>(now.v[j], l + j * kVec<DT>);
             if (!f(s, l)) return;
             now = next;
+            next = third;
         }
     }
 };
@@ -204,13 +241,8 @@ RQ_DEV void find_bin(Lds& lds, double before, double want, double share, double 
         double sum = 0.0;
 #pragma unroll 8
         for (int i = 0; i < PER; ++i) sum += lds.sums[lane * PER + i];
-        double upto = sum;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const double x = __shfl_up(upto, d);
-            if (lane >= d) upto += x;
-        }
-        if (want < 0.0) want = fmax(share * __shfl(upto, 63), quantum);
+        const double upto = scan64(sum);
+        if (want < 0.0) want = fmax(share * last64(upto), quantum);
         double at = before + (upto - sum);
         if (at < want && before + upto >= want) {
             int i = 0;
@@ -313,13 +345,14 @@ RQ_DEV uint32_t key_in_row(const Row<DT>& row, Lds& lds, const Bins& bins, doubl
 
 // The k-th largest of the keys that the waves hold, four bits at a time: `n` a lane, key(j) its j-th (0:
 // none).  `above` is the number of larger ones.  1 <= k <= their number.
-template <class K>
+// BITS: of the leading bits only, the others 0: not above the k-th largest.
+template <int BITS, class K>
 RQ_DEV uint32_t kth_key(Lds& lds, int n, K key, uint32_t k, uint32_t& above) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t prefix = 0;
     above = 0;
 #pragma unroll 1
-    for (int shift = 28, turn = 0; shift >= 0; shift -= 4, turn ^= 1) {
+    for (int shift = 28, turn = 0; shift >= 32 - BITS; shift -= 4, turn ^= 1) {
         uint32_t mine = 0;  // lane d: the keys of this wave that are at least prefix with digit d
         for (int j = 0; j < n; ++j) {
             const uint32_t x = key(j);
@@ -350,16 +383,13 @@ RQ_DEV bool gather(const Row<DT>& row, Lds& lds, P reaches) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t have = 0;
     row.each([&](int s, const float* l) {
-        uint32_t at = have;
         uint32_t in = 0;
 #pragma unroll
-        for (int i = 0; i < kLane; ++i) {
-            const bool is = l[i] > -INFINITY && reaches(l[i], key_of(l[i]));
-            const uint64_t who = __ballot(is);
-            in |= (uint32_t)is << i;
-            at += __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-            have += __popcll(who);
-        }
+        for (int i = 0; i < kLane; ++i) in |= (uint32_t)(l[i] > -INFINITY && reaches(l[i], key_of(l[i]))) << i;
+        if (!__any(in != 0)) return true;
+        const uint32_t upto = scan32(__popc(in));
+        uint32_t at = have + upto - __popc(in);
+        have += last32(upto);
         if (have > kPart) return false;
 #pragma unroll
         for (int i = 0; i < kLane; ++i) {
@@ -389,22 +419,26 @@ struct Place {
     int wave;
 };
 RQ_DEV Place find_wave(const Lds& lds, int64_t ties, double tie, float u, double quantum) {
-    Place f{0.0, 0.0, 0.0, 0, 0};
-    uint32_t so_far = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        f.whole += lds.wave_sum[i] + staying(ties, so_far, lds.wave_count[i]) * tie;
-        so_far += lds.wave_count[i];
-    }
+    const int i = threadIdx.x & 15;  // four rows of lanes do the same
+    const uint32_t equal = lds.wave_count[i];
+    uint32_t equals = equal;
+    equals += Moved32::of<0x111>(equals);
+    equals += Moved32::of<0x112>(equals);
+    equals += Moved32::of<0x114>(equals);
+    equals += Moved32::of<0x118>(equals);
+    const double here = lds.wave_sum[i] + staying(ties, equals - equal, equal) * tie;
+    double upto = here;
+    upto += Moved64::of<0x111>(upto);
+    upto += Moved64::of<0x112>(upto);
+    upto += Moved64::of<0x114>(upto);
+    upto += Moved64::of<0x118>(upto);
+    Place f;
+    f.whole = last64(upto);
     // at most one quantum below the whole: the last that stays, where u is 1 or more
     f.target = u > 0.f ? fmin((double)u * f.whole, f.whole - quantum) : 0.0;
-    for (int i = 0; i < kWaves; ++i) {
-        const double here = lds.wave_sum[i] + staying(ties, f.so_far, lds.wave_count[i]) * tie;
-        f.wave = i;
-        if (f.at + here > f.target) break;
-        f.at += here;
-        f.so_far += lds.wave_count[i];
-    }
+    f.wave = (int)__builtin_ctzll(__ballot(upto > f.target) | (1ull << 15));
+    f.at = __shfl(upto - here, f.wave);
+    f.so_far = __shfl(equals - equal, f.wave);
     return f;
 }
 
@@ -414,23 +448,6 @@ RQ_DEV void choose(const SampleArgs& p, int64_t r, int64_t at, float l, const We
         const double z = w.inf ? 0.0 : ((double)l - w.top) / (double)temperature;
         p.logprob[r] = (float)(z - log(whole));
     }
-}
-
-RQ_DEV uint32_t scan32(uint32_t x, int lane) {  // up to and with the lane's own
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
-    return x;
-}
-RQ_DEV double scan64(double x, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
-    return x;
 }
 
 template <int DT>
@@ -446,47 +463,37 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
     const float u = p.u[r];
     min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
 
+    // a NaN is above +inf as an integer without its sign; below, `low` is -inf where some logits are masked
     float top = -INFINITY, low = INFINITY;
-    uint32_t there = 0;
-    bool nan = false;
+    uint32_t size = 0;
     row.each([&](int, const float* l) {
 #pragma unroll
         for (int i = 0; i < kLane; ++i) {
-            nan |= l[i] != l[i];
-            const bool is = l[i] > -INFINITY;
-            there += is;
             top = fmaxf(top, l[i]);
-            low = is ? fminf(low, l[i]) : low;
+            low = fminf(low, l[i]);
+            size = std::max(size, __float_as_uint(l[i]) & 0x7fffffffu);
         }
         return true;
     });
-    const float lane_top = top;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        top = fmaxf(top, __shfl_xor(top, d));
-        low = fminf(low, __shfl_xor(low, d));
-    }
-    there = wave_sum32(there);
-    if (threadIdx.x == 0) {
-        lds.nan = 0;
-        lds.first = ~0ull;
-    }
-    __syncthreads();
-    if (__any(nan) && lane == 0) lds.nan = 1;
-    if (lane == 0) {
-        lds.wave_max[wave] = top;
-        lds.wave_min[wave] = low;
-        lds.wave_count[wave] = there;
+    const uint32_t lane_top = top > -INFINITY ? key_of(top) : 0;
+    if (threadIdx.x == 0) lds.first = ~0ull;
+    if (threadIdx.x < kTable) lds.table[threadIdx.x] = exp2((double)threadIdx.x / kTable);
+    {
+        const uint32_t a = wave_max32(key_of(top)), b = wave_max32(~key_of(low)), c = wave_max32(size);
+        if (lane == 0) {
+            lds.wave_max[wave] = a;
+            lds.wave_min[wave] = b;
+            lds.wave_count[wave] = c;
+        }
     }
     __syncthreads();
-    there = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        there += lds.wave_count[i];
-        top = fmaxf(top, lds.wave_max[i]);
-        low = fminf(low, lds.wave_min[i]);
+    {
+        const uint32_t a = wave_max32(lds.wave_max[lane & 15]), b = wave_max32(lds.wave_min[lane & 15]);
+        size = wave_max32(lds.wave_count[lane & 15]);
+        top = of_key(a);
+        low = of_key(~b);
     }
-    if (lds.nan || there == 0) {  // nothing to choose from
+    if (size > 0x7f800000u || top == -INFINITY) {  // nothing to choose from
         if (threadIdx.x == 0) {
             p.token[r] = -1;
             if (p.logprob) p.logprob[r] = NAN;
@@ -510,10 +517,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
         return;
     }
     const int bits = n <= (1 << 17) ? 36 : 33;
-    const Weights w{(double)top, 1.4426950408889634 / (double)temperature,
-                    6755399441055744.0 / (double)(1ll << bits), top == INFINITY};
+    const Weights w{(double)top, kTable * 1.4426950408889634 / (double)temperature,
+                    6755399441055744.0 / (double)(1ll << bits), lds.table, top == INFINITY};
     const double quantum = 1.0 / (double)(1ll << bits);
-    if (top_k < 0 || top_k >= (int64_t)there) top_k = 0;
+    if (top_k < 0 || top_k >= n) top_k = 0;
     const bool by_sum = top_p < 1.f;
     // past 26 temperatures below the largest, e_i is rounded to 0
     const Bins sum_bins(top, fminf(top - low, 26.f * temperature));
@@ -523,22 +530,24 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
     int64_t ties = 0;
     bool listed = false;
     if (top_k > 0) {
-        const uint32_t mine = lane_top > -INFINITY ? key_of(lane_top) : 0;
         uint32_t above;
-        if (top_k <= kThreads && __syncthreads_count(mine != 0) >= (int)top_k) {
-            const uint32_t bound = kth_key(lds, 1, [&](int) { return mine; }, (uint32_t)top_k, above);
+        if (top_k <= kThreads && __syncthreads_count(lane_top != 0) >= (int)top_k) {
+            const uint32_t bound = kth_key<16>(lds, 1, [&](int) { return lane_top; }, (uint32_t)top_k, above);
             listed = gather(row, lds, [&](float, uint32_t key) { return key >= bound; });
         }
         if (listed) {
             uint32_t longest = 0;
 #pragma unroll
             for (int i = 0; i < kWaves; ++i) longest = std::max(longest, lds.part_n[i]);
-            least = kth_key(lds, (longest + 63) / 64,
-                            [&](int j) {
-                                const uint32_t i = lane + 64 * j;
-                                return i < lds.part_n[wave] ? lds.part_key[wave][i] : 0u;
-                            },
-                            (uint32_t)top_k, above);
+            // the bits that the type's values have
+            least = kth_key<DT == RQ_BF16 ? 16 : DT == RQ_F16 ? 20 : 32>(
+                lds, (longest + 63) / 64,
+                [&](int j) {
+                    const uint32_t i = lane + 64 * j;
+                    return i < lds.part_n[wave] ? lds.part_key[wave][i] : 0u;
+                },
+                (uint32_t)top_k, above);
+            if (DT != RQ_F32 && !(least >> 31)) least |= DT == RQ_BF16 ? 0xffffu : 0xfffu;  // a negative value's complement
             ties = top_k - above;
         } else {
             // logits further below count as one bin: their range may be that of the type
@@ -552,14 +561,19 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
                     if (l[i] > -INFINITY) unsafeAtomicAdd(&lds.sums[bins.of(l[i])], 1.0);
                 return true;
             });
+            if (threadIdx.x == 0) lds.total = 0.0;
             find_bin<kBins>(lds, 0.0, (double)top_k, 0.0, 0.0);
-            least = key_in_row(row, lds, bins, before, any, [](float, uint32_t) { return 1.0; }, 0, 0.0);
-            ties = top_k - (int64_t)before;
-            listed = gather(row, lds, [&](float, uint32_t key) { return key >= least; });
+            if (lds.total > 0.0) {  // as many logits are there
+                least = key_in_row(row, lds, bins, before, any, [](float, uint32_t) { return 1.0; }, 0, 0.0);
+                ties = top_k - (int64_t)before;
+                listed = gather(row, lds, [&](float, uint32_t key) { return key >= least; });
+            } else {
+                top_k = 0;
+            }
         }
     }
     if (by_sum) {
-        const double tied = ties ? (double)ties * w.quanta(w.exact(of_key(least))) : 0.0;
+        const double tied = ties ? (double)ties * w.quanta(w.at(of_key(least))) : 0.0;
         double before, want;
         uint32_t key;
         clear_bins<kBins>(lds);
@@ -568,7 +582,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
                 const uint32_t k = lds.part_key[wave][i];
                 if (k <= least) continue;
-                const double x = w.quanta(w.exact(of_key(k)));
+                const double x = w.quanta(w.at(of_key(k)));
                 lds.part_e[wave][i] = x;
                 unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(k))], x);
             }
@@ -589,14 +603,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             __syncthreads();
         }
         const auto may_weigh = [&](float l, uint32_t k) { return k > least && l > -INFINITY; };
-        const auto weight = [&](float l, uint32_t) { return w.quanta(w.exact(l)); };
+        const auto weight = [&](float l, uint32_t) { return w.quanta(w.at(l)); };
         const bool from_row = !listed;
         if (from_row) {
             if (top_k == 0) {
                 row.each([&](int, const float* l) {
                     double x[kLane];
 #pragma unroll
-                    for (int i = 0; i < kLane; ++i) x[i] = w.quanta(w.exact(l[i]));
+                    for (int i = 0; i < kLane; ++i) x[i] = w.quanta(w.at(l[i]));
 #pragma unroll
                     for (int i = 0; i < kLane; ++i)
                         if (x[i] > 0.0) unsafeAtomicAdd(&lds.sums[sum_bins.of(l[i])], x[i]);
@@ -624,7 +638,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             if (listed) {
                 for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
                     const uint32_t k = lds.part_key[wave][i];
-                    const double x = w.quanta(w.exact(of_key(k)));
+                    const double x = w.quanta(w.at(of_key(k)));
                     lds.part_e[wave][i] = x;
                     if (x > 0.0 && sum_bins.of(of_key(k)) == bin) add_to_bin(lds, k, x);
                 }
@@ -640,7 +654,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             }
         }
         // as many of that class as are needed to reach it
-        const double each = w.quanta(w.exact(of_key(key)));
+        const double each = w.quanta(w.at(of_key(key)));
         double more = __builtin_ceil((want - before) / each);
         if (more > 1.0 && before + (more - 1.0) * each >= want) more -= 1.0;
         if (before + more * each < want) more += 1.0;
@@ -653,10 +667,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
         if (!w.inf) listed = gather(row, lds, [&](float l, uint32_t) { return !(l - top < border); });
     }
 
-    const double tie_e = ties ? w.exact(of_key(least)) : 0.0;
+    const double tie_e = ties ? w.at(of_key(least)) : 0.0;
     const double tie = ties && tie_e >= (double)min_p ? w.quanta(tie_e) : 0.0;
     const auto above = [&](float l, uint32_t key) {
-        const double e = w.exact(l);
+        const double e = w.at(l);
         return l > -INFINITY && key > least && e >= (double)min_p ? w.quanta(e) : 0.0;
     };
 
@@ -686,24 +700,32 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             const uint32_t key = i < mine ? lds.part_key[wave][i] : 0u;
             double x = i < mine ? lds.part_e[wave][i] : 0.0;
             const uint32_t is = i < mine && ties && key == least;
-            const uint32_t equals = scan32(is, lane);
+            const uint32_t equals = scan32(is);
             if (is) x = staying(ties, f.so_far + equals - 1, 1) ? tie : 0.0;
-            const double upto = scan64(x, lane);
+            const double upto = scan64(x);
             const uint64_t over = __ballot(f.at + upto > f.target);
             if (over) {
                 if (lane == __builtin_ctzll(over)) choose(p, r, lds.part_at[wave][i], of_key(key), w, temperature, f.whole);
                 return;
             }
-            f.at += __shfl(upto, 63);
-            f.so_far += __shfl(equals, 63);
+            f.at += last64(upto);
+            f.so_far += last32(equals);
         }
         return;
     }
 
     // from the row: each wave's part, then the one in which the token lies, by all waves
+    const bool everything = top_k == 0 && !by_sum && !(min_p > 0.f) && !w.inf;
     double sum = 0.0;
     uint32_t equal = 0;
     row.each([&](int, const float* l) {
+        if (everything) {  // -inf adds 0
+            double x[kLane];
+#pragma unroll
+            for (int i = 0; i < kLane; ++i) x[i] = w.quanta(w.exact(l[i]));
+            sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+            return true;
+        }
         bool some = false;
 #pragma unroll
         for (int i = 0; i < kLane; ++i) {
@@ -743,7 +765,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             lane_equal += ties && key == least;
             x[i] = above(l[i], key);
         }
-        uint32_t equals = scan32(lane_equal, lane);
+        uint32_t equals = scan32(lane_equal);
         __syncthreads();
         if (lane == 63) lds.wave_count[wave] = equals;
         __syncthreads();
@@ -758,7 +780,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             if (ties && key_of(l[i]) == least) x[i] = staying(ties, so_far++, 1) ? tie : 0.0;
             lane_sum += x[i];
         }
-        const double upto = scan64(lane_sum, lane);
+        const double upto = scan64(lane_sum);
         if (lane == 63) lds.wave_sum[wave] = upto;
         __syncthreads();
         double at = f.at, here = 0.0;
