@@ -76,6 +76,7 @@ struct Weights {
 
 constexpr int kBins = 2048;  // for sums below the largest logit
 constexpr int kBin = 1024;   // logits of one bin that are told apart in LDS
+constexpr int kFew = 400;    // of these, the number up to which each is compared with all
 constexpr int kPart = 384;   // logits of a wave's part of the row that are kept in LDS
 
 struct Lds {
@@ -234,23 +235,30 @@ RQ_DEV void clear_bins(Lds& lds) {
 // whole, at least `quantum`); lds.found, the total before it lds.found_sum, what was looked for lds.total.
 template <int BINS>
 RQ_DEV void find_bin(Lds& lds, double before, double want, double share, double quantum) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int PER = BINS > kThreads ? BINS / kThreads : 1;  // bins a thread
     __syncthreads();
-    if (threadIdx.x < 64) {
-        constexpr int PER = BINS / 64;
-        const int lane = threadIdx.x;
-        double sum = 0.0;
-#pragma unroll 8
-        for (int i = 0; i < PER; ++i) sum += lds.sums[lane * PER + i];
-        const double upto = scan64(sum);
-        if (want < 0.0) want = fmax(share * last64(upto), quantum);
-        double at = before + (upto - sum);
-        if (at < want && before + upto >= want) {
-            int i = 0;
-            while (i < PER - 1 && at + lds.sums[lane * PER + i] < want) at += lds.sums[lane * PER + i++];
-            lds.found = lane * PER + i;
+    double own[PER], sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += own[i] = (int)threadIdx.x * PER < BINS ? lds.sums[threadIdx.x * PER + i] : 0.0;
+    const double upto = scan64(sum);
+    if (lane == 63) lds.wave_sum[wave] = upto;
+    __syncthreads();
+    double waves = lds.wave_sum[lane & 15];
+    waves += Moved64::of<0x111>(waves);
+    waves += Moved64::of<0x112>(waves);
+    waves += Moved64::of<0x114>(waves);
+    waves += Moved64::of<0x118>(waves);
+    if (want < 0.0) want = fmax(share * last64(waves), quantum);
+    double at = before + (upto - sum) + (wave ? __shfl(waves, wave - 1) : 0.0);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (at < want && at + own[i] >= want) {
+            lds.found = threadIdx.x * PER + i;
             lds.found_sum = at;
             lds.total = want;
         }
+        at += own[i];
     }
     __syncthreads();
 }
@@ -377,32 +385,63 @@ RQ_DEV uint32_t kth_key(Lds& lds, int n, K key, uint32_t k, uint32_t& above) {
     return prefix;
 }
 
-// The row's logits for which reaches(l, key) holds into LDS, each wave's by index.  Whether they fit.
-template <int DT, class P>
-RQ_DEV bool gather(const Row<DT>& row, Lds& lds, P reaches) {
+// A value that at least k of the lanes' maxima reach, a little below the k-th largest: the largest maxima are
+// told apart by 256 bins between the smallest and the largest of them.  k <= the lanes that hold a logit.
+RQ_DEV float bound_of_maxima(Lds& lds, float mine, float top, uint32_t k) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t* const counts = (uint32_t*)lds.sums;
+    const uint32_t low = wave_max32(mine > -INFINITY ? ~key_of(mine) : 0u);
+    __syncthreads();
+    if (lane == 0) lds.wave_min[wave] = low;
+    if (threadIdx.x < 256) counts[threadIdx.x] = 0;
+    __syncthreads();
+    const float least = of_key(~wave_max32(lds.wave_min[lane & 15])), width = (top - least) * (1.f / 255.f);
+    if (!(width > 0.f) || !(width < INFINITY)) return least;  // all equal, or a range past the type's
+    const auto edge = [&](int b) { return top - (float)b * width; };
+    int bin = (int)fminf((top - mine) / width, 255.f);
+    while (bin < 255 && mine < edge(bin + 1)) ++bin;  // in its bin whatever the rounding: mine >= edge(bin + 1)
+    if (mine > -INFINITY) atomicAdd(&counts[bin], 1u);
+    __syncthreads();
+    uint32_t four[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += four[i] = counts[4 * lane + i];
+    uint32_t before = scan32(sum) - sum;
+    int found = -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (before < k && before + four[i] >= k) found = 4 * lane + i;
+        before += four[i];
+    }
+    const uint64_t who = __ballot(found >= 0);
+    if (!who) return least;
+    const int b = __shfl(found, __builtin_ctzll(who));
+    return b >= 255 ? least : fmaxf(least, edge(b + 1));
+}
+
+// The row's logits of `bound` (above -inf) and more into LDS, each wave's by index.  Whether they fit.
+template <int DT>
+RQ_DEV bool gather(const Row<DT>& row, Lds& lds, float bound) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t have = 0;
     row.each([&](int s, const float* l) {
+        const float most = fmaxf(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), fmaxf(fmaxf(l[4], l[5]), fmaxf(l[6], l[7])));
+        if (!__any(most >= bound)) return true;
         uint32_t in = 0;
 #pragma unroll
-        for (int i = 0; i < kLane; ++i) in |= (uint32_t)(l[i] > -INFINITY && reaches(l[i], key_of(l[i]))) << i;
-        if (!__any(in != 0)) return true;
+        for (int i = 0; i < kLane; ++i) in |= (uint32_t)(l[i] >= bound) << i;
         const uint32_t upto = scan32(__popc(in));
         uint32_t at = have + upto - __popc(in);
         have += last32(upto);
         if (have > kPart) return false;
-#pragma unroll
-        for (int i = 0; i < kLane; ++i) {
-            if (in >> i & 1) {
-                lds.part_key[wave][at] = key_of(l[i]);
-                lds.part_at[wave][at] = (uint32_t)(row.at(s) + i);
-                ++at;
-            }
-        }
+        const uint32_t first = (uint32_t)row.at(s);
+        for (; in; in &= in - 1) lds.part_at[wave][at++] = first + __builtin_ctz(in);
         return true;
     });
     if (lane == 0) lds.part_n[wave] = have;
-    return __syncthreads_and(have <= kPart);
+    if (!__syncthreads_and(have <= kPart)) return false;
+    for (uint32_t i = lane; i < have; i += 64) lds.part_key[wave][i] = key_of(load_dt(row.p, DT, lds.part_at[wave][i]));
+    __syncthreads();
+    return true;
 }
 
 // How many of `here` equal logits behind `so_far` others stay.
@@ -532,22 +571,53 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
     if (top_k > 0) {
         uint32_t above;
         if (top_k <= kThreads && __syncthreads_count(lane_top != 0) >= (int)top_k) {
-            const uint32_t bound = kth_key<16>(lds, 1, [&](int) { return lane_top; }, (uint32_t)top_k, above);
-            listed = gather(row, lds, [&](float, uint32_t key) { return key >= bound; });
+            listed = gather(row, lds, bound_of_maxima(lds, lane_top ? of_key(lane_top) : -INFINITY, top, (uint32_t)top_k));
         }
         if (listed) {
-            uint32_t longest = 0;
+            uint32_t longest = 0, all = 0;
 #pragma unroll
-            for (int i = 0; i < kWaves; ++i) longest = std::max(longest, lds.part_n[i]);
-            // the bits that the type's values have
-            least = kth_key<DT == RQ_BF16 ? 16 : DT == RQ_F16 ? 20 : 32>(
-                lds, (longest + 63) / 64,
-                [&](int j) {
-                    const uint32_t i = lane + 64 * j;
-                    return i < lds.part_n[wave] ? lds.part_key[wave][i] : 0u;
-                },
-                (uint32_t)top_k, above);
-            if (DT != RQ_F32 && !(least >> 31)) least |= DT == RQ_BF16 ? 0xffffu : 0xfffu;  // a negative value's complement
+            for (int i = 0; i < kWaves; ++i) {
+                longest = std::max(longest, lds.part_n[i]);
+                all += lds.part_n[i];
+            }
+            if (all <= kFew) {  // each against all
+                uint32_t base = 0;
+#pragma unroll
+                for (int i = 0; i < kWaves; ++i) base += i < wave ? lds.part_n[i] : 0;
+                for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) lds.bin_keys[base + i] = lds.part_key[wave][i];
+                if (threadIdx.x < 8) lds.bin_keys[all + threadIdx.x] = 0;
+                __syncthreads();
+                const uint32_t key = threadIdx.x < all ? lds.bin_keys[threadIdx.x] : 0;
+                uint32_t larger = 0, same = 0;
+                if (wave * 64 < all) {
+                    for (uint32_t j = 0; j < all; j += 8) {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const uint32_t other = lds.bin_keys[j + x];
+                            larger += other > key;
+                            same += other == key;
+                        }
+                    }
+                }
+                if (key && larger < top_k && larger + same >= top_k) {
+                    lds.found_key = key;
+                    lds.found = larger;
+                }
+                __syncthreads();
+                least = lds.found_key;
+                above = lds.found;
+                __syncthreads();
+            } else {
+                // the bits that the type's values have
+                least = kth_key<DT == RQ_BF16 ? 16 : DT == RQ_F16 ? 20 : 32>(
+                    lds, (longest + 63) / 64,
+                    [&](int j) {
+                        const uint32_t i = lane + 64 * j;
+                        return i < lds.part_n[wave] ? lds.part_key[wave][i] : 0u;
+                    },
+                    (uint32_t)top_k, above);
+                if (DT != RQ_F32 && !(least >> 31)) least |= DT == RQ_BF16 ? 0xffffu : 0xfffu;  // a negative value's complement
+            }
             ties = top_k - above;
         } else {
             // logits further below count as one bin: their range may be that of the type
@@ -566,7 +636,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             if (lds.total > 0.0) {  // as many logits are there
                 least = key_in_row(row, lds, bins, before, any, [](float, uint32_t) { return 1.0; }, 0, 0.0);
                 ties = top_k - (int64_t)before;
-                listed = gather(row, lds, [&](float, uint32_t key) { return key >= least; });
+                listed = gather(row, lds, of_key(least));
             } else {
                 top_k = 0;
             }
@@ -574,9 +644,32 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
     }
     if (by_sum) {
         const double tied = ties ? (double)ties * w.quanta(w.at(of_key(least))) : 0.0;
-        double before, want;
+        double before, want = -1.0;
         uint32_t key;
+        if (top_k == 0) {
+            // the whole; and as candidates some 60 of 1024 logits, of the largest: what the maxima of 31 of 32
+            // lanes reach
+            double sum = 0.0;
+            row.each([&](int, const float* l) {
+                double x[kLane];
+#pragma unroll
+                for (int i = 0; i < kLane; ++i) x[i] = w.quanta(w.at(l[i]));
+                sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+                return true;
+            });
+            sum = wave_sum64(sum);
+            __syncthreads();
+            if (lane == 0) lds.wave_sum[wave] = sum;
+            const int lanes = __syncthreads_count(lane_top != 0);
+            sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) sum += lds.wave_sum[i];
+            want = fmax(fmax((double)top_p, 0.0) * sum, quantum);
+            listed = gather(row, lds, bound_of_maxima(lds, lane_top ? of_key(lane_top) : -INFINITY, top,
+                                                      (uint32_t)(lanes - lanes / 32)));
+        }
         clear_bins<kBins>(lds);
+        if (threadIdx.x == 0) lds.total = -1.0;
         if (threadIdx.x == 0 && ties) unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(least))], tied);
         if (listed) {
             for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
@@ -586,7 +679,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
                 lds.part_e[wave][i] = x;
                 unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(k))], x);
             }
-            find_bin<kBins>(lds, 0.0, -1.0, fmax((double)top_p, 0.0), quantum);
+            find_bin<kBins>(lds, 0.0, want, fmax((double)top_p, 0.0), quantum);
+            if (lds.total < 0.0) listed = false;  // what is listed does not reach it
+        }
+        if (listed) {
             const int bin = lds.found;
             const double base = lds.found_sum;
             want = lds.total;
@@ -604,54 +700,22 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
         }
         const auto may_weigh = [&](float l, uint32_t k) { return k > least && l > -INFINITY; };
         const auto weight = [&](float l, uint32_t) { return w.quanta(w.at(l)); };
-        const bool from_row = !listed;
-        if (from_row) {
-            if (top_k == 0) {
-                row.each([&](int, const float* l) {
-                    double x[kLane];
+        if (!listed) {
+            clear_bins<kBins>(lds);
+            if (threadIdx.x == 0 && ties) unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(least))], tied);
+            row.each([&](int, const float* l) {
 #pragma unroll
-                    for (int i = 0; i < kLane; ++i) x[i] = w.quanta(w.at(l[i]));
-#pragma unroll
-                    for (int i = 0; i < kLane; ++i)
-                        if (x[i] > 0.0) unsafeAtomicAdd(&lds.sums[sum_bins.of(l[i])], x[i]);
-                    return true;
-                });
-            } else {
-                clear_bins<kBins>(lds);
-                if (threadIdx.x == 0 && ties) unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(least))], tied);
-                row.each([&](int, const float* l) {
-#pragma unroll
-                    for (int i = 0; i < kLane; ++i) {
-                        const uint32_t k = key_of(l[i]);
-                        if (!may_weigh(l[i], k)) continue;
-                        const double x = weight(l[i], k);
-                        if (x > 0.0) unsafeAtomicAdd(&lds.sums[sum_bins.of(l[i])], x);
-                    }
-                    return true;
-                });
-            }
+                for (int i = 0; i < kLane; ++i) {
+                    const uint32_t k = key_of(l[i]);
+                    if (!may_weigh(l[i], k)) continue;
+                    const double x = weight(l[i], k);
+                    if (x > 0.0) unsafeAtomicAdd(&lds.sums[sum_bins.of(l[i])], x);
+                }
+                return true;
+            });
             find_bin<kBins>(lds, 0.0, -1.0, fmax((double)top_p, 0.0), quantum);
             want = lds.total;
-            const int bin = lds.found;
-            const double base = lds.found_sum;
-            if (top_k == 0) listed = gather(row, lds, [&](float l, uint32_t) { return sum_bins.of(l) <= bin; });
-            if (listed) {
-                for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
-                    const uint32_t k = lds.part_key[wave][i];
-                    const double x = w.quanta(w.at(of_key(k)));
-                    lds.part_e[wave][i] = x;
-                    if (x > 0.0 && sum_bins.of(of_key(k)) == bin) add_to_bin(lds, k, x);
-                }
-                __syncthreads();
-            }
-            if (listed && lds.in_bin <= kBin) {
-                key = key_in_bin(lds, base, want, before, 0, false);
-            } else {
-                __syncthreads();
-                if (threadIdx.x == 0) lds.in_bin = 0;
-                __syncthreads();
-                key = key_in_row(row, lds, sum_bins, before, may_weigh, weight, least, tied);
-            }
+            key = key_in_row(row, lds, sum_bins, before, may_weigh, weight, least, tied);
         }
         // as many of that class as are needed to reach it
         const double each = w.quanta(w.at(of_key(key)));
@@ -664,7 +728,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
     if (!listed && top_k == 0 && !by_sum && min_p > 0.f) {
         // a little below the border (NaN where any logit may stay): the terms themselves decide
         const float border = (float)(log((double)min_p) * (double)temperature) * 1.0001f - 1e-6f * fabsf(top);
-        if (!w.inf) listed = gather(row, lds, [&](float l, uint32_t) { return !(l - top < border); });
+        // (of l, not of l - top: rounded by half a step of top's)
+        if (!w.inf && border > -INFINITY) listed = gather(row, lds, top + border - 1e-6f * fabsf(top));
     }
 
     const double tie_e = ties ? w.at(of_key(least)) : 0.0;
