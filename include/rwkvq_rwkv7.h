@@ -49,9 +49,11 @@ extern "C" {
  * sa [rq_wkv7_chunks(), heads, 16, 64], both or neither: what rq_wkv7_backward reads
  * (every 16th state, and S_{t-1} a_t of every token). */
 int64_t rq_wkv7_chunks(int64_t batch, int64_t time, int64_t seqs, int has_cu_seqlens);
+int64_t rq_wkv7_workspace_bytes(int64_t batch, int64_t time, int64_t heads, int64_t seqs, int has_cu_seqlens);
 int rq_wkv7(const void* r, const void* w, const void* k, const void* v, const void* a, const void* b,
             rq_dtype dt, int64_t batch, int64_t time, int64_t heads, const int32_t* cu_seqlens, int64_t seqs,
-            const float* state, void* y, rq_dtype y_dt, float* state_out, float* states, float* sa, void* stream);
+            const float* state, void* y, rq_dtype y_dt, float* state_out, float* states, float* sa, void* workspace,
+            int64_t workspace_bytes, void* stream);
 
 /* The gradients of rq_wkv7's inputs from dy (of y_dt) and dstate_out (fp32, NULL for
  * 0).  dr .. db are of dt, dstate is fp32; each may be NULL.  states and sa are those

@@ -16,9 +16,9 @@ using rq::valid_dt;
 
 namespace {
 
-// A grid holds fewer than 2^32 threads: 768 for each head of a sequence in the scan, 256 for each
+// A grid holds fewer than 2^32 threads: up to 1024 for each head of a sequence in the scan, 256 for each
 // head of a chunk and of a decode step.
-constexpr int64_t kMaxHeadsOfSeqs = 1 << 22, kMaxHeadsOfChunks = 1 << 23, kMaxTokens = 1ll << 31;
+constexpr int64_t kMaxHeadsOfSeqs = 1 << 21, kMaxHeadsOfChunks = 1 << 23, kMaxTokens = 1ll << 31;
 
 int check_shape(const char* what, int64_t batch, int64_t time, int64_t heads, bool packed, int64_t seqs) {
     if (batch < 0 || time < 0 || heads < 0 || seqs < 0)
@@ -66,6 +66,14 @@ int check_chunks(const char* what, const rq::WkvShape& s) {
 // any pointer stands for "packed" where only sizes count
 const int32_t kPacked = 0;
 
+// The segments of a scan with their workspace, whose bytes are a multiple of 16.
+rq::WkvSegments segments(const rq::WkvShape& shape, void* workspace) {
+    rq::WkvSegments g = rq::wkv_segments(shape);
+    g.ends = (float*)workspace;
+    g.begins = g.ends ? g.ends + 2 * g.slots * shape.heads * RQ_WKV7_HEAD * RQ_WKV7_HEAD : nullptr;
+    return g;
+}
+
 }  // namespace
 
 extern "C" {
@@ -76,9 +84,17 @@ int64_t rq_wkv7_chunks(int64_t batch, int64_t time, int64_t seqs, int has_cu_seq
     return rq::wkv_chunks({has_cu_seqlens ? &kPacked : nullptr, batch, time, 0, seqs});
 }
 
+int64_t rq_wkv7_workspace_bytes(int64_t batch, int64_t time, int64_t heads, int64_t seqs, int has_cu_seqlens) {
+    if (int rc = check_shape("rq_wkv7_workspace_bytes", batch, time, heads, has_cu_seqlens, seqs)) return rc;
+    ok();
+    const rq::WkvShape shape{has_cu_seqlens ? &kPacked : nullptr, batch, time, heads, seqs};
+    return 4 * rq::wkv_segment_floats(rq::wkv_segments(shape), heads);
+}
+
 int rq_wkv7(const void* r, const void* w, const void* k, const void* v, const void* a, const void* b, rq_dtype dt,
             int64_t batch, int64_t time, int64_t heads, const int32_t* cu_seqlens, int64_t seqs, const float* state,
-            void* y, rq_dtype y_dt, float* state_out, float* states, float* sa, void* stream) {
+            void* y, rq_dtype y_dt, float* state_out, float* states, float* sa, void* workspace, int64_t workspace_bytes,
+            void* stream) {
     const char* what = "rq_wkv7";
     if (int rc = check_types(what, dt, y_dt)) return rc;
     if (int rc = check_shape(what, batch, time, heads, cu_seqlens, seqs)) return rc;
@@ -89,8 +105,12 @@ int rq_wkv7(const void* r, const void* w, const void* k, const void* v, const vo
     if (heads == 0 || (batch * time == 0 && seqs == 0)) return ok();
     if (batch * time > 0)
         if (int rc = check_ptrs(what, {r, w, k, v, a, b, y}, {})) return rc;
-    if (int rc = check_ptrs(what, {}, {state, state_out, states, sa})) return rc;
+    if (int rc = check_ptrs(what, {}, {state, state_out, states, sa, workspace})) return rc;
     if (int rc = check_cu(what, cu_seqlens)) return rc;
+    const rq::WkvSegments seg = segments(shape, workspace);
+    const int64_t need = 4 * rq::wkv_segment_floats(seg, heads);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(RQ_EINVAL, "%s: needs a workspace of %lld bytes", what, (long long)need);
     hipStream_t s = (hipStream_t)stream;
     hipError_t e = hipSuccess;
     if (cu_seqlens && time > 0) {
@@ -99,7 +119,7 @@ int rq_wkv7(const void* r, const void* w, const void* k, const void* v, const vo
         e = rq::launch_wkv_rest(shape, y_dt, rest, 1, s);
     }
     if (e == hipSuccess && seqs > 0)
-        e = rq::launch_wkv_scan({shape, {r, w, k, v, a, b, dt}, false, v, dt, y, y_dt, state, state_out, states, sa}, s);
+        e = rq::launch_wkv_scan({shape, {r, w, k, v, a, b, dt}, false, v, dt, y, y_dt, state, state_out, states, sa, seg}, s);
     return rq::launch_status(e, what);
 }
 
@@ -110,7 +130,7 @@ int64_t rq_wkv7_backward_workspace_bytes(int64_t batch, int64_t time, int64_t he
     if (int rc = check_chunks(what, shape)) return rc;
     ok();
     const int64_t chunks = rq::wkv_chunks(shape);
-    return 4 * (state_floats(chunks, heads) + sa_floats(chunks, heads));
+    return 4 * (state_floats(chunks, heads) + sa_floats(chunks, heads) + rq::wkv_segment_floats(rq::wkv_segments(shape), heads));
 }
 
 int rq_wkv7_backward(const void* r, const void* w, const void* k, const void* v, const void* a, const void* b,
@@ -131,7 +151,9 @@ int rq_wkv7_backward(const void* r, const void* w, const void* k, const void* v,
     }
     if (int rc = check_ptrs(what, {}, {dstate_out, dstate, workspace})) return rc;
     if (int rc = check_cu(what, cu_seqlens)) return rc;
-    const int64_t need = 4 * (state_floats(chunks, heads) + sa_floats(chunks, heads));
+    const int64_t own = state_floats(chunks, heads) + sa_floats(chunks, heads);
+    const rq::WkvSegments seg = segments(shape, workspace ? (float*)workspace + own : nullptr);
+    const int64_t need = 4 * (own + rq::wkv_segment_floats(seg, heads));
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(RQ_EINVAL, "%s: needs a workspace of %lld bytes", what, (long long)need);
     float* const dstates = (float*)workspace;
@@ -144,7 +166,7 @@ int rq_wkv7_backward(const void* r, const void* w, const void* k, const void* v,
         e = rq::launch_wkv_rest(shape, dt, rest, 6, s);
     }
     if (e == hipSuccess)
-        e = rq::launch_wkv_scan({shape, in, true, dy, y_dt, dv, dt, dstate_out, dstate, dstates, dz}, s);
+        e = rq::launch_wkv_scan({shape, in, true, dy, y_dt, dv, dt, dstate_out, dstate, dstates, dz, seg}, s);
     if (e == hipSuccess && chunks > 0 && batch * time > 0 && (dr || dw || dk || da || db))
         e = rq::launch_wkv_grads({shape, in, dy, y_dt, states, sa, dstates, dz, dr, dw, dk, da, db}, s);
     return rq::launch_status(e, what);

@@ -374,112 +374,168 @@ RQ_DEV void form_matrix(const WkvInputs& in, const Arrays& from, const Rows* inv
     if (pair == 3) to.y_x[lane] = x;
 }
 
-constexpr int kScanThreads = 12 * 64;
+// A segment of a sequence: which, and its chunks in processing order.
+struct Segment {
+    int64_t seq, index, first, end;
+    bool last;
+};
 
-// Four scan waves, each with 16 of the 64 values, take chunk c while four waves form the matrices of chunk
-// c + 1 and four others the arrays of chunk c + 2, load chunk c + 3 and store the y of chunk c - 1.  A scan wave
+RQ_DEV Segment segment_of(const WkvShape& s, const WkvSegments& g, int64_t slot, Span& span) {
+    int64_t seq = slot, index = 0;
+    if (g.chunks && s.cu) {
+        // as the chunks' places (WkvShape), in units of a segment: the last sequence that begins here or before
+        const int64_t tokens = g.chunks * kChunk;
+        int64_t lo = 0, hi = s.seqs;
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) / 2;
+            if (clamp_token(s.cu[mid], s.time) / tokens + mid <= slot) lo = mid;
+            else hi = mid;
+        }
+        seq = lo;
+        index = slot - (clamp_token(s.cu[lo], s.time) / tokens + lo);
+    } else if (g.chunks) {
+        const int64_t per = ((s.time + kChunk - 1) / kChunk + g.chunks - 1) / g.chunks;
+        seq = slot / per;
+        index = slot % per;
+    }
+    span = span_of(s, seq);
+    const int64_t n = span.chunks();
+    if (!g.chunks) return {seq, 0, 0, n, true};
+    // an empty sequence has one segment, without a chunk; places behind the last segment begin behind the end
+    const int64_t first = index * g.chunks;
+    return {seq, index, first, std::min(first + g.chunks, n), first + g.chunks >= n};
+}
+RQ_DEV bool unused(const Segment& s) { return s.index < 0 || (s.index > 0 && s.first >= s.end); }
+
+// Four waves form the arrays of chunk c + 2, load chunk c + 3 and store the y of chunk c - 1, four others form
+// the matrices of chunk c + 1, while four scan waves, each with 16 of the 64 values, take chunk c.  A scan wave
 // holds its state transposed, acc[q][i] = S[value lane & 15][key 16q + 4g + i]: the layout in which a product's
 // result comes and in which the next takes it.  It reads nothing from memory: on this machine loads and
 // stores are waited for in their order, and a load behind a store waits for the store too.
-template <int DT, int XDT, int YDT, bool REV>
-__global__ __launch_bounds__(kScanThreads) void wkv7_scan_kernel(WkvScan p) {
+//
+// ENDS: only where a segment ends, from a state of 0 (four scan waves) and, without x, from the identity (four more).
+template <bool ENDS>
+constexpr int kScanThreads = (ENDS ? 16 : 12) * 64;
+
+template <int DT, int XDT, int YDT, bool REV, bool ENDS>
+__global__ __launch_bounds__(kScanThreads<ENDS>) void wkv7_scan_kernel(WkvScan p) {
     __shared__ ScanLds lds;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int g = lane >> 4, m = lane & 15;
-    const int64_t H = p.shape.heads, seq = blockIdx.x / H, head = blockIdx.x % H;
-    const Span span = span_of(p.shape, seq);
-    const int64_t n = span.chunks();
+    const int64_t H = p.shape.heads, slot = blockIdx.x / H, head = blockIdx.x % H;
+    Span span;
+    const Segment seg = segment_of(p.shape, p.seg, slot, span);
+    if (unused(seg) || (ENDS && seg.last)) return;
+    const int64_t n = span.chunks(), first = seg.first, end = seg.end;
     // the chunk's token of index i, i in processing order
     const auto token = [&](int64_t c, int i) { return REV ? kChunk * (n - 1 - c) + (kChunk - 1 - i) : kChunk * c + i; };
-
     const auto exists = [&](int64_t c) { return token(c, m) < span.len; };
     const auto row = [&](int64_t c) { return (span.start + (exists(c) ? token(c, m) : 0)) * H + head; };  // where n > 0
+    const auto odd = [&](int64_t c) { return (int)(c - first) & 1; };
+
     if (wave < 4) {
         Elementwise<DT, XDT, REV> el{lane, wave};
         const auto load = [&](int64_t c) {
-            if (c < n) el.load(p.in, p.x, row(c), exists(c));
+            if (c < end) el.load(p.in, p.x, row(c), exists(c));
         };
         const auto arrays = [&](int64_t c, int ring) {
-            if (c < n) el.run(lds.arrays[ring], lds.inverse[c & 1], lds.strong[ring][wave]);
+            if (c < end) el.run(lds.arrays[ring], lds.inverse[odd(c)], lds.strong[ring][wave]);
         };
         const auto store_y = [&](int64_t c) {
-            if (c < 0 || !p.y || !exists(c)) return;
+            if (ENDS || c < first || !p.y || !exists(c)) return;
             const int at = 16 * wave + 4 * g;
-            store4<YDT>(p.y, row(c) * kHead + at, *(const f32x4_t*)&lds.y[c & 1][m][at]);
+            store4<YDT>(p.y, row(c) * kHead + at, *(const f32x4_t*)&lds.y[odd(c)][m][at]);
         };
-        load(0);
-        arrays(0, 0);
-        load(1);
+        load(first);
+        arrays(first, 0);
+        load(first + 1);
         __syncthreads();
-        arrays(1, 1);
-        load(2);
+        arrays(first + 1, 1);
+        load(first + 2);
         __syncthreads();
         int ring = 2;  // of chunk c + 2
-        for (int64_t c = 0; c < n; ++c) {
+        for (int64_t c = first; c < end; ++c) {
             arrays(c + 2, ring);
             store_y(c - 1);
             load(c + 3);
             ring = ring == 2 ? 0 : ring + 1;
             __syncthreads();
         }
-        store_y(n - 1);
+        store_y(end - 1);
         return;
     }
     if (wave < 8) {
         const auto matrix = [&](int64_t c, int ring) {
-            if (c >= n) return;
+            if (c >= end) return;
             const int* f = lds.strong[ring];
-            form_matrix<DT, REV>(p.in, lds.arrays[ring], lds.inverse[c & 1], f[0] | f[1] | f[2] | f[3], lds.matrices[c & 1],
+            form_matrix<DT, REV>(p.in, lds.arrays[ring], lds.inverse[odd(c)], f[0] | f[1] | f[2] | f[3], lds.matrices[odd(c)],
                                  lane, wave - 4, row(c), exists(c));
         };
         __syncthreads();
-        matrix(0, 0);
+        matrix(first, 0);
         __syncthreads();
         int ring = 1;  // of chunk c + 1
-        for (int64_t c = 0; c < n; ++c) {
+        for (int64_t c = first; c < end; ++c) {
             matrix(c + 1, ring);
             ring = ring == 2 ? 0 : ring + 1;
             __syncthreads();
         }
         return;
     }
-    const int value = 16 * (wave - 8) + m;
-    const int64_t state_at = ((int64_t)blockIdx.x * kHead + value) * kHead + 4 * g;
+    const bool map = ENDS && wave >= 12;
+    const int value = 16 * (wave & 3) + m;
     f32x4_t acc[4];
+    {
+        const float* from = ENDS ? nullptr
+                            : seg.index ? p.seg.begins + ((slot * H + head) * kHead + value) * kHead
+                            : p.state   ? p.state + ((seg.seq * H + head) * kHead + value) * kHead
+                                        : nullptr;
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-        acc[q] = p.state ? *(const f32x4_t*)(p.state + state_at + 16 * q) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < 4; ++q) {
+            acc[q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            if (from) acc[q] = *(const f32x4_t*)(from + 16 * q + 4 * g);
+            if (map) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[q][i] = 16 * q + 4 * g + i == value ? 1.f : 0.f;
+            }
+        }
+    }
     __syncthreads();
     __syncthreads();
     int ring = 0;
-    for (int64_t c = 0; c < n; ++c) {
+    for (int64_t c = first; c < end; ++c) {
         const Arrays& b = lds.arrays[ring];
-        const Matrices& mat = lds.matrices[c & 1];
+        const Matrices& mat = lds.matrices[odd(c)];
         ring = ring == 2 ? 0 : ring + 1;
-        const int64_t slot = (span.chunk0 + (REV ? n - 1 - c : c)) * H + head;
-        if (p.states) {
-            float* to = p.states + (slot * kHead + value) * kHead + 4 * g;
+        const int64_t chunk = (span.chunk0 + (REV ? n - 1 - c : c)) * H + head;
+        if (!ENDS && p.states) {
+            float* to = p.states + (chunk * kHead + value) * kHead + 4 * g;
 #pragma unroll
             for (int q = 0; q < 4; ++q) *(f32x4_t*)(to + 16 * q) = acc[q];
         }
         const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-        f32x4_t to_sa[4], to_y[4], fs[4], fx[4], v;
+        f32x4_t to_sa[4], to_y[4], fs[4], fx[4], v = zero;
+        if (!map) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = b.x[4 * g + i][value];
+            for (int i = 0; i < 4; ++i) v[i] = b.x[4 * g + i][value];
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) to_sa[q] = *(const f32x4_t*)&b.to_sa[m][16 * q + 4 * g];
         const f32x4_t sa_x = mat.sa_x[lane], inv = mat.inv[lane];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) to_y[q] = *(const f32x4_t*)&b.to_y[m][16 * q + 4 * g];
-        const f32x4_t y_sa = mat.y_sa[lane], y_x = mat.y_x[lane];
-        f32x4_t z[2] = {zero, zero}, y[2] = {zero, zero};
-        z[0] = mma16(sa_x, v, z[0]);
+        f32x4_t z[2] = {zero, zero}, y[2] = {zero, zero}, y_sa, y_x;
+        if (!map) z[0] = mma16(sa_x, v, z[0]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) z[q & 1] = mma16(to_sa[q], acc[q], z[q & 1]);
         z[0] += z[1];
+        if constexpr (!ENDS) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) y[q & 1] = mma16(to_y[q], acc[q], y[q & 1]);
-        y[1] = mma16(y_x, v, y[1]);
+            for (int q = 0; q < 4; ++q) to_y[q] = *(const f32x4_t*)&b.to_y[m][16 * q + 4 * g];
+            y_sa = mat.y_sa[lane];
+            y_x = mat.y_x[lane];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) y[q & 1] = mma16(to_y[q], acc[q], y[q & 1]);
+            y[1] = mma16(y_x, v, y[1]);
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
 #pragma unroll
@@ -490,27 +546,72 @@ __global__ __launch_bounds__(kScanThreads) void wkv7_scan_kernel(WkvScan p) {
         }
         const f32x4_t sa = mma16(inv, z[0], zero);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            acc[q] *= *(const f32x4_t*)&b.decay[16 * q + 4 * g];
-            acc[q] = mma16(fx[q], v, acc[q]);
+        for (int q = 0; q < 4; ++q) acc[q] *= *(const f32x4_t*)&b.decay[16 * q + 4 * g];
+        if (!map) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[q] = mma16(fx[q], v, acc[q]);
         }
-        y[0] = mma16(y_sa, sa, y[0]);
+        if constexpr (!ENDS) y[0] = mma16(y_sa, sa, y[0]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)  // one step of each sum in turn
 #pragma unroll
             for (int q = 0; q < 4; ++q) acc[q] = mfma4(fs[q][i], sa[i], acc[q]);
+        if constexpr (!ENDS) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) lds.y[c & 1][4 * g + i][value] = y[0][i] + y[1][i];
-        if (p.sa) {  // rows in the order of time, the missing ones 0
+            for (int i = 0; i < 4; ++i) lds.y[odd(c)][4 * g + i][value] = y[0][i] + y[1][i];
+            if (p.sa) {  // rows in the order of time, the missing ones 0
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                p.sa[(slot * kChunk + (REV ? kChunk - 1 - (4 * g + i) : 4 * g + i)) * kHead + value] = sa[i];
+                for (int i = 0; i < 4; ++i)
+                    p.sa[(chunk * kChunk + (REV ? kChunk - 1 - (4 * g + i) : 4 * g + i)) * kHead + value] = sa[i];
+            }
         }
         __syncthreads();
     }
-    if (p.state_out) {
+    float* to = ENDS ? p.seg.ends + ((slot * H + head) * 2 * kHead + (map ? kHead : 0) + value) * kHead
+                : p.state_out && seg.last ? p.state_out + ((seg.seq * H + head) * kHead + value) * kHead
+                                          : nullptr;
+    if (to) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) *(f32x4_t*)(p.state_out + state_at + 16 * q) = acc[q];
+        for (int q = 0; q < 4; ++q) *(f32x4_t*)(to + 16 * q + 4 * g) = acc[q];
+    }
+}
+
+// The states at the segments' beginnings, S' = S M + N from one to the next: a block is a head of a sequence,
+// its waves the 16 tiles of 16 values and 16 keys, and the state goes round through LDS.
+__global__ __launch_bounds__(1024) void wkv7_join_kernel(WkvShape shape, WkvSegments seg, const float* state) {
+    __shared__ Rows lds[2][4];  // [value / 16][value % 16][key]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = lane >> 4, m = lane & 15, q = wave & 3, tile = wave >> 2;
+    const int64_t H = shape.heads, seq = blockIdx.x / H, head = blockIdx.x % H;
+    const Span span = span_of(shape, seq);
+    const int64_t count = (span.chunks() + seg.chunks - 1) / seg.chunks;
+    if (count < 2) return;
+    const int64_t slot0 = shape.cu ? span.start / (seg.chunks * kChunk) + seq
+                                   : seq * (((shape.time + kChunk - 1) / kChunk + seg.chunks - 1) / seg.chunks);
+    const int value = 16 * tile + m;
+    f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+    if (state) s = *(const f32x4_t*)(state + ((seq * H + head) * kHead + value) * kHead + 16 * q + 4 * g);
+    float map[16];  // M[key 16j + 4g + i][key 16q + m]
+    f32x4_t add;    // N[value][key 16q + 4g + i]
+    const auto load = [&](int64_t j) {
+        const float* from = seg.ends + ((slot0 + j) * H + head) * 2 * kHead * kHead;
+        add = *(const f32x4_t*)(from + value * kHead + 16 * q + 4 * g);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) map[x] = from[(kHead + 16 * (x >> 2) + 4 * g + (x & 3)) * kHead + 16 * q + m];
+    };
+    load(0);
+    for (int64_t j = 0; j + 1 < count; ++j) {
+        *(f32x4_t*)&lds[j & 1][tile][m][16 * q + 4 * g] = s;
+        __syncthreads();
+        f32x4_t sum[2] = {add, {0.f, 0.f, 0.f, 0.f}}, a[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) a[x] = f32x4_t{map[4 * x], map[4 * x + 1], map[4 * x + 2], map[4 * x + 3]};
+        if (j + 2 < count) load(j + 1);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            sum[x & 1] = mma16(a[x], *(const f32x4_t*)&lds[j & 1][tile][m][16 * x + 4 * g], sum[x & 1]);
+        s = sum[0] + sum[1];
+        *(f32x4_t*)(seg.begins + (((slot0 + j + 1) * H + head) * kHead + value) * kHead + 16 * q + 4 * g) = s;
     }
 }
 
@@ -896,12 +997,24 @@ __global__ __launch_bounds__(256) void wkv7_rest_kernel(WkvShape s, RestTensors 
     }
 }
 
+template <int DT, int XDT, int YDT, bool REV>
+hipError_t scan_all(const WkvScan& a, hipStream_t s) {
+    const int64_t heads = a.shape.heads;
+    if (a.seg.chunks) {
+        const dim3 grid((unsigned)(a.seg.slots * heads));
+        wkv7_scan_kernel<DT, XDT, YDT, REV, true><<<grid, kScanThreads<true>, 0, s>>>(a);
+        wkv7_join_kernel<<<dim3((unsigned)(a.shape.seqs * heads)), 1024, 0, s>>>(a.shape, a.seg, a.state);
+        wkv7_scan_kernel<DT, XDT, YDT, REV, false><<<grid, kScanThreads<false>, 0, s>>>(a);
+    } else {
+        wkv7_scan_kernel<DT, XDT, YDT, REV, false>
+            <<<dim3((unsigned)(a.shape.seqs * heads)), kScanThreads<false>, 0, s>>>(a);
+    }
+    return hipGetLastError();
+}
+
 template <int DT, int ODT>
 hipError_t scan_dt(const WkvScan& a, hipStream_t s) {
-    const dim3 grid((unsigned)(a.shape.seqs * a.shape.heads));
-    if (a.reverse) wkv7_scan_kernel<DT, ODT, DT, true><<<grid, kScanThreads, 0, s>>>(a);
-    else wkv7_scan_kernel<DT, DT, ODT, false><<<grid, kScanThreads, 0, s>>>(a);
-    return hipGetLastError();
+    return a.reverse ? scan_all<DT, ODT, DT, true>(a, s) : scan_all<DT, DT, ODT, false>(a, s);
 }
 
 template <int DT, int ODT>

@@ -104,7 +104,9 @@ SIGNATURES = {
     "rq_clip_grads": ([_vp, _i64, ctypes.c_float, ctypes.c_float, _vp, _vp, _i64, _vp], _i32),
     # include/rwkvq_rwkv7.h
     "rq_wkv7_chunks": ([_i64, _i64, _i64, _i32], _i64),
-    "rq_wkv7": ([_vp] * 6 + [_i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _vp], _i32),
+    "rq_wkv7": ([_vp] * 6 + [_i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _vp],
+                _i32),
+    "rq_wkv7_workspace_bytes": ([_i64, _i64, _i64, _i64, _i32], _i64),
     "rq_wkv7_backward_workspace_bytes": ([_i64, _i64, _i64, _i64, _i32], _i64),
     "rq_wkv7_backward": ([_vp] * 6 + [_i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _vp] +
                          [_vp] * 7 + [_vp, _i64, _vp], _i32),

@@ -61,9 +61,11 @@ def _wkv7_impl(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor,
             rc = L.rq_wkv7_step(_ptr(r), _ptr(w), _ptr(k), _ptr(v), _ptr(a), _ptr(b), dt, batch, heads,
                                 _addr(state), _ptr(y), odt, _ptr(last), stream)
         else:
+            ws = _queried_workspace("rq_wkv7_workspace_bytes", (batch, time, heads, seqs, cu is not None), r.device,
+                                    "wkv7")
             rc = L.rq_wkv7(_ptr(r), _ptr(w), _ptr(k), _ptr(v), _ptr(a), _ptr(b), dt, batch, time, heads,
                            0 if cu is None else cu.data_ptr(), seqs, _addr(state), _ptr(y), odt, _ptr(last),
-                           _addr(states), _addr(sa), stream)
+                           _addr(states), _addr(sa), _addr(ws), _size(ws), stream)
     if rc:
         check(rc, "wkv7")
     return y, last, states, sa

@@ -78,6 +78,51 @@ def test_packed_sequences(rq, dev, i, dt, train):
     check(rq, dev, 50 + i, 1, 0, 1 + i % 3, dt, "fp32" if i % 2 else dt, i % 4 != 3, train, LENS[i], rest)
 
 
+# few heads over many tokens: in segments, whole ones and one of a single token behind them, sequences of
+# one segment and of several side by side
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("b,t,h", [(1, 385, 1), (1, 700, 2), (2, 513, 1), (1, 1024, 3)])
+def test_segments(rq, dev, b, t, h, dt):
+    assert rq._lib.lib().rq_wkv7_workspace_bytes(b, t, h, b, 0) > 0
+    print(f"wkv7 segments b={b} t={t} h={h} {dt}", flush=True)
+    check(rq, dev, 60 + t, b, t, h, dt, "fp32", t % 2 == 0, True)
+    check(rq, dev, 61 + t, b, t, h, dt, dt, t % 2 == 1, False)
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_packed_segments(rq, dev, i):
+    lens = [[600, 3, 0, 401], [0, 0, 1, 800], [129, 128, 127, 385, 1, 0], [16, 900]][i]
+    rest = (0, 5, 40, 1)[i]
+    assert rq._lib.lib().rq_wkv7_workspace_bytes(1, sum(lens) + rest, 2, len(lens), 1) > 0
+    check(rq, dev, 90 + i, 1, 0, 2, ("fp32", "bf16", "f16", "fp32")[i], "fp32", i != 3, True, lens, rest)
+
+
+def test_segments_with_strong_decays_and_equal_directions(rq, dev):
+    def change(six, g):
+        w = six[1]
+        w.copy_(torch.randn(w.shape, generator=g) * 3 - 1)
+        w[:, 100:130, :, ::5] = math.inf
+    check(rq, dev, 95, 1, 450, 1, "fp32", "fp32", True, True, change=change)
+
+    def change(six, g):
+        u = torch.nn.functional.normalize(torch.randn(D, generator=g), dim=-1)
+        six[4].copy_(-u.expand_as(six[4]))
+        six[5].copy_(u.expand_as(six[5]))
+    check(rq, dev, 96, 1, 450, 1, "fp32", "fp32", True, True, change=change, w=-6.0)
+
+
+def test_wild_boundaries_in_segments(rq, dev):
+    """Nothing outside the tensors is touched."""
+    g = torch.Generator().manual_seed(97)
+    six = [x.to(dev).requires_grad_() for x in inputs(g, 1, 900, 2)]
+    wild = torch.tensor([850, 3, 700, -1, 2 ** 31 - 1, 0, 899], dtype=torch.int32, device=dev)
+    assert rq._lib.lib().rq_wkv7_workspace_bytes(1, 900, 2, 6, 1) > 0
+    y, last = rq.wkv7(*six, cu_seqlens=wild)
+    grads = torch.autograd.grad(y.sum() + last.sum(), six)
+    torch.cuda.synchronize()
+    assert y.shape == six[0].shape and len(grads) == 6
+
+
 def test_many_packed_sequences(rq, dev):
     lens = [(7 * i) % 23 for i in range(200)]
     check(rq, dev, 77, 1, 0, 2, "fp32", "fp32", True, True, lens, 5)

@@ -26,7 +26,7 @@ def test_every_declared_entry_point_is_exported_and_bound(L):
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     names = set(re.findall(r"^\s*\w+\s+(rq_\w+)\s*\(", text, flags=re.M))
     assert names == {"rq_wkv7", "rq_wkv7_backward", "rq_wkv7_step", "rq_wkv7_chunks",
-                     "rq_wkv7_backward_workspace_bytes", "rq_sample"}
+                     "rq_wkv7_workspace_bytes", "rq_wkv7_backward_workspace_bytes", "rq_sample"}
     for name in names:
         assert hasattr(L, name) and name in _lib.SIGNATURES
 
@@ -38,6 +38,13 @@ def test_chunks_and_workspaces(L):
     assert L.rq_wkv7_chunks(0, 5, 0, 0) == 0
     assert L.rq_wkv7_backward_workspace_bytes(1, 16, 2, 1, 0) >= 2 * 4 * (64 * 64 + 16 * 64)
     assert L.rq_wkv7_backward_workspace_bytes(1, 2 ** 30, 64, 1, 0) == -1 and "heads of chunks" in err(L)
+    # few heads over many tokens run in segments, which take room for 3 states each; many heads do not
+    one = 3 * 4 * 64 * 64
+    assert L.rq_wkv7_workspace_bytes(1, 16, 12, 1, 0) == 0 and L.rq_wkv7_workspace_bytes(8, 512, 32, 8, 0) == 0
+    for args in ((1, 8192, 12, 1, 0), (1, 2047, 32, 1, 0), (1, 8192, 12, 3, 1)):
+        n = L.rq_wkv7_workspace_bytes(*args)
+        assert n > 0 and n % (one * args[2]) == 0
+    assert L.rq_wkv7_workspace_bytes(2, 1, 1, 1, 0) == -1
 
 
 def test_packed_sequences_never_share_a_chunk():
@@ -55,16 +62,17 @@ def test_packed_sequences_never_share_a_chunk():
 
 
 def test_scan_refusals(L):
-    def fwd(x=P, dt=0, batch=1, time=4, heads=2, cu=0, seqs=1, state=0, y=P, ydt=0, so=0, st=0, sa=0, w=P):
-        return L.rq_wkv7(x, w, x, x, x, x, dt, batch, time, heads, cu, seqs, state, y, ydt, so, st, sa, None)
+    def fwd(x=P, dt=0, batch=1, time=4, heads=2, cu=0, seqs=1, state=0, y=P, ydt=0, so=0, st=0, sa=0, w=P, ws=0, nb=0):
+        return L.rq_wkv7(x, w, x, x, x, x, dt, batch, time, heads, cu, seqs, state, y, ydt, so, st, sa, ws, nb, None)
 
     for kw, text in (({"dt": 3}, "dtype"), ({"ydt": 1}, "y must have"), ({"time": -1}, "negative"), ({"x": 0}, "NULL"),
                      ({"y": 0}, "NULL"), ({"w": 0}, "NULL"), ({"seqs": 2}, "seqs"), ({"cu": P, "batch": 2}, "batch of 1"),
                      ({"cu": P, "seqs": 0}, "no sequence"), ({"st": P}, "together"), ({"sa": P}, "together"),
                      ({"time": 2 ** 31}, "2^31"), ({"batch": 2 ** 20, "seqs": 2 ** 20, "heads": 64}, "heads of sequences"),
-                     ({"time": 2 ** 30, "heads": 64, "st": P, "sa": P}, "heads of chunks")):
+                     ({"time": 2 ** 30, "heads": 64, "st": P, "sa": P}, "heads of chunks"),
+                     ({"time": 2 ** 16}, "workspace"), ({"time": 2 ** 16, "ws": P, "nb": 64}, "workspace")):
         assert fwd(**kw) == -1 and text in err(L), (kw, err(L))
-    for kw in ({"x": P + 2}, {"w": P + 8}, {"y": P + 4}, {"state": P + 8}, {"so": P + 4}, {"st": P + 4, "sa": P},
+    for kw in ({"x": P + 2}, {"w": P + 8}, {"y": P + 4}, {"state": P + 8}, {"so": P + 4}, {"st": P + 4, "sa": P}, {"ws": P + 8},
                {"cu": P + 2}):
         assert fwd(**kw) == -2 and "aligned" in err(L), kw
     assert fwd(heads=0) == 0 and fwd(batch=0, seqs=0) == 0
@@ -91,7 +99,7 @@ def test_step_refusals(L):
         return L.rq_wkv7_step(x, x, x, x, x, x, dt, batch, heads, state, y, ydt, so, None)
 
     for kw, text in (({"dt": 7}, "dtype"), ({"ydt": 1}, "y must have"), ({"batch": -1}, "negative"), ({"x": 0}, "NULL"),
-                     ({"y": 0}, "NULL"), ({"batch": 2 ** 22, "heads": 2}, "heads of sequences")):
+                     ({"y": 0}, "NULL"), ({"batch": 2 ** 21, "heads": 2}, "heads of sequences")):
         assert step(**kw) == -1 and text in err(L), (kw, err(L))
     for kw in ({"x": P + 2}, {"state": P + 8}, {"so": P + 8}, {"y": P + 2}):
         assert step(**kw) == -2 and "aligned" in err(L), kw
