@@ -22,7 +22,7 @@
 //   db = e^-L (e^Lend SA dS' + dMrb^T R~ + dMab^T A~), dk alike with V, dMrk, dMak
 //   dlog d_t: what of the loss passes token t's decay (grads_kernel).
 //
-// All products are fp32 MFMAs (v_mfma_f32_16x16x4_f32): the state lives in fp32 and
+// The scan's products are fp32 MFMAs (v_mfma_f32_16x16x4_f32): the state lives in fp32 and
 // feeds itself for thousands of tokens.
 //
 // e^-L overflows where the decays of a chunk are strong.  Below 2^-32 over one
@@ -55,6 +55,10 @@ RQ_DEV f32x4_t mma16(const f32x4_t& a, const f32x4_t& b, f32x4_t c) {
     for (int i = 0; i < 4; ++i) c = mfma4(a[i], b[i], c);
     return c;
 }
+
+// The same in all lanes, and known to be: branches on it are scalar.  MFMAs do not heed the execution mask, so that
+// one in a branch that lanes are masked out of instead of jumping over it would still write.
+RQ_DEV int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 RQ_DEV float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -420,7 +424,7 @@ constexpr int kScanThreads = (ENDS ? 16 : 12) * 64;
 template <int DT, int XDT, int YDT, bool REV, bool ENDS>
 __global__ __launch_bounds__(kScanThreads<ENDS>) void wkv7_scan_kernel(WkvScan p) {
     __shared__ ScanLds lds;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = wave_index();
     const int g = lane >> 4, m = lane & 15;
     const int64_t H = p.shape.heads, slot = blockIdx.x / H, head = blockIdx.x % H;
     Span span;
@@ -580,7 +584,7 @@ __global__ __launch_bounds__(kScanThreads<ENDS>) void wkv7_scan_kernel(WkvScan p
 // its waves the 16 tiles of 16 values and 16 keys, and the state goes round through LDS.
 __global__ __launch_bounds__(1024) void wkv7_join_kernel(WkvShape shape, WkvSegments seg, const float* state) {
     __shared__ Rows lds[2][4];  // [value / 16][value % 16][key]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = wave_index();
     const int g = lane >> 4, m = lane & 15, q = wave & 3, tile = wave >> 2;
     const int64_t H = shape.heads, seq = blockIdx.x / H, head = blockIdx.x % H;
     const Span span = span_of(shape, seq);
@@ -633,30 +637,119 @@ RQ_DEV float over_groups(float x) {
 
 constexpr int kPairRow = 20;  // LDS row of a [16, 16] matrix
 
+// The products of the gradients.  They are not fed back into anything, and where the tensors have 16 bits
+// their results are rounded to 8 or 11 significant ones: there an operand is the sum of two bf16 (16 bits of
+// it), a product three bf16 MFMAs of 32 steps, at a fifth of the fp32 MFMA's time and beside the VALU, which
+// the fp32 one holds up.  fp32 tensors keep fp32 products.
+struct Halves {
+    bf16x8_t hi, lo;
+};
+RQ_DEV Halves halves_of(const f32x4_t& x, const f32x4_t& y) {
+    Halves h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h.hi[i] = (__bf16)x[i];
+        h.hi[4 + i] = (__bf16)y[i];
+        h.lo[i] = (__bf16)(x[i] - (float)h.hi[i]);
+        h.lo[4 + i] = (__bf16)(y[i] - (float)h.hi[4 + i]);
+    }
+    return h;
+}
+// EXACT: an operand that is bf16 as it is (its lo is 0)
+template <bool EXACT_A, bool EXACT_B>
+RQ_DEV f32x4_t mma_halves(const Halves& a, const Halves& b, f32x4_t c) {
+    if constexpr (!EXACT_A) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.lo, b.hi, c, 0, 0, 0);
+    if constexpr (!EXACT_B) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.lo, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.hi, c, 0, 0, 0);
+}
+
+// A row or column of N / 4 lanes' shares, four numbers from each 16: N = 64 values, or the 16 tokens of two matrices.
+template <bool HALF, int N>
+struct Operand {
+    f32x4_t v[N / 16];
+    RQ_DEV explicit Operand(const f32x4_t* x) {
+#pragma unroll
+        for (int q = 0; q < N / 16; ++q) v[q] = x[q];
+    }
+};
+template <int N>
+struct Operand<true, N> {
+    Halves v[N / 32];
+    RQ_DEV explicit Operand(const f32x4_t* x) {
+#pragma unroll
+        for (int q = 0; q < N / 32; ++q) v[q] = halves_of(x[2 * q], x[2 * q + 1]);
+    }
+    RQ_DEV explicit Operand(const Halves& h) { v[0] = h; }
+};
+template <bool EXACT_A = false, bool EXACT_B = false, bool HALF, int N>
+RQ_DEV f32x4_t mma(const Operand<HALF, N>& a, const Operand<HALF, N>& b, f32x4_t c) {
+    if constexpr (HALF) {
+#pragma unroll
+        for (int q = 0; q < N / 32; ++q) c = mma_halves<EXACT_A, EXACT_B>(a.v[q], b.v[q], c);
+    } else {
+#pragma unroll
+        for (int q = 0; q < N / 16; ++q) c = mma16(a.v[q], b.v[q], c);
+    }
+    return c;
+}
+
 struct GradLds {
-    float m[4][kChunk][kPairRow];       // dMab, dMak, dMrb, dMrk, [s][t], s < t
+    uint32_t m[4][kChunk][kPairRow];    // dMab, dMak, dMrb, dMrk, [s][t], s < t: as they are, or their halves
     float own[2][kChunk];               // the diagonals of dMrb, dMrk
     float strong[4][5][kChunk][16];     // r, a, b, k and log2 d of a wave's 16 keys
 };
 
+template <bool HALF>
+RQ_DEV uint32_t pack_pair(float x) {
+    if constexpr (!HALF) return __float_as_uint(x);
+    const uint32_t hi = f32_to_bf16_bits(x);
+    return hi << 16 | f32_to_bf16_bits(x - bf16_bits_to_f32(hi));
+}
+template <bool HALF>
+RQ_DEV float pair_of(uint32_t u) {
+    return HALF ? __uint_as_float(u & 0xffff0000u) + __uint_as_float(u << 16) : __uint_as_float(u);
+}
+// The operand of two matrices' entries.
+template <bool HALF>
+RQ_DEV Operand<HALF, 32> pair_operand(const uint32_t* x, const uint32_t* y) {
+    if constexpr (HALF) {
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        const u32x4 hi = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302), __builtin_amdgcn_perm(x[3], x[2], 0x07060302),
+                          __builtin_amdgcn_perm(y[1], y[0], 0x07060302), __builtin_amdgcn_perm(y[3], y[2], 0x07060302)};
+        const u32x4 lo = {__builtin_amdgcn_perm(x[1], x[0], 0x05040100), __builtin_amdgcn_perm(x[3], x[2], 0x05040100),
+                          __builtin_amdgcn_perm(y[1], y[0], 0x05040100), __builtin_amdgcn_perm(y[3], y[2], 0x05040100)};
+        return Operand<true, 32>(Halves{__builtin_bit_cast(bf16x8_t, hi), __builtin_bit_cast(bf16x8_t, lo)});
+    } else {
+        f32x4_t v[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[0][i] = __uint_as_float(x[i]);
+            v[1][i] = __uint_as_float(y[i]);
+        }
+        return Operand<false, 32>(v);
+    }
+}
+
 // The parts of the gradients that come from the pairs within a chunk of strong decays, for the
 // lane's key and tokens 4g + i: gr, ga, gb, gk, and in `cross` what of the loss passes each
 // token's decay.
+template <bool HALF>
 __device__ __attribute__((noinline)) void strong_grads(const GradLds& lds, int wave, int lane, float* gr, float* ga,
                                                        float* gb, float* gk, float* cross) {
     const int g = lane >> 4, key = lane & 15;
     const auto& in = lds.strong[wave];
+    const auto pair = [&](int j, int s, int t) { return pair_of<HALF>(lds.m[j][s][t]); };
     for (int i = 0; i < 4; ++i) {
         const int own = 4 * g + i;
         gr[i] = ga[i] = gb[i] = gk[i] = cross[i] = 0.f;
         float e = in[4][own][key];  // log2 of the decay from s to own
         for (int s = own - 1; s >= 0; --s) {
-            gr[i] += (lds.m[2][s][own] * in[2][s][key] + lds.m[3][s][own] * in[3][s][key]) * exp2_hw(e);
+            gr[i] += (pair(2, s, own) * in[2][s][key] + pair(3, s, own) * in[3][s][key]) * exp2_hw(e);
             e += in[4][s][key];
         }
         e = 0.f;
         for (int s = own - 1; s >= 0; --s) {
-            ga[i] += (lds.m[0][s][own] * in[2][s][key] + lds.m[1][s][own] * in[3][s][key]) * exp2_hw(e);
+            ga[i] += (pair(0, s, own) * in[2][s][key] + pair(1, s, own) * in[3][s][key]) * exp2_hw(e);
             e += in[4][s][key];
         }
         e = 0.f;
@@ -664,29 +757,34 @@ __device__ __attribute__((noinline)) void strong_grads(const GradLds& lds, int w
             const float f = in[1][t][key] * exp2_hw(e);
             e += in[4][t][key];
             const float h = in[0][t][key] * exp2_hw(e);
-            gb[i] += lds.m[0][own][t] * f + lds.m[2][own][t] * h;
-            gk[i] += lds.m[1][own][t] * f + lds.m[3][own][t] * h;
+            gb[i] += pair(0, own, t) * f + pair(2, own, t) * h;
+            gk[i] += pair(1, own, t) * f + pair(3, own, t) * h;
         }
         for (int s = 0; s < own; ++s) {
             e = 0.f;
             for (int t = s + 1; t < kChunk; ++t) {
                 if (t > own)  // a's decays end before t
-                    cross[i] += in[1][t][key] * exp2_hw(e) *
-                                (lds.m[0][s][t] * in[2][s][key] + lds.m[1][s][t] * in[3][s][key]);
+                    cross[i] += in[1][t][key] * exp2_hw(e) * (pair(0, s, t) * in[2][s][key] + pair(1, s, t) * in[3][s][key]);
                 e += in[4][t][key];
                 if (t >= own)
-                    cross[i] += in[0][t][key] * exp2_hw(e) *
-                                (lds.m[2][s][t] * in[2][s][key] + lds.m[3][s][t] * in[3][s][key]);
+                    cross[i] += in[0][t][key] * exp2_hw(e) * (pair(2, s, t) * in[2][s][key] + pair(3, s, t) * in[3][s][key]);
             }
         }
     }
 }
 
-// Four contiguous values of a row as fp32.
+// Four contiguous values of a row as fp32, `at` bytes behind a pointer that all lanes share.
 template <int DT>
-RQ_DEV f32x4_t load4(const void* p, int64_t at, bool there) {
-    const f32x4_t x = unpack_raw4<DT>(load_raw4<DT>(p, at));
-    return there ? x : f32x4_t{0.f, 0.f, 0.f, 0.f};
+RQ_DEV f32x4_t load4(const uint8_t* p, uint32_t at) {
+    return unpack_raw4<DT>(*(const Raw4<DT>*)(p + at));
+}
+template <int DT>
+RQ_DEV typename dt_traits<DT>::storage load1(const uint8_t* p, uint32_t at) {
+    return *(const typename dt_traits<DT>::storage*)(p + at);
+}
+template <int DT>
+RQ_DEV void store1(uint8_t* p, uint32_t at, float x) {
+    *(typename dt_traits<DT>::storage*)(p + at) = dt_traits<DT>::from_f32(x);
 }
 
 // A block is one chunk of one head; each of its four waves has 16 keys, and one of the four pair
@@ -694,10 +792,12 @@ RQ_DEV f32x4_t load4(const void* p, int64_t at, bool there) {
 // keys (B); the results, tokens 4g + i of key lane & 15, are where the gradients are formed.
 template <int DT, int YDT>
 __global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
+    constexpr bool HALF = DT != RQ_F32, V_EXACT = DT == RQ_BF16, DY_EXACT = YDT == RQ_BF16;
+    constexpr uint32_t SIZE = DT == RQ_F32 ? 4 : 2, YSIZE = YDT == RQ_F32 ? 4 : 2;
     __shared__ GradLds lds;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = wave_index();
     const int g = lane >> 4, m = lane & 15;
-    const int64_t H = p.shape.heads, slot = blockIdx.x, head = slot % H, chunk = slot / H;
+    const uint32_t heads = (uint32_t)p.shape.heads, head = blockIdx.x % heads, chunk = blockIdx.x / heads;
     Span span;
     if (p.shape.cu) {  // the last sequence that begins at this chunk or before
         int64_t lo = 0, hi = p.shape.seqs;
@@ -708,82 +808,105 @@ __global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
         }
         span = span_of(p.shape, lo);
     } else {
-        span = span_of(p.shape, chunk / ((p.shape.time + kChunk - 1) / kChunk));
+        span = span_of(p.shape, chunk / (uint32_t)((p.shape.time + kChunk - 1) / kChunk));
     }
-    const int64_t c = chunk - span.chunk0;
+    const int64_t c = (int64_t)chunk - span.chunk0;
     if (c < 0 || c >= span.chunks()) return;
     const int64_t t0 = kChunk * c;
+    const int tokens = (int)std::min<int64_t>(kChunk, span.len - t0);
+    const int64_t first = ((span.start + t0) * heads + head) * kHead;  // the chunk's first element
+    const uint32_t stride = heads * kHead;                             // from token to token
+    const auto of_chunk = [&](const void* q, uint32_t size) { return (const uint8_t*)q + first * size; };
 
-    // rows of tokens: dy, dz, sa, v of token m, values 16q + 4g + i
-    const bool there = t0 + m < span.len;
-    const int64_t row = (span.start + t0 + (there ? m : 0)) * H + head;
+    // rows of tokens: dy, dz, sa, v of token m, values 16q + 4g + i.  A load under a condition would be waited for
+    // where the condition ends: tokens that are not there load the first.
+    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+    const uint32_t row = (m < tokens ? m : 0) * stride + 4 * g;
     f32x4_t dy[4], dz[4], sa[4], v[4];
+    const uint8_t* const dz_at = (const uint8_t*)(p.dz + (int64_t)blockIdx.x * kChunk * kHead);
+    const uint8_t* const sa_at = (const uint8_t*)(p.sa + (int64_t)blockIdx.x * kChunk * kHead);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        dy[q] = load4<YDT>(p.dy, row * kHead + 16 * q + 4 * g, there);
-        v[q] = load4<DT>(p.in.v, row * kHead + 16 * q + 4 * g, there);
-        dz[q] = load4<RQ_F32>(p.dz, (slot * kChunk + m) * kHead + 16 * q + 4 * g, true);
-        sa[q] = load4<RQ_F32>(p.sa, (slot * kChunk + m) * kHead + 16 * q + 4 * g, true);
+        dy[q] = load4<YDT>(of_chunk(p.dy, YSIZE), (row + 16 * q) * YSIZE);
+        v[q] = load4<DT>(of_chunk(p.in.v, SIZE), (row + 16 * q) * SIZE);
+        dz[q] = load4<RQ_F32>(dz_at, (m * kHead + 16 * q + 4 * g) * 4);
+        sa[q] = load4<RQ_F32>(sa_at, (m * kHead + 16 * q + 4 * g) * 4);
     }
     const int key = 16 * wave + m;
-    // this wave's tensors: tokens 4g + i of its key
-    float r[4], a[4], b[4], k[4], g2[4], l[4], w[4];
-    bool has[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t t = t0 + 4 * g + i;
-        has[i] = t < span.len;
-        const int64_t at = ((span.start + (has[i] ? t : t0)) * H + head) * kHead + key;
-        r[i] = load_dt(p.in.r, DT, at);
-        a[i] = load_dt(p.in.a, DT, at);
-        b[i] = load_dt(p.in.b, DT, at);
-        k[i] = load_dt(p.in.k, DT, at);
-        w[i] = load_dt(p.in.w, DT, at);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (!has[i]) r[i] = a[i] = b[i] = k[i] = 0.f;
-    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-    f32x4_t gr = zero, ga = zero, gb = zero, gk = zero;
-    float through = 0.f;  // sum over the values of S dS' of this key
-    const float* s_at = p.states + slot * kHead * kHead + key;
-    const float* d_at = p.dstates + slot * kHead * kHead + key;
+    // columns of keys: S and dS' of values 16q + 4g + i
+    f32x4_t s[4], d[4];
+    const uint8_t* const s_at = (const uint8_t*)(p.states + (int64_t)blockIdx.x * kHead * kHead);
+    const uint8_t* const d_at = (const uint8_t*)(p.dstates + (int64_t)blockIdx.x * kHead * kHead);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        f32x4_t s, d;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            s[i] = s_at[(16 * q + 4 * g + i) * kHead];
-            d[i] = d_at[(16 * q + 4 * g + i) * kHead];
-            through = fmaf(s[i], d[i], through);
+            const uint32_t at = ((16 * q + 4 * g + i) * kHead + key) * 4;
+            s[q][i] = *(const float*)(s_at + at);
+            d[q][i] = *(const float*)(d_at + at);
         }
-        gr = mma16(dy[q], s, gr);
-        ga = mma16(dz[q], s, ga);
-        gb = mma16(sa[q], d, gb);
-        gk = mma16(v[q], d, gk);
     }
-    through = over_groups(through);
+    // this wave's tensors: tokens 4g + i of its key
+    float r[4], a[4], b[4], k[4], g2[4], l[4];
+    uint32_t at[4];
     {
-        f32x4_t pm = zero;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) pm = mma16((wave & 1) ? v[q] : sa[q], wave < 2 ? dz[q] : dy[q], pm);
+        typename dt_traits<DT>::storage raw[5][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = 4 * g + i;
-            lds.m[wave][s][m] = s < m ? pm[i] : 0.f;
-            if (wave >= 2 && s == m) lds.own[wave - 2][m] = pm[i];
+            at[i] = ((4 * g + i < tokens ? 4 * g + i : 0) * stride + key) * SIZE;
+            raw[0][i] = load1<DT>(of_chunk(p.in.w, SIZE), at[i]);
+            raw[1][i] = load1<DT>(of_chunk(p.in.r, SIZE), at[i]);
+            raw[2][i] = load1<DT>(of_chunk(p.in.a, SIZE), at[i]);
+            raw[3][i] = load1<DT>(of_chunk(p.in.b, SIZE), at[i]);
+            raw[4][i] = load1<DT>(of_chunk(p.in.k, SIZE), at[i]);
         }
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        g2[i] = has[i] ? log2_decay(w[i]) : 0.f;
-        l[i] = i ? l[i - 1] + g2[i] : g2[i];
+        for (int i = 0; i < 4; ++i) {
+            const bool has = 4 * g + i < tokens;
+            g2[i] = has ? log2_decay(dt_traits<DT>::to_f32(raw[0][i])) : 0.f;
+            r[i] = has ? dt_traits<DT>::to_f32(raw[1][i]) : 0.f;
+            a[i] = has ? dt_traits<DT>::to_f32(raw[2][i]) : 0.f;
+            b[i] = has ? dt_traits<DT>::to_f32(raw[3][i]) : 0.f;
+            k[i] = has ? dt_traits<DT>::to_f32(raw[4][i]) : 0.f;
+            l[i] = i ? l[i - 1] + g2[i] : g2[i];
+        }
     }
     const float off = groups_before(l[3], g);
 #pragma unroll
     for (int i = 0; i < 4; ++i) l[i] += off;
     const float end = __shfl(l[3], 48 + m);
     const bool strong = __any(!(end >= kStrong));
+    if (m >= tokens) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) dy[q] = v[q] = zero;
+    }
+    f32x4_t gr = zero, ga = zero, gb = zero, gk = zero;
+    float through = 0.f;  // sum over the values of S dS' of this key
+    {
+        const Operand<HALF, 64> dy_o(dy), v_o(v), dz_o(dz), sa_o(sa);
+        // the wave's pair matrix
+        f32x4_t pm = zero;
+        if (wave == 0) pm = mma(sa_o, dz_o, pm);
+        if (wave == 1) pm = mma<V_EXACT, false>(v_o, dz_o, pm);
+        if (wave == 2) pm = mma<false, DY_EXACT>(sa_o, dy_o, pm);
+        if (wave == 3) pm = mma<V_EXACT, DY_EXACT>(v_o, dy_o, pm);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = 4 * g + i;
+            lds.m[wave][t][m] = pack_pair<HALF>(t < m ? pm[i] : 0.f);
+            if (wave >= 2 && t == m) lds.own[wave - 2][m] = pm[i];
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) through = fmaf(s[q][i], d[q][i], through);
+        const Operand<HALF, 64> s_o(s), d_o(d);
+        gr = mma<DY_EXACT, false>(dy_o, s_o, gr);
+        ga = mma(dz_o, s_o, ga);
+        gb = mma(sa_o, d_o, gb);
+        gk = mma<V_EXACT, false>(v_o, d_o, gk);
+    }
+    through = over_groups(through);
     if (strong) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -796,15 +919,14 @@ __global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
         }
     }
     __syncthreads();
-    float to_end[4], el[4], ex[4];  // e^(Lend - L), e^L, e^Lx
+    f32x4_t to_end, el, ex;  // e^(Lend - L), e^L, e^Lx
     {
         float after = groups_after((g2[0] + g2[1]) + (g2[2] + g2[3]), g);
         float prev = off;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             el[i] = exp2_hw(l[i]);
-            ex[i] = exp2_hw(prev);
-            prev = l[i];
+            ex[i] = i ? el[i - 1] : exp2_hw(prev);
         }
 #pragma unroll
         for (int i = 3; i >= 0; --i) {
@@ -826,7 +948,7 @@ __global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
     float cross[4];
     if (strong) {
         float pr[4], pa[4], pb[4], pk[4], pc[4];
-        strong_grads(lds, wave, lane, pr, pa, pb, pk, pc);
+        strong_grads<HALF>(lds, wave, lane, pr, pa, pb, pk, pc);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             gr[i] += pr[i];
@@ -836,31 +958,29 @@ __global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
             cross[i] = pc[i];
         }
     } else {
-        f32x4_t rs, as, bs, ks, pr = zero, pa = zero, pb = zero, pk = zero;
-        float il[4];
+        f32x4_t late[2], early[2], il, pr = zero, pa = zero, pb = zero, pk = zero;  // A~, R~ and B~, K~
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             il[i] = exp2_hw(-l[i]);
-            rs[i] = r[i] * el[i];
-            as[i] = a[i] * ex[i];
-            bs[i] = b[i] * il[i];
-            ks[i] = k[i] * il[i];
+            late[0][i] = a[i] * ex[i];
+            late[1][i] = r[i] * el[i];
+            early[0][i] = b[i] * il[i];
+            early[1][i] = k[i] * il[i];
         }
-        f32x4_t by_t[4], by_s[4];
+        const Operand<HALF, 32> late_o(late), early_o(early);
+        uint32_t by_t[4][4], by_s[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            by_s[j] = *(const f32x4_t*)&lds.m[j][m][4 * g];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) by_t[j][i] = lds.m[j][4 * g + i][m];
+            for (int i = 0; i < 4; ++i) {
+                by_s[j][i] = lds.m[j][m][4 * g + i];
+                by_t[j][i] = lds.m[j][4 * g + i][m];
+            }
         }
-        pa = mma16(by_t[0], bs, pa);
-        pa = mma16(by_t[1], ks, pa);
-        pr = mma16(by_t[2], bs, pr);
-        pr = mma16(by_t[3], ks, pr);
-        pb = mma16(by_s[0], as, pb);
-        pb = mma16(by_s[2], rs, pb);
-        pk = mma16(by_s[1], as, pk);
-        pk = mma16(by_s[3], rs, pk);
+        pa = mma(pair_operand<HALF>(by_t[0], by_t[1]), early_o, pa);
+        pr = mma(pair_operand<HALF>(by_t[2], by_t[3]), early_o, pr);
+        pb = mma(pair_operand<HALF>(by_s[0], by_s[2]), late_o, pb);
+        pk = mma(pair_operand<HALF>(by_s[1], by_s[3]), late_o, pk);
         // a pair (s, t) passes the decays behind s up to t (before t, for a): sums of what ends
         // minus what begins at each token and behind it
         float q[4], qa[4];
@@ -910,15 +1030,15 @@ __global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
         // d log d / dw = -exp(w), inf where the decay, and with it what passes it, is 0
         gw[i] = gw[i] == 0.f ? 0.f : gw[i] * (g2[i] * kLn2);
     }
+    const auto to_chunk = [&](void* q) { return (uint8_t*)q + first * SIZE; };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if (!has[i]) continue;
-        const int64_t at = ((span.start + t0 + 4 * g + i) * H + head) * kHead + key;
-        if (p.dr) store_dt(p.dr, DT, at, gr[i]);
-        if (p.dw) store_dt(p.dw, DT, at, gw[i]);
-        if (p.dk) store_dt(p.dk, DT, at, gk[i]);
-        if (p.da) store_dt(p.da, DT, at, ga[i]);
-        if (p.db) store_dt(p.db, DT, at, gb[i]);
+        if (4 * g + i >= tokens) continue;
+        if (p.dr) store1<DT>(to_chunk(p.dr), at[i], gr[i]);
+        if (p.dw) store1<DT>(to_chunk(p.dw), at[i], gw[i]);
+        if (p.dk) store1<DT>(to_chunk(p.dk), at[i], gk[i]);
+        if (p.da) store1<DT>(to_chunk(p.da), at[i], ga[i]);
+        if (p.db) store1<DT>(to_chunk(p.db), at[i], gb[i]);
     }
 }
 
