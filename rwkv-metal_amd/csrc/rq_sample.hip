@@ -194,21 +194,26 @@ struct Row {
 #pragma unroll
             for (int x = 0; x < 4; ++x) to.v[j].w[x] = w[4 * j + x];
     }
-    // f(step, eight logits) in the order of the index, while it gives true; three steps in flight
+    // f(step, eight logits) in the order of the index, while it gives true; three steps in flight, in registers by
+    // turns (a copy of what is on its way waits for it)
     template <class F>
     RQ_DEV void each(F f) const {
         if (steps == 0) return;
-        Raw8<DT> now, next, third;
-        fetch(0, now);
-        if (steps > 1) fetch(1, next);
-        for (int s = 0; s < steps; ++s) {
-            if (s + 2 < steps) fetch(s + 2, third);
-            float l[kLane];
+        constexpr int kTurns = 4;
+        Raw8<DT> held[kTurns];
 #pragma unroll
-            for (int j = 0; j < kLane / kVec<DT>; ++j) unpack_vec<DT>(now.v[j], l + j * kVec<DT>);
-            if (!f(s, l)) return;
-            now = next;
-            next = third;
+        for (int o = 0; o + 1 < kTurns; ++o) fetch(o < steps ? o : 0, held[o]);
+        for (int s0 = 0; s0 < steps; s0 += kTurns) {
+#pragma unroll
+            for (int o = 0; o < kTurns; ++o) {
+                const int s = s0 + o, ahead = s + kTurns - 1;
+                if (s >= steps) return;
+                fetch(ahead < steps ? ahead : 0, held[(o + kTurns - 1) % kTurns]);
+                float l[kLane];
+#pragma unroll
+                for (int j = 0; j < kLane / kVec<DT>; ++j) unpack_vec<DT>(held[o].v[j], l + j * kVec<DT>);
+                if (!f(s, l)) return;
+            }
         }
     }
 };

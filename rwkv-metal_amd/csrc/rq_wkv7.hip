@@ -100,11 +100,15 @@ struct Span {
     RQ_DEV int64_t chunks() const { return (len + kChunk - 1) / kChunk; }
 };
 
-RQ_DEV int64_t clamp_token(int32_t v, int64_t time) { return v < 0 ? 0 : (v > time ? time : v); }
+// A boundary, the same in all lanes: addresses that follow from it are scalar.
+RQ_DEV int64_t boundary(const WkvShape& s, int64_t n) {
+    const int32_t v = __builtin_amdgcn_readfirstlane(s.cu[n]);
+    return v < 0 ? 0 : (v > s.time ? s.time : v);
+}
 
 RQ_DEV Span span_of(const WkvShape& s, int64_t n) {
     if (!s.cu) return {n * s.time, s.time, n * ((s.time + kChunk - 1) / kChunk)};
-    const int64_t from = clamp_token(s.cu[n], s.time), to = clamp_token(s.cu[n + 1], s.time);
+    const int64_t from = boundary(s, n), to = boundary(s, n + 1);
     return {from, to > from ? to - from : 0, from / kChunk + n};
 }
 
@@ -392,11 +396,11 @@ RQ_DEV Segment segment_of(const WkvShape& s, const WkvSegments& g, int64_t slot,
         int64_t lo = 0, hi = s.seqs;
         while (hi - lo > 1) {
             const int64_t mid = (lo + hi) / 2;
-            if (clamp_token(s.cu[mid], s.time) / tokens + mid <= slot) lo = mid;
+            if (boundary(s, mid) / tokens + mid <= slot) lo = mid;
             else hi = mid;
         }
         seq = lo;
-        index = slot - (clamp_token(s.cu[lo], s.time) / tokens + lo);
+        index = slot - (boundary(s, lo) / tokens + lo);
     } else if (g.chunks) {
         const int64_t per = ((s.time + kChunk - 1) / kChunk + g.chunks - 1) / g.chunks;
         seq = slot / per;
@@ -472,8 +476,9 @@ __global__ __launch_bounds__(kScanThreads<ENDS>) void wkv7_scan_kernel(WkvScan p
         const auto matrix = [&](int64_t c, int ring) {
             if (c >= end) return;
             const int* f = lds.strong[ring];
-            form_matrix<DT, REV>(p.in, lds.arrays[ring], lds.inverse[odd(c)], f[0] | f[1] | f[2] | f[3], lds.matrices[odd(c)],
-                                 lane, wave - 4, row(c), exists(c));
+            const bool strong = __builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]);
+            form_matrix<DT, REV>(p.in, lds.arrays[ring], lds.inverse[odd(c)], strong, lds.matrices[odd(c)], lane, wave - 4,
+                                 row(c), exists(c));
         };
         __syncthreads();
         matrix(first, 0);
@@ -580,42 +585,56 @@ __global__ __launch_bounds__(kScanThreads<ENDS>) void wkv7_scan_kernel(WkvScan p
     }
 }
 
-// The states at the segments' beginnings, S' = S M + N from one to the next: a block is a head of a sequence,
-// its waves the 16 tiles of 16 values and 16 keys, and the state goes round through LDS.
-__global__ __launch_bounds__(1024) void wkv7_join_kernel(WkvShape shape, WkvSegments seg, const float* state) {
-    __shared__ Rows lds[2][4];  // [value / 16][value % 16][key]
-    const int lane = threadIdx.x & 63, wave = wave_index();
-    const int g = lane >> 4, m = lane & 15, q = wave & 3, tile = wave >> 2;
-    const int64_t H = shape.heads, seq = blockIdx.x / H, head = blockIdx.x % H;
+// The states at the segments' beginnings, S' = S M + N from one to the next: a block is 16 values of a head of
+// a sequence, its four waves 16 keys each.  A step's 64 x 64 x 64 product is 0.9 us of one CU's fp32 MFMAs, and a step
+// of all values in one block took 1.75 us; the values do not need each other.
+__global__ __launch_bounds__(256) void wkv7_join_kernel(WkvShape shape, WkvSegments seg, const float* state) {
+    __shared__ Rows states[2];              // [value][key]
+    __shared__ float maps[2][kHead][kRow];  // [from key][to key]
+    const int lane = threadIdx.x & 63, q = wave_index();
+    const int g = lane >> 4, m = lane & 15;
+    const int64_t H = shape.heads, which = blockIdx.x / 4, seq = which / H, head = which % H;
     const Span span = span_of(shape, seq);
     const int64_t count = (span.chunks() + seg.chunks - 1) / seg.chunks;
     if (count < 2) return;
     const int64_t slot0 = shape.cu ? span.start / (seg.chunks * kChunk) + seq
                                    : seq * (((shape.time + kChunk - 1) / kChunk + seg.chunks - 1) / seg.chunks);
-    const int value = 16 * tile + m;
+    const int value = 16 * (blockIdx.x & 3) + m, row = threadIdx.x >> 4, column = 4 * (threadIdx.x & 15);
     f32x4_t s = {0.f, 0.f, 0.f, 0.f};
     if (state) s = *(const f32x4_t*)(state + ((seq * H + head) * kHead + value) * kHead + 16 * q + 4 * g);
-    float map[16];  // M[key 16j + 4g + i][key 16q + m]
-    f32x4_t add;    // N[value][key 16q + 4g + i]
-    const auto load = [&](int64_t j) {
-        const float* from = seg.ends + ((slot0 + j) * H + head) * 2 * kHead * kHead;
-        add = *(const f32x4_t*)(from + value * kHead + 16 * q + 4 * g);
+    // of the next steps: the thread's share of M, N[value][key 16q + 4g + i].  Registers by turns, not handed on:
+    // a copy of what is on its way waits for it.
+    constexpr int kTurns = 4;
+    f32x4_t map[kTurns][4], add[kTurns];
+    const auto load = [&](int at, int64_t j) {
+        const float* from = seg.ends + ((slot0 + (j < count - 1 ? j : count - 2)) * H + head) * 2 * kHead * kHead;
 #pragma unroll
-        for (int x = 0; x < 16; ++x) map[x] = from[(kHead + 16 * (x >> 2) + 4 * g + (x & 3)) * kHead + 16 * q + m];
+        for (int x = 0; x < 4; ++x) map[at][x] = *(const f32x4_t*)(from + (kHead + 16 * x + row) * kHead + column);
+        add[at] = *(const f32x4_t*)(from + value * kHead + 16 * q + 4 * g);
     };
-    load(0);
-    for (int64_t j = 0; j + 1 < count; ++j) {
-        *(f32x4_t*)&lds[j & 1][tile][m][16 * q + 4 * g] = s;
-        __syncthreads();
-        f32x4_t sum[2] = {add, {0.f, 0.f, 0.f, 0.f}}, a[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) a[x] = f32x4_t{map[4 * x], map[4 * x + 1], map[4 * x + 2], map[4 * x + 3]};
-        if (j + 2 < count) load(j + 1);
+    for (int j = 0; j + 1 < kTurns; ++j) load(j, j);
+    for (int64_t j0 = 0; j0 + 1 < count; j0 += kTurns) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-            sum[x & 1] = mma16(a[x], *(const f32x4_t*)&lds[j & 1][tile][m][16 * x + 4 * g], sum[x & 1]);
-        s = sum[0] + sum[1];
-        *(f32x4_t*)(seg.begins + (((slot0 + j + 1) * H + head) * kHead + value) * kHead + 16 * q + 4 * g) = s;
+        for (int o = 0; o < kTurns; ++o) {
+            const int64_t j = j0 + o;
+            if (j + 1 >= count) return;
+            load((o + kTurns - 1) % kTurns, j + kTurns - 1);
+            *(f32x4_t*)&states[o & 1][m][16 * q + 4 * g] = s;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) *(f32x4_t*)&maps[o & 1][16 * x + row][column] = map[o][x];
+            __syncthreads();
+            f32x4_t sum[2] = {add[o], {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                f32x4_t a;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = maps[o & 1][16 * x + 4 * g + i][16 * q + m];
+                sum[x & 1] = mma16(a, *(const f32x4_t*)&states[o & 1][m][16 * x + 4 * g], sum[x & 1]);
+            }
+            s = sum[0] + sum[1];
+            *(f32x4_t*)(seg.begins + (((slot0 + j + 1) * H + head) * kHead + value) * kHead + 16 * q + 4 * g) = s;
+        }
     }
 }
 
@@ -803,7 +822,7 @@ __global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
         int64_t lo = 0, hi = p.shape.seqs;
         while (hi - lo > 1) {
             const int64_t mid = (lo + hi) / 2;
-            if (clamp_token(p.shape.cu[mid], p.shape.time) / kChunk + mid <= chunk) lo = mid;
+            if (boundary(p.shape, mid) / kChunk + mid <= chunk) lo = mid;
             else hi = mid;
         }
         span = span_of(p.shape, lo);
@@ -835,15 +854,15 @@ __global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
     const int key = 16 * wave + m;
     // columns of keys: S and dS' of values 16q + 4g + i
     f32x4_t s[4], d[4];
+    const uint32_t column = (4 * g * kHead + key) * 4;
     const uint8_t* const s_at = (const uint8_t*)(p.states + (int64_t)blockIdx.x * kHead * kHead);
     const uint8_t* const d_at = (const uint8_t*)(p.dstates + (int64_t)blockIdx.x * kHead * kHead);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t at = ((16 * q + 4 * g + i) * kHead + key) * 4;
-            s[q][i] = *(const float*)(s_at + at);
-            d[q][i] = *(const float*)(d_at + at);
+            s[q][i] = *(const float*)(s_at + 16 * q * kHead * 4 + (column + i * kHead * 4));
+            d[q][i] = *(const float*)(d_at + 16 * q * kHead * 4 + (column + i * kHead * 4));
         }
     }
     // this wave's tensors: tokens 4g + i of its key
@@ -1103,7 +1122,7 @@ struct RestTensors {
 // One block a token outside [cu[0], cu[seqs]), in grid-sized strides.
 template <int SIZE>
 __global__ __launch_bounds__(256) void wkv7_rest_kernel(WkvShape s, RestTensors to) {
-    const int64_t first = clamp_token(s.cu[0], s.time), last = clamp_token(s.cu[s.seqs], s.time);
+    const int64_t first = boundary(s, 0), last = boundary(s, s.seqs);
     const int64_t behind = last > first ? last : first;
     const int64_t rows = first + (s.time - behind), vecs = s.heads * kHead * SIZE / 16;
     for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
@@ -1123,7 +1142,7 @@ hipError_t scan_all(const WkvScan& a, hipStream_t s) {
     if (a.seg.chunks) {
         const dim3 grid((unsigned)(a.seg.slots * heads));
         wkv7_scan_kernel<DT, XDT, YDT, REV, true><<<grid, kScanThreads<true>, 0, s>>>(a);
-        wkv7_join_kernel<<<dim3((unsigned)(a.shape.seqs * heads)), 1024, 0, s>>>(a.shape, a.seg, a.state);
+        wkv7_join_kernel<<<dim3((unsigned)(4 * a.shape.seqs * heads)), 256, 0, s>>>(a.shape, a.seg, a.state);
         wkv7_scan_kernel<DT, XDT, YDT, REV, false><<<grid, kScanThreads<false>, 0, s>>>(a);
     } else {
         wkv7_scan_kernel<DT, XDT, YDT, REV, false>
