@@ -30,6 +30,27 @@ CHUNK = 16       # tokens between two states that are kept for the backward pass
 
 # -------------------------------------------------------------- recurrence
 
+_device_of, _address_of, _contiguous_one = Tensor.get_device, Tensor.data_ptr, Tensor.is_contiguous
+
+
+def _operands(ts: list) -> Tuple[list, list]:
+    """The tensors as the C entry points take them (on one GPU, contiguous, 16-byte aligned) and their
+    addresses.  Column by column: a decode step's launch is shorter than a loop of Python over its operands."""
+    devices = set(map(_device_of, ts))
+    if len(devices) != 1 or -1 in devices:
+        _on_gpu(*ts)
+    if not all(map(_contiguous_one, ts)):
+        ts = [t.contiguous() for t in ts]
+    at = list(map(_address_of, ts))
+    low = 0
+    for x in at:
+        low |= x
+    if low & 15:
+        ts = list(map(_ready, ts))
+        at = list(map(_ptr, ts))
+    return ts, at
+
+
 def _sizes(r: Tensor, cu: Optional[Tensor]) -> Tuple[int, int, int, int]:
     batch, time, heads = r.shape[:3]
     return batch, time, heads, batch if cu is None else cu.numel() - 1
@@ -42,9 +63,10 @@ def _chunks(batch: int, time: int, seqs: int, packed: bool) -> int:
 def _wkv7_impl(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state: Optional[Tensor],
                cu: Optional[Tensor], out_dtype: torch.dtype, keep: bool):
     """(y, last state, and where they are kept the states and S a that the backward pass reads)."""
-    _on_gpu(r, w, k, v, a, b, *[t for t in (state, cu) if t is not None])
-    r, w, k, v, a, b = map(_ready, (r, w, k, v, a, b))
-    state = None if state is None else _ready(state)
+    held, at = _operands([r, w, k, v, a, b] if state is None else [r, w, k, v, a, b, state])
+    r = held[0]
+    if cu is not None:
+        _on_gpu(r, cu)
     batch, time, heads, seqs = _sizes(r, cu)
     f32 = {"dtype": torch.float32, "device": r.device}
     y = torch.empty(r.shape, dtype=out_dtype, device=r.device)
@@ -58,14 +80,14 @@ def _wkv7_impl(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor,
     with _DeviceGuard(r.device):
         stream = _stream_on(r.device)
         if time == 1 and cu is None and not keep:
-            rc = L.rq_wkv7_step(_ptr(r), _ptr(w), _ptr(k), _ptr(v), _ptr(a), _ptr(b), dt, batch, heads,
-                                _addr(state), _ptr(y), odt, _ptr(last), stream)
+            rc = L.rq_wkv7_step(*at[:6], dt, batch, heads, at[6] if len(at) > 6 else 0, y.data_ptr(), odt,
+                                last.data_ptr(), stream)
         else:
             ws = _queried_workspace("rq_wkv7_workspace_bytes", (batch, time, heads, seqs, cu is not None), r.device,
                                     "wkv7")
-            rc = L.rq_wkv7(_ptr(r), _ptr(w), _ptr(k), _ptr(v), _ptr(a), _ptr(b), dt, batch, time, heads,
-                           0 if cu is None else cu.data_ptr(), seqs, _addr(state), _ptr(y), odt, _ptr(last),
-                           _addr(states), _addr(sa), _addr(ws), _size(ws), stream)
+            rc = L.rq_wkv7(*at[:6], dt, batch, time, heads, 0 if cu is None else cu.data_ptr(), seqs,
+                           at[6] if len(at) > 6 else 0, y.data_ptr(), odt, last.data_ptr(), _addr(states), _addr(sa),
+                           _addr(ws), _size(ws), stream)
     if rc:
         check(rc, "wkv7")
     return y, last, states, sa
@@ -73,9 +95,11 @@ def _wkv7_impl(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor,
 
 def _wkv7_backward_impl(r, w, k, v, a, b, cu, states, sa, dy, dlast, want_state: bool):
     """The gradients of the six and, where it is wanted, of the first state."""
-    _on_gpu(r, w, k, v, a, b, states, sa, dy, *[t for t in (dlast, cu) if t is not None])
-    r, w, k, v, a, b, dy = map(_ready, (r, w, k, v, a, b, dy))
-    dlast = None if dlast is None else _ready(dlast)
+    ts = [r, w, k, v, a, b, states, sa, dy]
+    held, at = _operands(ts if dlast is None else [*ts, dlast])
+    r, dy = held[0], held[8]
+    if cu is not None:
+        _on_gpu(r, cu)
     batch, time, heads, seqs = _sizes(r, cu)
     grads = [torch.empty_like(r) for _ in range(6)]
     dstate = None
@@ -85,10 +109,10 @@ def _wkv7_backward_impl(r, w, k, v, a, b, cu, states, sa, dy, dlast, want_state:
         stream = _stream_on(r.device)
         ws = _queried_workspace("rq_wkv7_backward_workspace_bytes", (batch, time, heads, seqs, cu is not None),
                                 r.device, "wkv7 backward")
-        rc = lib().rq_wkv7_backward(_ptr(r), _ptr(w), _ptr(k), _ptr(v), _ptr(a), _ptr(b), DTYPE_CODE[r.dtype],
-                                    batch, time, heads, 0 if cu is None else cu.data_ptr(), seqs, _ptr(states),
-                                    _ptr(sa), _ptr(dy), DTYPE_CODE[dy.dtype], _addr(dlast),
-                                    *[_ptr(g) for g in grads], _addr(dstate), _addr(ws), _size(ws), stream)
+        rc = lib().rq_wkv7_backward(*at[:6], DTYPE_CODE[r.dtype], batch, time, heads,
+                                    0 if cu is None else cu.data_ptr(), seqs, *at[6:9], DTYPE_CODE[dy.dtype],
+                                    at[9] if len(at) > 9 else 0, *map(_address_of, grads), _addr(dstate), _addr(ws),
+                                    _size(ws), stream)
     if rc:
         check(rc, "wkv7 backward")
     return (*grads, dstate)
@@ -187,20 +211,25 @@ class _Wkv7Function(torch.autograd.Function):
 def _same_dtype(six):
     """The six in one dtype, float32 where they come in several."""
     dt = six[0].dtype
-    if all(t.dtype == dt for t in six):
-        return six, dt
-    return [t.to(torch.float32) for t in six], torch.float32
+    for t in six:
+        if t.dtype is not dt:
+            return [t.to(torch.float32) for t in six], torch.float32
+    return six, dt
 
 
-def _check_inputs(six, dims: int) -> None:
-    for name, t in zip("rwkvab", six):
-        _float(t, name)
-        if t.shape != six[0].shape:
-            raise ValueError(f"r, w, k, v, a and b must have one shape (got {tuple(six[0].shape)} and "
-                             f"{tuple(t.shape)} of {name})")
-    if six[0].dim() != dims or six[0].shape[-1] != HEAD_SIZE:
+def _check_inputs(six, dims: int) -> torch.Size:
+    shape = six[0].shape
+    for t in six:
+        if t.dtype not in DTYPE_CODE or t.shape != shape:
+            for name, t in zip("rwkvab", six):
+                _float(t, name)
+                if t.shape != shape:
+                    raise ValueError(f"r, w, k, v, a and b must have one shape (got {tuple(shape)} and "
+                                     f"{tuple(t.shape)} of {name})")
+    if len(shape) != dims or shape[-1] != HEAD_SIZE:
         lead = "[batch, time, heads, 64]" if dims == 4 else "[batch, heads, 64]"
-        raise ValueError(f"r, w, k, v, a and b must be {lead} (got {tuple(six[0].shape)})")
+        raise ValueError(f"r, w, k, v, a and b must be {lead} (got {tuple(shape)})")
+    return shape
 
 
 def _check_state(state: Tensor, seqs: int, heads: int, name: str = "state") -> None:
@@ -238,10 +267,9 @@ def wkv7(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state
     Differentiable in all six and the first state, from both results (once).  The backward pass
     keeps every 16th state, a sixteenth of 16 KB for each token and head."""
     six = [r, w, k, v, a, b]
-    _check_inputs(six, 4)
+    batch, time, heads, _ = _check_inputs(six, 4)
     six, dt = _same_dtype(six)
     odt = _out_dtype(out_dtype, dt)
-    batch, time, heads = six[0].shape[:3]
     seqs = batch
     if cu_seqlens is not None:
         if cu_seqlens.dtype not in (torch.int32, torch.int64) or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
@@ -265,48 +293,46 @@ def wkv7(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state
 
 # --------------------------------------------------------------- one token
 
-def _step_impl(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state: Tensor, out: Tensor,
-               out_dtype: torch.dtype) -> Tensor:
-    _on_gpu(r, w, k, v, a, b, state, out)
-    r, w, k, v, a, b = map(_ready, (r, w, k, v, a, b))
-    y = torch.empty(r.shape, dtype=out_dtype, device=r.device)
-    with _DeviceGuard(r.device):
-        rc = lib().rq_wkv7_step(_ptr(r), _ptr(w), _ptr(k), _ptr(v), _ptr(a), _ptr(b), DTYPE_CODE[r.dtype],
-                                r.shape[0], r.shape[1], _ptr(state), _ptr(y), DTYPE_CODE[out_dtype], _ptr(out),
-                                _stream_on(r.device))
-    if rc:
-        check(rc, "wkv7_step")
-    return y
-
-
-@torch.no_grad()
 def wkv7_step(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state: Tensor,
               out: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
     """(y, new state) of one token of every sequence: r .. b [batch, heads, 64], state
     [batch, heads, 64, 64].  out: a contiguous float32 tensor for the new state, `state` itself for an
     update in place.  Without gradients (wkv7 over a time of 1 has them)."""
     six = [r, w, k, v, a, b]
-    _check_inputs(six, 3)
+    shape = _check_inputs(six, 3)
     six, dt = _same_dtype(six)
     odt = _out_dtype(out_dtype, dt)
-    _check_state(state, *six[0].shape[:2])
+    batch, heads, _ = shape
+    _check_state(state, batch, heads)
     if out is None:
         out = torch.empty(state.shape, dtype=torch.float32, device=state.device)
-    else:
-        _check_state(out, *six[0].shape[:2], "out")
+    elif out is not state:
+        _check_state(out, batch, heads, "out")
         if not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("out must be contiguous and 16-byte aligned")
-        if out.numel() and out.data_ptr() != state.data_ptr() and _overlap(out, state):
+        if out.data_ptr() != state.data_ptr() and _overlap(out, state):
             raise ValueError("out may be the state itself, but must not overlap it otherwise")
-    return _step_impl(*six, _ready(state), out, odt), out
+    elif not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError("out must be contiguous and 16-byte aligned")
+    held, at = _operands([*six, state, out])
+    device = held[0].device
+    y = torch.empty(shape, dtype=odt, device=device)
+    with _DeviceGuard(device):
+        rc = lib().rq_wkv7_step(*at[:6], DTYPE_CODE[dt], batch, heads, at[6], y.data_ptr(), DTYPE_CODE[odt], at[7],
+                                _stream_on(device))
+    if rc:
+        check(rc, "wkv7_step")
+    return y, out
 
 
 def _overlap(x: Tensor, y: Tensor) -> bool:
-    """Whether the memory that the two span has bytes in common."""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + 4 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-    (x0, x1), (y0, y1) = span(x), span(y)
-    return x0 < y1 and y0 < x1
+    """Whether the memory that the two span has bytes in common (x is contiguous)."""
+    if y.is_contiguous():
+        last = y.numel()
+    else:
+        last = 1 + sum((n - 1) * s for n, s in zip(y.shape, y.stride()))
+    x0, y0 = x.data_ptr(), y.data_ptr()
+    return x.numel() > 0 and x0 < y0 + 4 * last and y0 < x0 + 4 * x.numel()
 
 
 # ------------------------------------------------------------------ sampler
@@ -349,7 +375,6 @@ def _parameter(x, name: str, lead, whole: bool):
     return x.to(torch.int64 if whole else torch.float32), (0 if whole else 1.0)
 
 
-@torch.no_grad()
 def sample(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] = 1.0, top_k: Union[int, Tensor] = 0,
            top_p: Union[float, Tensor] = 1.0, min_p: Union[float, Tensor] = 0.0) -> Tuple[Tensor, Tensor]:
     """(tokens int64, their log-probabilities float32) for logits [..., vocab] and numbers u [...] in
@@ -375,4 +400,5 @@ def sample(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] = 1.0, t
     m, m_all = _parameter(min_p, "min_p", lead, False)
     given = [x for x in (t, k, p, m) if x is not None]
     op = _sample_impl if _eager(logits, u, *given) else _sample_op
-    return op(logits, u, t, k, p, m, t_all, min(k_all, 1 << 62), p_all, m_all)
+    with torch.no_grad():
+        return op(logits, u, t, k, p, m, t_all, min(k_all, 1 << 62), p_all, m_all)
