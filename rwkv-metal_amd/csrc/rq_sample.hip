@@ -311,13 +311,11 @@ RQ_DEV void add_to_bin(Lds& lds, uint32_t key, double x) {
     }
 }
 
-// The same over the whole row, once its bins are found (lds.found ...).  weight(l, key) is what a logit adds, and
+// The same over the whole row, once its bin is found.  weight(l, key) is what a logit adds, and
 // may_weigh(l, key) whether that is more than 0 without working it out.
 template <int DT, class M, class W>
-RQ_DEV uint32_t key_in_row(const Row<DT>& row, Lds& lds, const Bins& bins, double& before, M may_weigh, W weight,
-                           uint32_t extra_key, double extra) {
-    const int bin = lds.found;
-    const double base = lds.found_sum, want = lds.total;
+RQ_DEV uint32_t key_in_row(const Row<DT>& row, Lds& lds, const Bins& bins, int bin, double base, double want, double& before,
+                           M may_weigh, W weight, uint32_t extra_key, double extra) {
     row.each([&](int, const float* l) {
 #pragma unroll
         for (int i = 0; i < kLane; ++i) {
@@ -639,7 +637,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             if (threadIdx.x == 0) lds.total = 0.0;
             find_bin<kBins>(lds, 0.0, (double)top_k, 0.0, 0.0);
             if (lds.total > 0.0) {  // as many logits are there
-                least = key_in_row(row, lds, bins, before, any, [](float, uint32_t) { return 1.0; }, 0, 0.0);
+                least = key_in_row(row, lds, bins, (int)lds.found, lds.found_sum, lds.total, before, any, [](float, uint32_t) { return 1.0; }, 0, 0.0);
                 ties = top_k - (int64_t)before;
                 listed = gather(row, lds, of_key(least));
             } else {
@@ -648,79 +646,91 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
         }
     }
     if (by_sum) {
-        const double tied = ties ? (double)ties * w.quanta(w.at(of_key(least))) : 0.0;
-        double before, want = -1.0;
+        double before, want;
         uint32_t key;
         if (top_k == 0) {
-            // the whole; and as candidates some 60 of 1024 logits, of the largest: what the maxima of 31 of 32
-            // lanes reach
-            double sum = 0.0;
+            // sums by bins over the row, and then what lies in the border's bin and above
+            clear_bins<kBins>(lds);
             row.each([&](int, const float* l) {
                 double x[kLane];
 #pragma unroll
                 for (int i = 0; i < kLane; ++i) x[i] = w.quanta(w.at(l[i]));
-                sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-                return true;
-            });
-            sum = wave_sum64(sum);
-            __syncthreads();
-            if (lane == 0) lds.wave_sum[wave] = sum;
-            const int lanes = __syncthreads_count(lane_top != 0);
-            sum = 0.0;
 #pragma unroll
-            for (int i = 0; i < kWaves; ++i) sum += lds.wave_sum[i];
-            want = fmax(fmax((double)top_p, 0.0) * sum, quantum);
-            listed = gather(row, lds, bound_of_maxima(lds, lane_top ? of_key(lane_top) : -INFINITY, top,
-                                                      (uint32_t)(lanes - lanes / 32)));
-        }
-        clear_bins<kBins>(lds);
-        if (threadIdx.x == 0) lds.total = -1.0;
-        if (threadIdx.x == 0 && ties) unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(least))], tied);
-        if (listed) {
-            for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
-                const uint32_t k = lds.part_key[wave][i];
-                if (k <= least) continue;
-                const double x = w.quanta(w.at(of_key(k)));
-                lds.part_e[wave][i] = x;
-                unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(k))], x);
-            }
-            find_bin<kBins>(lds, 0.0, want, fmax((double)top_p, 0.0), quantum);
-            if (lds.total < 0.0) listed = false;  // what is listed does not reach it
-        }
-        if (listed) {
-            const int bin = lds.found;
-            const double base = lds.found_sum;
-            want = lds.total;
-            for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
-                const uint32_t k = lds.part_key[wave][i];
-                if (k > least && sum_bins.of(of_key(k)) == bin && lds.part_e[wave][i] > 0.0) add_to_bin(lds, k, lds.part_e[wave][i]);
-            }
-            __syncthreads();
-            if (lds.in_bin <= kBin) {
-                key = key_in_bin(lds, base, want, before, least, ties && sum_bins.of(of_key(least)) == bin);
-            } else {
-                listed = false;  // found again from the row
-            }
-            __syncthreads();
-        }
-        const auto may_weigh = [&](float l, uint32_t k) { return k > least && l > -INFINITY; };
-        const auto weight = [&](float l, uint32_t) { return w.quanta(w.at(l)); };
-        if (!listed) {
-            clear_bins<kBins>(lds);
-            if (threadIdx.x == 0 && ties) unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(least))], tied);
-            row.each([&](int, const float* l) {
-#pragma unroll
-                for (int i = 0; i < kLane; ++i) {
-                    const uint32_t k = key_of(l[i]);
-                    if (!may_weigh(l[i], k)) continue;
-                    const double x = weight(l[i], k);
-                    if (x > 0.0) unsafeAtomicAdd(&lds.sums[sum_bins.of(l[i])], x);
-                }
+                for (int i = 0; i < kLane; ++i)
+                    if (x[i] > 0.0) unsafeAtomicAdd(&lds.sums[sum_bins.of(l[i])], x[i]);
                 return true;
             });
             find_bin<kBins>(lds, 0.0, -1.0, fmax((double)top_p, 0.0), quantum);
             want = lds.total;
-            key = key_in_row(row, lds, sum_bins, before, may_weigh, weight, least, tied);
+            const int bin = lds.found;
+            const double base = lds.found_sum;
+            // a little below the bin, whatever the rounding
+            const float bound = top - (float)(bin + 1) / sum_bins.scale * 1.00001f - 1e-6f * fabsf(top);
+            if (bound > -INFINITY) listed = gather(row, lds, bound);
+            if (listed) {
+                for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
+                    const uint32_t k = lds.part_key[wave][i];
+                    if (sum_bins.of(of_key(k)) != bin) continue;
+                    const double x = w.quanta(w.at(of_key(k)));
+                    if (x > 0.0) add_to_bin(lds, k, x);
+                }
+                __syncthreads();
+            }
+            if (listed && lds.in_bin <= kBin) {
+                key = key_in_bin(lds, base, want, before, 0, false);
+            } else {
+                __syncthreads();
+                if (threadIdx.x == 0) lds.in_bin = 0;
+                __syncthreads();
+                key = key_in_row(row, lds, sum_bins, bin, base, want, before, [](float l, uint32_t) { return l > -INFINITY; },
+                                 [&](float l, uint32_t) { return w.quanta(w.at(l)); }, 0, 0.0);
+            }
+        } else {
+            const double tied = (double)ties * w.quanta(w.at(of_key(least)));
+            const bool with_tied = ties > 0;
+            clear_bins<kBins>(lds);
+            if (threadIdx.x == 0 && with_tied) unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(least))], tied);
+            if (listed) {
+                for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
+                    const uint32_t k = lds.part_key[wave][i];
+                    if (k <= least) continue;
+                    const double x = w.quanta(w.at(of_key(k)));
+                    lds.part_e[wave][i] = x;
+                    unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(k))], x);
+                }
+            } else {
+                row.each([&](int, const float* l) {
+#pragma unroll
+                    for (int i = 0; i < kLane; ++i) {
+                        if (!(l[i] > -INFINITY) || key_of(l[i]) <= least) continue;
+                        const double x = w.quanta(w.at(l[i]));
+                        if (x > 0.0) unsafeAtomicAdd(&lds.sums[sum_bins.of(l[i])], x);
+                    }
+                    return true;
+                });
+            }
+            find_bin<kBins>(lds, 0.0, -1.0, fmax((double)top_p, 0.0), quantum);
+            want = lds.total;
+            const int bin = lds.found;
+            const double base = lds.found_sum;
+            const bool tied_in_bin = with_tied && sum_bins.of(of_key(least)) == bin;
+            if (listed) {
+                for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
+                    const uint32_t k = lds.part_key[wave][i];
+                    if (k > least && sum_bins.of(of_key(k)) == bin && lds.part_e[wave][i] > 0.0) add_to_bin(lds, k, lds.part_e[wave][i]);
+                }
+                __syncthreads();
+            }
+            if (listed && lds.in_bin <= kBin) {
+                key = key_in_bin(lds, base, want, before, least, tied_in_bin);
+            } else {
+                __syncthreads();
+                if (threadIdx.x == 0) lds.in_bin = 0;
+                __syncthreads();
+                key = key_in_row(row, lds, sum_bins, bin, base, want, before,
+                                 [&](float l, uint32_t k) { return k > least && l > -INFINITY; },
+                                 [&](float l, uint32_t) { return w.quanta(w.at(l)); }, least, with_tied ? tied : 0.0);
+            }
         }
         // as many of that class as are needed to reach it
         const double each = w.quanta(w.at(of_key(key)));
@@ -785,6 +795,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
     }
 
     // from the row: each wave's part, then the one in which the token lies, by all waves
+    const float border = least ? of_key(least) : -INFINITY;
     const bool everything = top_k == 0 && !by_sum && !(min_p > 0.f) && !w.inf;
     double sum = 0.0;
     uint32_t equal = 0;
@@ -796,17 +807,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
             return true;
         }
-        bool some = false;
+        const float most = fmaxf(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), fmaxf(fmaxf(l[4], l[5]), fmaxf(l[6], l[7])));
+        if (!__any(most >= border)) return true;
+        double x[kLane];
 #pragma unroll
         for (int i = 0; i < kLane; ++i) {
-            const uint32_t key = key_of(l[i]);
-            some |= key > least && l[i] > -INFINITY;
-            equal += ties && key == least;
+            const double e = w.at(l[i]);
+            x[i] = l[i] > border && e >= (double)min_p ? w.quanta(e) : 0.0;
+            equal += ties && l[i] == border;
         }
-        if (__any(some)) {
-#pragma unroll
-            for (int i = 0; i < kLane; ++i) sum += above(l[i], key_of(l[i]));
-        }
+        sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         return true;
     });
     sum = wave_sum64(sum);
