@@ -49,15 +49,15 @@ constexpr int kTable = 32;  // powers 2^(j / 32): each in banks of its own
 // e^((l - top) / temperature) in float64: x = 32 log2 of it is split into a whole number and f, |f| <= 1/2; with
 // t = f ln 2 / 32, |t| <= 0.0109, four terms of the series of e^t leave t^5 / 120 = 1.3e-12, less than a quantum's share.
 struct Weights {
-    double top, scale;    // the largest logit, 32 log2(e) / temperature
+    double top, scale;    // the largest logit, 32 log2(e) / temperature; beside +inf a number past all others, 1
     double grid;          // 1.5 * 2^52 quanta: a sum with it is rounded to whole quanta
     const double* table;
     bool inf;             // the largest logit is +inf
-    RQ_DEV double exact(float l) const {
+    RQ_DEV double at(float l) const {
         constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52
         constexpr double k = 0.6931471805599453 / kTable;
         // past 2^-40 everything is rounded to 0
-        const double x = fmax(((double)l - top) * scale, -40.0 * kTable);
+        const double x = fmin(fmax(((double)l - top) * scale, -40.0 * kTable), 0.0);
         const double r = x + kWhole;
         const int n = (int)(uint32_t)__double_as_longlong(r);
         const double f = x - (r - kWhole);
@@ -70,8 +70,16 @@ struct Weights {
         power += (long long)(n >> 5) << 52;
         return s * __longlong_as_double(power);
     }
-    RQ_DEV double at(float l) const { return inf ? (l == INFINITY ? 1.0 : 0.0) : exact(l); }
     RQ_DEV double quanta(double e) const { return (e + grid) - grid; }
+};
+
+// Whole units, for sums in LDS: integer atomics run at twice the rate of float64 ones.
+struct Units {
+    double grid, unit;  // 1.5 * 2^52 units, and one
+    RQ_DEV unsigned long long of(double x) const {  // x <= 1
+        return (unsigned long long)(__double_as_longlong(x + grid) - __double_as_longlong(grid));
+    }
+    RQ_DEV unsigned long long of_sum(double x) const { return (unsigned long long)(x / unit); }
 };
 
 constexpr int kBins = 2048;  // for sums below the largest logit
@@ -81,7 +89,7 @@ constexpr int kPart = 384;   // logits of a wave's part of the row that are kept
 
 struct Lds {
     double table[kTable];
-    double sums[kBins];  // of the bins; of 256 of them by bits
+    unsigned long long sums[kBins];  // of the bins, in quanta; of 256 of them by bits
     double bin_sums[kBin];
     uint32_t bin_keys[kBin];
     uint32_t in_bin;
@@ -231,21 +239,21 @@ struct Bins {
 template <int BINS>
 RQ_DEV void clear_bins(Lds& lds) {
     __syncthreads();
-    for (int i = threadIdx.x; i < BINS; i += kThreads) lds.sums[i] = 0.0;
+    for (int i = threadIdx.x; i < BINS; i += kThreads) lds.sums[i] = 0;
     if (threadIdx.x == 0) lds.in_bin = 0;
     __syncthreads();
 }
 
 // The bin, from the first, in which the running total reaches `want` (less than 0: `share` of the
-// whole, at least `quantum`); lds.found, the total before it lds.found_sum, what was looked for lds.total.
+// whole, at least a unit); lds.found, the total before it lds.found_sum, what was looked for lds.total.
 template <int BINS>
-RQ_DEV void find_bin(Lds& lds, double before, double want, double share, double quantum) {
+RQ_DEV void find_bin(Lds& lds, const Units& units, double before, double want, double share) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     constexpr int PER = BINS > kThreads ? BINS / kThreads : 1;  // bins a thread
     __syncthreads();
     double own[PER], sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sum += own[i] = (int)threadIdx.x * PER < BINS ? lds.sums[threadIdx.x * PER + i] : 0.0;
+    for (int i = 0; i < PER; ++i) sum += own[i] = (int)threadIdx.x * PER < BINS ? (double)lds.sums[threadIdx.x * PER + i] * units.unit : 0.0;
     const double upto = scan64(sum);
     if (lane == 63) lds.wave_sum[wave] = upto;
     __syncthreads();
@@ -254,7 +262,7 @@ RQ_DEV void find_bin(Lds& lds, double before, double want, double share, double 
     waves += Moved64::of<0x112>(waves);
     waves += Moved64::of<0x114>(waves);
     waves += Moved64::of<0x118>(waves);
-    if (want < 0.0) want = fmax(share * last64(waves), quantum);
+    if (want < 0.0) want = fmax(share * last64(waves), units.unit);
     double at = before + (upto - sum) + (wave ? __shfl(waves, wave - 1) : 0.0);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -314,8 +322,8 @@ RQ_DEV void add_to_bin(Lds& lds, uint32_t key, double x) {
 // The same over the whole row, once its bin is found.  weight(l, key) is what a logit adds, and
 // may_weigh(l, key) whether that is more than 0 without working it out.
 template <int DT, class M, class W>
-RQ_DEV uint32_t key_in_row(const Row<DT>& row, Lds& lds, const Bins& bins, int bin, double base, double want, double& before,
-                           M may_weigh, W weight, uint32_t extra_key, double extra) {
+RQ_DEV uint32_t key_in_row(const Row<DT>& row, Lds& lds, const Bins& bins, const Units& units, int bin, double base, double want,
+                           double& before, M may_weigh, W weight, uint32_t extra_key, double extra) {
     row.each([&](int, const float* l) {
 #pragma unroll
         for (int i = 0; i < kLane; ++i) {
@@ -340,13 +348,13 @@ RQ_DEV uint32_t key_in_row(const Row<DT>& row, Lds& lds, const Bins& bins, int b
                 const uint32_t key = key_of(l[i]);
                 if ((key & mask) != prefix || !may_weigh(l[i], key) || bins.of(l[i]) != bin) continue;
                 const double x = weight(l[i], key);
-                if (x > 0.0) unsafeAtomicAdd(&lds.sums[255 - ((key >> shift) & 255)], x);
+                if (x > 0.0) atomicAdd(&lds.sums[255 - ((key >> shift) & 255)], units.of(x));
             }
             return true;
         });
         if (threadIdx.x == 0 && with_extra && (extra_key & mask) == prefix)
-            unsafeAtomicAdd(&lds.sums[255 - ((extra_key >> shift) & 255)], extra);
-        find_bin<256>(lds, before, want, 0.0, 0.0);
+            atomicAdd(&lds.sums[255 - ((extra_key >> shift) & 255)], units.of_sum(extra));
+        find_bin<256>(lds, units, before, want, 0.0);
         before = lds.found_sum;
         prefix |= (255u - lds.found) << shift;
         mask |= 0xffu << shift;
@@ -559,9 +567,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
         return;
     }
     const int bits = n <= (1 << 17) ? 36 : 33;
-    const Weights w{(double)top, kTable * 1.4426950408889634 / (double)temperature,
-                    6755399441055744.0 / (double)(1ll << bits), lds.table, top == INFINITY};
+    const bool inf = top == INFINITY;
+    const Weights w{inf ? 6.8e38 : (double)top, inf ? 1.0 : kTable * 1.4426950408889634 / (double)temperature,
+                    6755399441055744.0 / (double)(1ll << bits), lds.table, inf};
     const double quantum = 1.0 / (double)(1ll << bits);
+    const Units units{w.grid, quantum};
     if (top_k < 0 || top_k >= n) top_k = 0;
     const bool by_sum = top_p < 1.f;
     // past 26 temperatures below the largest, e_i is rounded to 0
@@ -631,13 +641,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             row.each([&](int, const float* l) {
 #pragma unroll
                 for (int i = 0; i < kLane; ++i)
-                    if (l[i] > -INFINITY) unsafeAtomicAdd(&lds.sums[bins.of(l[i])], 1.0);
+                    if (l[i] > -INFINITY) atomicAdd(&lds.sums[bins.of(l[i])], 1ull);
                 return true;
             });
             if (threadIdx.x == 0) lds.total = 0.0;
-            find_bin<kBins>(lds, 0.0, (double)top_k, 0.0, 0.0);
+            const Units ones{6755399441055744.0, 1.0};
+            find_bin<kBins>(lds, ones, 0.0, (double)top_k, 0.0);
             if (lds.total > 0.0) {  // as many logits are there
-                least = key_in_row(row, lds, bins, (int)lds.found, lds.found_sum, lds.total, before, any, [](float, uint32_t) { return 1.0; }, 0, 0.0);
+                least = key_in_row(row, lds, bins, ones, (int)lds.found, lds.found_sum, lds.total, before, any, [](float, uint32_t) { return 1.0; }, 0, 0.0);
                 ties = top_k - (int64_t)before;
                 listed = gather(row, lds, of_key(least));
             } else {
@@ -652,15 +663,15 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             // sums by bins over the row, and then what lies in the border's bin and above
             clear_bins<kBins>(lds);
             row.each([&](int, const float* l) {
-                double x[kLane];
+                unsigned long long x[kLane];
 #pragma unroll
-                for (int i = 0; i < kLane; ++i) x[i] = w.quanta(w.at(l[i]));
+                for (int i = 0; i < kLane; ++i) x[i] = units.of(w.at(l[i]));
 #pragma unroll
                 for (int i = 0; i < kLane; ++i)
-                    if (x[i] > 0.0) unsafeAtomicAdd(&lds.sums[sum_bins.of(l[i])], x[i]);
+                    if (x[i]) atomicAdd(&lds.sums[sum_bins.of(l[i])], x[i]);
                 return true;
             });
-            find_bin<kBins>(lds, 0.0, -1.0, fmax((double)top_p, 0.0), quantum);
+            find_bin<kBins>(lds, units, 0.0, -1.0, fmax((double)top_p, 0.0));
             want = lds.total;
             const int bin = lds.found;
             const double base = lds.found_sum;
@@ -682,21 +693,21 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
                 __syncthreads();
                 if (threadIdx.x == 0) lds.in_bin = 0;
                 __syncthreads();
-                key = key_in_row(row, lds, sum_bins, bin, base, want, before, [](float l, uint32_t) { return l > -INFINITY; },
+                key = key_in_row(row, lds, sum_bins, units, bin, base, want, before, [](float l, uint32_t) { return l > -INFINITY; },
                                  [&](float l, uint32_t) { return w.quanta(w.at(l)); }, 0, 0.0);
             }
         } else {
             const double tied = (double)ties * w.quanta(w.at(of_key(least)));
             const bool with_tied = ties > 0;
             clear_bins<kBins>(lds);
-            if (threadIdx.x == 0 && with_tied) unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(least))], tied);
+            if (threadIdx.x == 0 && with_tied) atomicAdd(&lds.sums[sum_bins.of(of_key(least))], units.of_sum(tied));
             if (listed) {
                 for (uint32_t i = lane; i < lds.part_n[wave]; i += 64) {
                     const uint32_t k = lds.part_key[wave][i];
                     if (k <= least) continue;
                     const double x = w.quanta(w.at(of_key(k)));
                     lds.part_e[wave][i] = x;
-                    unsafeAtomicAdd(&lds.sums[sum_bins.of(of_key(k))], x);
+                    atomicAdd(&lds.sums[sum_bins.of(of_key(k))], units.of(x));
                 }
             } else {
                 row.each([&](int, const float* l) {
@@ -704,12 +715,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
                     for (int i = 0; i < kLane; ++i) {
                         if (!(l[i] > -INFINITY) || key_of(l[i]) <= least) continue;
                         const double x = w.quanta(w.at(l[i]));
-                        if (x > 0.0) unsafeAtomicAdd(&lds.sums[sum_bins.of(l[i])], x);
+                        if (x > 0.0) atomicAdd(&lds.sums[sum_bins.of(l[i])], units.of(x));
                     }
                     return true;
                 });
             }
-            find_bin<kBins>(lds, 0.0, -1.0, fmax((double)top_p, 0.0), quantum);
+            find_bin<kBins>(lds, units, 0.0, -1.0, fmax((double)top_p, 0.0));
             want = lds.total;
             const int bin = lds.found;
             const double base = lds.found_sum;
@@ -727,7 +738,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
                 __syncthreads();
                 if (threadIdx.x == 0) lds.in_bin = 0;
                 __syncthreads();
-                key = key_in_row(row, lds, sum_bins, bin, base, want, before,
+                key = key_in_row(row, lds, sum_bins, units, bin, base, want, before,
                                  [&](float l, uint32_t k) { return k > least && l > -INFINITY; },
                                  [&](float l, uint32_t) { return w.quanta(w.at(l)); }, least, with_tied ? tied : 0.0);
             }
@@ -796,14 +807,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
 
     // from the row: each wave's part, then the one in which the token lies, by all waves
     const float border = least ? of_key(least) : -INFINITY;
-    const bool everything = top_k == 0 && !by_sum && !(min_p > 0.f) && !w.inf;
+    const bool everything = top_k == 0 && !by_sum && !(min_p > 0.f);
     double sum = 0.0;
     uint32_t equal = 0;
     row.each([&](int, const float* l) {
         if (everything) {  // -inf adds 0
             double x[kLane];
 #pragma unroll
-            for (int i = 0; i < kLane; ++i) x[i] = w.quanta(w.exact(l[i]));
+            for (int i = 0; i < kLane; ++i) x[i] = w.quanta(w.at(l[i]));
             sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
             return true;
         }
@@ -813,8 +824,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
 #pragma unroll
         for (int i = 0; i < kLane; ++i) {
             const double e = w.at(l[i]);
-            x[i] = l[i] > border && e >= (double)min_p ? w.quanta(e) : 0.0;
-            equal += ties && l[i] == border;
+            x[i] = l[i] > border ? w.quanta(e) : 0.0;
+            if (min_p > 0.f) x[i] = e >= (double)min_p ? x[i] : 0.0;
+        }
+        if (ties) {
+#pragma unroll
+            for (int i = 0; i < kLane; ++i) equal += l[i] == border;
         }
         sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         return true;

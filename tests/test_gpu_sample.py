@@ -83,6 +83,21 @@ def test_many_ties(rq, dev, vocab):
         check(rq, logits, u, **kw)
 
 
+def test_more_ties_than_a_bin_of_float_holds(rq, dev):
+    """Sums of 60000 equal terms, as one class and beside larger ones."""
+    n = 100003
+    g = torch.Generator().manual_seed(3)
+    logits = torch.zeros(4, n)
+    logits[1, torch.randperm(n, generator=g)[:500]] = 1.0
+    logits[2] = torch.randint(0, 2, (n,), generator=g).float()
+    logits[3] = torch.randint(0, 3, (n,), generator=g).float() * 0.5
+    logits, u = logits.to(dev), torch.rand(4, generator=g).to(dev)
+    for kw in ({"top_k": 60000, "top_p": 0.9}, {"top_p": 0.7}, {"top_k": 90000}, {"top_k": 60000, "top_p": 0.999, "temperature": 2.0},
+               {"temperature": 50.0, "top_p": 0.3}):
+        for dt in DT.values():
+            check(rq, logits.to(dt), u, **kw)
+
+
 def test_rows_with_parameters_of_their_own(rq, dev):
     g = torch.Generator().manual_seed(4)
     m, vocab = 60, 3001
