@@ -54,9 +54,6 @@ int check_cu(const char* what, const int32_t* cu) {
     return ((uintptr_t)cu & 3u) ? fail(RQ_EALIGN, "%s: cu_seqlens must be 4-byte aligned", what) : RQ_OK;
 }
 
-int64_t state_floats(int64_t chunks, int64_t heads) { return chunks * heads * RQ_WKV7_HEAD * RQ_WKV7_HEAD; }
-int64_t sa_floats(int64_t chunks, int64_t heads) { return chunks * heads * RQ_WKV7_CHUNK * RQ_WKV7_HEAD; }
-
 int check_chunks(const char* what, const rq::WkvShape& s) {
     if (s.heads && rq::wkv_chunks(s) > kMaxHeadsOfChunks / s.heads)
         return fail(RQ_EINVAL, "%s: more than %lld heads of chunks", what, (long long)kMaxHeadsOfChunks);
@@ -67,8 +64,8 @@ int check_chunks(const char* what, const rq::WkvShape& s) {
 const int32_t kPacked = 0;
 
 // The segments of a scan with their workspace, whose bytes are a multiple of 16.
-rq::WkvSegments segments(const rq::WkvShape& shape, void* workspace) {
-    rq::WkvSegments g = rq::wkv_segments(shape);
+rq::WkvSegments segments(const rq::WkvShape& shape, bool backward, void* workspace) {
+    rq::WkvSegments g = rq::wkv_segments(shape, backward);
     g.ends = (float*)workspace;
     g.begins = g.ends ? g.ends + 2 * g.slots * shape.heads * RQ_WKV7_HEAD * RQ_WKV7_HEAD : nullptr;
     return g;
@@ -88,7 +85,7 @@ int64_t rq_wkv7_workspace_bytes(int64_t batch, int64_t time, int64_t heads, int6
     if (int rc = check_shape("rq_wkv7_workspace_bytes", batch, time, heads, has_cu_seqlens, seqs)) return rc;
     ok();
     const rq::WkvShape shape{has_cu_seqlens ? &kPacked : nullptr, batch, time, heads, seqs};
-    return 4 * rq::wkv_segment_floats(rq::wkv_segments(shape), heads);
+    return 4 * rq::wkv_segment_floats(rq::wkv_segments(shape, false), heads);
 }
 
 int rq_wkv7(const void* r, const void* w, const void* k, const void* v, const void* a, const void* b, rq_dtype dt,
@@ -107,7 +104,7 @@ int rq_wkv7(const void* r, const void* w, const void* k, const void* v, const vo
         if (int rc = check_ptrs(what, {r, w, k, v, a, b, y}, {})) return rc;
     if (int rc = check_ptrs(what, {}, {state, state_out, states, sa, workspace})) return rc;
     if (int rc = check_cu(what, cu_seqlens)) return rc;
-    const rq::WkvSegments seg = segments(shape, workspace);
+    const rq::WkvSegments seg = segments(shape, false, workspace);
     const int64_t need = 4 * rq::wkv_segment_floats(seg, heads);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(RQ_EINVAL, "%s: needs a workspace of %lld bytes", what, (long long)need);
@@ -119,7 +116,7 @@ int rq_wkv7(const void* r, const void* w, const void* k, const void* v, const vo
         e = rq::launch_wkv_rest(shape, y_dt, rest, 1, s);
     }
     if (e == hipSuccess && seqs > 0)
-        e = rq::launch_wkv_scan({shape, {r, w, k, v, a, b, dt}, false, v, dt, y, y_dt, state, state_out, states, sa, seg}, s);
+        e = rq::launch_wkv_scan({shape, {r, w, k, v, a, b, dt}, false, v, dt, y, y_dt, state, state_out, states, sa, seg, {}}, s);
     return rq::launch_status(e, what);
 }
 
@@ -129,8 +126,7 @@ int64_t rq_wkv7_backward_workspace_bytes(int64_t batch, int64_t time, int64_t he
     const rq::WkvShape shape{has_cu_seqlens ? &kPacked : nullptr, batch, time, heads, seqs};
     if (int rc = check_chunks(what, shape)) return rc;
     ok();
-    const int64_t chunks = rq::wkv_chunks(shape);
-    return 4 * (state_floats(chunks, heads) + sa_floats(chunks, heads) + rq::wkv_segment_floats(rq::wkv_segments(shape), heads));
+    return 4 * rq::wkv_segment_floats(rq::wkv_segments(shape, true), heads);
 }
 
 int rq_wkv7_backward(const void* r, const void* w, const void* k, const void* v, const void* a, const void* b,
@@ -144,31 +140,25 @@ int rq_wkv7_backward(const void* r, const void* w, const void* k, const void* v,
     const rq::WkvShape shape{cu_seqlens, batch, time, heads, seqs};
     if (int rc = check_chunks(what, shape)) return rc;
     if (heads == 0 || (batch * time == 0 && seqs == 0)) return ok();
-    const int64_t chunks = rq::wkv_chunks(shape);
     if (batch * time > 0) {
         if (int rc = check_ptrs(what, {r, w, k, v, a, b, states, sa, dy}, {dr, dw, dk, dv, da, db})) return rc;
         if (cu_seqlens && seqs == 0) return fail(RQ_EINVAL, "%s: tokens but no sequence", what);
     }
     if (int rc = check_ptrs(what, {}, {dstate_out, dstate, workspace})) return rc;
     if (int rc = check_cu(what, cu_seqlens)) return rc;
-    const int64_t own = state_floats(chunks, heads) + sa_floats(chunks, heads);
-    const rq::WkvSegments seg = segments(shape, workspace ? (float*)workspace + own : nullptr);
-    const int64_t need = 4 * (own + rq::wkv_segment_floats(seg, heads));
+    const rq::WkvSegments seg = segments(shape, true, workspace);
+    const int64_t need = 4 * rq::wkv_segment_floats(seg, heads);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(RQ_EINVAL, "%s: needs a workspace of %lld bytes", what, (long long)need);
-    float* const dstates = (float*)workspace;
-    float* const dz = dstates ? dstates + state_floats(chunks, heads) : nullptr;
     hipStream_t s = (hipStream_t)stream;
-    const rq::WkvInputs in{r, w, k, v, a, b, dt};
     hipError_t e = hipSuccess;
     if (cu_seqlens && time > 0) {
         void* const rest[] = {dr, dw, dk, dv, da, db};
         e = rq::launch_wkv_rest(shape, dt, rest, 6, s);
     }
-    if (e == hipSuccess)
-        e = rq::launch_wkv_scan({shape, in, true, dy, y_dt, dv, dt, dstate_out, dstate, dstates, dz, seg}, s);
-    if (e == hipSuccess && chunks > 0 && batch * time > 0 && (dr || dw || dk || da || db))
-        e = rq::launch_wkv_grads({shape, in, dy, y_dt, states, sa, dstates, dz, dr, dw, dk, da, db}, s);
+    if (e == hipSuccess && seqs > 0)
+        e = rq::launch_wkv_scan({shape, {r, w, k, v, a, b, dt}, true, dy, y_dt, dv, dt, dstate_out, dstate, nullptr, nullptr, seg,
+                                 {states, sa, dr, dw, dk, da, db}}, s);
     return rq::launch_status(e, what);
 }
 

@@ -33,6 +33,12 @@ struct WkvSegments {
     float* begins;   // [slots, heads, 64, 64]
 };
 
+// Of the backward pass: what the forward one stored, and where the gradients go (each may be NULL).
+struct WkvGrads {
+    const float *states, *sa;
+    void *dr, *dw, *dk, *da, *db;
+};
+
 // One pass over the tokens, forwards or backwards in time.
 struct WkvScan {
     WkvShape shape;
@@ -44,19 +50,10 @@ struct WkvScan {
     int y_dt;
     const float* state;   // where the pass begins, or NULL for 0
     float* state_out;     // where it ends, or NULL
-    float* states;        // [chunks, heads, 64, 64]: the state with which the pass enters each chunk, or NULL
-    float* sa;            // [chunks, heads, 16, 64]: S a of every token (its gradient backwards), or NULL
+    float* states;        // forwards, [chunks, heads, 64, 64]: the state with which the pass enters each chunk, or NULL
+    float* sa;            // forwards, [chunks, heads, 16, 64]: S a of every token, or NULL
     WkvSegments seg;
-};
-
-// dr, dw, dk, da and db of every chunk from what the two passes stored.
-struct WkvGrads {
-    WkvShape shape;
-    WkvInputs in;
-    const void* dy;
-    int dy_dt;
-    const float *states, *sa, *dstates, *dz;
-    void *dr, *dw, *dk, *da, *db;  // each may be NULL
+    WkvGrads grads;       // backwards
 };
 
 struct WkvStep {
@@ -74,30 +71,40 @@ inline int64_t wkv_chunks(const WkvShape& s) {
     return s.cu ? s.time / RQ_WKV7_CHUNK + s.seqs : s.batch * ((s.time + RQ_WKV7_CHUNK - 1) / RQ_WKV7_CHUNK);
 }
 
-// The segments that take the least time by what was measured: a chunk of a block takes kScanUs, one
-// of a segment's end kEndsUs, a step from segment to segment kJoinUs, the further launches kMoreUs.
-inline WkvSegments wkv_segments(const WkvShape& s) {
-    constexpr double kScanUs = 2.4, kEndsUs = 2.7, kJoinUs = 0.6, kMoreUs = 12, kCus = 256;
+// The segments that take the least time by what was measured: a chunk of a block's scan takes kScanUs (kBackUs with
+// the gradients), one of a segment's end kEndsUs, and as much as two chunks to begin; a step from segment to segment
+// kJoinUs, the further launches kMoreUs.  A block has a CU to itself, and one block more than there are CUs is a
+// whole turn more: 12 heads of 8192 tokens took 93 us forwards in 264 blocks of 24 chunks, 67 us in 252 of 25.
+inline WkvSegments wkv_segments(const WkvShape& s, bool backward) {
+    constexpr double kScanUs = 2.4, kBackUs = 7, kEndsUs = 2.7, kJoinUs = 0.8, kMoreUs = 12;
+    constexpr int64_t kCus = 256, kBegin = 2;
     WkvSegments best{0, 0, nullptr, nullptr};
     if (s.seqs == 0 || s.heads == 0 || s.time == 0) return best;
     const int64_t all = wkv_chunks(s);
     const int64_t row = (s.time + RQ_WKV7_CHUNK - 1) / RQ_WKV7_CHUNK;
     // of a packed batch the lengths are not known here: one sequence may be this long
     const int64_t longest = s.cu ? std::min<int64_t>(row, 4 * row / s.seqs + 1) : row;
-    const double share = (double)all * s.heads / kCus;
-    double least = kScanUs * std::max((double)longest, share);
-    for (int64_t chunks = 8; chunks < longest; chunks += chunks < 32 ? 4 : chunks / 8) {
-        const double us = (kScanUs + kEndsUs) * std::max((double)chunks, share) +
+    const auto slots = [&](int64_t chunks) {
+        return s.cu ? s.time / (RQ_WKV7_CHUNK * chunks) + s.seqs : s.batch * ((row + chunks - 1) / chunks);
+    };
+    // chunks, one after another, of the CU that has most
+    const auto turns = [&](int64_t chunks, int64_t n) {
+        const int64_t blocks = n * s.heads;
+        const double share = (double)(all + kBegin * n) * s.heads / kCus;
+        if (s.cu) return std::max((double)(chunks + kBegin), share + (blocks > kCus ? 0.5 * chunks : 0));
+        return (double)(chunks + kBegin) * ((blocks + kCus - 1) / kCus);
+    };
+    const double scan = backward ? kBackUs : kScanUs;
+    double least = scan * turns(longest, s.seqs);
+    for (int64_t chunks = 4; chunks < longest; chunks += chunks < 64 ? 1 : chunks / 32) {
+        const double us = (scan + kEndsUs) * turns(chunks, slots(chunks)) +
                           kJoinUs * ((longest + chunks - 1) / chunks) + kMoreUs;
         if (us < least) {
             least = us;
             best.chunks = chunks;
         }
     }
-    if (best.chunks) {
-        const int64_t per = (row + best.chunks - 1) / best.chunks;
-        best.slots = s.cu ? s.time / (RQ_WKV7_CHUNK * best.chunks) + s.seqs : s.batch * per;
-    }
+    if (best.chunks) best.slots = slots(best.chunks);
     return best;
 }
 
@@ -106,7 +113,6 @@ inline int64_t wkv_segment_floats(const WkvSegments& g, int64_t heads) {
 }
 
 hipError_t launch_wkv_scan(const WkvScan& a, hipStream_t stream);
-hipError_t launch_wkv_grads(const WkvGrads& a, hipStream_t stream);
 hipError_t launch_wkv_step(const WkvStep& a, hipStream_t stream);
 // 0 in the rows of a packed batch that belong to no sequence; NULL tensors are left out.
 hipError_t launch_wkv_rest(const WkvShape& s, int dt, void* const* tensors, int n, hipStream_t stream);

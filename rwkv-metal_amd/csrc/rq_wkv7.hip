@@ -20,7 +20,7 @@
 //   dr = e^L (dY S + dMrb B~ + dMrk K~)             dMrb = incl(dY SA^T), dMrk = incl(dY V^T)
 //   da = e^Lx (dZ S + dMab B~ + dMak K~)            dMab = strict(dZ SA^T), dMak = strict(dZ V^T)
 //   db = e^-L (e^Lend SA dS' + dMrb^T R~ + dMab^T A~), dk alike with V, dMrk, dMak
-//   dlog d_t: what of the loss passes token t's decay (grads_kernel).
+//   dlog d_t: what of the loss passes token t's decay (chunk_grads).
 //
 // The scan's products are fp32 MFMAs (v_mfma_f32_16x16x4_f32): the state lives in fp32 and
 // feeds itself for thousands of tokens.
@@ -30,6 +30,7 @@
 // e^(L_t - L_s), whose exponents are sums of the terms between s and t and never
 // positive; that also serves decays of 0.
 #include <algorithm>
+#include <type_traits>
 
 #include "rq_common.h"
 #include "rq_error.h"
@@ -168,6 +169,10 @@ struct ScanLds {
     Rows y[2];
     int strong[3][4];    // whether a wave's channels hold strong decays
 };
+struct ScanGradLds : ScanLds {
+    Rows d[4];  // dS' of a chunk, [value / 16][value % 16][key]
+    Rows dz;    // dZ, [15 - token][value]
+};
 
 // X^T of X = (1 - M)^-1 from m[i] = M^T[4g + i][lane & 15], nonzero above the diagonal:
 // rows from the last, X^T[s] = e_s + sum over u > s of M^T[s, u] X^T[u], four at a time.
@@ -241,8 +246,6 @@ __device__ __attribute__((noinline)) f32x4_t strong_pairs(const float* late, con
     }
     return out;
 }
-
-// ------------------------------------------------------------------ the scan
 
 // Four contiguous values as they are stored.
 template <int DT>
@@ -382,6 +385,352 @@ RQ_DEV void form_matrix(const WkvInputs& in, const Arrays& from, const Rows* inv
     if (pair == 3) to.y_x[lane] = x;
 }
 
+// ----------------------------------------------------------- the gradients
+
+// Over a lane's four tokens and the four lanes of its key: lane (m, g) holds tokens 4g + i.
+RQ_DEV float groups_before(float x, int g) {  // the sum over the groups before the lane's own
+    float a = __shfl_up(x, 16), b = __shfl_up(x, 32), c = __shfl_up(x, 48);
+    return (g > 0 ? a : 0.f) + (g > 1 ? b : 0.f) + (g > 2 ? c : 0.f);
+}
+RQ_DEV float groups_after(float x, int g) {
+    float a = __shfl_down(x, 16), b = __shfl_down(x, 32), c = __shfl_down(x, 48);
+    return (g < 3 ? a : 0.f) + (g < 2 ? b : 0.f) + (g < 1 ? c : 0.f);
+}
+RQ_DEV float over_groups(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// The products of the gradients.  They are not fed back into anything, and where the tensors have 16 bits
+// their results are rounded to 8 or 11 significant ones: there an operand is the sum of two bf16 (16 bits of
+// it), a product three bf16 MFMAs of 32 steps, at a fifth of the fp32 MFMA's time and beside the VALU, which
+// the fp32 one holds up.  fp32 tensors keep fp32 products.
+struct Halves {
+    bf16x8_t hi, lo;
+};
+RQ_DEV Halves halves_of(const f32x4_t& x, const f32x4_t& y) {
+    Halves h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h.hi[i] = (__bf16)x[i];
+        h.hi[4 + i] = (__bf16)y[i];
+        h.lo[i] = (__bf16)(x[i] - (float)h.hi[i]);
+        h.lo[4 + i] = (__bf16)(y[i] - (float)h.hi[4 + i]);
+    }
+    return h;
+}
+// EXACT: an operand that is bf16 as it is (its lo is 0)
+template <bool EXACT_A, bool EXACT_B>
+RQ_DEV f32x4_t mma_halves(const Halves& a, const Halves& b, f32x4_t c) {
+    if constexpr (!EXACT_A) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.lo, b.hi, c, 0, 0, 0);
+    if constexpr (!EXACT_B) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.lo, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.hi, c, 0, 0, 0);
+}
+
+// A row or column of N / 4 lanes' shares, four numbers from each 16: N = 64 values, or the 16 tokens of two matrices.
+template <bool HALF, int N>
+struct Operand {
+    f32x4_t v[N / 16];
+    RQ_DEV explicit Operand(const f32x4_t* x) {
+#pragma unroll
+        for (int q = 0; q < N / 16; ++q) v[q] = x[q];
+    }
+    RQ_DEV Operand(f32x4_t x0, f32x4_t x1) : v{x0, x1} {}
+};
+template <int N>
+struct Operand<true, N> {
+    Halves v[N / 32];
+    RQ_DEV explicit Operand(const f32x4_t* x) {
+#pragma unroll
+        for (int q = 0; q < N / 32; ++q) v[q] = halves_of(x[2 * q], x[2 * q + 1]);
+    }
+    RQ_DEV Operand(f32x4_t x0, f32x4_t x1) : v{halves_of(x0, x1)} {}
+};
+
+// Of rows as they are stored: bf16 ones are their own high halves.  0 where the token is not there.
+template <bool HALF, int DT>
+RQ_DEV Operand<HALF, 64> row_operand(const Raw4<DT>* raw, bool there) {
+    if constexpr (HALF && DT == RQ_BF16) {
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        const f32x4_t zero[4] = {};
+        Operand<true, 64> o(zero);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const u32x4 u = {raw[2 * q].v[0], raw[2 * q].v[1], raw[2 * q + 1].v[0], raw[2 * q + 1].v[1]};
+            o.v[q].hi = __builtin_bit_cast(bf16x8_t, there ? u : u32x4{0, 0, 0, 0});
+        }
+        return o;
+    } else {
+        f32x4_t x[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = there ? unpack_raw4<DT>(raw[q]) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+        return Operand<HALF, 64>(x);
+    }
+}
+// Half h of an operand of 64.
+template <bool HALF>
+RQ_DEV Operand<HALF, 32> half_of(const Operand<HALF, 64>& x, int h) {
+    const f32x4_t zero[2] = {};
+    Operand<HALF, 32> o(zero);
+    if constexpr (HALF) {
+        o.v[0] = x.v[h];
+    } else {
+        o.v[0] = x.v[2 * h];
+        o.v[1] = x.v[2 * h + 1];
+    }
+    return o;
+}
+template <bool EXACT_A = false, bool EXACT_B = false, bool HALF, int N>
+RQ_DEV f32x4_t mma(const Operand<HALF, N>& a, const Operand<HALF, N>& b, f32x4_t c) {
+    if constexpr (HALF) {
+#pragma unroll
+        for (int q = 0; q < N / 32; ++q) c = mma_halves<EXACT_A, EXACT_B>(a.v[q], b.v[q], c);
+    } else {
+#pragma unroll
+        for (int q = 0; q < N / 16; ++q) c = mma16(a.v[q], b.v[q], c);
+    }
+    return c;
+}
+
+
+// A value of a row, `at` bytes behind a pointer that all lanes share.
+template <int DT>
+RQ_DEV typename dt_traits<DT>::storage load1(const uint8_t* p, uint32_t at) {
+    return *(const typename dt_traits<DT>::storage*)(p + at);
+}
+template <int DT>
+RQ_DEV void store1(uint8_t* p, uint32_t at, float x) {
+    *(typename dt_traits<DT>::storage*)(p + at) = dt_traits<DT>::from_f32(x);
+}
+
+// x of the token `t` (the same in all lanes) and the lane's key, from tokens 4g + i
+RQ_DEV float at_token(const f32x4_t& x, int t, int m) {
+    const float own = (t & 3) == 0 ? x[0] : (t & 3) == 1 ? x[1] : (t & 3) == 2 ? x[2] : x[3];
+    return __shfl(own, 16 * (t >> 2) + m);
+}
+
+// A chunk's dr, dw, dk, da and db for the 16 keys of a wave.  In products over the values a lane holds rows
+// of tokens (A) and columns of keys (B); the results, tokens 4g + i of key lane & 15, are where the gradients are
+// formed.  Each wave forms the four pair matrices for itself, and their transposes: no wave waits for another.
+// `d` is dS' [value][key], `dz` dZ [15 - token][value].
+template <int DT, int YDT>
+struct ChunkGrads {
+    static constexpr bool HALF = DT != RQ_F32, V_EXACT = DT == RQ_BF16, DY_EXACT = YDT == RQ_BF16;
+    static constexpr uint32_t SIZE = DT == RQ_F32 ? 4 : 2, YSIZE = YDT == RQ_F32 ? 4 : 2;
+    // of the chunk: its first element, its tokens; of the lane's tokens 4g + i
+    int64_t first;
+    int tokens;
+    uint32_t at[4];
+    typename dt_traits<DT>::storage raw[5][4];
+    Raw4<YDT> raw_dy[4];
+    Raw4<DT> raw_v[4];
+    f32x4_t sa[4], s[4];
+
+    RQ_DEV void load(const WkvScan& p, int64_t first_, int64_t chunk, int tokens_, int lane, int wave) {
+        const int g = lane >> 4, m = lane & 15, key = 16 * wave + m;
+        const uint32_t stride = (uint32_t)p.shape.heads * kHead;  // from token to token
+        first = first_;
+        tokens = tokens_;
+        const auto of_chunk = [&](const void* q, uint32_t size) { return (const uint8_t*)q + first * size; };
+        // a load under a condition would be waited for where the condition ends: tokens that are not there
+        // load the first
+        // The lane's offsets in 32 bits behind scalar pointers, made anew for each chunk: hoisted out of the loop over
+        // the chunks as 64-bit addresses they took 63 registers too many.
+        uint32_t row = (m < tokens ? m : 0) * stride + 4 * g, column = (4 * g * kHead + key) * 4, line = (m * kHead + 4 * g) * 4;
+        asm volatile("" : "+v"(row), "+v"(column), "+v"(line));
+        const uint8_t* const s_at = (const uint8_t*)(p.grads.states + chunk * kHead * kHead);
+        const uint8_t* const sa_at = (const uint8_t*)(p.grads.sa + chunk * kChunk * kHead);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            at[i] = ((4 * g + i < tokens ? 4 * g + i : 0) * stride + key) * SIZE;
+            asm volatile("" : "+v"(at[i]));
+            raw[0][i] = load1<DT>(of_chunk(p.in.w, SIZE), at[i]);
+            raw[1][i] = load1<DT>(of_chunk(p.in.r, SIZE), at[i]);
+            raw[2][i] = load1<DT>(of_chunk(p.in.a, SIZE), at[i]);
+            raw[3][i] = load1<DT>(of_chunk(p.in.b, SIZE), at[i]);
+            raw[4][i] = load1<DT>(of_chunk(p.in.k, SIZE), at[i]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[q][i] = *(const float*)(s_at + 16 * q * kHead * 4 + (column + i * kHead * 4));
+            raw_dy[q] = *(const Raw4<YDT>*)(of_chunk(p.x, YSIZE) + (row + 16 * q) * YSIZE);
+            raw_v[q] = *(const Raw4<DT>*)(of_chunk(p.in.v, SIZE) + (row + 16 * q) * SIZE);
+            sa[q] = *(const f32x4_t*)(sa_at + (line + 16 * q * 4));
+        }
+    }
+    RQ_DEV void run(const WkvScan& p, const Rows* d_rows, const Rows& dz_rows, int lane, int wave) const;
+};
+
+template <int DT, int YDT>
+RQ_DEV void ChunkGrads<DT, YDT>::run(const WkvScan& p, const Rows* d_rows, const Rows& dz_rows, int lane, int wave) const {
+    const int g = lane >> 4, m = lane & 15, key = 16 * wave + m;
+    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+    f32x4_t gr = zero, ga = zero, gb = zero, gk = zero;
+    float through = 0.f;  // sum over the values of S dS' of this key
+    f32x4_t by_t[4], by_s[4];  // dMab, dMak, dMrb, dMrk
+    {
+        const Operand<HALF, 64> dy_o = row_operand<HALF>(raw_dy, m < tokens), v_o = row_operand<HALF>(raw_v, m < tokens),
+                                sa_o(sa);
+        f32x4_t dz[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) dz[q] = *(const f32x4_t*)&dz_rows[kChunk - 1 - m][16 * q + 4 * g];
+        const Operand<HALF, 64> dz_o(dz);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            f32x4_t d[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    d[q][i] = d_rows[2 * h + q][4 * g + i][key];
+                    through = fmaf(s[2 * h + q][i], d[q][i], through);
+                }
+            }
+            const Operand<HALF, 32> s_o(s + 2 * h), d_o(d);
+            gr = mma<DY_EXACT, false>(half_of(dy_o, h), s_o, gr);
+            ga = mma(half_of(dz_o, h), s_o, ga);
+            gb = mma(half_of(sa_o, h), d_o, gb);
+            gk = mma<V_EXACT, false>(half_of(v_o, h), d_o, gk);
+            }
+        by_t[0] = mma(sa_o, dz_o, zero);
+        by_t[1] = mma<V_EXACT, false>(v_o, dz_o, zero);
+        by_t[2] = mma<false, DY_EXACT>(sa_o, dy_o, zero);
+        by_t[3] = mma<V_EXACT, DY_EXACT>(v_o, dy_o, zero);
+        by_s[0] = mma(dz_o, sa_o, zero);
+        by_s[1] = mma<false, V_EXACT>(dz_o, v_o, zero);
+        by_s[2] = mma<DY_EXACT, false>(dy_o, sa_o, zero);
+        by_s[3] = mma<DY_EXACT, V_EXACT>(dy_o, v_o, zero);
+    }
+    f32x4_t r, a, b, k, g2, l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool has = 4 * g + i < tokens;
+        g2[i] = has ? log2_decay(dt_traits<DT>::to_f32(raw[0][i])) : 0.f;
+        r[i] = has ? dt_traits<DT>::to_f32(raw[1][i]) : 0.f;
+        a[i] = has ? dt_traits<DT>::to_f32(raw[2][i]) : 0.f;
+        b[i] = has ? dt_traits<DT>::to_f32(raw[3][i]) : 0.f;
+        k[i] = has ? dt_traits<DT>::to_f32(raw[4][i]) : 0.f;
+        l[i] = i ? l[i - 1] + g2[i] : g2[i];
+    }
+    const float off = groups_before(l[3], g);
+    l += off;
+    const float end = __shfl(l[3], 48 + m);
+    const bool strong = __any(!(end >= kStrong));
+    through = over_groups(through);
+    // a token's own pair passes no decay: it stays out of the sums below, where it would cancel
+    f32x4_t own_b, own_k;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        own_b[i] = __shfl(by_t[2][i], 16 * g + 4 * g + i);
+        own_k[i] = __shfl(by_t[3][i], 16 * g + 4 * g + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (!(4 * g + i < m)) by_t[j][i] = 0.f;  // rows are sources, columns targets
+            if (!(m < 4 * g + i)) by_s[j][i] = 0.f;  // the other way round
+        }
+    }
+    f32x4_t to_end, el, ex;  // e^(Lend - L), e^L, e^Lx
+    {
+        float after = groups_after((g2[0] + g2[1]) + (g2[2] + g2[3]), g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            el[i] = exp2_hw(l[i]);
+            ex[i] = i ? el[i - 1] : exp2_hw(off);
+        }
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {
+            to_end[i] = exp2_hw(after);
+            after += g2[i];
+        }
+    }
+    gb *= to_end;
+    gk *= to_end;
+    gr *= el;
+    ga *= ex;
+    const f32x4_t enters = b * gb + k * gk, leaves_r = r * gr, leaves_a = a * ga;  // what each token adds to, and takes from, the state
+    f32x4_t pr = zero, pa = zero, pb = zero, pk = zero, cross = zero;
+    if (strong) {
+        // pair by pair, from the sums of the terms between the two tokens
+#pragma unroll 1
+        for (int src = 0; src < kChunk - 1; ++src) {
+            const float bs = at_token(b, src, m), ks = at_token(k, src, m);
+            float e = 0.f;
+#pragma unroll 1
+            for (int t = src + 1; t < kChunk; ++t) {
+                const float h = exp2_hw(e);
+                e += at_token(g2, t, m);
+                const float f = exp2_hw(e), rt = at_token(r, t, m) * f, at_ = at_token(a, t, m) * h;
+                const float m0 = at_token(by_t[0], src, t), m1 = at_token(by_t[1], src, t), m2 = at_token(by_t[2], src, t),
+                            m3 = at_token(by_t[3], src, t);
+                const float of_a = m0 * bs + m1 * ks, of_r = m2 * bs + m3 * ks;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int own = 4 * g + i;
+                    pr[i] += own == t ? of_r * f : 0.f;
+                    pa[i] += own == t ? of_a * h : 0.f;
+                    pb[i] += own == src ? m0 * at_ + m2 * rt : 0.f;
+                    pk[i] += own == src ? m1 * at_ + m3 * rt : 0.f;
+                    cross[i] += own > src && own <= t ? of_r * rt : 0.f;
+                    cross[i] += own > src && own < t ? of_a * at_ : 0.f;  // a's decays end before t
+                }
+            }
+        }
+    } else {
+        f32x4_t il;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) il[i] = exp2_hw(-l[i]);
+        const Operand<HALF, 32> early(b * il, k * il), late(a * ex, r * el);  // B~, K~ and A~, R~
+        pa = mma(Operand<HALF, 32>(by_t[0], by_t[1]), early, pa) * ex;
+        pr = mma(Operand<HALF, 32>(by_t[2], by_t[3]), early, pr) * el;
+        pb = mma(Operand<HALF, 32>(by_s[0], by_s[2]), late, pb) * il;
+        pk = mma(Operand<HALF, 32>(by_s[1], by_s[3]), late, pk) * il;
+        // a pair (s, t) passes the decays behind s up to t (before t, for a): sums of what ends
+        // minus what begins at each token and behind it
+        const f32x4_t q = r * pr - b * pb - k * pk, qa = a * pa;
+        float sum = groups_after((q[0] + qa[0]) + (q[1] + qa[1]) + (q[2] + qa[2]) + (q[3] + qa[3]), g);
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {
+            cross[i] = sum + q[i];
+            sum += q[i] + qa[i];
+        }
+    }
+    gr += pr + own_b * b + own_k * k;
+    ga += pa;
+    gb += pb + own_b * r;
+    gk += pk + own_k * r;
+    // the state's own way through the chunk, what entered before and what leaves at or behind
+    const float whole = exp2_hw(end) * through;
+    float into = groups_before((enters[0] + enters[1]) + (enters[2] + enters[3]), g);
+    float out_of = groups_after((leaves_r[0] + leaves_a[0]) + (leaves_r[1] + leaves_a[1]) +
+                                    (leaves_r[2] + leaves_a[2]) + (leaves_r[3] + leaves_a[3]), g);
+    f32x4_t gw;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        gw[i] = cross[i] + whole + into;
+        into += enters[i];
+    }
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+        gw[i] += out_of + leaves_r[i];
+        out_of += leaves_r[i] + leaves_a[i];
+        // d log d / dw = -exp(w), inf where the decay, and with it what passes it, is 0
+        gw[i] = gw[i] == 0.f ? 0.f : gw[i] * (g2[i] * kLn2);
+    }
+    const auto to_chunk = [&](void* q) { return (uint8_t*)q + first * SIZE; };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (4 * g + i >= tokens) continue;
+        if (p.grads.dr) store1<DT>(to_chunk(p.grads.dr), at[i], gr[i]);
+        if (p.grads.dw) store1<DT>(to_chunk(p.grads.dw), at[i], gw[i]);
+        if (p.grads.dk) store1<DT>(to_chunk(p.grads.dk), at[i], gk[i]);
+        if (p.grads.da) store1<DT>(to_chunk(p.grads.da), at[i], ga[i]);
+        if (p.grads.db) store1<DT>(to_chunk(p.grads.db), at[i], gb[i]);
+    }
+}
+
+// ------------------------------------------------------------------ the scan
+
 // A segment of a sequence: which, and its chunks in processing order.
 struct Segment {
     int64_t seq, index, first, end;
@@ -422,12 +771,20 @@ RQ_DEV bool unused(const Segment& s) { return s.index < 0 || (s.index > 0 && s.f
 // stores are waited for in their order, and a load behind a store waits for the store too.
 //
 // ENDS: only where a segment ends, from a state of 0 (four scan waves) and, without x, from the identity (four more).
-template <bool ENDS>
-constexpr int kScanThreads = (ENDS ? 16 : 12) * 64;
+//
+// Backwards (GRADS) the scan waves also form the other gradients of their chunk, from its dS' and dZ in LDS, with
+// what else they need on its way from memory while they scan.  That takes more than the 168 registers of twelve
+// waves: there are eight, four for the arrays and the matrices, and a second barrier between scan and gradients.
+// Four waves of their own for chunk c - 1 (one barrier, a load's whole wait in each turn) took 8.7 us a chunk
+// against 6.7; a kernel of its own behind the scan, its dS' and dZ through memory, 145 + 100 us for 4096 tokens
+// of 32 heads against 220.
+template <bool REV, bool ENDS>
+constexpr int kScanThreads = (ENDS ? 16 : REV ? 8 : 12) * 64;
 
 template <int DT, int XDT, int YDT, bool REV, bool ENDS>
-__global__ __launch_bounds__(kScanThreads<ENDS>) void wkv7_scan_kernel(WkvScan p) {
-    __shared__ ScanLds lds;
+__global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(WkvScan p) {
+    constexpr bool GRADS = REV && !ENDS;
+    __shared__ std::conditional_t<GRADS, ScanGradLds, ScanLds> lds;
     const int lane = threadIdx.x & 63, wave = wave_index();
     const int g = lane >> 4, m = lane & 15;
     const int64_t H = p.shape.heads, slot = blockIdx.x / H, head = blockIdx.x % H;
@@ -441,6 +798,13 @@ __global__ __launch_bounds__(kScanThreads<ENDS>) void wkv7_scan_kernel(WkvScan p
     const auto row = [&](int64_t c) { return (span.start + (exists(c) ? token(c, m) : 0)) * H + head; };  // where n > 0
     const auto odd = [&](int64_t c) { return (int)(c - first) & 1; };
 
+    const auto matrix = [&](int64_t c, int ring) {
+        if (c >= end) return;
+        const int* f = lds.strong[ring];
+        const bool strong = __builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]);
+        form_matrix<DT, REV>(p.in, lds.arrays[ring], lds.inverse[odd(c)], strong, lds.matrices[odd(c)], lane, wave & 3, row(c),
+                             exists(c));
+    };
     if (wave < 4) {
         Elementwise<DT, XDT, REV> el{lane, wave};
         const auto load = [&](int64_t c) {
@@ -458,28 +822,28 @@ __global__ __launch_bounds__(kScanThreads<ENDS>) void wkv7_scan_kernel(WkvScan p
         arrays(first, 0);
         load(first + 1);
         __syncthreads();
+        if (GRADS) matrix(first, 0);
         arrays(first + 1, 1);
         load(first + 2);
         __syncthreads();
-        int ring = 2;  // of chunk c + 2
+        int next = 1, ring = 2;  // of chunks c + 1 and c + 2
         for (int64_t c = first; c < end; ++c) {
             arrays(c + 2, ring);
-            store_y(c - 1);
+            if (!GRADS) store_y(c - 1);
             load(c + 3);
-            ring = ring == 2 ? 0 : ring + 1;
             __syncthreads();
+            if (GRADS) {
+                matrix(c + 1, next);
+                store_y(c);
+                __syncthreads();
+            }
+            next = ring;
+            ring = ring == 2 ? 0 : ring + 1;
         }
-        store_y(end - 1);
+        if (!GRADS) store_y(end - 1);
         return;
     }
-    if (wave < 8) {
-        const auto matrix = [&](int64_t c, int ring) {
-            if (c >= end) return;
-            const int* f = lds.strong[ring];
-            const bool strong = __builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]);
-            form_matrix<DT, REV>(p.in, lds.arrays[ring], lds.inverse[odd(c)], strong, lds.matrices[odd(c)], lane, wave - 4,
-                                 row(c), exists(c));
-        };
+    if (!GRADS && wave < 8) {
         __syncthreads();
         matrix(first, 0);
         __syncthreads();
@@ -517,7 +881,15 @@ __global__ __launch_bounds__(kScanThreads<ENDS>) void wkv7_scan_kernel(WkvScan p
         const Matrices& mat = lds.matrices[odd(c)];
         ring = ring == 2 ? 0 : ring + 1;
         const int64_t chunk = (span.chunk0 + (REV ? n - 1 - c : c)) * H + head;
-        if (!ENDS && p.states) {
+        ChunkGrads<DT, XDT> grads;
+        if constexpr (GRADS) {
+            const int64_t t0 = kChunk * (n - 1 - c);
+            grads.load(p, ((span.start + t0) * H + head) * kHead, chunk, (int)std::min<int64_t>(kChunk, span.len - t0), lane,
+                       wave & 3);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *(f32x4_t*)&lds.d[wave & 3][m][16 * q + 4 * g] = acc[q];
+        }
+        if (!ENDS && !REV && p.states) {
             float* to = p.states + (chunk * kHead + value) * kHead + 4 * g;
 #pragma unroll
             for (int q = 0; q < 4; ++q) *(f32x4_t*)(to + 16 * q) = acc[q];
@@ -568,13 +940,20 @@ __global__ __launch_bounds__(kScanThreads<ENDS>) void wkv7_scan_kernel(WkvScan p
         if constexpr (!ENDS) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) lds.y[odd(c)][4 * g + i][value] = y[0][i] + y[1][i];
-            if (p.sa) {  // rows in the order of time, the missing ones 0
+            if constexpr (GRADS) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    p.sa[(chunk * kChunk + (REV ? kChunk - 1 - (4 * g + i) : 4 * g + i)) * kHead + value] = sa[i];
+                for (int i = 0; i < 4; ++i) lds.dz[4 * g + i][value] = sa[i];
+            }
+            if (!REV && p.sa) {  // 0 for tokens that are not there
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p.sa[(chunk * kChunk + 4 * g + i) * kHead + value] = sa[i];
             }
         }
         __syncthreads();
+        if constexpr (GRADS) {
+            grads.run(p, lds.d, lds.dz, lane, wave & 3);
+            __syncthreads();
+        }
     }
     float* to = ENDS ? p.seg.ends + ((slot * H + head) * 2 * kHead + (map ? kHead : 0) + value) * kHead
                 : p.state_out && seg.last ? p.state_out + ((seg.seq * H + head) * kHead + value) * kHead
@@ -635,429 +1014,6 @@ __global__ __launch_bounds__(256) void wkv7_join_kernel(WkvShape shape, WkvSegme
             s = sum[0] + sum[1];
             *(f32x4_t*)(seg.begins + (((slot0 + j + 1) * H + head) * kHead + value) * kHead + 16 * q + 4 * g) = s;
         }
-    }
-}
-
-// ----------------------------------------------------------- the gradients
-
-// Over a lane's four tokens and the four lanes of its key: lane (m, g) holds tokens 4g + i.
-RQ_DEV float groups_before(float x, int g) {  // the sum over the groups before the lane's own
-    float a = __shfl_up(x, 16), b = __shfl_up(x, 32), c = __shfl_up(x, 48);
-    return (g > 0 ? a : 0.f) + (g > 1 ? b : 0.f) + (g > 2 ? c : 0.f);
-}
-RQ_DEV float groups_after(float x, int g) {
-    float a = __shfl_down(x, 16), b = __shfl_down(x, 32), c = __shfl_down(x, 48);
-    return (g < 3 ? a : 0.f) + (g < 2 ? b : 0.f) + (g < 1 ? c : 0.f);
-}
-RQ_DEV float over_groups(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
-}
-
-constexpr int kPairRow = 20;  // LDS row of a [16, 16] matrix
-
-// The products of the gradients.  They are not fed back into anything, and where the tensors have 16 bits
-// their results are rounded to 8 or 11 significant ones: there an operand is the sum of two bf16 (16 bits of
-// it), a product three bf16 MFMAs of 32 steps, at a fifth of the fp32 MFMA's time and beside the VALU, which
-// the fp32 one holds up.  fp32 tensors keep fp32 products.
-struct Halves {
-    bf16x8_t hi, lo;
-};
-RQ_DEV Halves halves_of(const f32x4_t& x, const f32x4_t& y) {
-    Halves h;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        h.hi[i] = (__bf16)x[i];
-        h.hi[4 + i] = (__bf16)y[i];
-        h.lo[i] = (__bf16)(x[i] - (float)h.hi[i]);
-        h.lo[4 + i] = (__bf16)(y[i] - (float)h.hi[4 + i]);
-    }
-    return h;
-}
-// EXACT: an operand that is bf16 as it is (its lo is 0)
-template <bool EXACT_A, bool EXACT_B>
-RQ_DEV f32x4_t mma_halves(const Halves& a, const Halves& b, f32x4_t c) {
-    if constexpr (!EXACT_A) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.lo, b.hi, c, 0, 0, 0);
-    if constexpr (!EXACT_B) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.lo, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.hi, c, 0, 0, 0);
-}
-
-// A row or column of N / 4 lanes' shares, four numbers from each 16: N = 64 values, or the 16 tokens of two matrices.
-template <bool HALF, int N>
-struct Operand {
-    f32x4_t v[N / 16];
-    RQ_DEV explicit Operand(const f32x4_t* x) {
-#pragma unroll
-        for (int q = 0; q < N / 16; ++q) v[q] = x[q];
-    }
-};
-template <int N>
-struct Operand<true, N> {
-    Halves v[N / 32];
-    RQ_DEV explicit Operand(const f32x4_t* x) {
-#pragma unroll
-        for (int q = 0; q < N / 32; ++q) v[q] = halves_of(x[2 * q], x[2 * q + 1]);
-    }
-    RQ_DEV explicit Operand(const Halves& h) { v[0] = h; }
-};
-template <bool EXACT_A = false, bool EXACT_B = false, bool HALF, int N>
-RQ_DEV f32x4_t mma(const Operand<HALF, N>& a, const Operand<HALF, N>& b, f32x4_t c) {
-    if constexpr (HALF) {
-#pragma unroll
-        for (int q = 0; q < N / 32; ++q) c = mma_halves<EXACT_A, EXACT_B>(a.v[q], b.v[q], c);
-    } else {
-#pragma unroll
-        for (int q = 0; q < N / 16; ++q) c = mma16(a.v[q], b.v[q], c);
-    }
-    return c;
-}
-
-struct GradLds {
-    uint32_t m[4][kChunk][kPairRow];    // dMab, dMak, dMrb, dMrk, [s][t], s < t: as they are, or their halves
-    float own[2][kChunk];               // the diagonals of dMrb, dMrk
-    float strong[4][5][kChunk][16];     // r, a, b, k and log2 d of a wave's 16 keys
-};
-
-template <bool HALF>
-RQ_DEV uint32_t pack_pair(float x) {
-    if constexpr (!HALF) return __float_as_uint(x);
-    const uint32_t hi = f32_to_bf16_bits(x);
-    return hi << 16 | f32_to_bf16_bits(x - bf16_bits_to_f32(hi));
-}
-template <bool HALF>
-RQ_DEV float pair_of(uint32_t u) {
-    return HALF ? __uint_as_float(u & 0xffff0000u) + __uint_as_float(u << 16) : __uint_as_float(u);
-}
-// The operand of two matrices' entries.
-template <bool HALF>
-RQ_DEV Operand<HALF, 32> pair_operand(const uint32_t* x, const uint32_t* y) {
-    if constexpr (HALF) {
-        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-        const u32x4 hi = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302), __builtin_amdgcn_perm(x[3], x[2], 0x07060302),
-                          __builtin_amdgcn_perm(y[1], y[0], 0x07060302), __builtin_amdgcn_perm(y[3], y[2], 0x07060302)};
-        const u32x4 lo = {__builtin_amdgcn_perm(x[1], x[0], 0x05040100), __builtin_amdgcn_perm(x[3], x[2], 0x05040100),
-                          __builtin_amdgcn_perm(y[1], y[0], 0x05040100), __builtin_amdgcn_perm(y[3], y[2], 0x05040100)};
-        return Operand<true, 32>(Halves{__builtin_bit_cast(bf16x8_t, hi), __builtin_bit_cast(bf16x8_t, lo)});
-    } else {
-        f32x4_t v[2];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[0][i] = __uint_as_float(x[i]);
-            v[1][i] = __uint_as_float(y[i]);
-        }
-        return Operand<false, 32>(v);
-    }
-}
-
-// The parts of the gradients that come from the pairs within a chunk of strong decays, for the
-// lane's key and tokens 4g + i: gr, ga, gb, gk, and in `cross` what of the loss passes each
-// token's decay.
-template <bool HALF>
-__device__ __attribute__((noinline)) void strong_grads(const GradLds& lds, int wave, int lane, float* gr, float* ga,
-                                                       float* gb, float* gk, float* cross) {
-    const int g = lane >> 4, key = lane & 15;
-    const auto& in = lds.strong[wave];
-    const auto pair = [&](int j, int s, int t) { return pair_of<HALF>(lds.m[j][s][t]); };
-    for (int i = 0; i < 4; ++i) {
-        const int own = 4 * g + i;
-        gr[i] = ga[i] = gb[i] = gk[i] = cross[i] = 0.f;
-        float e = in[4][own][key];  // log2 of the decay from s to own
-        for (int s = own - 1; s >= 0; --s) {
-            gr[i] += (pair(2, s, own) * in[2][s][key] + pair(3, s, own) * in[3][s][key]) * exp2_hw(e);
-            e += in[4][s][key];
-        }
-        e = 0.f;
-        for (int s = own - 1; s >= 0; --s) {
-            ga[i] += (pair(0, s, own) * in[2][s][key] + pair(1, s, own) * in[3][s][key]) * exp2_hw(e);
-            e += in[4][s][key];
-        }
-        e = 0.f;
-        for (int t = own + 1; t < kChunk; ++t) {
-            const float f = in[1][t][key] * exp2_hw(e);
-            e += in[4][t][key];
-            const float h = in[0][t][key] * exp2_hw(e);
-            gb[i] += pair(0, own, t) * f + pair(2, own, t) * h;
-            gk[i] += pair(1, own, t) * f + pair(3, own, t) * h;
-        }
-        for (int s = 0; s < own; ++s) {
-            e = 0.f;
-            for (int t = s + 1; t < kChunk; ++t) {
-                if (t > own)  // a's decays end before t
-                    cross[i] += in[1][t][key] * exp2_hw(e) * (pair(0, s, t) * in[2][s][key] + pair(1, s, t) * in[3][s][key]);
-                e += in[4][t][key];
-                if (t >= own)
-                    cross[i] += in[0][t][key] * exp2_hw(e) * (pair(2, s, t) * in[2][s][key] + pair(3, s, t) * in[3][s][key]);
-            }
-        }
-    }
-}
-
-// Four contiguous values of a row as fp32, `at` bytes behind a pointer that all lanes share.
-template <int DT>
-RQ_DEV f32x4_t load4(const uint8_t* p, uint32_t at) {
-    return unpack_raw4<DT>(*(const Raw4<DT>*)(p + at));
-}
-template <int DT>
-RQ_DEV typename dt_traits<DT>::storage load1(const uint8_t* p, uint32_t at) {
-    return *(const typename dt_traits<DT>::storage*)(p + at);
-}
-template <int DT>
-RQ_DEV void store1(uint8_t* p, uint32_t at, float x) {
-    *(typename dt_traits<DT>::storage*)(p + at) = dt_traits<DT>::from_f32(x);
-}
-
-// A block is one chunk of one head; each of its four waves has 16 keys, and one of the four pair
-// matrices for all.  In products over the values a lane holds rows of tokens (A) and columns of
-// keys (B); the results, tokens 4g + i of key lane & 15, are where the gradients are formed.
-template <int DT, int YDT>
-__global__ __launch_bounds__(256) void wkv7_grads_kernel(WkvGrads p) {
-    constexpr bool HALF = DT != RQ_F32, V_EXACT = DT == RQ_BF16, DY_EXACT = YDT == RQ_BF16;
-    constexpr uint32_t SIZE = DT == RQ_F32 ? 4 : 2, YSIZE = YDT == RQ_F32 ? 4 : 2;
-    __shared__ GradLds lds;
-    const int lane = threadIdx.x & 63, wave = wave_index();
-    const int g = lane >> 4, m = lane & 15;
-    const uint32_t heads = (uint32_t)p.shape.heads, head = blockIdx.x % heads, chunk = blockIdx.x / heads;
-    Span span;
-    if (p.shape.cu) {  // the last sequence that begins at this chunk or before
-        int64_t lo = 0, hi = p.shape.seqs;
-        while (hi - lo > 1) {
-            const int64_t mid = (lo + hi) / 2;
-            if (boundary(p.shape, mid) / kChunk + mid <= chunk) lo = mid;
-            else hi = mid;
-        }
-        span = span_of(p.shape, lo);
-    } else {
-        span = span_of(p.shape, chunk / (uint32_t)((p.shape.time + kChunk - 1) / kChunk));
-    }
-    const int64_t c = (int64_t)chunk - span.chunk0;
-    if (c < 0 || c >= span.chunks()) return;
-    const int64_t t0 = kChunk * c;
-    const int tokens = (int)std::min<int64_t>(kChunk, span.len - t0);
-    const int64_t first = ((span.start + t0) * heads + head) * kHead;  // the chunk's first element
-    const uint32_t stride = heads * kHead;                             // from token to token
-    const auto of_chunk = [&](const void* q, uint32_t size) { return (const uint8_t*)q + first * size; };
-
-    // rows of tokens: dy, dz, sa, v of token m, values 16q + 4g + i.  A load under a condition would be waited for
-    // where the condition ends: tokens that are not there load the first.
-    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-    const uint32_t row = (m < tokens ? m : 0) * stride + 4 * g;
-    f32x4_t dy[4], dz[4], sa[4], v[4];
-    const uint8_t* const dz_at = (const uint8_t*)(p.dz + (int64_t)blockIdx.x * kChunk * kHead);
-    const uint8_t* const sa_at = (const uint8_t*)(p.sa + (int64_t)blockIdx.x * kChunk * kHead);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        dy[q] = load4<YDT>(of_chunk(p.dy, YSIZE), (row + 16 * q) * YSIZE);
-        v[q] = load4<DT>(of_chunk(p.in.v, SIZE), (row + 16 * q) * SIZE);
-        dz[q] = load4<RQ_F32>(dz_at, (m * kHead + 16 * q + 4 * g) * 4);
-        sa[q] = load4<RQ_F32>(sa_at, (m * kHead + 16 * q + 4 * g) * 4);
-    }
-    const int key = 16 * wave + m;
-    // columns of keys: S and dS' of values 16q + 4g + i
-    f32x4_t s[4], d[4];
-    const uint32_t column = (4 * g * kHead + key) * 4;
-    const uint8_t* const s_at = (const uint8_t*)(p.states + (int64_t)blockIdx.x * kHead * kHead);
-    const uint8_t* const d_at = (const uint8_t*)(p.dstates + (int64_t)blockIdx.x * kHead * kHead);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[q][i] = *(const float*)(s_at + 16 * q * kHead * 4 + (column + i * kHead * 4));
-            d[q][i] = *(const float*)(d_at + 16 * q * kHead * 4 + (column + i * kHead * 4));
-        }
-    }
-    // this wave's tensors: tokens 4g + i of its key
-    float r[4], a[4], b[4], k[4], g2[4], l[4];
-    uint32_t at[4];
-    {
-        typename dt_traits<DT>::storage raw[5][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            at[i] = ((4 * g + i < tokens ? 4 * g + i : 0) * stride + key) * SIZE;
-            raw[0][i] = load1<DT>(of_chunk(p.in.w, SIZE), at[i]);
-            raw[1][i] = load1<DT>(of_chunk(p.in.r, SIZE), at[i]);
-            raw[2][i] = load1<DT>(of_chunk(p.in.a, SIZE), at[i]);
-            raw[3][i] = load1<DT>(of_chunk(p.in.b, SIZE), at[i]);
-            raw[4][i] = load1<DT>(of_chunk(p.in.k, SIZE), at[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool has = 4 * g + i < tokens;
-            g2[i] = has ? log2_decay(dt_traits<DT>::to_f32(raw[0][i])) : 0.f;
-            r[i] = has ? dt_traits<DT>::to_f32(raw[1][i]) : 0.f;
-            a[i] = has ? dt_traits<DT>::to_f32(raw[2][i]) : 0.f;
-            b[i] = has ? dt_traits<DT>::to_f32(raw[3][i]) : 0.f;
-            k[i] = has ? dt_traits<DT>::to_f32(raw[4][i]) : 0.f;
-            l[i] = i ? l[i - 1] + g2[i] : g2[i];
-        }
-    }
-    const float off = groups_before(l[3], g);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) l[i] += off;
-    const float end = __shfl(l[3], 48 + m);
-    const bool strong = __any(!(end >= kStrong));
-    if (m >= tokens) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) dy[q] = v[q] = zero;
-    }
-    f32x4_t gr = zero, ga = zero, gb = zero, gk = zero;
-    float through = 0.f;  // sum over the values of S dS' of this key
-    {
-        const Operand<HALF, 64> dy_o(dy), v_o(v), dz_o(dz), sa_o(sa);
-        // the wave's pair matrix
-        f32x4_t pm = zero;
-        if (wave == 0) pm = mma(sa_o, dz_o, pm);
-        if (wave == 1) pm = mma<V_EXACT, false>(v_o, dz_o, pm);
-        if (wave == 2) pm = mma<false, DY_EXACT>(sa_o, dy_o, pm);
-        if (wave == 3) pm = mma<V_EXACT, DY_EXACT>(v_o, dy_o, pm);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int t = 4 * g + i;
-            lds.m[wave][t][m] = pack_pair<HALF>(t < m ? pm[i] : 0.f);
-            if (wave >= 2 && t == m) lds.own[wave - 2][m] = pm[i];
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) through = fmaf(s[q][i], d[q][i], through);
-        const Operand<HALF, 64> s_o(s), d_o(d);
-        gr = mma<DY_EXACT, false>(dy_o, s_o, gr);
-        ga = mma(dz_o, s_o, ga);
-        gb = mma(sa_o, d_o, gb);
-        gk = mma<V_EXACT, false>(v_o, d_o, gk);
-    }
-    through = over_groups(through);
-    if (strong) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            auto& in = lds.strong[wave];
-            in[0][4 * g + i][m] = r[i];
-            in[1][4 * g + i][m] = a[i];
-            in[2][4 * g + i][m] = b[i];
-            in[3][4 * g + i][m] = k[i];
-            in[4][4 * g + i][m] = g2[i];
-        }
-    }
-    __syncthreads();
-    f32x4_t to_end, el, ex;  // e^(Lend - L), e^L, e^Lx
-    {
-        float after = groups_after((g2[0] + g2[1]) + (g2[2] + g2[3]), g);
-        float prev = off;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            el[i] = exp2_hw(l[i]);
-            ex[i] = i ? el[i - 1] : exp2_hw(prev);
-        }
-#pragma unroll
-        for (int i = 3; i >= 0; --i) {
-            to_end[i] = exp2_hw(after);
-            after += g2[i];
-        }
-    }
-    float enters[4], leaves_r[4], leaves_a[4];  // what each token adds to, and takes from, the state
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        gb[i] *= to_end[i];
-        gk[i] *= to_end[i];
-        gr[i] *= el[i];
-        ga[i] *= ex[i];
-        enters[i] = b[i] * gb[i] + k[i] * gk[i];
-        leaves_r[i] = r[i] * gr[i];
-        leaves_a[i] = a[i] * ga[i];
-    }
-    float cross[4];
-    if (strong) {
-        float pr[4], pa[4], pb[4], pk[4], pc[4];
-        strong_grads<HALF>(lds, wave, lane, pr, pa, pb, pk, pc);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            gr[i] += pr[i];
-            ga[i] += pa[i];
-            gb[i] += pb[i];
-            gk[i] += pk[i];
-            cross[i] = pc[i];
-        }
-    } else {
-        f32x4_t late[2], early[2], il, pr = zero, pa = zero, pb = zero, pk = zero;  // A~, R~ and B~, K~
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            il[i] = exp2_hw(-l[i]);
-            late[0][i] = a[i] * ex[i];
-            late[1][i] = r[i] * el[i];
-            early[0][i] = b[i] * il[i];
-            early[1][i] = k[i] * il[i];
-        }
-        const Operand<HALF, 32> late_o(late), early_o(early);
-        uint32_t by_t[4][4], by_s[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                by_s[j][i] = lds.m[j][m][4 * g + i];
-                by_t[j][i] = lds.m[j][4 * g + i][m];
-            }
-        }
-        pa = mma(pair_operand<HALF>(by_t[0], by_t[1]), early_o, pa);
-        pr = mma(pair_operand<HALF>(by_t[2], by_t[3]), early_o, pr);
-        pb = mma(pair_operand<HALF>(by_s[0], by_s[2]), late_o, pb);
-        pk = mma(pair_operand<HALF>(by_s[1], by_s[3]), late_o, pk);
-        // a pair (s, t) passes the decays behind s up to t (before t, for a): sums of what ends
-        // minus what begins at each token and behind it
-        float q[4], qa[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            pr[i] *= el[i];
-            pa[i] *= ex[i];
-            pb[i] *= il[i];
-            pk[i] *= il[i];
-            q[i] = r[i] * pr[i] - b[i] * pb[i] - k[i] * pk[i];
-            qa[i] = a[i] * pa[i];
-            gr[i] += pr[i];
-            ga[i] += pa[i];
-            gb[i] += pb[i];
-            gk[i] += pk[i];
-        }
-        float sum = groups_after((q[0] + qa[0]) + (q[1] + qa[1]) + (q[2] + qa[2]) + (q[3] + qa[3]), g);
-#pragma unroll
-        for (int i = 3; i >= 0; --i) {
-            cross[i] = sum + q[i];
-            sum += q[i] + qa[i];
-        }
-    }
-    // a token's own pair passes no decay: kept out of the sums above, where it would cancel
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float ob = lds.own[0][4 * g + i], ok = lds.own[1][4 * g + i];
-        gr[i] += ob * b[i] + ok * k[i];
-        gb[i] += ob * r[i];
-        gk[i] += ok * r[i];
-    }
-    // the state's own way through the chunk, what entered before and what leaves at or behind
-    const float whole = exp2_hw(end) * through;
-    float into = groups_before((enters[0] + enters[1]) + (enters[2] + enters[3]), g);
-    float out_of = groups_after((leaves_r[0] + leaves_a[0]) + (leaves_r[1] + leaves_a[1]) +
-                                    (leaves_r[2] + leaves_a[2]) + (leaves_r[3] + leaves_a[3]), g);
-    float gw[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        gw[i] = cross[i] + whole + into;
-        into += enters[i];
-    }
-#pragma unroll
-    for (int i = 3; i >= 0; --i) {
-        gw[i] += out_of + leaves_r[i];
-        out_of += leaves_r[i] + leaves_a[i];
-        // d log d / dw = -exp(w), inf where the decay, and with it what passes it, is 0
-        gw[i] = gw[i] == 0.f ? 0.f : gw[i] * (g2[i] * kLn2);
-    }
-    const auto to_chunk = [&](void* q) { return (uint8_t*)q + first * SIZE; };
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (4 * g + i >= tokens) continue;
-        if (p.dr) store1<DT>(to_chunk(p.dr), at[i], gr[i]);
-        if (p.dw) store1<DT>(to_chunk(p.dw), at[i], gw[i]);
-        if (p.dk) store1<DT>(to_chunk(p.dk), at[i], gk[i]);
-        if (p.da) store1<DT>(to_chunk(p.da), at[i], ga[i]);
-        if (p.db) store1<DT>(to_chunk(p.db), at[i], gb[i]);
     }
 }
 
@@ -1141,12 +1097,12 @@ hipError_t scan_all(const WkvScan& a, hipStream_t s) {
     const int64_t heads = a.shape.heads;
     if (a.seg.chunks) {
         const dim3 grid((unsigned)(a.seg.slots * heads));
-        wkv7_scan_kernel<DT, XDT, YDT, REV, true><<<grid, kScanThreads<true>, 0, s>>>(a);
+        wkv7_scan_kernel<DT, XDT, YDT, REV, true><<<grid, kScanThreads<REV, true>, 0, s>>>(a);
         wkv7_join_kernel<<<dim3((unsigned)(4 * a.shape.seqs * heads)), 256, 0, s>>>(a.shape, a.seg, a.state);
-        wkv7_scan_kernel<DT, XDT, YDT, REV, false><<<grid, kScanThreads<false>, 0, s>>>(a);
+        wkv7_scan_kernel<DT, XDT, YDT, REV, false><<<grid, kScanThreads<REV, false>, 0, s>>>(a);
     } else {
         wkv7_scan_kernel<DT, XDT, YDT, REV, false>
-            <<<dim3((unsigned)(a.shape.seqs * heads)), kScanThreads<false>, 0, s>>>(a);
+            <<<dim3((unsigned)(a.shape.seqs * heads)), kScanThreads<REV, false>, 0, s>>>(a);
     }
     return hipGetLastError();
 }
@@ -1154,12 +1110,6 @@ hipError_t scan_all(const WkvScan& a, hipStream_t s) {
 template <int DT, int ODT>
 hipError_t scan_dt(const WkvScan& a, hipStream_t s) {
     return a.reverse ? scan_all<DT, ODT, DT, true>(a, s) : scan_all<DT, DT, ODT, false>(a, s);
-}
-
-template <int DT, int ODT>
-hipError_t grads_dt(const WkvGrads& a, hipStream_t s) {
-    wkv7_grads_kernel<DT, ODT><<<dim3((unsigned)(wkv_chunks(a.shape) * a.shape.heads)), 256, 0, s>>>(a);
-    return hipGetLastError();
 }
 
 template <int DT, int ODT>
@@ -1181,8 +1131,6 @@ namespace rq {
 hipError_t launch_wkv_scan(const WkvScan& a, hipStream_t s) {
     RQ_BY_TYPES(scan_dt, a.in.dt, (a.reverse ? a.x_dt : a.y_dt), a, s)
 }
-
-hipError_t launch_wkv_grads(const WkvGrads& a, hipStream_t s) { RQ_BY_TYPES(grads_dt, a.in.dt, a.dy_dt, a, s) }
 
 hipError_t launch_wkv_step(const WkvStep& a, hipStream_t s) { RQ_BY_TYPES(step_dt, a.in.dt, a.y_dt, a, s) }
 

@@ -36,7 +36,7 @@ def test_chunks_and_workspaces(L):
     assert L.rq_wkv7_chunks(2, 33, 4, 1) == -1 and L.rq_wkv7_chunks(2, 33, 3, 0) == -1
     assert L.rq_wkv7_chunks(-1, 33, -1, 0) == -1 and "negative" in err(L)
     assert L.rq_wkv7_chunks(0, 5, 0, 0) == 0
-    assert L.rq_wkv7_backward_workspace_bytes(1, 16, 2, 1, 0) >= 2 * 4 * (64 * 64 + 16 * 64)
+    assert L.rq_wkv7_backward_workspace_bytes(1, 16, 2, 1, 0) == 0
     assert L.rq_wkv7_backward_workspace_bytes(1, 2 ** 30, 64, 1, 0) == -1 and "heads of chunks" in err(L)
     # few heads over many tokens run in segments, which take room for 3 states each; many heads do not
     one = 3 * 4 * 64 * 64
@@ -79,9 +79,10 @@ def test_scan_refusals(L):
 
 
 def test_backward_refusals(L):
-    need = L.rq_wkv7_backward_workspace_bytes(1, 4, 2, 1, 0)
+    need = L.rq_wkv7_backward_workspace_bytes(1, 4000, 2, 1, 0)
+    assert need > 0
 
-    def bwd(x=P, dt=0, batch=1, time=4, heads=2, cu=0, seqs=1, st=P, sa=P, dy=P, ydt=0, dso=0, g=P, ds=0, ws=P, nb=need):
+    def bwd(x=P, dt=0, batch=1, time=4000, heads=2, cu=0, seqs=1, st=P, sa=P, dy=P, ydt=0, dso=0, g=P, ds=0, ws=P, nb=need):
         return L.rq_wkv7_backward(x, x, x, x, x, x, dt, batch, time, heads, cu, seqs, st, sa, dy, ydt, dso, g, g, g, g,
                                   g, g, ds, ws, nb, None)
 
