@@ -74,7 +74,7 @@ inline int64_t wkv_chunks(const WkvShape& s) {
 // The segments that take the least time by what was measured: a chunk of a block's scan takes kScanUs (kBackUs with
 // the gradients), one of a segment's end kEndsUs, and as much as two chunks to begin; a step from segment to segment
 // kJoinUs, the further launches kMoreUs.  A block has a CU to itself, and one block more than there are CUs is a
-// whole turn more: 12 heads of 8192 tokens took 93 us forwards in 264 blocks of 24 chunks, 67 us in 252 of 25.
+// whole turn more: 12 heads of 8192 tokens took 93 us forwards in 264 blocks of 24 chunks, 73 us in 252 of 25.
 inline WkvSegments wkv_segments(const WkvShape& s, bool backward) {
     constexpr double kScanUs = 2.4, kBackUs = 7, kEndsUs = 2.7, kJoinUs = 0.8, kMoreUs = 12;
     constexpr int64_t kCus = 256, kBegin = 2;

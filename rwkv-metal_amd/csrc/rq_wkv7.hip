@@ -775,9 +775,9 @@ RQ_DEV bool unused(const Segment& s) { return s.index < 0 || (s.index > 0 && s.f
 // Backwards (GRADS) the scan waves also form the other gradients of their chunk, from its dS' and dZ in LDS, with
 // what else they need on its way from memory while they scan.  That takes more than the 168 registers of twelve
 // waves: there are eight, four for the arrays and the matrices, and a second barrier between scan and gradients.
-// Four waves of their own for chunk c - 1 (one barrier, a load's whole wait in each turn) took 8.7 us a chunk
-// against 6.7; a kernel of its own behind the scan, its dS' and dZ through memory, 145 + 100 us for 4096 tokens
-// of 32 heads against 220.
+// Four waves of their own for chunk c - 1 (one barrier, but a load's whole wait in each turn) took 8.9 us a chunk
+// against 7.4; a kernel of its own behind the scan, dS' and dZ through memory, 145 + 100 us for 8 x 512 tokens
+// of 32 heads against 238.
 template <bool REV, bool ENDS>
 constexpr int kScanThreads = (ENDS ? 16 : REV ? 8 : 12) * 64;
 
