@@ -169,9 +169,14 @@ struct ScanLds {
     Rows y[2];
     int strong[3][4];    // whether a wave's channels hold strong decays
 };
+// For the gradients of a chunk; rows of tokens are [15 - token].
+struct GradRows {
+    Rows d[4];   // dS', [value / 16][value % 16][key]
+    Rows dz, v, sa;
+    Rows io[5];  // log2 d, r, a, b and k; then, each in its place, dw, dr, da, db and dk
+};
 struct ScanGradLds : ScanLds {
-    Rows d[4];  // dS' of a chunk, [value / 16][value % 16][key]
-    Rows dz;    // dZ, [15 - token][value]
+    GradRows grads;
 };
 
 // X^T of X = (1 - M)^-1 from m[i] = M^T[4g + i][lane & 15], nonzero above the diagonal:
@@ -408,15 +413,22 @@ RQ_DEV float over_groups(float x) {
 struct Halves {
     bf16x8_t hi, lo;
 };
+RQ_DEV uint32_t two_bf16(float a, float b) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, pair{(__bf16)a, (__bf16)b});
+}
 RQ_DEV Halves halves_of(const f32x4_t& x, const f32x4_t& y) {
     Halves h;
+    uint32_t hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        h.hi[i] = (__bf16)x[i];
-        h.hi[4 + i] = (__bf16)y[i];
-        h.lo[i] = (__bf16)(x[i] - (float)h.hi[i]);
-        h.lo[4 + i] = (__bf16)(y[i] - (float)h.hi[4 + i]);
+        const float a = i < 2 ? x[2 * i] : y[2 * i - 4], b = i < 2 ? x[2 * i + 1] : y[2 * i - 3];
+        hi[i] = two_bf16(a, b);
+        lo[i] = two_bf16(a - __uint_as_float(hi[i] << 16), b - __uint_as_float(hi[i] & 0xffff0000u));
     }
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    h.hi = __builtin_bit_cast(bf16x8_t, u32x4{hi[0], hi[1], hi[2], hi[3]});
+    h.lo = __builtin_bit_cast(bf16x8_t, u32x4{lo[0], lo[1], lo[2], lo[3]});
     return h;
 }
 // EXACT: an operand that is bf16 as it is (its lo is 0)
@@ -447,26 +459,6 @@ struct Operand<true, N> {
     RQ_DEV Operand(f32x4_t x0, f32x4_t x1) : v{halves_of(x0, x1)} {}
 };
 
-// Of rows as they are stored: bf16 ones are their own high halves.  0 where the token is not there.
-template <bool HALF, int DT>
-RQ_DEV Operand<HALF, 64> row_operand(const Raw4<DT>* raw, bool there) {
-    if constexpr (HALF && DT == RQ_BF16) {
-        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-        const f32x4_t zero[4] = {};
-        Operand<true, 64> o(zero);
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const u32x4 u = {raw[2 * q].v[0], raw[2 * q].v[1], raw[2 * q + 1].v[0], raw[2 * q + 1].v[1]};
-            o.v[q].hi = __builtin_bit_cast(bf16x8_t, there ? u : u32x4{0, 0, 0, 0});
-        }
-        return o;
-    } else {
-        f32x4_t x[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) x[q] = there ? unpack_raw4<DT>(raw[q]) : f32x4_t{0.f, 0.f, 0.f, 0.f};
-        return Operand<HALF, 64>(x);
-    }
-}
 // Half h of an operand of 64.
 template <bool HALF>
 RQ_DEV Operand<HALF, 32> half_of(const Operand<HALF, 64>& x, int h) {
@@ -509,73 +501,26 @@ RQ_DEV float at_token(const f32x4_t& x, int t, int m) {
     return __shfl(own, 16 * (t >> 2) + m);
 }
 
-// A chunk's dr, dw, dk, da and db for the 16 keys of a wave.  In products over the values a lane holds rows
-// of tokens (A) and columns of keys (B); the results, tokens 4g + i of key lane & 15, are where the gradients are
-// formed.  Each wave forms the four pair matrices for itself, and their transposes: no wave waits for another.
-// `d` is dS' [value][key], `dz` dZ [15 - token][value].
+// A chunk's dr, dw, dk, da and db for the 16 keys of a wave, s[q][i] = S[value 16q + 4g + i][key].  In products over the
+// values a lane holds rows of tokens (A) and columns of keys (B); the results, tokens 4g + i of key lane & 15, are
+// where the gradients are formed.  Each wave forms the four pair matrices for itself, and their transposes: no wave
+// waits for another.
 template <int DT, int YDT>
-struct ChunkGrads {
-    static constexpr bool HALF = DT != RQ_F32, V_EXACT = DT == RQ_BF16, DY_EXACT = YDT == RQ_BF16;
-    static constexpr uint32_t SIZE = DT == RQ_F32 ? 4 : 2, YSIZE = YDT == RQ_F32 ? 4 : 2;
-    // of the chunk: its first element, its tokens; of the lane's tokens 4g + i
-    int64_t first;
-    int tokens;
-    uint32_t at[4];
-    typename dt_traits<DT>::storage raw[5][4];
-    Raw4<YDT> raw_dy[4];
-    Raw4<DT> raw_v[4];
-    f32x4_t sa[4], s[4];
-
-    RQ_DEV void load(const WkvScan& p, int64_t first_, int64_t chunk, int tokens_, int lane, int wave) {
-        const int g = lane >> 4, m = lane & 15, key = 16 * wave + m;
-        const uint32_t stride = (uint32_t)p.shape.heads * kHead;  // from token to token
-        first = first_;
-        tokens = tokens_;
-        const auto of_chunk = [&](const void* q, uint32_t size) { return (const uint8_t*)q + first * size; };
-        // a load under a condition would be waited for where the condition ends: tokens that are not there
-        // load the first
-        // The lane's offsets in 32 bits behind scalar pointers, made anew for each chunk: hoisted out of the loop over
-        // the chunks as 64-bit addresses they took 63 registers too many.
-        uint32_t row = (m < tokens ? m : 0) * stride + 4 * g, column = (4 * g * kHead + key) * 4, line = (m * kHead + 4 * g) * 4;
-        asm volatile("" : "+v"(row), "+v"(column), "+v"(line));
-        const uint8_t* const s_at = (const uint8_t*)(p.grads.states + chunk * kHead * kHead);
-        const uint8_t* const sa_at = (const uint8_t*)(p.grads.sa + chunk * kChunk * kHead);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            at[i] = ((4 * g + i < tokens ? 4 * g + i : 0) * stride + key) * SIZE;
-            asm volatile("" : "+v"(at[i]));
-            raw[0][i] = load1<DT>(of_chunk(p.in.w, SIZE), at[i]);
-            raw[1][i] = load1<DT>(of_chunk(p.in.r, SIZE), at[i]);
-            raw[2][i] = load1<DT>(of_chunk(p.in.a, SIZE), at[i]);
-            raw[3][i] = load1<DT>(of_chunk(p.in.b, SIZE), at[i]);
-            raw[4][i] = load1<DT>(of_chunk(p.in.k, SIZE), at[i]);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[q][i] = *(const float*)(s_at + 16 * q * kHead * 4 + (column + i * kHead * 4));
-            raw_dy[q] = *(const Raw4<YDT>*)(of_chunk(p.x, YSIZE) + (row + 16 * q) * YSIZE);
-            raw_v[q] = *(const Raw4<DT>*)(of_chunk(p.in.v, SIZE) + (row + 16 * q) * SIZE);
-            sa[q] = *(const f32x4_t*)(sa_at + (line + 16 * q * 4));
-        }
-    }
-    RQ_DEV void run(const WkvScan& p, const Rows* d_rows, const Rows& dz_rows, int lane, int wave) const;
-};
-
-template <int DT, int YDT>
-RQ_DEV void ChunkGrads<DT, YDT>::run(const WkvScan& p, const Rows* d_rows, const Rows& dz_rows, int lane, int wave) const {
+RQ_DEV void chunk_grads(const f32x4_t* s, const Rows& dy_rows, GradRows& lds, int lane, int wave) {
+    constexpr bool HALF = DT != RQ_F32, V_EXACT = DT == RQ_BF16, DY_EXACT = YDT == RQ_BF16;
     const int g = lane >> 4, m = lane & 15, key = 16 * wave + m;
     const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
     f32x4_t gr = zero, ga = zero, gb = zero, gk = zero;
     float through = 0.f;  // sum over the values of S dS' of this key
     f32x4_t by_t[4], by_s[4];  // dMab, dMak, dMrb, dMrk
     {
-        const Operand<HALF, 64> dy_o = row_operand<HALF>(raw_dy, m < tokens), v_o = row_operand<HALF>(raw_v, m < tokens),
-                                sa_o(sa);
-        f32x4_t dz[4];
+        const auto rows = [&](const Rows& from) {
+            f32x4_t x[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) dz[q] = *(const f32x4_t*)&dz_rows[kChunk - 1 - m][16 * q + 4 * g];
-        const Operand<HALF, 64> dz_o(dz);
+            for (int q = 0; q < 4; ++q) x[q] = *(const f32x4_t*)&from[kChunk - 1 - m][16 * q + 4 * g];
+            return Operand<HALF, 64>(x);
+        };
+        const Operand<HALF, 64> dy_o = rows(dy_rows), v_o = rows(lds.v), sa_o = rows(lds.sa), dz_o = rows(lds.dz);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             f32x4_t d[2];
@@ -583,7 +528,7 @@ RQ_DEV void ChunkGrads<DT, YDT>::run(const WkvScan& p, const Rows* d_rows, const
             for (int q = 0; q < 2; ++q) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    d[q][i] = d_rows[2 * h + q][4 * g + i][key];
+                    d[q][i] = lds.d[2 * h + q][4 * g + i][key];
                     through = fmaf(s[2 * h + q][i], d[q][i], through);
                 }
             }
@@ -602,15 +547,15 @@ RQ_DEV void ChunkGrads<DT, YDT>::run(const WkvScan& p, const Rows* d_rows, const
         by_s[2] = mma<DY_EXACT, false>(dy_o, sa_o, zero);
         by_s[3] = mma<DY_EXACT, V_EXACT>(dy_o, v_o, zero);
     }
-    f32x4_t r, a, b, k, g2, l;
+    f32x4_t g2, r, a, b, k, l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const bool has = 4 * g + i < tokens;
-        g2[i] = has ? log2_decay(dt_traits<DT>::to_f32(raw[0][i])) : 0.f;
-        r[i] = has ? dt_traits<DT>::to_f32(raw[1][i]) : 0.f;
-        a[i] = has ? dt_traits<DT>::to_f32(raw[2][i]) : 0.f;
-        b[i] = has ? dt_traits<DT>::to_f32(raw[3][i]) : 0.f;
-        k[i] = has ? dt_traits<DT>::to_f32(raw[4][i]) : 0.f;
+        const int at = kChunk - 1 - (4 * g + i);
+        g2[i] = lds.io[0][at][key];
+        r[i] = lds.io[1][at][key];
+        a[i] = lds.io[2][at][key];
+        b[i] = lds.io[3][at][key];
+        k[i] = lds.io[4][at][key];
         l[i] = i ? l[i - 1] + g2[i] : g2[i];
     }
     const float off = groups_before(l[3], g);
@@ -717,16 +662,62 @@ RQ_DEV void ChunkGrads<DT, YDT>::run(const WkvScan& p, const Rows* d_rows, const
         // d log d / dw = -exp(w), inf where the decay, and with it what passes it, is 0
         gw[i] = gw[i] == 0.f ? 0.f : gw[i] * (g2[i] * kLn2);
     }
-    const auto to_chunk = [&](void* q) { return (uint8_t*)q + first * SIZE; };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if (4 * g + i >= tokens) continue;
-        if (p.grads.dr) store1<DT>(to_chunk(p.grads.dr), at[i], gr[i]);
-        if (p.grads.dw) store1<DT>(to_chunk(p.grads.dw), at[i], gw[i]);
-        if (p.grads.dk) store1<DT>(to_chunk(p.grads.dk), at[i], gk[i]);
-        if (p.grads.da) store1<DT>(to_chunk(p.grads.da), at[i], ga[i]);
-        if (p.grads.db) store1<DT>(to_chunk(p.grads.db), at[i], gb[i]);
+        const int at = kChunk - 1 - (4 * g + i);
+        lds.io[0][at][key] = gw[i];
+        lds.io[1][at][key] = gr[i];
+        lds.io[2][at][key] = ga[i];
+        lds.io[3][at][key] = gb[i];
+        lds.io[4][at][key] = gk[i];
     }
+}
+
+// A producer wave's share of what the gradients of a chunk read and give: 16 channels of its 16 tokens, as in
+// Elementwise.
+template <int DT>
+struct GradTensors {
+    bool there;
+    Raw4<DT> w, r, a, b, k, v;
+    f32x4_t sa;
+
+    // `sa_row`: of the lane's token, which is there also for tokens that are not
+    RQ_DEV void load(const WkvScan& p, int64_t row, bool exists, int64_t sa_row, int lane, int wave) {
+        there = exists;
+        const int c = 16 * wave + 4 * (lane >> 4);
+        const int64_t at = row * kHead + c;
+        w = load_raw4<DT>(p.in.w, at);
+        r = load_raw4<DT>(p.in.r, at);
+        a = load_raw4<DT>(p.in.a, at);
+        b = load_raw4<DT>(p.in.b, at);
+        k = load_raw4<DT>(p.in.k, at);
+        v = load_raw4<DT>(p.in.v, at);
+        sa = *(const f32x4_t*)(p.grads.sa + sa_row * kHead + c);
+    }
+    RQ_DEV void put(GradRows& lds, int lane, int wave) const {
+        const int m = lane & 15, c = 16 * wave + 4 * (lane >> 4);
+        const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+        f32x4_t g2 = unpack_raw4<DT>(w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g2[i] = there ? log2_decay(g2[i]) : 0.f;
+        *(f32x4_t*)&lds.io[0][m][c] = g2;
+        *(f32x4_t*)&lds.io[1][m][c] = there ? unpack_raw4<DT>(r) : zero;
+        *(f32x4_t*)&lds.io[2][m][c] = there ? unpack_raw4<DT>(a) : zero;
+        *(f32x4_t*)&lds.io[3][m][c] = there ? unpack_raw4<DT>(b) : zero;
+        *(f32x4_t*)&lds.io[4][m][c] = there ? unpack_raw4<DT>(k) : zero;
+        *(f32x4_t*)&lds.v[m][c] = there ? unpack_raw4<DT>(v) : zero;
+        *(f32x4_t*)&lds.sa[m][c] = sa;
+    }
+};
+template <int DT>
+RQ_DEV void store_grads(const WkvGrads& to, const GradRows& lds, int64_t row, int lane, int wave) {
+    const int m = lane & 15, c = 16 * wave + 4 * (lane >> 4);
+    const int64_t at = row * kHead + c;
+    if (to.dw) store4<DT>(to.dw, at, *(const f32x4_t*)&lds.io[0][m][c]);
+    if (to.dr) store4<DT>(to.dr, at, *(const f32x4_t*)&lds.io[1][m][c]);
+    if (to.da) store4<DT>(to.da, at, *(const f32x4_t*)&lds.io[2][m][c]);
+    if (to.db) store4<DT>(to.db, at, *(const f32x4_t*)&lds.io[3][m][c]);
+    if (to.dk) store4<DT>(to.dk, at, *(const f32x4_t*)&lds.io[4][m][c]);
 }
 
 // ------------------------------------------------------------------ the scan
@@ -772,12 +763,13 @@ RQ_DEV bool unused(const Segment& s) { return s.index < 0 || (s.index > 0 && s.f
 //
 // ENDS: only where a segment ends, from a state of 0 (four scan waves) and, without x, from the identity (four more).
 //
-// Backwards (GRADS) the scan waves also form the other gradients of their chunk, from its dS' and dZ in LDS, with
-// what else they need on its way from memory while they scan.  That takes more than the 168 registers of twelve
-// waves: there are eight, four for the arrays and the matrices, and a second barrier between scan and gradients.
-// Four waves of their own for chunk c - 1 (one barrier, but a load's whole wait in each turn) took 8.9 us a chunk
-// against 7.4; a kernel of its own behind the scan, dS' and dZ through memory, 145 + 100 us for 8 x 512 tokens
-// of 32 heads against 238.
+// Backwards (GRADS) the scan waves also form the other gradients of their chunk, from its dS' and dZ in LDS.  That takes more
+// than the 168 registers of twelve waves: there are eight, four for the arrays and the matrices, and a second barrier
+// between scan and gradients.  The first four have time left: what the gradients need but the state, and the
+// gradients on their way to memory, pass through them and LDS, in whole rows; by the scan waves' own loads and stores of single
+// 16-bit numbers a chunk took 7.4 us against 6.4.  Four waves of their own for chunk c - 1, with these loads, took
+// 8.9 us; a kernel of its own behind the scan, dS' and dZ through memory, 145 + 100 us for 8 x 512 tokens of 32 heads
+// against 205.
 template <bool REV, bool ENDS>
 constexpr int kScanThreads = (ENDS ? 16 : REV ? 8 : 12) * 64;
 
@@ -818,7 +810,19 @@ __global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(Wk
             const int at = 16 * wave + 4 * g;
             store4<YDT>(p.y, row(c) * kHead + at, *(const f32x4_t*)&lds.y[odd(c)][m][at]);
         };
+        GradTensors<DT> of_grads;
+        const auto load_of_grads = [&](int64_t c) {
+            if (c < end)
+                of_grads.load(p, row(c), exists(c),
+                              ((span.chunk0 + n - 1 - c) * H + head) * kChunk + (kChunk - 1 - m), lane, wave);
+        };
+        const auto store_of_grads = [&](int64_t c) {
+            if constexpr (GRADS) {
+                if (c >= first && exists(c)) store_grads<DT>(p.grads, lds.grads, row(c), lane, wave);
+            }
+        };
         load(first);
+        if (GRADS) load_of_grads(first);
         arrays(first, 0);
         load(first + 1);
         __syncthreads();
@@ -828,6 +832,11 @@ __global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(Wk
         __syncthreads();
         int next = 1, ring = 2;  // of chunks c + 1 and c + 2
         for (int64_t c = first; c < end; ++c) {
+            if constexpr (GRADS) {
+                store_of_grads(c - 1);
+                of_grads.put(lds.grads, lane, wave);
+                load_of_grads(c + 1);
+            }
             arrays(c + 2, ring);
             if (!GRADS) store_y(c - 1);
             load(c + 3);
@@ -840,7 +849,8 @@ __global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(Wk
             next = ring;
             ring = ring == 2 ? 0 : ring + 1;
         }
-        if (!GRADS) store_y(end - 1);
+        if (GRADS) store_of_grads(end - 1);
+        else store_y(end - 1);
         return;
     }
     if (!GRADS && wave < 8) {
@@ -881,13 +891,17 @@ __global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(Wk
         const Matrices& mat = lds.matrices[odd(c)];
         ring = ring == 2 ? 0 : ring + 1;
         const int64_t chunk = (span.chunk0 + (REV ? n - 1 - c : c)) * H + head;
-        ChunkGrads<DT, XDT> grads;
+        f32x4_t s[4];  // of the gradients: keys 16 (wave & 3) + m
         if constexpr (GRADS) {
-            const int64_t t0 = kChunk * (n - 1 - c);
-            grads.load(p, ((span.start + t0) * H + head) * kHead, chunk, (int)std::min<int64_t>(kChunk, span.len - t0), lane,
-                       wave & 3);
+            const float* from = p.grads.states + chunk * kHead * kHead;
+            uint32_t at = 4 * g * kHead + value;
+            asm volatile("" : "+v"(at));  // 32 bits behind a scalar pointer; hoisted as 64-bit addresses they took too many registers
 #pragma unroll
-            for (int q = 0; q < 4; ++q) *(f32x4_t*)&lds.d[wave & 3][m][16 * q + 4 * g] = acc[q];
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[q][i] = from[at + (16 * q + i) * kHead];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *(f32x4_t*)&lds.grads.d[wave & 3][m][16 * q + 4 * g] = acc[q];
         }
         if (!ENDS && !REV && p.states) {
             float* to = p.states + (chunk * kHead + value) * kHead + 4 * g;
@@ -942,7 +956,7 @@ __global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(Wk
             for (int i = 0; i < 4; ++i) lds.y[odd(c)][4 * g + i][value] = y[0][i] + y[1][i];
             if constexpr (GRADS) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) lds.dz[4 * g + i][value] = sa[i];
+                for (int i = 0; i < 4; ++i) lds.grads.dz[4 * g + i][value] = sa[i];
             }
             if (!REV && p.sa) {  // 0 for tokens that are not there
 #pragma unroll
@@ -951,7 +965,7 @@ __global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(Wk
         }
         __syncthreads();
         if constexpr (GRADS) {
-            grads.run(p, lds.d, lds.dz, lane, wave & 3);
+            chunk_grads<DT, XDT>(s, b.x, lds.grads, lane, wave & 3);
             __syncthreads();
         }
     }
