@@ -108,16 +108,11 @@ int rq_wkv7(const void* r, const void* w, const void* k, const void* v, const vo
     const int64_t need = 4 * rq::wkv_segment_floats(seg, heads);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(RQ_EINVAL, "%s: needs a workspace of %lld bytes", what, (long long)need);
-    hipStream_t s = (hipStream_t)stream;
-    hipError_t e = hipSuccess;
-    if (cu_seqlens && time > 0) {
-        void* const rest[] = {y};
-        if (seqs == 0) return fail(RQ_EINVAL, "%s: tokens but no sequence", what);
-        e = rq::launch_wkv_rest(shape, y_dt, rest, 1, s);
-    }
-    if (e == hipSuccess && seqs > 0)
-        e = rq::launch_wkv_scan({shape, {r, w, k, v, a, b, dt}, false, v, dt, y, y_dt, state, state_out, states, sa, seg, {}}, s);
-    return rq::launch_status(e, what);
+    if (seqs == 0) return fail(RQ_EINVAL, "%s: tokens but no sequence", what);
+    return rq::launch_status(
+        rq::launch_wkv_scan({shape, {r, w, k, v, a, b, dt}, false, v, dt, y, y_dt, state, state_out, states, sa, seg, {}},
+                            (hipStream_t)stream),
+        what);
 }
 
 int64_t rq_wkv7_backward_workspace_bytes(int64_t batch, int64_t time, int64_t heads, int64_t seqs, int has_cu_seqlens) {
@@ -150,16 +145,11 @@ int rq_wkv7_backward(const void* r, const void* w, const void* k, const void* v,
     const int64_t need = 4 * rq::wkv_segment_floats(seg, heads);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(RQ_EINVAL, "%s: needs a workspace of %lld bytes", what, (long long)need);
-    hipStream_t s = (hipStream_t)stream;
-    hipError_t e = hipSuccess;
-    if (cu_seqlens && time > 0) {
-        void* const rest[] = {dr, dw, dk, dv, da, db};
-        e = rq::launch_wkv_rest(shape, dt, rest, 6, s);
-    }
-    if (e == hipSuccess && seqs > 0)
-        e = rq::launch_wkv_scan({shape, {r, w, k, v, a, b, dt}, true, dy, y_dt, dv, dt, dstate_out, dstate, nullptr, nullptr, seg,
-                                 {states, sa, dr, dw, dk, da, db}}, s);
-    return rq::launch_status(e, what);
+    return rq::launch_status(
+        rq::launch_wkv_scan({shape, {r, w, k, v, a, b, dt}, true, dy, y_dt, dv, dt, dstate_out, dstate, nullptr, nullptr, seg,
+                             {states, sa, dr, dw, dk, da, db}},
+                            (hipStream_t)stream),
+        what);
 }
 
 int rq_wkv7_step(const void* r, const void* w, const void* k, const void* v, const void* a, const void* b, rq_dtype dt,

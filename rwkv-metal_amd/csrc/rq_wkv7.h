@@ -39,7 +39,7 @@ struct WkvGrads {
     void *dr, *dw, *dk, *da, *db;
 };
 
-// One pass over the tokens, forwards or backwards in time.
+// One pass over the tokens, forwards or backwards in time.  Rows of a packed batch that belong to no sequence become 0.
 struct WkvScan {
     WkvShape shape;
     WkvInputs in;
@@ -114,7 +114,5 @@ inline int64_t wkv_segment_floats(const WkvSegments& g, int64_t heads) {
 
 hipError_t launch_wkv_scan(const WkvScan& a, hipStream_t stream);
 hipError_t launch_wkv_step(const WkvStep& a, hipStream_t stream);
-// 0 in the rows of a packed batch that belong to no sequence; NULL tensors are left out.
-hipError_t launch_wkv_rest(const WkvShape& s, int dt, void* const* tensors, int n, hipStream_t stream);
 
 }  // namespace rq

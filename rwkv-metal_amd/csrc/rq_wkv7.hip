@@ -30,6 +30,7 @@
 // e^(L_t - L_s), whose exponents are sums of the terms between s and t and never
 // positive; that also serves decays of 0.
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "rq_common.h"
@@ -755,6 +756,21 @@ RQ_DEV Segment segment_of(const WkvShape& s, const WkvSegments& g, int64_t slot,
 }
 RQ_DEV bool unused(const Segment& s) { return s.index < 0 || (s.index > 0 && s.first >= s.end); }
 
+// 0 in the tokens outside [cu[0], cu[seqs]): each block takes its share of them, without a launch of their own (3 us).
+template <int DT>
+RQ_DEV void clear_rest(const WkvShape& s, std::initializer_list<void*> tensors) {
+    const int64_t first = boundary(s, 0), last = boundary(s, s.seqs), behind = last > first ? last : first;
+    const int64_t rows = first + (s.time - behind), vecs = s.heads * kHead * (DT == RQ_F32 ? 4 : 2) / 16;
+    for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
+        const int64_t t = i < first ? i : behind + (i - first);
+        for (void* p : tensors) {
+            if (!p) continue;
+            uint4* at = (uint4*)p + t * vecs;
+            for (int64_t x = threadIdx.x; x < vecs; x += blockDim.x) at[x] = make_uint4(0, 0, 0, 0);
+        }
+    }
+}
+
 // Four waves form the arrays of chunk c + 2, load chunk c + 3 and store the y of chunk c - 1, four others form
 // the matrices of chunk c + 1, while four scan waves, each with 16 of the 64 values, take chunk c.  A scan wave
 // holds its state transposed, acc[q][i] = S[value lane & 15][key 16q + 4g + i]: the layout in which a product's
@@ -780,6 +796,10 @@ __global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(Wk
     const int lane = threadIdx.x & 63, wave = wave_index();
     const int g = lane >> 4, m = lane & 15;
     const int64_t H = p.shape.heads, slot = blockIdx.x / H, head = blockIdx.x % H;
+    if (!ENDS && p.shape.cu) {
+        if constexpr (GRADS) clear_rest<YDT>(p.shape, {p.grads.dr, p.grads.dw, p.grads.dk, p.y, p.grads.da, p.grads.db});
+        else clear_rest<YDT>(p.shape, {p.y});
+    }
     Span span;
     const Segment seg = segment_of(p.shape, p.seg, slot, span);
     if (unused(seg) || (ENDS && seg.last)) return;
@@ -1083,29 +1103,6 @@ __global__ __launch_bounds__(256) void wkv7_step_kernel(WkvStep p) {
     if (part == 0) store_dt(p.y, YDT, row * kHead + value, y);
 }
 
-// ------------------------------------------------- rows of no sequence
-
-struct RestTensors {
-    void* p[6];
-};
-
-// One block a token outside [cu[0], cu[seqs]), in grid-sized strides.
-template <int SIZE>
-__global__ __launch_bounds__(256) void wkv7_rest_kernel(WkvShape s, RestTensors to) {
-    const int64_t first = boundary(s, 0), last = boundary(s, s.seqs);
-    const int64_t behind = last > first ? last : first;
-    const int64_t rows = first + (s.time - behind), vecs = s.heads * kHead * SIZE / 16;
-    for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
-        const int64_t t = i < first ? i : behind + (i - first);
-#pragma unroll
-        for (int j = 0; j < 6; ++j) {
-            if (!to.p[j]) continue;
-            uint4* at = (uint4*)to.p[j] + t * vecs;
-            for (int64_t x = threadIdx.x; x < vecs; x += 256) at[x] = make_uint4(0, 0, 0, 0);
-        }
-    }
-}
-
 template <int DT, int XDT, int YDT, bool REV>
 hipError_t scan_all(const WkvScan& a, hipStream_t s) {
     const int64_t heads = a.shape.heads;
@@ -1147,14 +1144,5 @@ hipError_t launch_wkv_scan(const WkvScan& a, hipStream_t s) {
 }
 
 hipError_t launch_wkv_step(const WkvStep& a, hipStream_t s) { RQ_BY_TYPES(step_dt, a.in.dt, a.y_dt, a, s) }
-
-hipError_t launch_wkv_rest(const WkvShape& s, int dt, void* const* tensors, int n, hipStream_t stream) {
-    RestTensors to{};
-    for (int i = 0; i < n; ++i) to.p[i] = tensors[i];
-    const unsigned blocks = (unsigned)std::min<int64_t>(s.time, 1024);
-    if (dt == RQ_F32) wkv7_rest_kernel<4><<<dim3(blocks), 256, 0, stream>>>(s, to);
-    else wkv7_rest_kernel<2><<<dim3(blocks), 256, 0, stream>>>(s, to);
-    return hipGetLastError();
-}
 
 }  // namespace rq
