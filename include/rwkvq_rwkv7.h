@@ -34,7 +34,8 @@ extern "C" {
  *     y_t = S_t r_t
  *
  * r, w, k, v, a, b: [batch, time, heads, 64] of dt; y the same of y_dt (dt or
- * RQ_F32).  A token with w = -inf, k = 0 and b = 0 leaves the state as it was.
+ * RQ_F32).  A token with w = -inf, k = 0 and b = 0 (and finite r, v, a) leaves the state as it was.
+ * Tokens are taken in chunks of 16: a NaN or an infinity may reach the y before it in its own chunk.
  *
  * cu_seqlens NULL: `seqs` is batch, every row of the batch a sequence.  Else
  * batch is 1 and sequence n has the tokens cu_seqlens[n] .. cu_seqlens[n + 1] - 1 of

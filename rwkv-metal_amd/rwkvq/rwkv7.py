@@ -262,10 +262,12 @@ def wkv7(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state
     last.  Nothing waits for their values: boundaries outside the batch are moved into it, and
     where they decrease the results are undefined.
 
-    In a padded batch a token with w = -inf, k = 0 and b = 0 leaves the state as it was.
+    In a padded batch a token with w = -inf, k = 0 and b = 0 leaves the state as it was; its r, v and a have to
+    be finite.  Tokens are taken in chunks of 16 from a sequence's first: a NaN or an infinity reaches everything
+    behind it, and may reach the outputs before it in its own chunk (never another sequence or head).
 
-    Differentiable in all six and the first state, from both results (once).  The backward pass
-    keeps every 16th state, a sixteenth of 16 KB for each token and head."""
+    Differentiable in all six and the first state, from both results (once).  For the backward pass 1.25 KB
+    are kept for each token and head (every 16th state, and S a)."""
     six = [r, w, k, v, a, b]
     batch, time, heads, _ = _check_inputs(six, 4)
     six, dt = _same_dtype(six)
