@@ -177,14 +177,14 @@ struct Row {
         steps = (int)std::min<int64_t>(per, (left + kStep - 1) / kStep);
     }
     RQ_DEV int64_t at(int s) const { return from + (int64_t)s * kStep + lane * kLane; }
-    RQ_DEV void fetch(int s, Raw8<DT>& to) const {
-        const int64_t i = at(s);
-        if (s < whole) {
+    RQ_DEV void fetch(int s, Raw8<DT>& to) const {  // a whole step
+        const uint8_t* q = p + at(s) * kSize<DT>;
 #pragma unroll
-            for (int j = 0; j < kLane / kVec<DT>; ++j) to.v[j] = *(const Bytes16*)(p + (i + j * kVec<DT>)*kSize<DT>);
-            return;
-        }
-        uint32_t w[kLane / kVec<DT> * 4];  // -inf past the end
+        for (int j = 0; j < kLane / kVec<DT>; ++j) to.v[j] = *(const Bytes16*)(q + j * kVec<DT> * kSize<DT>);
+    }
+    RQ_DEV void fetch_last(int s, Raw8<DT>& to) const {  // -inf past the end
+        const int64_t i = at(s);
+        uint32_t w[kLane / kVec<DT> * 4];
         if constexpr (DT == RQ_F32) {
 #pragma unroll
             for (int j = 0; j < kLane; ++j) w[j] = i + j < n ? ((const uint32_t*)p)[i + j] : 0xff800000u;
@@ -202,26 +202,40 @@ struct Row {
 #pragma unroll
             for (int x = 0; x < 4; ++x) to.v[j].w[x] = w[4 * j + x];
     }
-    // f(step, eight logits) in the order of the index, while it gives true; three steps in flight, in registers by
-    // turns (a copy of what is on its way waits for it)
+    template <class F>
+    static RQ_DEV void take(int s, const Raw8<DT>& held, F f) {
+        float l[kLane];
+#pragma unroll
+        for (int j = 0; j < kLane / kVec<DT>; ++j) unpack_vec<DT>(held.v[j], l + j * kVec<DT>);
+        f(s, l);
+    }
+    // f(step, eight logits) in the order of the index; three steps in flight, in registers by turns (a copy of what is
+    // on its way waits for it, and so does the end of a condition or a loop that a load may leave early: with
+    // these a pass took 700 cycles a step more)
     template <class F>
     RQ_DEV void each(F f) const {
-        if (steps == 0) return;
         constexpr int kTurns = 4;
-        Raw8<DT> held[kTurns];
+        if (whole > 0) {
+            Raw8<DT> held[kTurns];
 #pragma unroll
-        for (int o = 0; o + 1 < kTurns; ++o) fetch(o < steps ? o : 0, held[o]);
-        for (int s0 = 0; s0 < steps; s0 += kTurns) {
+            for (int o = 0; o + 1 < kTurns; ++o) fetch(o < whole ? o : 0, held[o]);
+            int s0 = 0;
+            for (; s0 + kTurns <= whole; s0 += kTurns) {
 #pragma unroll
-            for (int o = 0; o < kTurns; ++o) {
-                const int s = s0 + o, ahead = s + kTurns - 1;
-                if (s >= steps) return;
-                fetch(ahead < steps ? ahead : 0, held[(o + kTurns - 1) % kTurns]);
-                float l[kLane];
-#pragma unroll
-                for (int j = 0; j < kLane / kVec<DT>; ++j) unpack_vec<DT>(held[o].v[j], l + j * kVec<DT>);
-                if (!f(s, l)) return;
+                for (int o = 0; o < kTurns; ++o) {
+                    const int ahead = s0 + o + kTurns - 1;
+                    fetch(ahead < whole ? ahead : 0, held[(o + kTurns - 1) % kTurns]);
+                    take(s0 + o, held[o], f);
+                }
             }
+#pragma unroll
+            for (int o = 0; o + 1 < kTurns; ++o)
+                if (s0 + o < whole) take(s0 + o, held[o], f);
+        }
+        if (whole < steps) {
+            Raw8<DT> last;
+            fetch_last(whole, last);
+            take(whole, last, f);
         }
     }
 };
@@ -332,7 +346,6 @@ RQ_DEV uint32_t key_in_row(const Row<DT>& row, Lds& lds, const Bins& bins, const
             const double x = weight(l[i], key);
             if (x > 0.0) add_to_bin(lds, key, x);
         }
-        return true;
     });
     __syncthreads();
     const bool with_extra = extra > 0.0 && bins.of(of_key(extra_key)) == bin;
@@ -350,7 +363,6 @@ RQ_DEV uint32_t key_in_row(const Row<DT>& row, Lds& lds, const Bins& bins, const
                 const double x = weight(l[i], key);
                 if (x > 0.0) atomicAdd(&lds.sums[255 - ((key >> shift) & 255)], units.of(x));
             }
-            return true;
         });
         if (threadIdx.x == 0 && with_extra && (extra_key & mask) == prefix)
             atomicAdd(&lds.sums[255 - ((extra_key >> shift) & 255)], units.of_sum(extra));
@@ -436,17 +448,16 @@ RQ_DEV bool gather(const Row<DT>& row, Lds& lds, float bound) {
     uint32_t have = 0;
     row.each([&](int s, const float* l) {
         const float most = fmaxf(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), fmaxf(fmaxf(l[4], l[5]), fmaxf(l[6], l[7])));
-        if (!__any(most >= bound)) return true;
+        if (have > kPart || !__any(most >= bound)) return;
         uint32_t in = 0;
 #pragma unroll
         for (int i = 0; i < kLane; ++i) in |= (uint32_t)(l[i] >= bound) << i;
         const uint32_t upto = scan32(__popc(in));
         uint32_t at = have + upto - __popc(in);
         have += last32(upto);
-        if (have > kPart) return false;
+        if (have > kPart) return;
         const uint32_t first = (uint32_t)row.at(s);
         for (; in; in &= in - 1) lds.part_at[wave][at++] = first + __builtin_ctz(in);
-        return true;
     });
     if (lane == 0) lds.part_n[wave] = have;
     if (!__syncthreads_and(have <= kPart)) return false;
@@ -507,7 +518,7 @@ RQ_DEV void choose(const SampleArgs& p, int64_t r, int64_t at, float l, const We
 template <int DT>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
     __shared__ Lds lds;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // known to be the same in all lanes
     const int64_t r = blockIdx.x, n = p.vocab;
     const Row<DT> row(p.logits, r, n, wave, lane);
     const float temperature = p.temperature ? p.temperature[r] : p.temperature_all;
@@ -527,7 +538,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             low = fminf(low, l[i]);
             size = std::max(size, __float_as_uint(l[i]) & 0x7fffffffu);
         }
-        return true;
     });
     const uint32_t lane_top = top > -INFINITY ? key_of(top) : 0;
     if (threadIdx.x == 0) lds.first = ~0ull;
@@ -560,7 +570,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
 #pragma unroll
             for (int i = kLane - 1; i >= 0; --i)
                 if (l[i] == top) first = std::min<unsigned long long>(first, row.at(s) + i);
-            return true;
         });
         if (first != ~0ull) atomicMin(&lds.first, first);
         __syncthreads();
@@ -646,7 +655,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
 #pragma unroll
                 for (int i = 0; i < kLane; ++i)
                     if (l[i] > -INFINITY) atomicAdd(&lds.sums[bins.of(l[i])], 1ull);
-                return true;
             });
             if (threadIdx.x == 0) lds.total = 0.0;
             const Units ones{6755399441055744.0, 1.0};
@@ -673,7 +681,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
 #pragma unroll
                 for (int i = 0; i < kLane; ++i)
                     if (x[i]) atomicAdd(&lds.sums[sum_bins.of(l[i])], x[i]);
-                return true;
             });
             find_bin<kBins>(lds, units, 0.0, -1.0, fmax((double)top_p, 0.0));
             want = lds.total;
@@ -721,7 +728,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
                         const double x = w.quanta(w.at(l[i]));
                         if (x > 0.0) atomicAdd(&lds.sums[sum_bins.of(l[i])], units.of(x));
                     }
-                    return true;
                 });
             }
             find_bin<kBins>(lds, units, 0.0, -1.0, fmax((double)top_p, 0.0));
@@ -820,10 +826,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
 #pragma unroll
             for (int i = 0; i < kLane; ++i) x[i] = w.quanta(w.at(l[i]));
             sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-            return true;
+            return;
         }
         const float most = fmaxf(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), fmaxf(fmaxf(l[4], l[5]), fmaxf(l[6], l[7])));
-        if (!__any(most >= border)) return true;
+        if (!__any(most >= border)) return;
         double x[kLane];
 #pragma unroll
         for (int i = 0; i < kLane; ++i) {
@@ -836,7 +842,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
             for (int i = 0; i < kLane; ++i) equal += l[i] == border;
         }
         sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-        return true;
     });
     sum = wave_sum64(sum);
     equal = wave_sum32(equal);
