@@ -184,23 +184,22 @@ struct Row {
     }
     RQ_DEV void fetch_last(int s, Raw8<DT>& to) const {  // -inf past the end
         const int64_t i = at(s);
-        uint32_t w[kLane / kVec<DT> * 4];
-        if constexpr (DT == RQ_F32) {
+        uint32_t w[kLane];
 #pragma unroll
-            for (int j = 0; j < kLane; ++j) w[j] = i + j < n ? ((const uint32_t*)p)[i + j] : 0xff800000u;
-        } else {
-            constexpr uint32_t kNone = DT == RQ_BF16 ? 0xff80u : 0xfc00u;
-#pragma unroll
-            for (int j = 0; j < kLane; j += 2) {
-                const uint32_t lo = i + j < n ? ((const uint16_t*)p)[i + j] : kNone;
-                const uint32_t hi = i + j + 1 < n ? ((const uint16_t*)p)[i + j + 1] : kNone;
-                w[j / 2] = lo | (hi << 16);
-            }
+        for (int j = 0; j < kLane; ++j) {
+            const int64_t x = std::min(i + j, n - 1);
+            if constexpr (DT == RQ_F32) w[j] = ((const uint32_t*)p)[x];
+            else w[j] = ((const uint16_t*)p)[x];
         }
+        constexpr uint32_t kNone = DT == RQ_F32 ? 0xff800000u : DT == RQ_BF16 ? 0xff80u : 0xfc00u;
 #pragma unroll
-        for (int j = 0; j < kLane / kVec<DT>; ++j)
+        for (int j = 0; j < kLane; ++j) w[j] = i + j < n ? w[j] : kNone;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) to.v[j].w[x] = w[4 * j + x];
+        for (int j = 0; j < kLane; ++j) {
+            uint32_t& word = to.v[j / kVec<DT>].w[DT == RQ_F32 ? j % 4 : j / 2];
+            if constexpr (DT == RQ_F32) word = w[j];
+            else word = j % 2 ? word | (w[j] << 16) : w[j];
+        }
     }
     template <class F>
     static RQ_DEV void take(int s, const Raw8<DT>& held, F f) {
