@@ -894,8 +894,9 @@ __global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(Wk
     f32x4_t acc[4];
     {
         const float* from = ENDS ? nullptr
-                            : seg.index ? p.seg.begins + ((slot * H + head) * kHead + value) * kHead
-                            : p.state   ? p.state + ((seg.seq * H + head) * kHead + value) * kHead
+                            : p.seg.chunks && !(seg.index == 0 && seg.last)
+                                ? p.seg.begins + ((slot * H + head) * kHead + value) * kHead
+                            : p.state ? p.state + ((seg.seq * H + head) * kHead + value) * kHead
                                         : nullptr;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -1019,6 +1020,8 @@ __global__ __launch_bounds__(256) void wkv7_join_kernel(WkvShape shape, WkvSegme
     const int value = 16 * (blockIdx.x & 3) + m, row = threadIdx.x >> 4, column = 4 * (threadIdx.x & 15);
     f32x4_t s = {0.f, 0.f, 0.f, 0.f};
     if (state) s = *(const f32x4_t*)(state + ((seq * H + head) * kHead + value) * kHead + 16 * q + 4 * g);
+    // the first segment's too: the last one's block may write the same memory before the first one's has read it
+    *(f32x4_t*)(seg.begins + ((slot0 * H + head) * kHead + value) * kHead + 16 * q + 4 * g) = s;
     // of the next steps: the thread's share of M, N[value][key 16q + 4g + i].  Registers by turns, not handed on:
     // a copy of what is on its way waits for it.
     constexpr int kTurns = 4;

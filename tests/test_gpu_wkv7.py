@@ -123,6 +123,29 @@ def test_wild_boundaries_in_segments(rq, dev):
     assert y.shape == six[0].shape and len(grads) == 6
 
 
+@pytest.mark.parametrize("lens", [None, [600, 3, 0, 401]])
+def test_a_state_in_place_in_segments(rq, dev, lens):
+    """The C entry point with one buffer for the state before and after: the last segment's block may
+    end before the first one's begins."""
+    g = torch.Generator().manual_seed(98)
+    L, h, t = rq._lib.lib(), 3, 1004
+    six = [x.to(dev) for x in inputs(g, 1, t, h)]
+    seqs = 1 if lens is None else len(lens)
+    cu = None if lens is None else torch.tensor([0, 600, 603, 603, 1004], dtype=torch.int32, device=dev)
+    state = torch.randn(seqs, h, D, D, generator=g).to(dev)
+    want_y, want_last = rq.wkv7(*six, state, cu_seqlens=cu)
+    need = L.rq_wkv7_workspace_bytes(1, t, h, seqs, int(cu is not None))
+    assert need > 0
+    ws, y = torch.empty(need, dtype=torch.uint8, device=dev), torch.empty_like(six[0])
+    rc = L.rq_wkv7(*[x.data_ptr() for x in six], rq._lib.DTYPE_CODE[torch.float32], 1, t, h,
+                   0 if cu is None else cu.data_ptr(), seqs, state.data_ptr(), y.data_ptr(),
+                   rq._lib.DTYPE_CODE[torch.float32], state.data_ptr(), 0, 0, ws.data_ptr(), need,
+                   torch.cuda.current_stream(dev).cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y, want_y) and torch.equal(state, want_last)
+
+
 def test_many_packed_sequences(rq, dev):
     lens = [(7 * i) % 23 for i in range(200)]
     check(rq, dev, 77, 1, 0, 2, "fp32", "fp32", True, True, lens, 5)
