@@ -16,8 +16,9 @@ using rq::valid_dt;
 
 namespace {
 
-// A grid holds fewer than 2^32 threads: up to 1024 for each head of a sequence in the scan, 256 for each
-// head of a chunk and of a decode step.
+// A grid holds fewer than 2^32 threads: up to 1024 for each head of a sequence or segment in the scan, 4 x 256 in the
+// joins, 256 in a decode step.  A chunk's state is 16 KB: 2^23 of them and the tensors they belong to are more than the
+// card's memory.
 constexpr int64_t kMaxHeadsOfSeqs = 1 << 21, kMaxHeadsOfChunks = 1 << 23, kMaxTokens = 1ll << 31;
 
 int check_shape(const char* what, int64_t batch, int64_t time, int64_t heads, bool packed, int64_t seqs) {
