@@ -472,6 +472,50 @@ def test_captured_and_replayed(rq, dev):
                 assert torch.equal(x, z)
 
 
+def test_captured_segments_of_one_pool(rq, dev):
+    """Two graphs that share a pool, and with it the memory of their workspaces: each replay behind the other and behind
+    eager work gives the eager bits."""
+    g = torch.Generator().manual_seed(99)
+    six = [x.to(dev) for x in inputs(g, 1, 701, 2, dtype=torch.bfloat16)]
+    state = torch.randn(1, 2, D, D, generator=g).to(dev)
+    dy = torch.randn(1, 701, 2, D, generator=g).to(torch.bfloat16).to(dev)
+    cu = torch.tensor([0, 450, 450, 699], dtype=torch.int32, device=dev)
+    states = torch.randn(3, 2, D, D, generator=g).to(dev)
+    leaves = [x.clone().requires_grad_() for x in six]
+
+    def train():
+        y, last = rq.wkv7(*leaves, state)
+        return [y, last, *torch.autograd.grad(y, leaves, dy)]
+
+    def serve():
+        return list(rq.wkv7(*six, states, cu_seqlens=cu))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        train()
+        serve()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, pool = [], None
+    for f in (train, serve):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            out = f()
+        pool = graph.pool()
+        graphs.append((graph, out, f))
+    for i in range(3):
+        with torch.no_grad():
+            for x, z in zip(six, leaves):
+                x.copy_(x.roll(7 * i + 1, 1))
+                z.copy_(x)
+        for graph, out, f in (graphs, graphs[::-1])[i % 2]:
+            graph.replay()
+            got = [x.detach().clone() for x in out]
+            torch.cuda.synchronize()
+            for x, z in zip(got, f()):
+                assert torch.equal(x, z)
+
+
 def test_offsets_past_32_bits(rq, dev):
     """A packed row of 17 million tokens of one head, 4.35e9 bytes of each tensor and 1.7e10 of states,
     the sequences at its end."""
