@@ -22,8 +22,8 @@
 //   db = e^-L (e^Lend SA dS' + dMrb^T R~ + dMab^T A~), dk alike with V, dMrk, dMak
 //   dlog d_t: what of the loss passes token t's decay (chunk_grads).
 //
-// The scan's products are fp32 MFMAs (v_mfma_f32_16x16x4_f32): the state lives in fp32 and
-// feeds itself for thousands of tokens.
+// All products are fp32 MFMAs (v_mfma_f32_16x16x4_f32): the state lives in fp32 and feeds itself for thousands of
+// tokens, and the gradients of 16-bit tensors are rounded once, where they are stored.
 //
 // e^-L overflows where the decays of a chunk are strong.  Below 2^-32 over one
 // chunk (RWKV-7's own decays reach 2^-14) a chunk's pair matrices are formed by VALU from
@@ -175,6 +175,7 @@ struct GradRows {
     Rows d[4];   // dS', [value / 16][value % 16][key]
     Rows dz, v, sa;
     Rows io[5];  // log2 d, r, a, b and k; then, each in its place, dw, dr, da, db and dk
+    float pairs[4][kChunk][kChunk + 4];  // dMab, dMak, dMrb and dMrk
 };
 struct ScanGradLds : ScanLds {
     GradRows grads;
@@ -407,94 +408,20 @@ RQ_DEV float over_groups(float x) {
     return x + __shfl_xor(x, 32);
 }
 
-// The products of the gradients.  They are not fed back into anything, and where the tensors have 16 bits
-// their results are rounded to 8 or 11 significant ones: there an operand is the sum of two bf16 (16 bits of
-// it), a product three bf16 MFMAs of 32 steps, at a fifth of the fp32 MFMA's time and beside the VALU, which
-// the fp32 one holds up.  fp32 tensors keep fp32 products.
-struct Halves {
-    bf16x8_t hi, lo;
-};
-RQ_DEV uint32_t two_bf16(float a, float b) {
-    typedef __bf16 pair __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, pair{(__bf16)a, (__bf16)b});
-}
-RQ_DEV Halves halves_of(const f32x4_t& x, const f32x4_t& y) {
-    Halves h;
-    uint32_t hi[4], lo[4];
+// A product over the 64 values: lane (m, g) holds values 16q + 4g + i of row m of A and of column m of B.
+RQ_DEV f32x4_t mma64(const f32x4_t* a, const f32x4_t* b, f32x4_t c) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float a = i < 2 ? x[2 * i] : y[2 * i - 4], b = i < 2 ? x[2 * i + 1] : y[2 * i - 3];
-        hi[i] = two_bf16(a, b);
-        lo[i] = two_bf16(a - __uint_as_float(hi[i] << 16), b - __uint_as_float(hi[i] & 0xffff0000u));
-    }
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    h.hi = __builtin_bit_cast(bf16x8_t, u32x4{hi[0], hi[1], hi[2], hi[3]});
-    h.lo = __builtin_bit_cast(bf16x8_t, u32x4{lo[0], lo[1], lo[2], lo[3]});
-    return h;
-}
-// EXACT: an operand that is bf16 as it is (its lo is 0)
-template <bool EXACT_A, bool EXACT_B>
-RQ_DEV f32x4_t mma_halves(const Halves& a, const Halves& b, f32x4_t c) {
-    if constexpr (!EXACT_A) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.lo, b.hi, c, 0, 0, 0);
-    if constexpr (!EXACT_B) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.lo, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.hi, c, 0, 0, 0);
-}
-
-// A row or column of N / 4 lanes' shares, four numbers from each 16: N = 64 values, or the 16 tokens of two matrices.
-template <bool HALF, int N>
-struct Operand {
-    f32x4_t v[N / 16];
-    RQ_DEV explicit Operand(const f32x4_t* x) {
-#pragma unroll
-        for (int q = 0; q < N / 16; ++q) v[q] = x[q];
-    }
-    RQ_DEV Operand(f32x4_t x0, f32x4_t x1) : v{x0, x1} {}
-};
-template <int N>
-struct Operand<true, N> {
-    Halves v[N / 32];
-    RQ_DEV explicit Operand(const f32x4_t* x) {
-#pragma unroll
-        for (int q = 0; q < N / 32; ++q) v[q] = halves_of(x[2 * q], x[2 * q + 1]);
-    }
-    RQ_DEV Operand(f32x4_t x0, f32x4_t x1) : v{halves_of(x0, x1)} {}
-};
-
-// Half h of an operand of 64.
-template <bool HALF>
-RQ_DEV Operand<HALF, 32> half_of(const Operand<HALF, 64>& x, int h) {
-    const f32x4_t zero[2] = {};
-    Operand<HALF, 32> o(zero);
-    if constexpr (HALF) {
-        o.v[0] = x.v[h];
-    } else {
-        o.v[0] = x.v[2 * h];
-        o.v[1] = x.v[2 * h + 1];
-    }
-    return o;
-}
-template <bool EXACT_A = false, bool EXACT_B = false, bool HALF, int N>
-RQ_DEV f32x4_t mma(const Operand<HALF, N>& a, const Operand<HALF, N>& b, f32x4_t c) {
-    if constexpr (HALF) {
-#pragma unroll
-        for (int q = 0; q < N / 32; ++q) c = mma_halves<EXACT_A, EXACT_B>(a.v[q], b.v[q], c);
-    } else {
-#pragma unroll
-        for (int q = 0; q < N / 16; ++q) c = mma16(a.v[q], b.v[q], c);
-    }
+    for (int q = 0; q < 4; ++q) c = mma16(a[q], b[q], c);
     return c;
 }
-
-
-// A value of a row, `at` bytes behind a pointer that all lanes share.
-template <int DT>
-RQ_DEV typename dt_traits<DT>::storage load1(const uint8_t* p, uint32_t at) {
-    return *(const typename dt_traits<DT>::storage*)(p + at);
-}
-template <int DT>
-RQ_DEV void store1(uint8_t* p, uint32_t at, float x) {
-    *(typename dt_traits<DT>::storage*)(p + at) = dt_traits<DT>::from_f32(x);
-}
+// Row m of a chunk's tokens.
+struct TokenRow {
+    f32x4_t v[4];
+    RQ_DEV TokenRow(const Rows& from, int lane) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = *(const f32x4_t*)&from[kChunk - 1 - (lane & 15)][16 * q + 4 * (lane >> 4)];
+    }
+};
 
 // x of the token `t` (the same in all lanes) and the lane's key, from tokens 4g + i
 RQ_DEV float at_token(const f32x4_t& x, int t, int m) {
@@ -502,51 +429,45 @@ RQ_DEV float at_token(const f32x4_t& x, int t, int m) {
     return __shfl(own, 16 * (t >> 2) + m);
 }
 
+// One of dMab, dMak, dMrb and dMrk, by wave: [target][source].
+RQ_DEV void pair_grads(const Rows& dy, GradRows& lds, int lane, int wave) {
+    const TokenRow source(wave & 1 ? lds.v : lds.sa, lane), target(wave < 2 ? lds.dz : dy, lane);
+    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+    *(f32x4_t*)&lds.pairs[wave][lane & 15][4 * (lane >> 4)] = mma64(source.v, target.v, zero);
+}
+
 // A chunk's dr, dw, dk, da and db for the 16 keys of a wave, s[q][i] = S[value 16q + 4g + i][key].  In products over the
 // values a lane holds rows of tokens (A) and columns of keys (B); the results, tokens 4g + i of key lane & 15, are
-// where the gradients are formed.  Each wave forms the four pair matrices for itself, and their transposes: no wave
-// waits for another.
-template <int DT, int YDT>
+// where the gradients are formed.  The pair matrices are the same for all keys: each wave forms one of the four.
 RQ_DEV void chunk_grads(const f32x4_t* s, const Rows& dy_rows, GradRows& lds, int lane, int wave) {
-    constexpr bool HALF = DT != RQ_F32, V_EXACT = DT == RQ_BF16, DY_EXACT = YDT == RQ_BF16;
     const int g = lane >> 4, m = lane & 15, key = 16 * wave + m;
     const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-    f32x4_t gr = zero, ga = zero, gb = zero, gk = zero;
+    f32x4_t gr, ga, gb, gk;
     float through = 0.f;  // sum over the values of S dS' of this key
-    f32x4_t by_t[4], by_s[4];  // dMab, dMak, dMrb, dMrk
+    pair_grads(dy_rows, lds, lane, wave);
     {
-        const auto rows = [&](const Rows& from) {
-            f32x4_t x[4];
+        const TokenRow dy(dy_rows, lane), dz(lds.dz, lane), sa(lds.sa, lane), v(lds.v, lane);
+        f32x4_t d[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) x[q] = *(const f32x4_t*)&from[kChunk - 1 - m][16 * q + 4 * g];
-            return Operand<HALF, 64>(x);
-        };
-        const Operand<HALF, 64> dy_o = rows(dy_rows), v_o = rows(lds.v), sa_o = rows(lds.sa), dz_o = rows(lds.dz);
+        for (int q = 0; q < 4; ++q) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            f32x4_t d[2];
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    d[q][i] = lds.d[2 * h + q][4 * g + i][key];
-                    through = fmaf(s[2 * h + q][i], d[q][i], through);
-                }
+            for (int i = 0; i < 4; ++i) {
+                d[q][i] = lds.d[q][4 * g + i][key];
+                through = fmaf(s[q][i], d[q][i], through);
             }
-            const Operand<HALF, 32> s_o(s + 2 * h), d_o(d);
-            gr = mma<DY_EXACT, false>(half_of(dy_o, h), s_o, gr);
-            ga = mma(half_of(dz_o, h), s_o, ga);
-            gb = mma(half_of(sa_o, h), d_o, gb);
-            gk = mma<V_EXACT, false>(half_of(v_o, h), d_o, gk);
-            }
-        by_t[0] = mma(sa_o, dz_o, zero);
-        by_t[1] = mma<V_EXACT, false>(v_o, dz_o, zero);
-        by_t[2] = mma<false, DY_EXACT>(sa_o, dy_o, zero);
-        by_t[3] = mma<V_EXACT, DY_EXACT>(v_o, dy_o, zero);
-        by_s[0] = mma(dz_o, sa_o, zero);
-        by_s[1] = mma<false, V_EXACT>(dz_o, v_o, zero);
-        by_s[2] = mma<DY_EXACT, false>(dy_o, sa_o, zero);
-        by_s[3] = mma<DY_EXACT, V_EXACT>(dy_o, v_o, zero);
+        }
+        gr = mma64(dy.v, s, zero);
+        ga = mma64(dz.v, s, zero);
+        gb = mma64(sa.v, d, zero);
+        gk = mma64(v.v, d, zero);
+    }
+    __syncthreads();
+    f32x4_t by_t[4], by_s[4];  // dMab, dMak, dMrb, dMrk: of target m and of source m
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        by_t[j] = *(const f32x4_t*)&lds.pairs[j][m][4 * g];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) by_s[j][i] = lds.pairs[j][4 * g + i][m];
     }
     f32x4_t g2, r, a, b, k, l;
 #pragma unroll
@@ -626,11 +547,11 @@ RQ_DEV void chunk_grads(const f32x4_t* s, const Rows& dy_rows, GradRows& lds, in
         f32x4_t il;
 #pragma unroll
         for (int i = 0; i < 4; ++i) il[i] = exp2_hw(-l[i]);
-        const Operand<HALF, 32> early(b * il, k * il), late(a * ex, r * el);  // B~, K~ and A~, R~
-        pa = mma(Operand<HALF, 32>(by_t[0], by_t[1]), early, pa) * ex;
-        pr = mma(Operand<HALF, 32>(by_t[2], by_t[3]), early, pr) * el;
-        pb = mma(Operand<HALF, 32>(by_s[0], by_s[2]), late, pb) * il;
-        pk = mma(Operand<HALF, 32>(by_s[1], by_s[3]), late, pk) * il;
+        const f32x4_t bt = b * il, kt = k * il, at = a * ex, rt = r * el;  // B~, K~, A~, R~
+        pa = mma16(by_t[1], kt, mma16(by_t[0], bt, pa)) * ex;
+        pr = mma16(by_t[3], kt, mma16(by_t[2], bt, pr)) * el;
+        pb = mma16(by_s[2], rt, mma16(by_s[0], at, pb)) * il;
+        pk = mma16(by_s[3], rt, mma16(by_s[1], at, pk)) * il;
         // a pair (s, t) passes the decays behind s up to t (before t, for a): sums of what ends
         // minus what begins at each token and behind it
         const f32x4_t q = r * pr - b * pb - k * pk, qa = a * pa;
@@ -867,6 +788,7 @@ __global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(Wk
             __syncthreads();
             if (GRADS) {
                 matrix(c + 1, next);
+                __syncthreads();
                 store_y(c);
                 __syncthreads();
             }
@@ -990,7 +912,7 @@ __global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(Wk
         }
         __syncthreads();
         if constexpr (GRADS) {
-            chunk_grads<DT, XDT>(s, b.x, lds.grads, lane, wave & 3);
+            chunk_grads(s, b.x, lds.grads, lane, wave & 3);
             __syncthreads();
         }
     }
