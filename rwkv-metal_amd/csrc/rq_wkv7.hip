@@ -429,6 +429,13 @@ RQ_DEV float at_token(const f32x4_t& x, int t, int m) {
     return __shfl(own, 16 * (t >> 2) + m);
 }
 
+// A wave's accesses of LDS before it are done before those behind it, for all its lanes: the machine keeps their order, and
+// this has the compiler keep it too, which takes a lane's addresses for its own.
+RQ_DEV void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // One of dMab, dMak, dMrb and dMrk, by wave: [target][source].
 RQ_DEV void pair_grads(const Rows& dy, GradRows& lds, int lane, int wave) {
     const TokenRow source(wave & 1 ? lds.v : lds.sa, lane), target(wave < 2 ? lds.dz : dy, lane);
@@ -462,13 +469,6 @@ RQ_DEV void chunk_grads(const f32x4_t* s, const Rows& dy_rows, GradRows& lds, in
         gk = mma64(v.v, d, zero);
     }
     __syncthreads();
-    f32x4_t by_t[4], by_s[4];  // dMab, dMak, dMrb, dMrk: of target m and of source m
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        by_t[j] = *(const f32x4_t*)&lds.pairs[j][m][4 * g];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) by_s[j][i] = lds.pairs[j][4 * g + i][m];
-    }
     f32x4_t g2, r, a, b, k, l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -485,17 +485,11 @@ RQ_DEV void chunk_grads(const f32x4_t* s, const Rows& dy_rows, GradRows& lds, in
     const float end = __shfl(l[3], 48 + m);
     const bool strong = __any(!(end >= kStrong));
     through = over_groups(through);
-    // a token's own pair passes no decay: it stays out of the sums below, where it would cancel
-    f32x4_t own_b, own_k;
+    f32x4_t own_b, own_k;  // a token's own pair passes no decay: it stays out of the sums below
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        own_b[i] = __shfl(by_t[2][i], 16 * g + 4 * g + i);
-        own_k[i] = __shfl(by_t[3][i], 16 * g + 4 * g + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (!(4 * g + i < m)) by_t[j][i] = 0.f;  // rows are sources, columns targets
-            if (!(m < 4 * g + i)) by_s[j][i] = 0.f;  // the other way round
-        }
+        own_b[i] = lds.pairs[2][4 * g + i][4 * g + i];
+        own_k[i] = lds.pairs[3][4 * g + i][4 * g + i];
     }
     f32x4_t to_end, el, ex;  // e^(Lend - L), e^L, e^Lx
     {
@@ -516,6 +510,9 @@ RQ_DEV void chunk_grads(const f32x4_t* s, const Rows& dy_rows, GradRows& lds, in
     gr *= el;
     ga *= ex;
     const f32x4_t enters = b * gb + k * gk, leaves_r = r * gr, leaves_a = a * ga;  // what each token adds to, and takes from, the state
+    // of the pairs of tokens s < t: their parts of dr, da, db and dk, and of each token's decay those that pass it (s < i <= t;
+    // of a, that reads the state before its own decay, s < i < t).  Only these: a difference of sums over all pairs
+    // would leave the rounding of pairs that lie to one side of the token, which may be any number of times larger.
     f32x4_t pr = zero, pa = zero, pb = zero, pk = zero, cross = zero;
     if (strong) {
         // pair by pair, from the sums of the terms between the two tokens
@@ -528,8 +525,8 @@ RQ_DEV void chunk_grads(const f32x4_t* s, const Rows& dy_rows, GradRows& lds, in
                 const float h = exp2_hw(e);
                 e += at_token(g2, t, m);
                 const float f = exp2_hw(e), rt = at_token(r, t, m) * f, at_ = at_token(a, t, m) * h;
-                const float m0 = at_token(by_t[0], src, t), m1 = at_token(by_t[1], src, t), m2 = at_token(by_t[2], src, t),
-                            m3 = at_token(by_t[3], src, t);
+                const float m0 = lds.pairs[0][t][src], m1 = lds.pairs[1][t][src], m2 = lds.pairs[2][t][src],
+                            m3 = lds.pairs[3][t][src];
                 const float of_a = m0 * bs + m1 * ks, of_r = m2 * bs + m3 * ks;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -544,22 +541,94 @@ RQ_DEV void chunk_grads(const f32x4_t* s, const Rows& dy_rows, GradRows& lds, in
             }
         }
     } else {
+        // between groups of four tokens by products, a step's contraction over the four of one group
         f32x4_t il;
 #pragma unroll
         for (int i = 0; i < 4; ++i) il[i] = exp2_hw(-l[i]);
-        const f32x4_t bt = b * il, kt = k * il, at = a * ex, rt = r * el;  // B~, K~, A~, R~
-        pa = mma16(by_t[1], kt, mma16(by_t[0], bt, pa)) * ex;
-        pr = mma16(by_t[3], kt, mma16(by_t[2], bt, pr)) * el;
-        pb = mma16(by_s[2], rt, mma16(by_s[0], at, pb)) * il;
-        pk = mma16(by_s[3], rt, mma16(by_s[1], at, pk)) * il;
-        // a pair (s, t) passes the decays behind s up to t (before t, for a): sums of what ends
-        // minus what begins at each token and behind it
-        const f32x4_t q = r * pr - b * pb - k * pk, qa = a * pa;
-        float sum = groups_after((q[0] + qa[0]) + (q[1] + qa[1]) + (q[2] + qa[2]) + (q[3] + qa[3]), g);
+        const f32x4_t rt = r * el, at = a * ex, bt = b * il, kt = k * il;  // R~, A~, B~, K~
 #pragma unroll
-        for (int i = 3; i >= 0; --i) {
-            cross[i] = sum + q[i];
-            sum += q[i] + qa[i];
+        for (int i = 0; i < 4; ++i) {  // to the lanes of the contraction; the wave's own keys
+            const int row = kChunk - 1 - (4 * g + i);
+            lds.io[1][row][key] = rt[i];
+            lds.io[2][row][key] = at[i];
+            lds.io[3][row][key] = bt[i];
+            lds.io[4][row][key] = kt[i];
+        }
+        wave_lds_order();
+        f32x4_t of_r[3], of_a[3];  // of the sources of group 0, 1, 2; for the targets of later groups only
+#pragma unroll
+        for (int o = 0; o < 3; ++o) {
+            const int row = kChunk - 1 - (4 * o + g);
+            const float b_ = lds.io[3][row][key], k_ = lds.io[4][row][key];
+            of_a[o] = mfma4(lds.pairs[0][m][4 * o + g], b_, zero);
+            of_r[o] = mfma4(lds.pairs[2][m][4 * o + g], b_, zero);
+            of_a[o] = mfma4(lds.pairs[1][m][4 * o + g], k_, of_a[o]);
+            of_r[o] = mfma4(lds.pairs[3][m][4 * o + g], k_, of_r[o]);
+        }
+#pragma unroll
+        for (int o = 1; o < 4; ++o) {  // the targets of group o, for the sources of earlier ones
+            const int row = kChunk - 1 - (4 * o + g), t = 4 * o + g;
+            const float r_ = lds.io[1][row][key], a_ = lds.io[2][row][key];
+            const bool earlier = m < 4 * o;
+            pb = mfma4(earlier ? lds.pairs[0][t][m] : 0.f, a_, pb);
+            pk = mfma4(earlier ? lds.pairs[1][t][m] : 0.f, a_, pk);
+            pb = mfma4(earlier ? lds.pairs[2][t][m] : 0.f, r_, pb);
+            pk = mfma4(earlier ? lds.pairs[3][t][m] : 0.f, r_, pk);
+        }
+        float over[2] = {0.f, 0.f};  // what the pairs with the lane's group as target and group 0, groups 0 and 1 as source add to a decay between
+#pragma unroll
+        for (int o = 0; o < 3; ++o) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = rt[i] * of_r[o][i] + at[i] * of_a[o][i];
+                if (o == 0) over[0] += x;
+                if (o < 2) over[1] += x;
+                pr[i] += o < g ? of_r[o][i] : 0.f;
+                pa[i] += o < g ? of_a[o][i] : 0.f;
+            }
+        }
+        {
+            const float from2 = __shfl(over[0], 32 + m), from3 = __shfl(over[0], 48 + m), both = __shfl(over[1], 48 + m);
+            cross += g == 1 ? from2 + from3 : g == 2 ? both : 0.f;
+        }
+        pr *= el;
+        pa *= ex;
+        pb *= il;
+        pk *= il;
+        float behind = 0.f, ahead = 0.f;
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {  // of an earlier group's sources, read in this one
+            behind += r[i] * pr[i];
+            cross[i] += behind;
+            behind += a[i] * pa[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // of this group's sources, read in a later one
+            cross[i] += ahead;
+            ahead += b[i] * pb[i] + k[i] * pk[i];
+        }
+        // within the group
+        float d[4];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) d[i] = exp2_hw(g2[i]);
+#pragma unroll
+        for (int t = 1; t < 4; ++t) {
+            f32x4_t pairs[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pairs[j] = *(const f32x4_t*)&lds.pairs[j][4 * g + t][4 * g];
+            float h = 1.f;  // the decays between the two
+#pragma unroll
+            for (int s = t - 1; s >= 0; --s) {
+                const float f = h * d[t], rf = r[t] * f, ah = a[t] * h;
+                const float to_r = pairs[2][s] * b[s] + pairs[3][s] * k[s], to_a = pairs[0][s] * b[s] + pairs[1][s] * k[s];
+                pr[t] += to_r * f;
+                pa[t] += to_a * h;
+                pb[s] += pairs[0][s] * ah + pairs[2][s] * rf;
+                pk[s] += pairs[1][s] * ah + pairs[3][s] * rf;
+#pragma unroll
+                for (int i = s + 1; i <= t; ++i) cross[i] += i < t ? to_r * rf + to_a * ah : to_r * rf;
+                if (s > 0) h *= d[s];
+            }
         }
     }
     gr += pr + own_b * b + own_k * k;
@@ -584,6 +653,7 @@ RQ_DEV void chunk_grads(const f32x4_t* s, const Rows& dy_rows, GradRows& lds, in
         // d log d / dw = -exp(w), inf where the decay, and with it what passes it, is 0
         gw[i] = gw[i] == 0.f ? 0.f : gw[i] * (g2[i] * kLn2);
     }
+    wave_lds_order();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int at = kChunk - 1 - (4 * g + i);

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from wkv_ref import D, DT, NAMES, inputs
+from wkv_ref import D, DT, NAMES, bound, inputs, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,38 @@ def test_gradients_of_16_bit_tensors_are_rounded_once(rq, dev, i, dt, out, decay
         assert x.dtype == (torch.float32 if name == "state" else DT[dt])
         same = (x == z) | (x.isnan() & z.isnan())
         assert same.all(), f"d{name}: {(~same).sum().item()} of {x.numel()} differ"
+
+
+# A token that decays hard among others that hardly do: the pairs of tokens to one side of it are any number of times
+# larger than those that pass its decay, and have no part in its dw.  Over chunk, group and segment boundaries; strong enough
+# (5: the pairwise form) and not.
+LONE = [("first", [0], 3.0, -8.0), ("mid", [7], 3.0, -6.0), ("mid", [9], 3.0, -4.0), ("edge", [0], -0.5, -8.0),
+        ("several", [2, 3, 13, 16, 21, 36], 2.5, -7.0), ("strong", [6, 20], 5.0, -8.0), ("chunk's last", [15, 31], 3.0, -8.0)]
+
+
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("i", range(len(LONE)))
+def test_decay_gradients_token_by_token(rq, dev, i, dt, given):
+    """Every token's dw by its own norm.  The bound is that of a gradient over the whole tensor (wkv_ref): each of
+    a token's terms passes the same roundings, and none of it is larger than what it adds to the token's own."""
+    name, at, w, others = LONE[i]
+    print(f"wkv7 dw {name} w={w} others={others} {dt} state={given}", flush=True)
+    t, h = 40, 4
+    g = torch.Generator().manual_seed(400 + i)
+    six = inputs(g, 1, t, h, dtype=DT[dt], w=others)
+    six[1][:, at] = w
+    state = torch.randn(1, h, D, D, generator=g) if given else torch.zeros(1, h, D, D)
+    dstate = torch.randn(1, h, D, D, generator=g)
+    dy = torch.randn(1, t, h, D, generator=g).to(DT[dt])
+    want = reference(six, state, dy, dstate)["dw"]
+    got = grads(rq, dev, six, state, dy, dstate, None, DT[dt])[1]
+    e = bound("dw", DT[dt], t)
+    # the smallest steps of the type are not relative: half of one for each value
+    least = math.sqrt(h * D) * torch.finfo(DT[dt]).smallest_normal * torch.finfo(DT[dt]).eps / 2
+    off = (got.double().cpu() - want).norm(dim=(2, 3))[0]
+    norm = want.norm(dim=(2, 3))[0]
+    worst = (off / (e * norm + least)).max().item()
+    assert worst <= 1, f"{worst:.3g} times the bound at token {(off / (e * norm + least)).argmax().item()}"
+    if not given:
+        assert (got[:, 0] == 0).all()   # nothing passes the first token's decay
