@@ -239,10 +239,11 @@ struct Row {
     }
 };
 
-// Bins of equal width that grow as the logits fall.
+// Bins of equal width that grow as the logits fall.  The scale stays finite (3.4e38) where the range is below 6e-36: a bin's
+// lower edge follows from it.
 struct Bins {
     float top, scale;
-    RQ_DEV Bins(float top_, float range) : top(top_), scale((float)(kBins - 1) / range) {}
+    RQ_DEV Bins(float top_, float range) : top(top_), scale(fminf((float)(kBins - 1) / range, 3.4e38f)) {}
     RQ_DEV int of(float l) const {
         const float x = l == top ? 0.f : (top - l) * scale;
         return x < (float)(kBins - 1) ? (int)x : kBins - 1;
