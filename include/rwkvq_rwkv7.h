@@ -81,8 +81,8 @@ int rq_wkv7_step(const void* r, const void* w, const void* k, const void* v, con
  *   4. the first by index at which the running sum of what stays exceeds u times the whole.
  * Equal logits rank by index.  A temperature of 0 takes the largest logit.  logprob[i] (or NULL) is the log of the
  * token's share of what stays.  -inf logits never come; +inf ones share everything.  A row with a NaN, or of
- * -inf alone, gives token -1 and a NaN.  The sums are taken in float64 from terms rounded to 2^-36
- * (2^-33 past 2^17 logits), exactly.
+ * -inf alone, gives token -1 and a NaN.  The sums are exact, of terms of float64 rounded to 2^-36
+ * (2^-33 past 2^17 logits); a token whose e_j is below half of that never comes.
  *
  * temperature, top_k, top_p, min_p: one for each row, or NULL for the value behind it.  Values on the
  * device are not checked: a temperature that is not above 0 is 0, top_k below 1 is 0, a top_p of 0 or less keeps the

@@ -18,10 +18,10 @@
 // from the top; and for the sums of what stays.
 //
 // The sums decide which token comes, so they are exact: every e_i is a float64 rounded to
-// a multiple of 2^-36 (coarser for a vocabulary past 2^17), and a row's sum of such
+// a multiple of 2^-36 (2^-33 for a vocabulary past 2^17), and a row's sum of such
 // numbers needs no more than 53 bits.  The order in which they are added does not
-// matter then, and tokens that the rounding takes to 0 have less than 2^-36 of the most
-// likely one's probability.
+// matter then.  Tokens whose e_i is below half of that are rounded to 0 and never come: each has less than 2^-37
+// (2^-34) of the most likely one's probability, and n of them at most n times as much of the whole.
 #include <algorithm>
 
 #include "rq_common.h"

@@ -390,8 +390,9 @@ def sample(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] = 1.0, t
 
     Equal logits rank by index.  Each parameter is a number, or a tensor [...] with one for each row
     (numbers of 32 bits).  A temperature of 0, or a top_k of 1, takes the largest.  -inf logits never
-    come; a row of nothing else, or with a NaN in it, gives -1 and a NaN.  The sums are exact
-    (terms of float64 rounded to 2^-36 of the largest), so the same inputs give the same tokens.  Without gradients."""
+    come; a row of nothing else, or with a NaN in it, gives -1 and a NaN.  The sums are exact, of terms of float64
+    rounded to 2^-36 of the largest (2^-33 for a vocabulary past 2^17), so the same inputs give the same tokens; one
+    whose e_i is below half of that never comes.  Without gradients."""
     _float(logits, "logits")
     if logits.dim() < 1 or u.dtype != torch.float32 or u.shape != logits.shape[:-1]:
         raise ValueError(f"u must be float32 of shape {tuple(logits.shape[:-1])} (got {u.dtype} {tuple(u.shape)})")

@@ -1,4 +1,6 @@
-"""The sampler on rows whose logits lie closer together than its bins."""
+"""The sampler on rows whose logits lie closer together, or further apart, than its bins and quanta."""
+import math
+
 import pytest
 import torch
 
@@ -39,3 +41,30 @@ def test_temperatures_next_to_nothing(rq, dev):
         for kw in ({"top_p": 0.9}, {"top_p": 0.9, "top_k": 40}, {"min_p": 0.1}):
             token, logprob = rq.sample(logits, u, temperature=t, **kw)
             assert torch.equal(token, logits.argmax(-1)) and (logprob == 0).all(), (t, kw)
+
+
+@pytest.mark.parametrize("vocab", [70000, 131072, 131073, 2 ** 20])
+def test_terms_next_to_the_quantum(rq, dev, vocab):
+    """A term is rounded to whole quanta of 2^-36, past 2^17 logits 2^-33: tokens below half of one never come, and the sums
+    and the log-probabilities are those of the rounded terms."""
+    bits = 36 if vocab <= 2 ** 17 else 33
+    at = vocab // 3
+    u = torch.tensor([0.0, 0.5, 1 - 2.0 ** -10, 1 - 2.0 ** -24], device=dev)
+    for quanta in (0.4, 0.6, 1.4, 2.6):
+        logits = torch.full((len(u), vocab), math.log(quanta * 2.0 ** -bits))
+        logits[:, at] = 0.0
+        logits = logits.to(dev)
+        tail = round(quanta)
+        term = torch.full((vocab,), tail, dtype=torch.int64)
+        term[at] = 2 ** bits
+        upto = term.cumsum(0).double()   # below 2^53: exact
+        whole = int(upto[-1])
+        want = [min(int((upto <= min(x * whole, whole - 1)).sum()), vocab - 1) for x in u.double().tolist()]
+        if tail == 0:
+            assert want == [at] * len(u)
+        for kw in ({}, {"top_p": 1 - 2.0 ** -24}) if tail == 0 else ({},):
+            token, logprob = rq.sample(logits, u, **kw)
+            assert token.tolist() == want, (quanta, kw)
+            z = torch.where(token.cpu() == at, 0.0, logits[0, at - 1].double().cpu().item())
+            share = z - math.log(whole / 2 ** bits)
+            assert ((logprob.double().cpu() - share).abs() <= 2.0 ** -24 * share.abs() + 2.0 ** -45).all()
