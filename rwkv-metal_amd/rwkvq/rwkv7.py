@@ -21,7 +21,8 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._lib import DTYPE_CODE, check, lib
-from .ops import _DeviceGuard, _eager, _float, _on_gpu, _ptr, _ready, _stream_on
+from .ops import (_PLAIN, _DeviceGuard, _dispatch_modes, _eager, _float, _function_modes, _functorch_active,
+                  _is_compiling, _on_gpu, _ptr, _ready, _stream_on, _tracing)
 from .train import _addr, _queried_workspace, _records, _size
 
 HEAD_SIZE = 64   # channels of a head
@@ -31,6 +32,7 @@ CHUNK = 16       # tokens between two states that are kept for the backward pass
 # -------------------------------------------------------------- recurrence
 
 _device_of, _address_of, _contiguous_one = Tensor.get_device, Tensor.data_ptr, Tensor.is_contiguous
+_PLAIN_TYPES = frozenset(_PLAIN)
 
 
 def _operands(ts: list) -> Tuple[list, list]:
@@ -295,36 +297,78 @@ def wkv7(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state
 
 # --------------------------------------------------------------- one token
 
+def _plain(ts: list) -> bool:
+    """_eager, column by column."""
+    if _is_compiling() or _dispatch_modes() or _function_modes() or _functorch_active() or _tracing() is not None:
+        return False
+    return _PLAIN_TYPES.issuperset(map(type, ts)) and -1 not in map(_device_of, ts)
+
+
+def _wkv7_step_into(six: list, state: Tensor, out: Tensor, out_dtype: torch.dtype) -> Tensor:
+    """y, with the new state in `out`."""
+    if not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError("out must be contiguous and 16-byte aligned")
+    if out is not state and out.data_ptr() != state.data_ptr() and _overlap(out, state):
+        raise ValueError("out may be the state itself, but must not overlap it otherwise")
+    held, at = _operands([*six, state, out])
+    r = held[0]
+    y = torch.empty(r.shape, dtype=out_dtype, device=r.device)
+    with _DeviceGuard(r.device):
+        rc = lib().rq_wkv7_step(*at[:6], DTYPE_CODE[r.dtype], r.shape[0], r.shape[1], at[6], y.data_ptr(),
+                                DTYPE_CODE[out_dtype], at[7], _stream_on(r.device))
+    if rc:
+        check(rc, "wkv7_step")
+    return y
+
+
+def _wkv7_step_op_impl(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state: Tensor,
+                       out_dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
+    out = torch.empty(state.shape, dtype=torch.float32, device=state.device)
+    return _wkv7_step_into([r, w, k, v, a, b], state, out, out_dtype), out
+
+
+def _wkv7_step_out_op_impl(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor,
+                           state: Optional[Tensor], out: Tensor, out_dtype: torch.dtype) -> Tensor:
+    return _wkv7_step_into([r, w, k, v, a, b], out if state is None else state, out, out_dtype)
+
+
+_wkv7_step_op = torch.library.custom_op("rwkvq::wkv7_step", _wkv7_step_op_impl, mutates_args=())
+# state None: the one in `out`
+_wkv7_step_out_op = torch.library.custom_op("rwkvq::wkv7_step_out", _wkv7_step_out_op_impl, mutates_args=("out",))
+
+
+@_wkv7_step_op.register_fake
+def _(r, w, k, v, a, b, state, out_dtype):
+    return r.new_empty(r.shape, dtype=out_dtype), state.new_empty(state.shape)
+
+
+@_wkv7_step_out_op.register_fake
+def _(r, w, k, v, a, b, state, out, out_dtype):
+    return r.new_empty(r.shape, dtype=out_dtype)
+
+
 def wkv7_step(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state: Tensor,
               out: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
     """(y, new state) of one token of every sequence: r .. b [batch, heads, 64], state
     [batch, heads, 64, 64].  out: a contiguous float32 tensor for the new state, `state` itself for an
     update in place.  Without gradients (wkv7 over a time of 1 has them)."""
     six = [r, w, k, v, a, b]
-    shape = _check_inputs(six, 3)
+    batch, heads, _ = _check_inputs(six, 3)
     six, dt = _same_dtype(six)
     odt = _out_dtype(out_dtype, dt)
-    batch, heads, _ = shape
     _check_state(state, batch, heads)
-    if out is None:
-        out = torch.empty(state.shape, dtype=torch.float32, device=state.device)
-    elif out is not state:
+    ts = [*six, state]
+    if out is not None and out is not state:
         _check_state(out, batch, heads, "out")
-        if not out.is_contiguous() or out.data_ptr() % 16:
-            raise ValueError("out must be contiguous and 16-byte aligned")
-        if out.data_ptr() != state.data_ptr() and _overlap(out, state):
-            raise ValueError("out may be the state itself, but must not overlap it otherwise")
-    elif not out.is_contiguous() or out.data_ptr() % 16:
-        raise ValueError("out must be contiguous and 16-byte aligned")
-    held, at = _operands([*six, state, out])
-    device = held[0].device
-    y = torch.empty(shape, dtype=odt, device=device)
-    with _DeviceGuard(device):
-        rc = lib().rq_wkv7_step(*at[:6], DTYPE_CODE[dt], batch, heads, at[6], y.data_ptr(), DTYPE_CODE[odt], at[7],
-                                _stream_on(device))
-    if rc:
-        check(rc, "wkv7_step")
-    return y, out
+        ts.append(out)
+    if _plain(ts):
+        if out is None:
+            out = torch.empty(state.shape, dtype=torch.float32, device=state.device)
+        return _wkv7_step_into(six, state, out, odt), out
+    with torch.no_grad():
+        if out is None:
+            return _wkv7_step_op(*six, state, odt)
+        return _wkv7_step_out_op(*six, None if out is state else state, out, odt), out
 
 
 def _overlap(x: Tensor, y: Tensor) -> bool:
