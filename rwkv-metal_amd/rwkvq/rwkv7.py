@@ -19,6 +19,7 @@ import torch
 from torch import Tensor
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from ._lib import DTYPE_CODE, check, lib
 from .ops import (_PLAIN, _DeviceGuard, _dispatch_modes, _eager, _float, _function_modes, _functorch_active,
@@ -298,10 +299,10 @@ def wkv7(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state
 # --------------------------------------------------------------- one token
 
 def _plain(ts: list) -> bool:
-    """_eager, column by column."""
+    """_eager, column by column; that all are on the last one's device is left to _operands."""
     if _is_compiling() or _dispatch_modes() or _function_modes() or _functorch_active() or _tracing() is not None:
         return False
-    return _PLAIN_TYPES.issuperset(map(type, ts)) and -1 not in map(_device_of, ts)
+    return _PLAIN_TYPES.issuperset(map(type, ts)) and ts[-1].is_cuda
 
 
 def _wkv7_step_into(six: list, state: Tensor, out: Tensor, out_dtype: torch.dtype) -> Tensor:
@@ -351,7 +352,7 @@ def wkv7_step(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, 
               out: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
     """(y, new state) of one token of every sequence: r .. b [batch, heads, 64], state
     [batch, heads, 64, 64].  out: a contiguous float32 tensor for the new state, `state` itself for an
-    update in place.  Without gradients (wkv7 over a time of 1 has them)."""
+    update in place; it must not require gradients.  Without gradients (wkv7 over a time of 1 has them)."""
     six = [r, w, k, v, a, b]
     batch, heads, _ = _check_inputs(six, 3)
     six, dt = _same_dtype(six)
@@ -361,10 +362,16 @@ def wkv7_step(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, 
     if out is not None and out is not state:
         _check_state(out, batch, heads, "out")
         ts.append(out)
+    if out is not None and out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out is written to without gradients: it must not require them")
     if _plain(ts):
         if out is None:
             out = torch.empty(state.shape, dtype=torch.float32, device=state.device)
-        return _wkv7_step_into(six, state, out, odt), out
+            return _wkv7_step_into(six, state, out, odt), out
+        y = _wkv7_step_into(six, state, out, odt)
+        if not out.is_inference():  # what was saved of it for a backward pass is no longer there
+            increment_version(out)
+        return y, out
     with torch.no_grad():
         if out is None:
             return _wkv7_step_op(*six, state, odt)

@@ -1,0 +1,53 @@
+"""Calls of the recurrence that its documentation allows and that are easily forgotten: steps whose state something
+else still needs, tracing, forward mode, memory around the tensors."""
+import math
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from wkv_ref import D, DT, NAMES, inputs
+
+pytestmark = pytest.mark.gpu
+
+
+def token(dev, batch=3, heads=2, dt=torch.bfloat16, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    six = [x.to(dev) for x in inputs(g, batch, heads, dtype=dt)]
+    return six, torch.randn(batch, heads, D, D, generator=g).to(dev)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_a_saved_state_that_is_written_to(rq, dev, in_place):
+    """As torch's own operations in place: an error where the old values are needed."""
+    six, state = token(dev)
+    out = state if in_place else torch.zeros_like(state)
+    weight = torch.ones_like(state).requires_grad_()
+    loss = (out * weight).sum()       # keeps `out` for weight's gradient
+    version = out._version
+    rq.wkv7_step(*six, state, out=out)
+    assert out._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    view = torch.zeros(2, *state.shape, device=dev)
+    version = view._version
+    rq.wkv7_step(*six, state, out=view[1])
+    assert view._version > version and (view[0] == 0).all()
+
+
+def test_an_output_that_requires_gradients(rq, dev):
+    six, state = token(dev)
+    leaf = torch.zeros_like(state).requires_grad_()
+    for out in (leaf, leaf * 2):
+        with pytest.raises(ValueError, match="gradients"):
+            rq.wkv7_step(*six, state, out=out)
+    with pytest.raises(ValueError, match="gradients"):
+        rq.wkv7_step(*six, leaf, out=leaf)
+    want = rq.wkv7_step(*six, state)[1]
+    with torch.no_grad():
+        rq.wkv7_step(*six, state, out=leaf)
+    assert torch.equal(leaf, want)
+    with torch.inference_mode():
+        mine = state.clone()
+        y, new = rq.wkv7_step(*six, mine, out=mine)
+    assert torch.equal(new, want)
