@@ -211,6 +211,12 @@ class _Wkv7Function(torch.autograd.Function):
     _once = staticmethod(once_differentiable(_run.__func__))
 
 
+def _no_tangents(*ts: Tensor) -> None:
+    """Refuses operands with a forward-mode tangent, which would be lost: there is no formula for one."""
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError("wkv7, wkv7_step and sample have no forward-mode derivatives")
+
+
 def _same_dtype(six):
     """The six in one dtype, float32 where they come in several."""
     dt = six[0].dtype
@@ -288,11 +294,12 @@ def wkv7(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state
     if state is not None:
         _check_state(state, seqs, heads)
     ts = six if state is None else [*six, state]
+    if not _is_compiling() and forward_ad._current_level >= 0:
+        _no_tangents(*ts)
     if _eager(*ts):
         if not torch.is_grad_enabled() or not any(t.requires_grad for t in ts):
             return _wkv7_impl(*six, state, cu_seqlens, odt, False)[:2]
-        if forward_ad._current_level < 0:
-            return _Wkv7Function.apply(*six, state, cu_seqlens, odt)
+        return _Wkv7Function.apply(*six, state, cu_seqlens, odt)
     return _wkv7_op(*six, state, cu_seqlens, odt, _records(*ts))[:2]
 
 
@@ -364,6 +371,8 @@ def wkv7_step(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, 
         ts.append(out)
     if out is not None and out.requires_grad and torch.is_grad_enabled():
         raise ValueError("out is written to without gradients: it must not require them")
+    if not _is_compiling() and forward_ad._current_level >= 0:
+        _no_tangents(*ts)
     if _plain(ts):
         if out is None:
             out = torch.empty(state.shape, dtype=torch.float32, device=state.device)
@@ -453,6 +462,8 @@ def sample(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] = 1.0, t
     p, p_all = _parameter(top_p, "top_p", lead, False)
     m, m_all = _parameter(min_p, "min_p", lead, False)
     given = [x for x in (t, k, p, m) if x is not None]
+    if not _is_compiling() and forward_ad._current_level >= 0:
+        _no_tangents(logits, u, *given)
     op = _sample_impl if _eager(logits, u, *given) else _sample_op
     with torch.no_grad():
         return op(logits, u, t, k, p, m, t_all, min(k_all, 1 << 62), p_all, m_all)

@@ -89,3 +89,36 @@ def test_refusals_of_recorded_steps(rq):
         rq.wkv7_step(*[x[0] for x in six], state)
     with pytest.raises(RuntimeError, match="only on a ROCm GPU"):
         rq.wkv7_step(*[torch.zeros(1, 1, 64)] * 6, torch.zeros(1, 1, 64, 64))
+
+
+def test_forward_mode_is_refused(rq):
+    """Of an operand with a tangent, whether or not anything requires gradients; the others run."""
+    from torch.autograd import forward_ad
+    six, state = token()
+    seq = [meta(1, 9, 2, 64) for _ in range(6)]
+    first, logits, u = meta(1, 2, 64, 64, dt=torch.float32), meta(3, 50), meta(3, dt=torch.float32)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.empty_like(t))
+
+        for needs in (False, True):
+            for i in (0, 1, 5):
+                args = [x.detach().requires_grad_(needs) for x in seq]
+                args[i] = dual(args[i])
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    rq.wkv7(*args)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            rq.wkv7(*seq, dual(first))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            rq.wkv7_step(*six[:3], dual(six[3]), *six[4:], state)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            rq.wkv7_step(*six, dual(state))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            rq.wkv7_step(*six, state, out=dual(torch.empty_like(state)))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            rq.sample(dual(logits), u)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            rq.sample(logits, u, temperature=dual(u))
+        rq.wkv7(*seq, first)
+        rq.wkv7_step(*six, state)
+        rq.sample(logits, u)
