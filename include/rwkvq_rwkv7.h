@@ -68,7 +68,8 @@ int rq_wkv7_backward(const void* r, const void* w, const void* k, const void* v,
                      float* dstate, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* One token of every sequence: r .. b and y [batch, heads, 64], state and state_out
- * [batch, heads, 64, 64] (they may be one buffer; state NULL for 0). */
+ * [batch, heads, 64, 64] (they may be one buffer; state NULL for 0).  Otherwise what is written must
+ * not overlap what is read: there is no order between the heads. */
 int rq_wkv7_step(const void* r, const void* w, const void* k, const void* v, const void* a, const void* b,
                  rq_dtype dt, int64_t batch, int64_t heads, const float* state, void* y, rq_dtype y_dt,
                  float* state_out, void* stream);

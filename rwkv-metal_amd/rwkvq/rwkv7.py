@@ -320,6 +320,12 @@ def _wkv7_step_into(six: list, state: Tensor, out: Tensor, out_dtype: torch.dtyp
         raise ValueError("out may be the state itself, but must not overlap it otherwise")
     held, at = _operands([*six, state, out])
     r = held[0]
+    first, size = at[7], r.numel() * r.element_size()
+    behind = first + 4 * out.numel()
+    if size and min(at[:6]) < behind and max(at[:6]) + size > first:
+        # a block writes its head's state while others still read their tokens
+        if any(x < behind and x + size > first for x in at[:6]):
+            raise ValueError("out must not overlap r, w, k, v, a or b")
     y = torch.empty(r.shape, dtype=out_dtype, device=r.device)
     with _DeviceGuard(r.device):
         rc = lib().rq_wkv7_step(*at[:6], DTYPE_CODE[r.dtype], r.shape[0], r.shape[1], at[6], y.data_ptr(),
@@ -359,7 +365,7 @@ def wkv7_step(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, 
               out: Optional[Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
     """(y, new state) of one token of every sequence: r .. b [batch, heads, 64], state
     [batch, heads, 64, 64].  out: a contiguous float32 tensor for the new state, `state` itself for an
-    update in place; it must not require gradients.  Without gradients (wkv7 over a time of 1 has them)."""
+    update in place; it must not require gradients, nor share memory with r .. b.  Without gradients (wkv7 over a time of 1 has them)."""
     six = [r, w, k, v, a, b]
     batch, heads, _ = _check_inputs(six, 3)
     six, dt = _same_dtype(six)

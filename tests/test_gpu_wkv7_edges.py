@@ -51,3 +51,28 @@ def test_an_output_that_requires_gradients(rq, dev):
         mine = state.clone()
         y, new = rq.wkv7_step(*six, mine, out=mine)
     assert torch.equal(new, want)
+
+
+def test_an_output_over_the_token_is_refused(rq, dev):
+    """Before anything is launched; memory side by side is not refused."""
+    batch, heads = 3, 2
+    size, n = batch * heads * D * D, batch * heads * D
+    memory = torch.zeros(size + 6 * n, device=dev)
+    state = torch.randn(batch, heads, D, D, device=dev)
+    out = memory[:size].view(state.shape)
+    beside = [memory[size + i * n:size + (i + 1) * n].view(batch, heads, D) for i in range(6)]
+    want, _ = rq.wkv7_step(*beside, state)
+    got, new = rq.wkv7_step(*beside, state, out=out)
+    assert torch.equal(got, want) and new is out
+    inside = memory[size - n // 2:size + n // 2].view(batch, heads, D)   # its first half
+    for i in range(6):
+        six = [inside if j == i else x for j, x in enumerate(beside)]
+        with pytest.raises(ValueError, match="overlap"):
+            rq.wkv7_step(*six, state, out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            rq.wkv7_step(*six, out, out=out)
+    # a strided one is copied first
+    apart = memory[:2 * n].view(n, 2)[:, 0].view(batch, heads, D)
+    rq.wkv7_step(apart, *beside[1:], state, out=out)
+    for x in rq.wkv7_step(*[x[:0] for x in beside], state[:0], out=out[:0]):
+        assert x.numel() == 0
