@@ -265,7 +265,7 @@ def wkv7(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state
     64 values, 64 keys] before the first token, 0 by default.  y has the inputs' dtype or
     out_dtype (float32 is the other choice); the state, its products and all sums are float32.
 
-    cu_seqlens: packed sequences in a batch of one; n + 1 int32 values on the GPU, from 0,
+    cu_seqlens: packed sequences in a batch of one; n + 1 int32 or int64 values on the GPU, from 0,
     not decreasing.  Sequence i is the tokens cu_seqlens[i] to cu_seqlens[i + 1] with state i of
     [n, heads, 64, 64] (an empty one keeps its state); y and the gradients are 0 behind the
     last.  Nothing waits for their values: boundaries outside the batch are moved into it, and
@@ -290,7 +290,9 @@ def wkv7(r: Tensor, w: Tensor, k: Tensor, v: Tensor, a: Tensor, b: Tensor, state
         seqs = cu_seqlens.numel() - 1
         if seqs == 0 and time:
             raise ValueError("cu_seqlens holds no sequence")
-        cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+        if cu_seqlens.dtype == torch.int64:  # into the batch before the type takes the high bits off
+            cu_seqlens = cu_seqlens.clamp(0, time).to(torch.int32)
+        cu_seqlens = cu_seqlens.contiguous()
     if state is not None:
         _check_state(state, seqs, heads)
     ts = six if state is None else [*six, state]

@@ -76,3 +76,21 @@ def test_an_output_over_the_token_is_refused(rq, dev):
     rq.wkv7_step(apart, *beside[1:], state, out=out)
     for x in rq.wkv7_step(*[x[:0] for x in beside], state[:0], out=out[:0]):
         assert x.numel() == 0
+
+
+def test_boundaries_of_64_bits(rq, dev):
+    """Moved into the batch by their value, whatever their low 32 bits say."""
+    g = torch.Generator().manual_seed(2)
+    six = [x.to(dev).requires_grad_() for x in inputs(g, 1, 30, 2)]
+    dy = torch.randn(1, 30, 2, D, generator=g).to(dev)
+    far = torch.tensor([-2 ** 32, 10, 10, 2 ** 32 + 12], device=dev)
+    near = torch.tensor([0, 10, 10, 30], dtype=torch.int32, device=dev)
+    got, want = [], []
+    for cu, res in ((far, got), (near, want)):
+        y, last = rq.wkv7(*six, cu_seqlens=cu)
+        res += [y, last, *torch.autograd.grad(y, six, dy)]
+    for x, z in zip(got, want):
+        assert torch.equal(x, z)
+    far = torch.tensor([2 ** 33, 2 ** 33 + 5, 2 ** 40], device=dev)   # all behind the end
+    y, last = rq.wkv7(*six, cu_seqlens=far)
+    assert (y == 0).all() and (last == 0).all()
