@@ -435,7 +435,11 @@ def _(logits, u, temperature, top_k, top_p, min_p, temperature_all, top_k_all, t
 def _parameter(x, name: str, lead, whole: bool):
     """(a value for each row, a value for all) of a parameter that is one or the other."""
     if not isinstance(x, Tensor):
-        return None, (int(x) if whole else float(x))
+        if not whole:
+            return None, float(x)
+        if int(x) != x:
+            raise ValueError(f"{name} must be an integer (got {x})")
+        return None, max(-1, min(int(x), 1 << 62))  # any negative number is refused as -1 is
     if x.is_floating_point() if whole else not x.is_floating_point():
         raise ValueError(f"{name} must hold {'integers' if whole else 'floating numbers'} (got {x.dtype})")
     if x.shape != lead:
@@ -474,4 +478,4 @@ def sample(logits: Tensor, u: Tensor, temperature: Union[float, Tensor] = 1.0, t
         _no_tangents(logits, u, *given)
     op = _sample_impl if _eager(logits, u, *given) else _sample_op
     with torch.no_grad():
-        return op(logits, u, t, k, p, m, t_all, min(k_all, 1 << 62), p_all, m_all)
+        return op(logits, u, t, k, p, m, t_all, k_all, p_all, m_all)

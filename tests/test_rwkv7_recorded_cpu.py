@@ -122,3 +122,15 @@ def test_forward_mode_is_refused(rq):
         rq.wkv7(*seq, first)
         rq.wkv7_step(*six, state)
         rq.sample(logits, u)
+
+
+def test_top_k_is_a_whole_number(rq, monkeypatch):
+    logits, u = meta(3, 50), meta(3, dt=torch.float32)
+    seen = []
+    monkeypatch.setattr(rq.rwkv7, "_sample_op", lambda *a: seen.append(a[7]) or (u, u))
+    for x, want in ((5, 5), (5.0, 5), (True, 1), (2 ** 80, 2 ** 62), (-3, -1), (-2 ** 80, -1)):
+        rq.sample(logits, u, top_k=x)
+        assert seen[-1] == want
+    for x in (2.5, 0.9):
+        with pytest.raises(ValueError, match="top_k must be an integer"):
+            rq.sample(logits, u, top_k=x)
