@@ -97,20 +97,31 @@ class Model(nn.Module):
         self.head = rwkvq.QuantizedLinear.from_linear(nn.Linear(d, vocab, bias=False, **kw))
 
     def forward(self, idx, state=None, cu=None):
-        """(logits, state) of whole sequences, idx [batch, time] or packed [1, time].  The state is
-        a list with (the last token's input, the recurrence's states) of each block."""
+        """(logits, state) of whole sequences, idx [batch, time] or packed [1, time] with their boundaries `cu`.
+        The state is a list with (the last token's input, the recurrence's states) of each block, for each
+        sequence; a sequence without a token keeps its own."""
         x, after = self.emb(idx), []
         if cu is not None:
-            first = cu[:-1].long()
+            start, end = cu[:-1].long(), cu[1:].long()
+            # rows: what the sequences had last, then the tokens.  A token's predecessor is the row before its own, a
+            # sequence's first token's what that sequence had last
+            seqs, time = torch.arange(start.numel(), device=idx.device), idx.shape[1]
+            source = torch.arange(time + 1, device=idx.device) + (len(seqs) - 1)
+            source[torch.where(end > start, start, time)] = seqs
+            source, left = source[:time], torch.where(end > start, end - 1 + len(seqs), seqs)
         for i, b in enumerate(self.blocks):
             n = b.norm1(x)
-            last = F.pad(n, (0, 0, 1, -1))  # each token's predecessor
-            if cu is not None:              # none in another sequence
-                last = last.index_fill(1, first, 0)
-            elif state is not None:
-                last = torch.cat([state[i][0][:, None], last[:, 1:]], 1)
+            if cu is not None:
+                before = n.new_zeros(len(seqs), n.shape[-1]) if state is None else state[i][0]
+                rows = torch.cat([before, n[0]])
+                last, kept = rows[source][None], rows[left]
+            else:
+                last = F.pad(n, (0, 0, 1, -1))  # each token's predecessor
+                if state is not None:
+                    last = torch.cat([state[i][0][:, None], last[:, 1:]], 1)
+                kept = n[:, -1]
             y, s = b.time(n, last, None if state is None else state[i][1], cu)
-            after.append((n[:, -1], s))
+            after.append((kept, s))
             x = x + y
             x = b.value(b.key(b.norm2(x)), residual=x)
         return self.head(self.norm(x)), after
