@@ -103,7 +103,6 @@ struct Lds {
     unsigned long long first;
     double found_sum, total;
     uint32_t found, found_key;
-    int nan;
 };
 
 // Over a wave by data-parallel moves: rows of 16 lanes, then the rows.
