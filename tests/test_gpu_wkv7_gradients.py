@@ -81,3 +81,25 @@ def test_decay_gradients_token_by_token(rq, dev, i, dt, given):
     assert worst <= 1, f"{worst:.3g} times the bound at token {(off / (e * norm + least)).argmax().item()}"
     if not given:
         assert (got[:, 0] == 0).all()   # nothing passes the first token's decay
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("i", range(len(LONE)))
+def test_everything_token_by_token(rq, dev, i, dt):
+    """y and the other gradients by each token's own norm, in the same company."""
+    name, at, w, others = LONE[i]
+    print(f"wkv7 by tokens {name} w={w} others={others} {dt}", flush=True)
+    t, h = 40, 4
+    g = torch.Generator().manual_seed(450 + i)
+    six = inputs(g, 1, t, h, dtype=DT[dt], w=others)
+    six[1][:, at] = w
+    state, dstate = torch.randn(1, h, D, D, generator=g), torch.randn(1, h, D, D, generator=g)
+    dy = torch.randn(1, t, h, D, generator=g).to(DT[dt])
+    want = reference(six, state, dy, dstate)
+    got = dict(zip(["d" + n for n in NAMES], grads(rq, dev, six, state, dy, dstate, None, DT[dt])))
+    got["y"] = rq.wkv7(*[x.to(dev) for x in six], state.to(dev))[0]
+    least = math.sqrt(h * D) * torch.finfo(DT[dt]).smallest_normal * torch.finfo(DT[dt]).eps / 2
+    for n, x in got.items():
+        off = (x.double().cpu() - want[n]).norm(dim=(2, 3))[0]
+        worst = off / (bound(n, DT[dt], t) * want[n].norm(dim=(2, 3))[0] + least)
+        assert worst.max() <= 1, f"{n}: {worst.max().item():.3g} times the bound at token {worst.argmax().item()}"
