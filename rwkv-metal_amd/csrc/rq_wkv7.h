@@ -76,7 +76,7 @@ inline int64_t wkv_chunks(const WkvShape& s) {
 // kJoinUs, the further launches kMoreUs.  A block has a CU to itself, and one block more than there are CUs is a
 // whole turn more: 12 heads of 8192 tokens took 93 us forwards in 264 blocks of 24 chunks, 73 us in 252 of 25.
 inline WkvSegments wkv_segments(const WkvShape& s, bool backward) {
-    constexpr double kScanUs = 2.4, kBackUs = 6, kEndsUs = 2.7, kJoinUs = 0.8, kMoreUs = 12;
+    constexpr double kScanUs = 2.4, kBackUs = 7, kEndsUs = 2.7, kJoinUs = 0.8, kMoreUs = 12;
     constexpr int64_t kCus = 256, kBegin = 2;
     WkvSegments best{0, 0, nullptr, nullptr};
     if (s.seqs == 0 || s.heads == 0 || s.time == 0) return best;

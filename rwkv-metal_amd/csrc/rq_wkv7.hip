@@ -429,6 +429,10 @@ RQ_DEV float at_token(const f32x4_t& x, int t, int m) {
     return __shfl(own, 16 * (t >> 2) + m);
 }
 
+RQ_DEV float of_lane(float x, int lane) {  // the same in all lanes
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+
 // A wave's accesses of LDS before it are done before those behind it, for all its lanes: the machine keeps their order, and
 // this has the compiler keep it too, which takes a lane's addresses for its own.
 RQ_DEV void wave_lds_order() {
@@ -519,14 +523,14 @@ RQ_DEV void chunk_grads(const f32x4_t* s, const Rows& dy_rows, GradRows& lds, in
 #pragma unroll 1
         for (int src = 0; src < kChunk - 1; ++src) {
             const float bs = at_token(b, src, m), ks = at_token(k, src, m);
+            const float of_m[4] = {lds.pairs[0][m][src], lds.pairs[1][m][src], lds.pairs[2][m][src], lds.pairs[3][m][src]};
             float e = 0.f;
 #pragma unroll 1
             for (int t = src + 1; t < kChunk; ++t) {
                 const float h = exp2_hw(e);
                 e += at_token(g2, t, m);
                 const float f = exp2_hw(e), rt = at_token(r, t, m) * f, at_ = at_token(a, t, m) * h;
-                const float m0 = lds.pairs[0][t][src], m1 = lds.pairs[1][t][src], m2 = lds.pairs[2][t][src],
-                            m3 = lds.pairs[3][t][src];
+                const float m0 = of_lane(of_m[0], t), m1 = of_lane(of_m[1], t), m2 = of_lane(of_m[2], t), m3 = of_lane(of_m[3], t);
                 const float of_a = m0 * bs + m1 * ks, of_r = m2 * bs + m3 * ks;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -857,9 +861,9 @@ __global__ __launch_bounds__((kScanThreads<REV, ENDS>)) void wkv7_scan_kernel(Wk
             load(c + 3);
             __syncthreads();
             if (GRADS) {
-                matrix(c + 1, next);
-                __syncthreads();
                 store_y(c);
+                __syncthreads();
+                matrix(c + 1, next);
                 __syncthreads();
             }
             next = ring;
