@@ -512,8 +512,9 @@ RQ_DEV void choose(const SampleArgs& p, int64_t r, int64_t at, float l, const We
 
 // A block of 16 waves for each row, whatever their number: bound by a CU's VALU where all of a row needs its e_i (some 30
 // operations, most in float64) and by the latency of its passes elsewhere.  Rows of 65536: one with top_p 30 us, 128 with
-// top_k 50 and top_p 19 us, 512 of which everything stays 45 us (67 MB at 1.5 TB/s).  A row's work over several CUs
-// would need two launches more, for the largest logit and for the bins, about 22 us for the one row.
+// top_k 50 and top_p 19 us, 512 of which everything stays 45 us (67 MB at 1.5 TB/s; VALU instructions for 60 % of the cycles at
+// four each, and float64 ones take more).  A row's work over several CUs is not built: it needs launches more, for the
+// largest logit and for the bins, and a workspace.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs p) {
     __shared__ Lds lds;

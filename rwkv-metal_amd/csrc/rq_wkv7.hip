@@ -20,7 +20,9 @@
 //   dr = e^L (dY S + dMrb B~ + dMrk K~)             dMrb = incl(dY SA^T), dMrk = incl(dY V^T)
 //   da = e^Lx (dZ S + dMab B~ + dMak K~)            dMab = strict(dZ SA^T), dMak = strict(dZ V^T)
 //   db = e^-L (e^Lend SA dS' + dMrb^T R~ + dMab^T A~), dk alike with V, dMrk, dMak
-//   dlog d_t: what of the loss passes token t's decay (chunk_grads).
+//   dlog d_i = e^Lend sum_v S dS' + sum_{s<i} b_s e^(Lend-L_s) (SA dS')_s (and k, V)
+//            + sum_{t>=i} r_t e^L_t (dY S)_t + sum_{t>i} a_t e^Lx_t (dZ S)_t
+//            + sum_{s<i<=t} r_t e^(L_t-L_s) (dMrb_ts b_s + dMrk_ts k_s) + sum_{s<i<t} a_t e^(Lx_t-L_s) (dMab_ts b_s + dMak_ts k_s)
 //
 // All products are fp32 MFMAs (v_mfma_f32_16x16x4_f32): the state lives in fp32 and feeds itself for thousands of
 // tokens, and the gradients of 16-bit tensors are rounded once, where they are stored.
@@ -771,20 +773,23 @@ RQ_DEV void clear_rest(const WkvShape& s, std::initializer_list<void*> tensors) 
 // holds its state transposed, acc[q][i] = S[value lane & 15][key 16q + 4g + i]: the layout in which a product's
 // result comes and in which the next takes it.  It reads nothing from memory: on this machine loads and
 // stores are waited for in their order, and a load behind a store waits for the store too.
-// What bounds it is a SIMD's issue: of a chunk's 2.35 us (5000 cycles; 2.9 us with the states written for the
-// backward pass) the scan wave's 79 fp32 MFMAs and the matrix wave's 16 take 3000, during which the SIMD's VALU stands still, and the
-// VALU of its three waves most of the rest.  32 heads of 8 x 512 tokens take 93 us forwards, 205 backwards, at 2.2
-// TB/s of HBM.  Of one sequence of 2047 tokens: 100 us in eight segments, 290 us whole.
+// What bounds it: of a chunk's 2.35 us (2.9 us with the states written for the backward pass) the scan wave's 80 fp32
+// MFMAs and the matrix wave's 16 keep a SIMD's matrix core busy for 42 %, its three waves' other instructions take 16 % of its
+// issue, a CU's LDS is busy for 19 %; the rest is the way from one product to the next.  Backwards 6.9 us a chunk: 39, 23 and 27
+// %.  32 heads of 8 x 512 tokens take 93 us forwards, 226 backwards, at 2.2 TB/s of HBM.  Of one sequence of 2047
+// tokens: 100 us in eight segments, 290 us whole.
 //
 // ENDS: only where a segment ends, from a state of 0 (four scan waves) and, without x, from the identity (four more).
 //
 // Backwards (GRADS) the scan waves also form the other gradients of their chunk, from its dS' and dZ in LDS.  That takes more
-// than the 168 registers of twelve waves: there are eight, four for the arrays and the matrices, and a second barrier
-// between scan and gradients.  The first four have time left: what the gradients need but the state, and the
-// gradients on their way to memory, pass through them and LDS, in whole rows; by the scan waves' own loads and stores of single
-// 16-bit numbers a chunk took 7.4 us against 6.4.  Four waves of their own for chunk c - 1, with these loads, took
-// 8.9 us; a kernel of its own behind the scan, dS' and dZ through memory, 145 + 100 us for 8 x 512 tokens of 32 heads
-// against 205.
+// than the 168 registers of twelve waves: there are eight, four for the arrays and the matrices.  A chunk has three phases, with
+// a barrier behind each: the scan; the pair matrices, one a wave, and the products over the values; the pairs.  The next
+// chunk's matrices are formed in the third: in the second they shared the matrix cores, 7.3 us a chunk against 6.9, and of
+// strong decays the two pairwise loops came one after the other (4.9 ms against 6.0 for 8 x 512 tokens of 32 heads, with
+// the forward pass).  The first four waves have time left: what the gradients need but the state, and the
+// gradients on their way to memory, pass through them and LDS, in whole rows.  In an earlier form, of two phases and 6.4 us a chunk,
+// the scan waves' own loads and stores of single 16-bit numbers took 7.4 us, four waves of their own for chunk c - 1
+// 8.9 us, and a kernel of its own behind the scan, dS' and dZ through memory, 145 + 100 us for 8 x 512 tokens against 205.
 template <bool REV, bool ENDS>
 constexpr int kScanThreads = (ENDS ? 16 : REV ? 8 : 12) * 64;
 
