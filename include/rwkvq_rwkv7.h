@@ -48,7 +48,9 @@ extern "C" {
  * state: [seqs, heads, 64, 64] before the first token, NULL for 0; state_out the same
  * after the last, or NULL; the two may be one buffer.  states [rq_wkv7_chunks(), heads, 64, 64] and
  * sa [rq_wkv7_chunks(), heads, 16, 64], both or neither: what rq_wkv7_backward reads
- * (every 16th state, and S_{t-1} a_t of every token). */
+ * (every 16th state, and S_{t-1} a_t of every token).
+ *
+ * At most 2^21 heads of sequences (seqs * heads), and where states are kept 2^23 heads of chunks. */
 int64_t rq_wkv7_chunks(int64_t batch, int64_t time, int64_t seqs, int has_cu_seqlens);
 int64_t rq_wkv7_workspace_bytes(int64_t batch, int64_t time, int64_t heads, int64_t seqs, int has_cu_seqlens);
 int rq_wkv7(const void* r, const void* w, const void* k, const void* v, const void* a, const void* b,
@@ -74,7 +76,7 @@ int rq_wkv7_step(const void* r, const void* w, const void* k, const void* v, con
                  rq_dtype dt, int64_t batch, int64_t heads, const float* state, void* y, rq_dtype y_dt,
                  float* state_out, void* stream);
 
-/* token[i] from the logits [rows, vocab] of dt (vocab at most 2^20, no alignment of the rows) and
+/* token[i] from the logits [rows, vocab] of dt (at most 2^21 rows, vocab at most 2^20, no alignment of the rows) and
  * u[i] in [0, 1), in this order, with e_j = exp((l_j - max l) / temperature):
  *   1. the top_k largest stay (0: all);
  *   2. of these, from the largest, those before whom less than top_p of their sum lies (1: all);
